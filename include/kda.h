@@ -444,6 +444,83 @@ kda_status kda_gqa_full_backward_saved_bf16(const void* dout, const void* q, con
                                             int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int causal,
                                             float rope_theta, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------- local attention --
+ * The attention half of a decoder layer whose queries see a sliding window
+ * and the sequence's first tokens.  No reference counterpart (the neighbours
+ * of gqa_full).  Rows are head_dim contiguous values; *_strides are host
+ * arrays of the element strides of the leading axes (batch, token, head), so
+ * slices of a packed projection and layers of a cache are taken as they are:
+ * every row must start on 16 bytes.  An axis of one entry may have any stride. */
+
+/* rope_table: table [length][D/2][2] = cos, sin of position * theta^(-2 i / D)
+ * (angles in double precision). */
+kda_status kda_rope_table_f32(float* table, int64_t length, int64_t D, float theta, void* stream);
+
+/* qk_norm_rope: for each head row x of q (B,S,QH,D) and k (B,S,KH,D),
+ *   y = rotate(x / sqrt(mean x^2 + eps) * g, table[position])
+ * (half-split rotation), written contiguous to q_out, k_out in the inputs'
+ * type (bf16, or fp32 with f32 != 0); gq, gk (D,) fp32; D 64, 128 or 256.
+ * positions: int32 [B][S], or NULL for 0 .. S-1.  A position outside
+ * [0, table_len) gives NaN rows and sets bit 8 of the device error word. */
+kda_status kda_qk_norm_rope(const void* q, const void* k, const float* gq, const float* gk, const float* table,
+                            int64_t table_len, const int* positions, float eps, void* q_out, void* k_out, int64_t B,
+                            int64_t S, int64_t QH, int64_t KH, int64_t D, const int64_t* q_strides,
+                            const int64_t* k_strides, int f32, void* stream);
+
+/* qk_norm_rope_append (bf16): the same for S new tokens of each request at
+ * positions lengths[b] + s (int32 [B], tokens already cached): q_out (B,S,QH,D)
+ * contiguous, the rotated k and v as it is into the caches (B,cache_len,KH,D,
+ * strided) at those positions.  lengths[b] < 0: an idle slot, zeros and no
+ * write.  A position outside the cache or the table: NaN, no write, bit 8 of
+ * the device error word. */
+kda_status kda_qk_norm_rope_append_bf16(const void* q, const void* k, const void* v, const float* gq,
+                                        const float* gk, const float* table, int64_t table_len, const int* lengths,
+                                        float eps, void* q_out, void* k_cache, void* v_cache, int64_t cache_len,
+                                        int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
+                                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                        const int64_t* k_cache_strides, const int64_t* v_cache_strides, void* stream);
+
+/* Gradients of qk_norm_rope given those of its outputs (contiguous): dq, dk
+ * contiguous in the inputs' type, dgq, dgk fp32 (D,), summed in a fixed order. */
+size_t kda_qk_norm_rope_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int f32);
+kda_status kda_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q, const void* k,
+                                     const float* gq, const float* gk, const float* table, int64_t table_len,
+                                     const int* positions, float eps, void* dq, void* dk, float* dgq, float* dgk,
+                                     int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
+                                     const int64_t* q_strides, const int64_t* k_strides, int f32, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* gqa_window (bf16, D 128): causal attention in which query i sees key j <= i
+ * where i - j < window or j < sinks; scores scaled by 1/sqrt(D).  out
+ * (B,S,QH,D) contiguous; lse, if not NULL, [B][QH][S] fp32: each row's
+ * log2-sum-exp of the scaled scores, for the backward. */
+size_t kda_gqa_window_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D);
+kda_status kda_gqa_window_bf16(const void* q, const void* k, const void* v, void* out, float* lse, int64_t B,
+                               int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window, int64_t sinks,
+                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of gqa_window given dout and the forward's out (B,S,QH,D,
+ * contiguous) and lse: dq, dk, dv bf16, contiguous. */
+size_t kda_gqa_window_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
+                                              int64_t window, int64_t sinks);
+kda_status kda_gqa_window_backward_bf16(const void* dout, const void* q, const void* k, const void* v,
+                                        const void* out, const float* lse, void* dq, void* dk, void* dv, int64_t B,
+                                        int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window, int64_t sinks,
+                                        const int64_t* q_strides, const int64_t* k_strides,
+                                        const int64_t* v_strides, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+
+/* gqa_window_decode (bf16, D 128): gqa_window of the newest token of each
+ * request, q (B,QH,D) (strides of batch and head), against the caches
+ * (B,T,KH,D, strided) of which lengths[b] tokens are valid, the newest among
+ * them; out (B,QH,D) contiguous.  lengths[b] <= 0: zeros; a length past T is
+ * cut to T and sets bit 8 of the device error word.  No workspace. */
+kda_status kda_gqa_window_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const int* lengths,
+                                      void* out, int64_t B, int64_t T, int64_t QH, int64_t KH, int64_t D,
+                                      int64_t window, int64_t sinks, const int64_t* q_strides,
+                                      const int64_t* k_strides, const int64_t* v_strides, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

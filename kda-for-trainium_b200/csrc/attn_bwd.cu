@@ -80,10 +80,12 @@ struct BwdParams {
   int B, S, QH, KH, rep;
   int nkb;          // key (and query) blocks per sequence
   int causal;
+  int window, sinks;  // sliding window (kWindow): keys [0, sinks) and the `window` keys up to the query
+  int row_stride;     // rows per (b, h) of lse and di: S, or (kWindow) S rounded up to whole blocks
   float sl2;        // softmax scale * log2(e)
   float scale;      // softmax scale (applied to dK here, to dQ by the conversion)
-  const float* lse;  // [B][QH][S]
-  const float* di;   // [B][QH][S]
+  const float* lse;  // [B][QH][row_stride]
+  const float* di;   // [B][QH][row_stride]
   float* dq;         // fp32 [B][QH][S][128] (the transposed dQ), zeroed before the launch, unscaled
   __nv_bfloat16* dk;  // [B][S][KH][128]
   __nv_bfloat16* dv;
@@ -103,10 +105,13 @@ struct Smem {
 };
 
 // Query blocks a key block visits (per head of its group): causal keeps the
-// blocks at or after it (128-row blocks on both sides).
+// blocks at or after it (128-row blocks on both sides), a window those up to
+// the last query that sees the block's last key, unless the block holds sinks.
+template <bool kWindow>
 __device__ __forceinline__ void q_range(const BwdParams& p, int j, int& q0, int& nq) {
-  q0 = p.causal ? j : 0;
+  q0 = kWindow || p.causal ? j : 0;
   nq = p.nkb - q0;
+  if (kWindow && j * kBlk >= p.sinks) nq = min(nq, (kBlk - 1 + p.window - 1) / kBlk + 1);
 }
 
 // Query block of step `it` (head it / nq of the group): each key block starts
@@ -136,6 +141,7 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   return v;
 }
 
+template <bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -166,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int j = static_cast<int>(blockIdx.x) / (p.B * p.KH);
   const int b = bg / p.KH, g = bg - (bg / p.KH) * p.KH;
   int q0, nq;
-  q_range(p, j, q0, nq);
+  q_range<kWindow>(p, j, q0, nq);
   const int n_iter = p.rep * nq;
 
   if (threadIdx.x == 0) {
@@ -223,8 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int h = g * p.rep + it / nq;
         const int s0 = q_block(j, q0, nq, it) * kBlk;
         const int qb = it & 1;
-        const int64_t drow = (static_cast<int64_t>(b) * p.QH + h) * p.S + s0;  // dout / lse / di row
-        const int valid = p.S - s0 < kBlk ? p.S - s0 : kBlk;  // query rows of the block inside S
+        const int64_t drow = (static_cast<int64_t>(b) * p.QH + h) * p.row_stride + s0;  // lse / di (dout) row
+        const int valid = !kWindow && p.S - s0 < kBlk ? p.S - s0 : kBlk;  // query rows of the block that lse, di have
         const uint32_t vbytes = static_cast<uint32_t>(valid) * 4u;
         // Q_i into buffer i % 2 once dK of block i - 2 is done
         if (it >= 2) ok = mbar_wait(&q_free[qb], static_cast<uint32_t>((it >> 1) - 1) & 1u, err, kErrWaitEmpty);
@@ -243,7 +249,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         mbar_arrive_expect_tx(do_full, kTile);
         for (int hh = 0; hh < 2; ++hh)
-          tma_load_2d(smem + Smem::kDO + hh * kHalf, &tmDO, do_full, hh * 64, static_cast<int>(drow));
+          if (kWindow)
+            tma_load_4d(smem + Smem::kDO + hh * kHalf, &tmDO, do_full, hh * 64, h, s0, b);
+          else
+            tma_load_2d(smem + Smem::kDO + hh * kHalf, &tmDO, do_full, hh * 64, static_cast<int>(drow));
         // di_i once the row warps are done with dS(i - 1)
         if (it >= 1) ok = mbar_wait(ds_ready, pprev, err, kErrWaitEmpty);
         if (!ok) break;
@@ -402,9 +411,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t prow = smem_u32(smem + Smem::kP) + static_cast<uint32_t>(kr * 128);
     const uint32_t dsrow = smem_u32(smem + Smem::kDS) + static_cast<uint32_t>(kr * 128);
     const uint32_t rsw = static_cast<uint32_t>(kr & 7);
-    // live queries of this key row: [qlo, S) -- from the key itself when causal,
-    // none when the key is past S
-    const int qlo = kpos >= p.S ? p.S : (p.causal ? kpos : 0);
+    // live queries of this key row: [qlo, qhi) -- from the key itself when causal,
+    // up to S or (a window, not a sink) the last query that sees it; none when
+    // the key is past S
+    const int qlo = kpos >= p.S ? p.S : (kWindow || p.causal ? kpos : 0);
+    const int qhi = kWindow && kpos >= p.sinks ? min(p.S, kpos + p.window) : p.S;
     bool ok = true;
     for (int it = 0; it < n_iter && ok; ++it) {
       const uint32_t par = static_cast<uint32_t>(it) & 1u;
@@ -421,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // [8u, 8u + 8) of a 64-query half = unit u).
       auto p_chunk = [&](const int k, const int odd, const uint32_t (&sv)[32]) {
         const int c = 2 * k + odd;
-        const uint32_t live = range_mask(qlo - s0 - c * 32, p.S - s0 - c * 32);
+        const uint32_t live = range_mask(qlo - s0 - c * 32, qhi - s0 - c * 32);
         float e[32];
 #pragma unroll
         for (int i4 = 0; i4 < 8; ++i4) {
@@ -464,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // masked entry (P = 0) stays 0 whatever di holds past S
       auto ds_chunk = [&](const int k, const int odd, const uint32_t (&dv)[32]) {
         const int c = 2 * k + odd;
-        const uint32_t live = range_mask(qlo - s0 - c * 32, p.S - s0 - c * 32);
+        const uint32_t live = range_mask(qlo - s0 - c * 32, qhi - s0 - c * 32);
         float w[32];
 #pragma unroll
         for (int u4 = 0; u4 < 4; ++u4) {
@@ -615,6 +626,37 @@ kda_status tmap_bshd(CUtensorMap* m, const void* base, int64_t B, int64_t S, int
   return make_tmap_bf16(m, base, 4, dims, strides, box);
 }
 
+// Opt-ins of one instantiation (once per device), the zeroed fp32 dq, the
+// kernel, and dq's conversion.
+template <bool kWindow>
+kda_status launch_bwd(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CUtensorMap& tdo,
+                      const BwdParams& p, __nv_bfloat16* dq, cudaStream_t st) {
+  if (cudaMemsetAsync(p.dq, 0, attn_backward_scratch_bytes(p.B, p.S, p.QH), st) != cudaSuccess)
+    return launch_status("attn_backward: memset");
+  static std::atomic<bool> attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, attn_bwd_kernel<kWindow>) != cudaSuccess) return launch_status("attn_backward: attributes");
+    if (fa.numRegs < kRegsNeeded) {
+      set_error("attn_backward: kernel compiled to %d registers/thread, its register split needs %d", fa.numRegs,
+                kRegsNeeded);
+      return KDA_UNSUPPORTED;
+    }
+    if (cudaFuncSetAttribute(attn_bwd_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Smem::kBytes)) != cudaSuccess)
+      return launch_status("attn_backward: cudaFuncSetAttribute");
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  const unsigned grid = static_cast<unsigned>(p.B * p.KH * p.nkb);
+  attn_bwd_kernel<kWindow><<<grid, kThreads, Smem::kBytes, st>>>(tk, tv, tq, tdo, p, kda_err_ptr_attn_bwd());
+  KDA_BWD_TRY(launch_status("attn_bwd_kernel"));
+  const int64_t n8 = static_cast<int64_t>(p.B) * p.S * p.QH * kD / 8;
+  dq_to_bf16_kernel<<<static_cast<unsigned>((n8 + 255) / 256), 256, 0, st>>>(p.dq, dq, n8, p.S, p.QH, p.scale);
+  return launch_status("attn_backward: dq to bf16");
+}
+
 }  // namespace
 
 size_t attn_backward_scratch_bytes(int64_t B, int64_t S, int64_t QH) {
@@ -639,8 +681,6 @@ kda_status attn_backward_flash(const __nv_bfloat16* q, const __nv_bfloat16* k, c
     const uint32_t box[2] = {64, static_cast<uint32_t>(kBlk)};
     KDA_BWD_TRY(make_tmap_bf16(&tdo, dout, 2, dims, strides, box));
   }
-  if (cudaMemsetAsync(dq32, 0, attn_backward_scratch_bytes(B, S, QH), st) != cudaSuccess)
-    return launch_status("attn_backward: memset");
   BwdParams p{};
   p.B = static_cast<int>(B);
   p.S = static_cast<int>(S);
@@ -649,6 +689,7 @@ kda_status attn_backward_flash(const __nv_bfloat16* q, const __nv_bfloat16* k, c
   p.rep = static_cast<int>(QH / KH);
   p.nkb = static_cast<int>((S + kBlk - 1) / kBlk);
   p.causal = causal ? 1 : 0;
+  p.row_stride = p.S;
   p.scale = 1.0f / sqrtf(static_cast<float>(kD));
   p.sl2 = p.scale * 1.4426950408889634f;
   p.lse = lse;
@@ -656,28 +697,110 @@ kda_status attn_backward_flash(const __nv_bfloat16* q, const __nv_bfloat16* k, c
   p.dq = dq32;
   p.dk = dk;
   p.dv = dv;
-  static std::atomic<bool> attr_set[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, attn_bwd_kernel) != cudaSuccess) return launch_status("attn_backward: attributes");
-    if (fa.numRegs < kRegsNeeded) {
-      set_error("attn_backward: kernel compiled to %d registers/thread, its register split needs %d", fa.numRegs,
-                kRegsNeeded);
-      return KDA_UNSUPPORTED;
-    }
-    if (cudaFuncSetAttribute(attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(Smem::kBytes)) != cudaSuccess)
-      return launch_status("attn_backward: cudaFuncSetAttribute");
-    attr_set[dev].store(true, std::memory_order_release);
-  }
-  const unsigned grid = static_cast<unsigned>(B * KH * p.nkb);
-  attn_bwd_kernel<<<grid, kThreads, Smem::kBytes, st>>>(tk, tv, tq, tdo, p, kda_err_ptr_attn_bwd());
-  KDA_BWD_TRY(launch_status("attn_bwd_kernel"));
-  const int64_t n8 = B * S * QH * kD / 8;
-  dq_to_bf16_kernel<<<static_cast<unsigned>((n8 + 255) / 256), 256, 0, st>>>(dq32, dq, n8, p.S, p.QH, p.scale);
-  return launch_status("attn_backward: dq to bf16");
+  return launch_bwd<false>(tk, tv, tq, tdo, p, dq, st);
 }
 
 }  // namespace kda
+
+using namespace kda;
+
+// ------------------------------------------------- sliding window with sinks
+namespace kda {
+namespace {
+// di[b][h][s] = sum_d dout * out (fp32) and a copy of lse, both with rows
+// padded to whole query blocks (zeros) so that every block's 512 bytes load
+// aligned.  dout, out [B][S][QH][128]; 16 lanes per row, 8 values each.
+__global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* __restrict__ dout,
+                                                          const __nv_bfloat16* __restrict__ out,
+                                                          const float* __restrict__ lse, float* __restrict__ di,
+                                                          float* __restrict__ lse_pad, int S, int SP, int QH) {
+  const int lane = threadIdx.x & 15;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);  // (s, h) of batch entry blockIdx.y
+  const int b = blockIdx.y;
+  const int h = static_cast<int>(i % QH);
+  const int s = static_cast<int>(i / QH);
+  const bool in = s < S;
+  float acc = 0.f;
+  if (in) {
+    const int64_t row = (static_cast<int64_t>(b) * S + s) * QH + h;
+    float fa[8], fb[8];
+    unpack_bf16x8(reinterpret_cast<const uint4*>(dout + row * kD)[lane], fa);
+    unpack_bf16x8(reinterpret_cast<const uint4*>(out + row * kD)[lane], fb);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fb[e], acc);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0 && s < SP) {
+    const int64_t bh = static_cast<int64_t>(b) * QH + h;
+    di[bh * SP + s] = acc;
+    lse_pad[bh * SP + s] = in ? lse[bh * S + s] : 0.f;
+  }
+}
+
+size_t al256(size_t n) { return (n + 255) & ~size_t(255); }
+int64_t padded_rows(int64_t S) { return (S + kBlk - 1) / kBlk * kBlk; }
+}  // namespace
+}  // namespace kda
+
+extern "C" size_t kda_gqa_window_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
+                                                         int64_t window, int64_t sinks) {
+  if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || D != kD || window <= 0 || sinks < 0) return 0;
+  return 2 * al256(static_cast<size_t>(B) * QH * padded_rows(S) * 4) + attn_backward_scratch_bytes(B, S, QH);
+}
+
+extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void* q, const void* k, const void* v,
+                                                   const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                                   int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
+                                                   int64_t window, int64_t sinks, const int64_t* q_strides,
+                                                   const int64_t* k_strides, const int64_t* v_strides,
+                                                   void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "gqa_window_backward";
+  KDA_BWD_TRY(gqa_window_check(op, B, S, QH, KH, D, window, sinks));
+  KDA_CHECK_ARG(dout && q && k && v && out && lse && dq && dk && dv && q_strides && k_strides && v_strides,
+                "%s: null pointer", op);
+  const int64_t dense_q[3] = {S * QH * kD, QH * kD, kD}, dense_k[3] = {S * KH * kD, KH * kD, kD};
+  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
+                          head_rows_ok(dout, dense_q) && head_rows_ok(out, dense_q) && head_rows_ok(dq, dense_q) &&
+                          head_rows_ok(dk, dense_k) && head_rows_ok(dv, dense_k),
+                      "%s: pointers and rows must be 16-byte aligned", op);
+  const size_t need = kda_gqa_window_backward_workspace_size(B, S, QH, KH, D, window, sinks);
+  KDA_CHECK_ARG(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes required, got %zu", op, need,
+                workspace_bytes);
+  KDA_CHECK_SUPPORTED((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "%s: workspace must be 16-byte aligned",
+                      op);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t SP = padded_rows(S);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  const size_t rows = al256(static_cast<size_t>(B) * QH * SP * 4);
+  BwdParams p{};
+  float* di = reinterpret_cast<float*>(w);
+  float* lse_pad = reinterpret_cast<float*>(w + rows);
+  p.dq = reinterpret_cast<float*>(w + 2 * rows);
+  window_rows_kernel<<<dim3(static_cast<unsigned>((SP * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
+      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, di, lse_pad,
+      static_cast<int>(S), static_cast<int>(SP), static_cast<int>(QH));
+  KDA_BWD_TRY(launch_status("gqa_window_backward: rows"));
+  CUtensorMap tk, tv, tq, tdo;
+  KDA_BWD_TRY(tmap_head_rows(&tk, k, B, S, KH, k_strides[0], k_strides[1], k_strides[2]));
+  KDA_BWD_TRY(tmap_head_rows(&tv, v, B, S, KH, v_strides[0], v_strides[1], v_strides[2]));
+  KDA_BWD_TRY(tmap_head_rows(&tq, q, B, S, QH, q_strides[0], q_strides[1], q_strides[2]));
+  KDA_BWD_TRY(tmap_head_rows(&tdo, dout, B, S, QH, dense_q[0], dense_q[1], dense_q[2]));
+  p.B = static_cast<int>(B);
+  p.S = static_cast<int>(S);
+  p.QH = static_cast<int>(QH);
+  p.KH = static_cast<int>(KH);
+  p.rep = static_cast<int>(QH / KH);
+  p.nkb = static_cast<int>(SP / kBlk);
+  p.causal = 1;
+  p.window = static_cast<int>(window < S ? window : S);
+  p.sinks = static_cast<int>(sinks < S ? sinks : S);
+  p.row_stride = static_cast<int>(SP);
+  p.scale = 1.0f / sqrtf(static_cast<float>(kD));
+  p.sl2 = p.scale * 1.4426950408889634f;
+  p.lse = lse_pad;
+  p.di = di;
+  p.dk = static_cast<__nv_bfloat16*>(dk);
+  p.dv = static_cast<__nv_bfloat16*>(dv);
+  return launch_bwd<true>(tk, tv, tq, tdo, p, static_cast<__nv_bfloat16*>(dq), st);
+}

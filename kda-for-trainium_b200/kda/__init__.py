@@ -14,9 +14,10 @@ provides the numpy-in / numpy-out shim ``kda.compat.<op>``.
 from ._lib import KdaError, lib as _load_lib
 from .ops import (  # noqa: F401
     adamw, adamw_multi, add_rmsnorm_matmul, bmm, bmm_softmax, device_error, gqa_full, gqa_full_backward,
-    gqa_full_lse, lora,
-    mamba, matmul, matmul_add_rmsnorm, rmsnorm_matmul, rmsnorm_matmul_backward, rope_single_freq_apply, silu, swiglu,
-    swiglu_backward, swiglu_gu, transpose_matmul,
+    gqa_full_lse, gqa_window, gqa_window_backward, gqa_window_decode, gqa_window_lse, lora,
+    mamba, matmul, matmul_add_rmsnorm, qk_norm_rope, qk_norm_rope_append, qk_norm_rope_backward, rmsnorm_matmul,
+    rmsnorm_matmul_backward, rope_single_freq_apply, rope_table, silu, swiglu, swiglu_backward, swiglu_gu,
+    transpose_matmul,
 )
 
 OPS = ("silu", "rmsnorm_matmul", "add_rmsnorm_matmul", "matmul_add_rmsnorm", "swiglu", "matmul",
@@ -28,4 +29,6 @@ _load_lib()
 from . import compat, library  # noqa: E402,F401  (torch.ops.kda.<op> and the numpy shim)
 
 __all__ = list(OPS) + ["adamw_multi", "rmsnorm_matmul_backward", "swiglu_backward", "gqa_full_backward",
-                       "gqa_full_lse", "swiglu_gu", "KdaError", "device_error"]
+                       "gqa_full_lse", "swiglu_gu", "rope_table", "qk_norm_rope", "qk_norm_rope_backward",
+                       "qk_norm_rope_append", "gqa_window", "gqa_window_lse", "gqa_window_backward",
+                       "gqa_window_decode", "KdaError", "device_error"]

@@ -94,6 +94,19 @@ PROTOTYPES = {
     "kda_zero1_adamw_f32": (INT, [P, P, INT, INT, I64, I64, P, P, D, D, D, D, D, I64, P]),
     "kda_gqa_full_f32_workspace_size": (SZ, [I64, I64, I64, I64, I64]),
     "kda_gqa_full_f32": (INT, [P, P, P, P, I64, I64, I64, I64, I64, INT, F, INT, P, SZ, P]),
+    "kda_rope_table_f32": (INT, [P, I64, I64, F, P]),
+    "kda_qk_norm_rope": (INT, [P, P, P, P, P, I64, P, F, P, P, I64, I64, I64, I64, I64, P, P, INT, P]),
+    "kda_qk_norm_rope_append_bf16": (INT, [P, P, P, P, P, P, I64, P, F, P, P, P, I64, I64, I64, I64, I64, I64, P, P,
+                                           P, P, P, P]),
+    "kda_qk_norm_rope_backward_workspace_size": (SZ, [I64, I64, I64, I64, I64, INT]),
+    "kda_qk_norm_rope_backward": (INT, [P, P, P, P, P, P, P, I64, P, F, P, P, P, P, I64, I64, I64, I64, I64, P, P,
+                                        INT, P, SZ, P]),
+    "kda_gqa_window_workspace_size": (SZ, [I64, I64, I64, I64, I64]),
+    "kda_gqa_window_bf16": (INT, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P, SZ, P]),
+    "kda_gqa_window_backward_workspace_size": (SZ, [I64, I64, I64, I64, I64, I64, I64]),
+    "kda_gqa_window_backward_bf16": (INT, [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P,
+                                           SZ, P]),
+    "kda_gqa_window_decode_bf16": (INT, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P]),
 }
 
 

@@ -5,6 +5,8 @@ differentiable op for training code.
     y.backward(dy)                                   # x.grad, w.grad, g.grad from the kernels
     y = kda.autograd.swiglu(x, w_up, w_down, w_gate)  # bf16; all four gradients from the kernels
     o = kda.autograd.gqa_full(q, k, v, causal=True, rope_theta=1e4)  # bf16; dq, dk, dv from the kernels
+    q, k = kda.autograd.qk_norm_rope(q, k, gq, gk, table)            # dq, dk, dgq, dgk from the kernels
+    o = kda.autograd.gqa_window(q, k, v, 1024, sinks=4)              # bf16; dq, dk, dv from the kernels
 """
 
 from __future__ import annotations
@@ -78,3 +80,45 @@ def gqa_full(q, k, v, causal=False, rope_theta=None):
     (B, QH, S, D)): the forward keeps its row log2-sum-exp, the gradients come
     from ``kda.gqa_full_backward`` on the saved forward."""
     return _GQA.apply(q, k, v, causal, rope_theta)
+
+
+class _QKNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, gq, gk, table, positions, eps):
+        ctx.save_for_backward(q, k, gq, gk, table, positions)
+        ctx.eps = float(eps)
+        return ops.qk_norm_rope(q, k, gq, gk, table, positions=positions, eps=eps)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        q, k, gq, gk, table, positions = ctx.saved_tensors
+        grads = ops.qk_norm_rope_backward(dq.to(q.dtype).contiguous(), dk.to(q.dtype).contiguous(), q, k, gq, gk,
+                                          table, positions=positions, eps=ctx.eps)
+        return (*grads, None, None, None)
+
+
+def qk_norm_rope(q, k, gq, gk, table, *, positions=None, eps=1e-6):
+    """Differentiable ``kda.qk_norm_rope``: gradients for q, k, gq and gk come
+    from ``kda.qk_norm_rope_backward``."""
+    return _QKNormRope.apply(q, k, gq, gk, table, positions, eps)
+
+
+class _GQAWindow(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks):
+        out, lse = ops.gqa_window_lse(q, k, v, window, sinks)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.window, ctx.sinks = int(window), int(sinks)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        grads = ops.gqa_window_backward(dout.to(torch.bfloat16).contiguous(), q, k, v, out, lse, ctx.window, ctx.sinks)
+        return (*grads, None, None)
+
+
+def gqa_window(q, k, v, window, sinks=0):
+    """Differentiable ``kda.gqa_window`` (bf16): the forward keeps its row
+    log2-sum-exp, the gradients come from ``kda.gqa_window_backward``."""
+    return _GQAWindow.apply(q, k, v, window, sinks)

@@ -1,4 +1,5 @@
-"""The fourteen operators as ``torch.library`` custom ops: ``torch.ops.kda.<op>``.
+"""The fourteen operators as ``torch.library`` custom ops: ``torch.ops.kda.<op>``,
+and the forwards of the local-attention operators beside them.
 
 Each op calls the same ``kda.ops`` function (and so the same libkda.so entry
 point, with the same host checks raising ``ValueError`` before any launch) and
@@ -179,6 +180,51 @@ def _(q, k, v, causal=False, rope_theta=None, out_layout="bhsd"):
     B, S, QH, D = q.shape
     shape = (B, QH, S, D) if out_layout == "bhsd" else (B, S, QH, D)
     return q.new_empty(shape, dtype=_contraction_dtype(q))
+
+
+# ------------------------------------------------------------- local attention
+@torch.library.custom_op("kda::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, gq: torch.Tensor, gk: torch.Tensor, table: torch.Tensor,
+                 positions: Optional[torch.Tensor] = None, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.qk_norm_rope(q, k, gq, gk, table, positions=positions, eps=eps)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, gq, gk, table, positions=None, eps=1e-6):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("kda::qk_norm_rope_append", mutates_args=("k_cache", "v_cache"))
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gq: torch.Tensor, gk: torch.Tensor,
+                        table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                        eps: float = 1e-6) -> torch.Tensor:
+    return ops.qk_norm_rope_append(q, k, v, gq, gk, table, k_cache, v_cache, lengths, eps=eps)
+
+
+@qk_norm_rope_append.register_fake
+def _(q, k, v, gq, gk, table, k_cache, v_cache, lengths, eps=1e-6):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("kda::gqa_window", mutates_args=())
+def gqa_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0) -> torch.Tensor:
+    return ops.gqa_window(q, k, v, window, sinks)
+
+
+@gqa_window.register_fake
+def _(q, k, v, window, sinks=0):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("kda::gqa_window_decode", mutates_args=())
+def gqa_window_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                      window: int, sinks: int = 0) -> torch.Tensor:
+    return ops.gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks)
+
+
+@gqa_window_decode.register_fake
+def _(q, k_cache, v_cache, lengths, window, sinks=0):
+    return q.new_empty(q.shape)
 
 
 OPS = ("silu", "rmsnorm_matmul", "add_rmsnorm_matmul", "matmul_add_rmsnorm", "swiglu", "matmul",

@@ -376,3 +376,111 @@ def gqa_full(q, k, v, causal=False, rope_theta=None, out_layout="bhsd", heads=No
     if out_layout == "bshd":
         return np.ascontiguousarray(out.transpose(0, 2, 1, 3))
     return out
+
+
+# --------------------------------------------------------------------------- #
+# local attention (no reference forward: the neighbours of gqa_full), float64
+# --------------------------------------------------------------------------- #
+def rope_table(length, head_dim, theta=10000.0):
+    """cos, sin of position * theta^(-2 i / head_dim): (length, head_dim / 2, 2), float64."""
+    ang = np.arange(length)[:, None] * theta ** (-2.0 * np.arange(head_dim // 2) / head_dim)
+    return np.stack([np.cos(ang), np.sin(ang)], axis=-1)
+
+
+def _norm_rope(x, g, cs, eps):
+    n = x / np.sqrt(np.mean(x * x, axis=-1, keepdims=True) + eps) * g
+    a, b = np.split(n, 2, axis=-1)
+    c, s = cs[..., None, :, 0], cs[..., None, :, 1]
+    return np.concatenate([a * c - b * s, a * s + b * c], axis=-1)
+
+
+def qk_norm_rope(q, k, gq, gk, table, positions=None, eps=1e-6):
+    """Head rows of q (B,S,QH,D) and k (B,S,KH,D): x / sqrt(mean x^2 + eps) * g,
+    then the half-split rotation by table[position]."""
+    q, k, gq, gk, table = (np.asarray(t, dtype=np.float64) for t in (q, k, gq, gk, table))
+    cs = table[: q.shape[1]][None] if positions is None else table[np.asarray(positions)]
+    return _norm_rope(q, gq, cs, eps), _norm_rope(k, gk, cs, eps)
+
+
+def qk_norm_rope_backward(dq, dk, q, k, gq, gk, table, positions=None, eps=1e-6):
+    """(dq, dk, dgq, dgk): with dn = the rotation's transpose of dy, t = g dn and
+    r = 1 / sqrt(mean x^2 + eps): dx = r t - x r^3 mean(x t); dg = sum x r dn."""
+    table = np.asarray(table, dtype=np.float64)
+    cs = table[: q.shape[1]][None] if positions is None else table[np.asarray(positions)]
+    c, s = cs[..., None, :, 0], cs[..., None, :, 1]
+    dx, dg = [], []
+    for dy, x, g in ((dq, q, gq), (dk, k, gk)):
+        dy, x, g = (np.asarray(t, dtype=np.float64) for t in (dy, x, g))
+        a, b = np.split(dy, 2, axis=-1)
+        dn = np.concatenate([a * c + b * s, b * c - a * s], axis=-1)
+        r = 1.0 / np.sqrt(np.mean(x * x, axis=-1, keepdims=True) + eps)
+        t = g * dn
+        dx.append(r * t - x * r ** 3 * np.mean(x * t, axis=-1, keepdims=True))
+        dg.append(np.sum(x * r * dn, axis=(0, 1, 2)))
+    return dx[0], dx[1], dg[0], dg[1]
+
+
+def window_mask(S, window, sinks):
+    """(S, S): query i sees key j <= i where i - j < window or j < sinks."""
+    i, j = np.arange(S)[:, None], np.arange(S)[None, :]
+    return (j <= i) & ((i - j < window) | (j < sinks))
+
+
+def _window_probs(q, k, window, sinks):
+    S, D = q.shape
+    s = np.where(window_mask(S, window, sinks), q @ k.T / np.sqrt(D), -np.inf)
+    m = s.max(-1, keepdims=True)
+    p = np.exp(s - m)
+    z = p.sum(-1, keepdims=True)
+    return p / z, (m + np.log(z))[:, 0] / np.log(2.0)
+
+
+def gqa_window(q, k, v, window, sinks=0):
+    """(out (B,S,QH,D), lse (B,QH,S) in log2) of the windowed attention."""
+    q, k, v = (np.asarray(t, dtype=np.float64) for t in (q, k, v))
+    B, S, QH, D = q.shape
+    rep = QH // k.shape[2]
+    out, lse = np.zeros_like(q), np.zeros((B, QH, S))
+    for b in range(B):
+        for h in range(QH):
+            p, lse[b, h] = _window_probs(q[b, :, h], k[b, :, h // rep], window, sinks)
+            out[b, :, h] = p @ v[b, :, h // rep]
+    return out, lse
+
+
+def gqa_window_backward(dout, q, k, v, window, sinks=0):
+    """(dq, dk, dv) of ``gqa_window``: dS = P (dP - rowsum(P dP)), dP = dout v^T."""
+    dout, q, k, v = (np.asarray(t, dtype=np.float64) for t in (dout, q, k, v))
+    B, S, QH, D = q.shape
+    rep = QH // k.shape[2]
+    dq, dk, dv = np.zeros_like(q), np.zeros_like(k), np.zeros_like(v)
+    for b in range(B):
+        for h in range(QH):
+            g = h // rep
+            p, _ = _window_probs(q[b, :, h], k[b, :, g], window, sinks)
+            dp = dout[b, :, h] @ v[b, :, g].T
+            ds = p * (dp - np.sum(p * dp, -1, keepdims=True)) / np.sqrt(D)
+            dq[b, :, h] = ds @ k[b, :, g]
+            dk[b, :, g] += ds.T @ q[b, :, h]
+            dv[b, :, g] += p.T @ dout[b, :, h]
+    return dq, dk, dv
+
+
+def gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks=0):
+    """The newest token's row of ``gqa_window`` for each request: q (B,QH,D), the
+    first lengths[b] rows of the caches (B,T,KH,D); zeros where there are none."""
+    q, k, v = (np.asarray(t, dtype=np.float64) for t in (q, k_cache, v_cache))
+    B, QH, D = q.shape
+    rep = QH // k.shape[2]
+    out = np.zeros_like(q)
+    for b in range(B):
+        n = int(lengths[b])
+        if n <= 0:
+            continue
+        j = np.arange(n)
+        j = j[(j >= n - window) | (j < sinks)]
+        for h in range(QH):
+            s = k[b, j, h // rep] @ q[b, h] / np.sqrt(D)
+            p = np.exp(s - s.max())
+            out[b, h] = (p / p.sum()) @ v[b, j, h // rep]
+    return out
