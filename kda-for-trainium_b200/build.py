@@ -4,7 +4,8 @@
 
 Each ``csrc/*.cu`` is compiled separately (in parallel, skipped when up to
 date) into ``_build/`` and linked with the static CUDA runtime into
-``kda/libkda.so``.  The library does not link libcuda: the driver entry point
+``kda/libkda.so``; ``csrc/binding.cpp`` (the local-attention operators' native
+Python binding, against the installed torch) becomes ``kda/_binding.so``.  The library does not link libcuda: the driver entry point
 it needs (``cuTensorMapEncodeTiled``) is resolved at run time, so the library
 loads -- and its symbols can be inspected -- on a machine without a GPU.
 """
@@ -25,6 +26,7 @@ CSRC = PKG / "csrc"
 INCLUDE = REPO / "include"
 BUILD = REPO / "_build"
 LIB = PKG / "kda" / "libkda.so"
+BINDING = PKG / "kda" / "_binding.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -60,6 +62,34 @@ def _compile(src: Path, force: bool, verbose: bool, extra) -> Path:
     return obj
 
 
+def _build_binding(force: bool, verbose: bool) -> Path:
+    """kda/_binding.so: host code only, resolved against the libkda.so beside it."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    src = CSRC / "binding.cpp"
+    stamp = BUILD / "binding.torch"  # the torch it was compiled against
+    newest = max(src.stat().st_mtime, (INCLUDE / "kda.h").stat().st_mtime)
+    if (not force and BINDING.exists() and BINDING.stat().st_mtime >= newest and stamp.exists()
+            and stamp.read_text() == torch.__version__):
+        return BINDING
+    cuda_inc = Path(nvcc()).resolve().parent.parent / "include"
+    inc = [*include_paths(), str(cuda_inc), sysconfig.get_paths()["include"], str(INCLUDE)]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(src), "-o", str(BINDING),
+           *(f"-I{p}" for p in inc), *(f"-L{p}" for p in library_paths()), "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           "-lc10", "-lc10_cuda", f"-L{LIB.parent}", "-l:libkda.so", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(torch.__version__)
+    return BINDING
+
+
 def build(verbose: bool = False, force: bool = False, jobs: int = 0, extra=()) -> Path:
     BUILD.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
@@ -69,12 +99,13 @@ def build(verbose: bool = False, force: bool = False, jobs: int = 0, extra=()) -
     newest = max(o.stat().st_mtime for o in objs)
     if force or not LIB.exists() or LIB.stat().st_mtime < newest:
         cmd = [nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *map(str, objs),
-               "-Xlinker", "--no-undefined", "-lrt", "-ldl", "-lpthread"]
+               "-Xlinker", "-soname=libkda.so", "-Xlinker", "--no-undefined", "-lrt", "-ldl", "-lpthread"]
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _build_binding(force, verbose)
     return LIB
 
 

@@ -136,6 +136,18 @@ def lib():
     return _lib
 
 
+def binding():
+    """The native binding of the local-attention operators.  It resolves the C
+    ABI in the library that ``lib()`` has loaded (matched by its soname)."""
+    lib()
+    try:
+        from . import _binding
+    except ImportError as e:
+        raise ImportError(f"kda/_binding.so is missing or was built against another torch ({e}); build it with "
+                          f"`python kda-for-trainium_b200/build.py`") from e
+    return _binding
+
+
 _attached = set()
 
 

@@ -614,37 +614,9 @@ def gqa_full_backward(dout, q, k, v, causal=False, rope_theta=None, *, fwd_out=N
 
 
 # ------------------------------------------------------------ local attention
-def _rows(t, name, dtypes, shape, device=None):
-    """Check a tensor of head rows that may be a view (a slice of a packed
-    projection, a layer of a cache): the last axis contiguous, every row on a
-    16-byte boundary, no expanded axis.  Returns its other strides (elements)
-    as a C array; an axis of one entry counts as stride 0."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    if not isinstance(dtypes, tuple):
-        dtypes = (dtypes,)
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} must have dtype {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    got = tuple(t.shape)
-    if len(got) != len(shape) or any(w is not None and w != n for w, n in zip(shape, got)):
-        raise ValueError(f"{name} must have shape ({', '.join('*' if w is None else str(w) for w in shape)}), got {got}")
-    if 0 in got:
-        raise ValueError(f"{name} must not be empty, got shape {got}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    es = t.element_size()
-    st = t.stride()
-    bad = st[-1] != 1 or t.data_ptr() % 16
-    out = []
-    for n, x in zip(got[:-1], st[:-1]):
-        bad = bad or (n > 1 and (x <= 0 or x * es % 16))
-        out.append(x if n > 1 else 0)
-    if bad:
-        raise ValueError(f"{name} must have a contiguous last axis, rows on 16-byte boundaries and no expanded axis, "
-                         f"got strides {st}")
-    return (C.c_int64 * len(out))(*out)
+# One native call each (csrc/binding.cpp): argument checks, outputs, workspace,
+# current stream and the C entry point.
+_native = _lib.binding()
 
 
 def rope_table(length, head_dim, theta=10000.0, *, device="cuda"):
@@ -662,23 +634,6 @@ def rope_table(length, head_dim, theta=10000.0, *, device="cuda"):
     return tab
 
 
-def _norm_rope_args(q, k, gq, gk, table, positions, dtypes=(_bf16, _f32)):
-    qs = _rows(q, "q", dtypes, (None, None, None, None))
-    B, S, QH, D = q.shape
-    if D not in (64, 128, 256):
-        raise ValueError(f"head_dim must be 64, 128 or 256, got {D}")
-    dev = q.device
-    ks = _rows(k, "k", q.dtype, (B, S, None, D), dev)
-    _check(gq, "gq", _f32, shape=(D,), device=dev)
-    _check(gk, "gk", _f32, shape=(D,), device=dev)
-    _check(table, "table", _f32, ndim=3, device=dev)
-    if table.shape[0] < 1 or table.shape[1] != D // 2 or table.shape[2] != 2:
-        raise ValueError(f"table must be (positions, {D // 2}, 2), got {tuple(table.shape)}")
-    if positions is not None:
-        _check(positions, "positions", torch.int32, shape=(B, S), device=dev)
-    return qs, ks, B, S, QH, k.shape[2], D
-
-
 def qk_norm_rope(q, k, gq, gk, table, *, positions=None, eps=1e-6, q_out=None, k_out=None):
     """Per-head RMS norm of queries and keys and the half-split rotation, in one
     pass: y = rotate(x / sqrt(mean_d x^2 + eps) * g), q (B,S,QH,D), k (B,S,KH,D)
@@ -686,13 +641,7 @@ def qk_norm_rope(q, k, gq, gk, table, *, positions=None, eps=1e-6, q_out=None, k
     128 or 256.  ``table`` is ``rope_table``'s; ``positions`` int32 (B,S) picks
     its rows (default 0 .. S-1).  A position outside the table gives NaN and
     sets ``device_error``.  Returns (q', k'), contiguous, in q's dtype."""
-    qs, ks, B, S, QH, KH, D = _norm_rope_args(q, k, gq, gk, table, positions)
-    qo = _out(q_out, (B, S, QH, D), q.dtype, q.device, "q_out")
-    ko = _out(k_out, (B, S, KH, D), q.dtype, q.device, "k_out")
-    with _on(q):
-        _lib.call("kda_qk_norm_rope", _p(q), _p(k), _p(gq), _p(gk), _p(table), table.shape[0], _p(positions),
-                  float(eps), _p(qo), _p(ko), B, S, QH, KH, D, qs, ks, int(q.dtype == _f32), _stream(q))
-    return qo, ko
+    return _native.qk_norm_rope(q, k, gq, gk, table, positions, eps, q_out, k_out)
 
 
 def qk_norm_rope_backward(dq_out, dk_out, q, k, gq, gk, table, *, positions=None, eps=1e-6, workspace=None):
@@ -700,21 +649,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, gq, gk, table, *, positions=None
     outputs (contiguous, q's dtype): returns (dq, dk) shaped like q and k,
     contiguous, and (dgq, dgk) fp32, summed over tokens and heads in a fixed
     order."""
-    qs, ks, B, S, QH, KH, D = _norm_rope_args(q, k, gq, gk, table, positions)
-    dev = q.device
-    _check(dq_out, "dq_out", q.dtype, shape=(B, S, QH, D), device=dev)
-    _check(dk_out, "dk_out", q.dtype, shape=(B, S, KH, D), device=dev)
-    dq = torch.empty((B, S, QH, D), dtype=q.dtype, device=dev)
-    dk = torch.empty((B, S, KH, D), dtype=q.dtype, device=dev)
-    dgq, dgk = torch.empty_like(gq), torch.empty_like(gk)
-    f32 = int(q.dtype == _f32)
-    with _on(q):
-        nb = _ws_size("kda_qk_norm_rope_backward_workspace_size", B, S, QH, KH, D, f32)
-        ws = _workspace(workspace, nb, dev)
-        _lib.call("kda_qk_norm_rope_backward", _p(dq_out), _p(dk_out), _p(q), _p(k), _p(gq), _p(gk), _p(table),
-                  table.shape[0], _p(positions), float(eps), _p(dq), _p(dk), _p(dgq), _p(dgk), B, S, QH, KH, D, qs,
-                  ks, f32, _p(ws), nb, _stream(q))
-    return dq, dk, dgq, dgk
+    return _native.qk_norm_rope_backward(dq_out, dk_out, q, k, gq, gk, table, positions, eps, workspace)
 
 
 def qk_norm_rope_append(q, k, v, gq, gk, table, k_cache, v_cache, lengths, *, eps=1e-6, q_out=None):
@@ -725,42 +660,7 @@ def qk_norm_rope_append(q, k, v, gq, gk, table, k_cache, v_cache, lengths, *, ep
     marks an idle slot: its q' is zero and nothing is written.  A position
     outside the cache or the table gives NaN, writes nothing and sets
     ``device_error``.  ``lengths`` is left as it is."""
-    qs, ks, B, S, QH, KH, D = _norm_rope_args(q, k, gq, gk, table, None, (_bf16,))
-    dev = q.device
-    vs = _rows(v, "v", _bf16, (B, S, KH, D), dev)
-    kcs = _rows(k_cache, "k_cache", _bf16, (B, None, KH, D), dev)
-    T = k_cache.shape[1]
-    vcs = _rows(v_cache, "v_cache", _bf16, (B, T, KH, D), dev)
-    _check(lengths, "lengths", torch.int32, shape=(B,), device=dev)
-    qo = _out(q_out, (B, S, QH, D), _bf16, dev, "q_out")
-    with _on(q):
-        _lib.call("kda_qk_norm_rope_append_bf16", _p(q), _p(k), _p(v), _p(gq), _p(gk), _p(table), table.shape[0],
-                  _p(lengths), float(eps), _p(qo), _p(k_cache), _p(v_cache), T, B, S, QH, KH, D, qs, ks, vs, kcs,
-                  vcs, _stream(q))
-    return qo
-
-
-def _window_args(q, k, v):
-    qs = _rows(q, "q", _bf16, (None, None, None, 128))
-    B, S, QH, D = q.shape
-    ks = _rows(k, "k", _bf16, (B, S, None, D), q.device)
-    KH = k.shape[2]
-    vs = _rows(v, "v", _bf16, (B, S, KH, D), q.device)
-    if QH % KH:
-        raise ValueError(f"query heads {QH} must be a multiple of kv heads {KH}")
-    return qs, ks, vs, B, S, QH, KH, D
-
-
-def _gqa_window(q, k, v, window, sinks, out, lse, workspace):
-    qs, ks, vs, B, S, QH, KH, D = _window_args(q, k, v)
-    y = _out(out, (B, S, QH, D), _bf16, q.device)
-    rows = torch.empty((B, QH, S), dtype=_f32, device=q.device) if lse else None
-    nb = _ws_size("kda_gqa_window_workspace_size", B, S, QH, KH, D)
-    ws = _workspace(workspace, nb, q.device)
-    with _on(q):
-        _lib.call("kda_gqa_window_bf16", _p(q), _p(k), _p(v), _p(y), _p(rows), B, S, QH, KH, D, int(window),
-                  int(sinks), qs, ks, vs, _p(ws), nb, _stream(q))
-    return y, rows
+    return _native.qk_norm_rope_append(q, k, v, gq, gk, table, k_cache, v_cache, lengths, eps, q_out)
 
 
 def gqa_window(q, k, v, window, sinks=0, *, out=None, workspace=None):
@@ -768,34 +668,20 @@ def gqa_window(q, k, v, window, sinks=0, *, out=None, workspace=None):
     sees key j <= i where i - j < window or j < sinks.  q (B,S,QH,128), k, v
     (B,S,KH,128) bf16, views are fine; returns (B,S,QH,128).  No rotation (see
     ``qk_norm_rope``); scores scaled by 1 / sqrt(128)."""
-    return _gqa_window(q, k, v, window, sinks, out, False, workspace)[0]
+    return _native.gqa_window(q, k, v, window, sinks, out, False, workspace)[0]
 
 
 def gqa_window_lse(q, k, v, window, sinks=0, *, workspace=None):
     """``gqa_window`` that also returns each query row's log2-sum-exp of the
     scaled scores, (B, QH, S) fp32: the forward of a training step."""
-    return _gqa_window(q, k, v, window, sinks, None, True, workspace)
+    return _native.gqa_window(q, k, v, window, sinks, None, True, workspace)
 
 
 def gqa_window_backward(dout, q, k, v, out, lse, window, sinks=0, *, workspace=None):
     """Gradients of ``gqa_window(q, k, v, window, sinks)`` given dout
     (B,S,QH,128) bf16 and ``gqa_window_lse``'s two outputs: returns (dq, dk, dv)
     bf16, shaped like q, k, v, contiguous."""
-    qs, ks, vs, B, S, QH, KH, D = _window_args(q, k, v)
-    dev = q.device
-    _check(dout, "dout", _bf16, shape=(B, S, QH, D), device=dev)
-    _check(out, "out", _bf16, shape=(B, S, QH, D), device=dev)
-    _check(lse, "lse", _f32, shape=(B, QH, S), device=dev)
-    dq = torch.empty((B, S, QH, D), dtype=_bf16, device=dev)
-    dk = torch.empty((B, S, KH, D), dtype=_bf16, device=dev)
-    dv = torch.empty((B, S, KH, D), dtype=_bf16, device=dev)
-    window, sinks = int(window), int(sinks)
-    nb = _ws_size("kda_gqa_window_backward_workspace_size", B, S, QH, KH, D, window, sinks)
-    ws = _workspace(workspace, nb, dev)
-    with _on(q):
-        _lib.call("kda_gqa_window_backward_bf16", _p(dout), _p(q), _p(k), _p(v), _p(out), _p(lse), _p(dq), _p(dk),
-                  _p(dv), B, S, QH, KH, D, window, sinks, qs, ks, vs, _p(ws), nb, _stream(q))
-    return dq, dk, dv
+    return _native.gqa_window_backward(dout, q, k, v, out, lse, window, sinks, workspace)
 
 
 def gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks=0, *, out=None):
@@ -805,20 +691,7 @@ def gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks=0, *, out=None
     first ``sinks``.  A request without tokens (length 0 or less) gives zeros; a
     length past the cache is cut to it and sets ``device_error``.  Returns
     (B,QH,128)."""
-    qs = _rows(q, "q", _bf16, (None, None, 128))
-    B, QH, D = q.shape
-    dev = q.device
-    ks = _rows(k_cache, "k_cache", _bf16, (B, None, None, D), dev)
-    T, KH = k_cache.shape[1], k_cache.shape[2]
-    vs = _rows(v_cache, "v_cache", _bf16, (B, T, KH, D), dev)
-    if QH % KH:
-        raise ValueError(f"query heads {QH} must be a multiple of kv heads {KH}")
-    _check(lengths, "lengths", torch.int32, shape=(B,), device=dev)
-    y = _out(out, (B, QH, D), _bf16, dev)
-    with _on(q):
-        _lib.call("kda_gqa_window_decode_bf16", _p(q), _p(k_cache), _p(v_cache), _p(lengths), _p(y), B, T, QH, KH, D,
-                  int(window), int(sinks), qs, ks, vs, _stream(q))
-    return y
+    return _native.gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks, out)
 
 
 def device_error(clear: bool = True) -> int:
