@@ -14,6 +14,8 @@
 // rotation needs no exchange and the two loads and stores are 16 bytes wide;
 // the sums over the row are shuffles among those lanes.  All arithmetic is
 // fp32; bf16 rows are rounded once, when they are stored.
+#include <algorithm>
+
 #include "common.cuh"
 
 KDA_DEFINE_ERROR_WORD(qk_norm)
@@ -35,29 +37,33 @@ __device__ __forceinline__ void st_stream(void* p, uint4 v) {
   asm volatile("st.global.cs.v4.b32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// The 16 bytes of a lane as fp32 values and back.
+// The 16 bytes of a lane as pairs of fp32 values (for the packed f32x2
+// instructions, two values per issue slot) and back.
 template <typename T>
 struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int kN = 8;
-  static __device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) { unpack_bf16x8(v, f); }
-  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                      pack_bf16x2(f[6], f[7]));
+  static __device__ __forceinline__ void unpack(const uint4 v, float2 (&f)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
+    return make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y),
+                      pack_bf16x2(f[3].x, f[3].y));
   }
 };
 template <>
 struct Vec<float> {
   static constexpr int kN = 4;
-  static __device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
-    f[0] = __uint_as_float(v.x);
-    f[1] = __uint_as_float(v.y);
-    f[2] = __uint_as_float(v.z);
-    f[3] = __uint_as_float(v.w);
+  static __device__ __forceinline__ void unpack(const uint4 v, float2 (&f)[2]) {
+    f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+    f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
-  static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[2]) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x),
+                      __float_as_uint(f[1].y));
   }
 };
 
@@ -80,7 +86,8 @@ struct FwdParams {
   const int* lengths;        // append: [B], tokens already in the cache (negative: idle slot)
   int64_t table_len, cache_len;
   int B, S, QH, KH;
-  int cq, ck;                // head chunks of a token's queries, of its keys (append: and of its values)
+  int hp;                    // heads per item
+  unsigned cq, ck;           // items of a token's queries, of its keys (append: and of its values)
   float eps;
 };
 
@@ -92,46 +99,53 @@ __device__ __forceinline__ float row_sum(float s) {
 }
 
 template <int N>
-__device__ __forceinline__ void load_f32(const float* p, float (&f)[N]) {
+__device__ __forceinline__ void load_f32x2(const float* p, float2 (&f)[N]) {
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
+  for (int i = 0; i < N / 2; ++i) {
     const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
-    f[4 * i] = v.x;
-    f[4 * i + 1] = v.y;
-    f[4 * i + 2] = v.z;
-    f[4 * i + 3] = v.w;
+    f[2 * i] = make_float2(v.x, v.y);
+    f[2 * i + 1] = make_float2(v.z, v.w);
   }
 }
 
-// One group of LPR lanes per item = U heads of one token (all queries, all
-// keys or all values): the U rows' loads are issued before anything waits.
+// N pairs of cosines and sines from the table's interleaved (cos, sin).
+template <int N>
+__device__ __forceinline__ void load_angles(const float* p, float2 (&c)[N], float2 (&s)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
+    c[i] = make_float2(v.x, v.z);
+    s[i] = make_float2(v.y, v.w);
+  }
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
+
+// One group of LPR lanes per item = up to hp heads of one token (queries, keys
+// or values), U rows at a time, whose loads are issued before anything waits.
+// The norm's weights and the token's angles fold into four coefficients per
+// pair of values once per item:
+//   y0 = r (x0 g0 cos - x1 g1 sin),  y1 = r (x0 g0 sin + x1 g1 cos)
 template <typename T, int D, int U, bool kAppend>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const FwdParams p, unsigned* err) {
   constexpr int VE = Vec<T>::kN;
   constexpr int LPR = D / (2 * VE);
   const int lane = threadIdx.x % LPR;  // owns values [VE lane, + VE) of both halves
-  const int nc = p.cq + p.ck * (kAppend ? 2 : 1);
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LPR;
-  const bool live = item < static_cast<int64_t>(p.B) * p.S * nc;  // whole groups; idle ones keep up the shuffles
-  const int64_t tok = live ? item / nc : 0;
-  int c = live ? static_cast<int>(item - tok * nc) : 0;
-  const int b = static_cast<int>(tok / p.S);
-  const int s = static_cast<int>(tok - static_cast<int64_t>(b) * p.S);
+  const unsigned nc = p.cq + p.ck * (kAppend ? 2 : 1);
+  const unsigned item = (blockIdx.x * static_cast<unsigned>(kThreads) + threadIdx.x) / LPR;
+  const bool live = item < static_cast<unsigned>(p.B) * static_cast<unsigned>(p.S) * nc;  // idle groups keep up the shuffles
+  const unsigned tok = live ? item / nc : 0;
+  unsigned c = live ? item - tok * nc : 0;
+  const int b = static_cast<int>(tok / static_cast<unsigned>(p.S));
+  const int s = static_cast<int>(tok - static_cast<unsigned>(b) * static_cast<unsigned>(p.S));
   const int kind = c < p.cq ? 0 : c < p.cq + p.ck ? 1 : 2;
   c -= kind == 0 ? 0 : kind == 1 ? p.cq : p.cq + p.ck;
   const Rows in = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
   const RowsOut out = kind == 0 ? p.qo : kind == 1 ? p.ko : p.vo;
-  const int h0 = c * U;
-  const int nh = min(U, (kind == 0 ? p.QH : p.KH) - h0);
-
+  const int h0 = static_cast<int>(c) * p.hp;
+  const int nh = live ? min(p.hp, (kind == 0 ? p.QH : p.KH) - h0) : 0;
   const T* src = static_cast<const T*>(in.p) + b * in.sb + s * in.ss + h0 * in.sh + lane * VE;
-  uint4 lo[U], hi[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (live && u < nh) {
-      lo[u] = ld_stream(src + u * in.sh);
-      hi[u] = ld_stream(src + u * in.sh + D / 2);
-    }
 
   int64_t pos = s, row = s;  // table row; row of the output
   bool idle = false;         // append: a slot without a request
@@ -147,43 +161,59 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const FwdParams p, 
   const bool bad = pos < 0 || pos >= p.table_len || (kAppend && pos >= p.cache_len);
   if (bad && live && lane == 0) atomicOr(err, static_cast<unsigned>(kErrRange));
   T* dst = static_cast<T*>(out.p) + b * out.sb + row * out.ss + h0 * out.sh + lane * VE;
-  const bool write = live && (!kAppend || kind == 0 || !(bad || idle));
+  const bool write = !kAppend || kind == 0 || !(bad || idle);
 
-  if (kAppend && kind == 2) {  // values go to the cache as they are
+  constexpr int N = VE / 2;
+  float2 k00[N], k01[N], k10[N], k11[N];  // y0 = r (x0 k00 + x1 k01), y1 = r (x0 k10 + x1 k11)
+  {
+    float2 cs[N], sn[N], g0[N], g1[N];
+    const float* g = kind == 0 ? p.gq : p.gk;
+    load_angles(p.table + ((bad ? 0 : pos) * (D / 2) + lane * VE) * 2, cs, sn);
+    load_f32x2(g + lane * VE, g0);
+    load_f32x2(g + D / 2 + lane * VE, g1);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (write && u < nh) {
-        st_stream(dst + u * out.sh, lo[u]);
-        st_stream(dst + u * out.sh + D / 2, hi[u]);
-      }
-  }
-  float cs[2 * VE], g0[VE], g1[VE];
-  const float* g = kind == 0 ? p.gq : p.gk;
-  load_f32(p.table + ((bad ? 0 : pos) * (D / 2) + lane * VE) * 2, cs);
-  load_f32(g + lane * VE, g0);
-  load_f32(g + D / 2 + lane * VE, g1);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const bool on = live && u < nh && kind != 2;
-    float x0[VE], x1[VE];
-    Vec<T>::unpack(on ? lo[u] : make_uint4(0u, 0u, 0u, 0u), x0);
-    Vec<T>::unpack(on ? hi[u] : make_uint4(0u, 0u, 0u, 0u), x1);
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
-    const float r = rsqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
-    float y0[VE], y1[VE];
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const float n0 = x0[i] * r * g0[i], n1 = x1[i] * r * g1[i];
-      y0[i] = n0 * cs[2 * i] - n1 * cs[2 * i + 1];
-      y1[i] = n0 * cs[2 * i + 1] + n1 * cs[2 * i];
-      if (bad) y0[i] = y1[i] = __int_as_float(0x7fffffff);
-      if (kAppend && idle) y0[i] = y1[i] = 0.f;
+    for (int i = 0; i < N; ++i) {
+      k00[i] = __fmul2_rn(g0[i], cs[i]);
+      k01[i] = neg(__fmul2_rn(g1[i], sn[i]));
+      k10[i] = __fmul2_rn(g0[i], sn[i]);
+      k11[i] = __fmul2_rn(g1[i], cs[i]);
+      if (bad) k00[i] = k10[i] = both(__int_as_float(0x7fffffff));
     }
-    if (write && on) {
-      st_stream(dst + u * out.sh, Vec<T>::pack(y0));
-      st_stream(dst + u * out.sh + D / 2, Vec<T>::pack(y1));
+  }
+  // all groups of a warp make hp / U rounds (the shuffles need every lane)
+  for (int h = 0; h < p.hp; h += U) {
+    uint4 lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      lo[u] = hi[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (h + u < nh) {
+        lo[u] = ld_stream(src + (h + u) * in.sh);
+        hi[u] = ld_stream(src + (h + u) * in.sh + D / 2);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float2 x0[N], x1[N];
+      Vec<T>::unpack(lo[u], x0);
+      Vec<T>::unpack(hi[u], x1);
+      float2 ss = both(0.f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) ss = __ffma2_rn(x0[i], x0[i], __ffma2_rn(x1[i], x1[i], ss));
+      const float2 r = both(rsqrtf(row_sum<LPR>(ss.x + ss.y) * (1.0f / D) + p.eps));
+      if (h + u >= nh || !write) continue;  // after the shuffles
+      if (!kAppend || kind != 2) {          // (values go to the cache as they are)
+        float2 y0[N], y1[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          y0[i] = __fmul2_rn(r, __ffma2_rn(x0[i], k00[i], __fmul2_rn(x1[i], k01[i])));
+          y1[i] = __fmul2_rn(r, __ffma2_rn(x0[i], k10[i], __fmul2_rn(x1[i], k11[i])));
+        }
+        lo[u] = Vec<T>::pack(y0);
+        hi[u] = Vec<T>::pack(y1);
+        if (kAppend && idle) lo[u] = hi[u] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      st_stream(dst + (h + u) * out.sh, lo[u]);
+      st_stream(dst + (h + u) * out.sh + D / 2, hi[u]);
     }
   }
 }
@@ -197,100 +227,106 @@ struct BwdParams {
   int64_t table_len;
   int B, S;
   int H[2];
+  int hp[2];                 // heads per item
   int blocks[2];             // CTAs of the queries, of the keys
   float* partial;            // [blocks[0] + blocks[1]][D]: each CTA's share of dg
   float eps;
 };
 
 // CTAs [0, blocks[0]) walk the queries, the others the keys; a group of LPR
-// lanes takes U heads of a token at a time.  Each thread sums its columns of
+// lanes takes up to hp heads of a token, U at a time.  Each thread sums its columns of
 // dg over all its rows in registers; the CTA's sums go to `partial` in a fixed
 // order, so the result does not depend on timing.
 template <typename T, int D, int U>
-__global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(const BwdParams p, unsigned* err) {
+__global__ void __launch_bounds__(kThreads, 2) norm_rope_bwd_kernel(const BwdParams p, unsigned* err) {
   constexpr int VE = Vec<T>::kN;
   constexpr int LPR = D / (2 * VE);
   constexpr int kGroups = kThreads / LPR;
-  __shared__ float red[kThreads / 32][D];
+  __shared__ __align__(8) float red[kThreads / 32][D];
+  pdl_trigger();  // the join may take its place while this runs
   const int lane = threadIdx.x % LPR;
   const int w = static_cast<int>(blockIdx.x) < p.blocks[0] ? 0 : 1;
   const int block = static_cast<int>(blockIdx.x) - (w ? p.blocks[0] : 0);
   const Rows xr = p.x[w], dyr = p.dy[w];
   const RowsOut dxr = p.dx[w];
-  const int H = p.H[w];
-  const int nc = (H + U - 1) / U;
-  const int64_t items = static_cast<int64_t>(p.B) * p.S * nc;
-  float g0[VE], g1[VE], a0[VE], a1[VE];
-  load_f32(p.g[w] + lane * VE, g0);
-  load_f32(p.g[w] + D / 2 + lane * VE, g1);
+  const int H = p.H[w], hp = p.hp[w];
+  const unsigned nc = static_cast<unsigned>((H + hp - 1) / hp);
+  const unsigned items = static_cast<unsigned>(p.B) * static_cast<unsigned>(p.S) * nc;
+  constexpr int N = VE / 2;
+  float2 g0[N], g1[N], a0[N], a1[N];
+  load_f32x2(p.g[w] + lane * VE, g0);
+  load_f32x2(p.g[w] + D / 2 + lane * VE, g1);
 #pragma unroll
-  for (int i = 0; i < VE; ++i) a0[i] = a1[i] = 0.f;
+  for (int i = 0; i < N; ++i) a0[i] = a1[i] = both(0.f);
 
   // every group of a warp makes the same number of rounds (the shuffles need all lanes)
-  const int64_t step = static_cast<int64_t>(p.blocks[w]) * kGroups;
-  for (int64_t base = static_cast<int64_t>(block) * kGroups; base < items; base += step) {
-    const int64_t item = base + threadIdx.x / LPR;
+  const unsigned step = static_cast<unsigned>(p.blocks[w]) * kGroups;
+  for (unsigned base = static_cast<unsigned>(block) * kGroups; base < items; base += step) {
+    const unsigned item = base + threadIdx.x / LPR;
     const bool live = item < items;
-    const int64_t tok = live ? item / nc : 0;
-    const int h0 = live ? static_cast<int>(item - tok * nc) * U : 0;
-    const int nh = min(U, H - h0);
-    const int b = static_cast<int>(tok / p.S);
-    const int s = static_cast<int>(tok - static_cast<int64_t>(b) * p.S);
+    const unsigned tok = live ? item / nc : 0;
+    const int h0 = live ? static_cast<int>(item - tok * nc) * hp : 0;
+    const int nh = live ? min(hp, H - h0) : 0;
+    const int b = static_cast<int>(tok / static_cast<unsigned>(p.S));
+    const int s = static_cast<int>(tok - static_cast<unsigned>(b) * static_cast<unsigned>(p.S));
     const T* xs = static_cast<const T*>(xr.p) + b * xr.sb + s * xr.ss + h0 * xr.sh + lane * VE;
     const T* ds = static_cast<const T*>(dyr.p) + b * dyr.sb + s * dyr.ss + h0 * dyr.sh + lane * VE;
     T* dst = static_cast<T*>(dxr.p) + b * dxr.sb + s * dxr.ss + h0 * dxr.sh + lane * VE;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    uint4 xl[U], xh[U], dl[U], dh[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      xl[u] = xh[u] = dl[u] = dh[u] = zero;
-      if (live && u < nh) {
-        xl[u] = ld_stream(xs + u * xr.sh);
-        xh[u] = ld_stream(xs + u * xr.sh + D / 2);
-        dl[u] = ld_stream(ds + u * dyr.sh);
-        dh[u] = ld_stream(ds + u * dyr.sh + D / 2);
-      }
-    }
     int64_t pos = s;
     if (p.positions) pos = __ldg(p.positions + tok);
     const bool bad = pos < 0 || pos >= p.table_len;
     if (bad && live && lane == 0) atomicOr(err, static_cast<unsigned>(kErrRange));
-    float cs[2 * VE];
-    load_f32(p.table + ((bad ? 0 : pos) * (D / 2) + lane * VE) * 2, cs);
+    float2 cs[N], sn[N];
+    load_angles(p.table + ((bad ? 0 : pos) * (D / 2) + lane * VE) * 2, cs, sn);
+    if (bad) {  // the position's rows come out as NaN
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x0[VE], x1[VE], y0[VE], y1[VE];
-      Vec<T>::unpack(xl[u], x0);
-      Vec<T>::unpack(xh[u], x1);
-      Vec<T>::unpack(dl[u], y0);
-      Vec<T>::unpack(dh[u], y1);
-      float ss = 0.f, xt = 0.f;
+      for (int i = 0; i < N; ++i) cs[i] = both(__int_as_float(0x7fffffff));
+    }
+    for (int h = 0; h < hp; h += U) {
+      uint4 xl[U], xh[U], dl[U], dh[U];
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        // dn = the rotation's transpose applied to dy
-        const float n0 = y0[i] * cs[2 * i] + y1[i] * cs[2 * i + 1];
-        const float n1 = y1[i] * cs[2 * i] - y0[i] * cs[2 * i + 1];
-        y0[i] = bad ? __int_as_float(0x7fffffff) : n0;
-        y1[i] = bad ? __int_as_float(0x7fffffff) : n1;
-        ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
-        xt = fmaf(x0[i], y0[i] * g0[i], fmaf(x1[i], y1[i] * g1[i], xt));
-      }
-      const float r = rsqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
-      const float k = row_sum<LPR>(xt) * (1.0f / D) * r * r;  // dx = r (t - x r^2 mean(x t))
-      const bool on = live && u < nh;
-      float o0[VE], o1[VE];
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        o0[i] = r * (y0[i] * g0[i] - x0[i] * k);
-        o1[i] = r * (y1[i] * g1[i] - x1[i] * k);
-        if (on) {  // a row that is not there has r = 1 / sqrt(eps), infinite for eps = 0
-          a0[i] = fmaf(x0[i] * r, y0[i], a0[i]);
-          a1[i] = fmaf(x1[i] * r, y1[i], a1[i]);
+      for (int u = 0; u < U; ++u) {
+        xl[u] = xh[u] = dl[u] = dh[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (h + u < nh) {
+          xl[u] = ld_stream(xs + (h + u) * xr.sh);
+          xh[u] = ld_stream(xs + (h + u) * xr.sh + D / 2);
+          dl[u] = ld_stream(ds + (h + u) * dyr.sh);
+          dh[u] = ld_stream(ds + (h + u) * dyr.sh + D / 2);
         }
       }
-      if (on) {
-        st_stream(dst + u * dxr.sh, Vec<T>::pack(o0));
-        st_stream(dst + u * dxr.sh + D / 2, Vec<T>::pack(o1));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float2 x0[N], x1[N], y0[N], y1[N];
+        Vec<T>::unpack(xl[u], x0);
+        Vec<T>::unpack(xh[u], x1);
+        Vec<T>::unpack(dl[u], y0);
+        Vec<T>::unpack(dh[u], y1);
+        float2 ss = both(0.f), xt = both(0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          // dn = the rotation's transpose applied to dy
+          const float2 n0 = __ffma2_rn(y0[i], cs[i], __fmul2_rn(y1[i], sn[i]));
+          const float2 n1 = __ffma2_rn(y1[i], cs[i], neg(__fmul2_rn(y0[i], sn[i])));
+          y0[i] = n0;
+          y1[i] = n1;
+          ss = __ffma2_rn(x0[i], x0[i], __ffma2_rn(x1[i], x1[i], ss));
+          xt = __ffma2_rn(x0[i], __fmul2_rn(n0, g0[i]), __ffma2_rn(x1[i], __fmul2_rn(n1, g1[i]), xt));
+        }
+        const float rs = rsqrtf(row_sum<LPR>(ss.x + ss.y) * (1.0f / D) + p.eps);
+        const float2 r = both(rs);
+        // dx = r t - x r^3 mean(x t)
+        const float2 k = both(-row_sum<LPR>(xt.x + xt.y) * (1.0f / D) * rs * rs * rs);
+        if (h + u >= nh) continue;  // after the shuffles; no row, no share of dg
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float2 m0 = __fmul2_rn(r, y0[i]), m1 = __fmul2_rn(r, y1[i]);
+          a0[i] = __ffma2_rn(x0[i], m0, a0[i]);
+          a1[i] = __ffma2_rn(x1[i], m1, a1[i]);
+          x0[i] = __ffma2_rn(m0, g0[i], __fmul2_rn(x0[i], k));
+          x1[i] = __ffma2_rn(m1, g1[i], __fmul2_rn(x1[i], k));
+        }
+        st_stream(dst + (h + u) * dxr.sh, Vec<T>::pack(x0));
+        st_stream(dst + (h + u) * dxr.sh + D / 2, Vec<T>::pack(x1));
       }
     }
   }
@@ -298,16 +334,18 @@ __global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(const BwdParams
 #pragma unroll
   for (int o = LPR; o < 32; o <<= 1)
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      a0[i] += __shfl_xor_sync(kFull, a0[i], o);
-      a1[i] += __shfl_xor_sync(kFull, a1[i], o);
+    for (int i = 0; i < N; ++i) {
+      a0[i].x += __shfl_xor_sync(kFull, a0[i].x, o);
+      a0[i].y += __shfl_xor_sync(kFull, a0[i].y, o);
+      a1[i].x += __shfl_xor_sync(kFull, a1[i].x, o);
+      a1[i].y += __shfl_xor_sync(kFull, a1[i].y, o);
     }
   const int warp = threadIdx.x >> 5;
   if ((threadIdx.x & 31) < LPR)
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      red[warp][lane * VE + i] = a0[i];
-      red[warp][D / 2 + lane * VE + i] = a1[i];
+    for (int i = 0; i < N; ++i) {
+      *reinterpret_cast<float2*>(&red[warp][lane * VE + 2 * i]) = a0[i];
+      *reinterpret_cast<float2*>(&red[warp][D / 2 + lane * VE + 2 * i]) = a1[i];
     }
   __syncthreads();
   for (int d = threadIdx.x; d < D; d += kThreads) {
@@ -323,6 +361,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(const BwdParams
 __global__ void __launch_bounds__(1024) dg_join_kernel(const float* __restrict__ partial, float* __restrict__ dgq,
                                                        float* __restrict__ dgk, int D, int bq, int bk) {
   __shared__ float red[32][33];
+  pdl_wait();  // the rows' kernel is done
   const int col = blockIdx.x * 32 + (threadIdx.x & 31);
   const int slice = threadIdx.x >> 5;
   const int w = blockIdx.y;
@@ -351,20 +390,40 @@ __global__ void __launch_bounds__(256) rope_table_any_kernel(float2* __restrict_
   tab[i] = make_float2(static_cast<float>(cs), static_cast<float>(sn));
 }
 
-// Forward CTAs take U heads of a token per group of lanes.
-constexpr int kFwdHeads = 4;
-constexpr int kBwdHeads = 2;
+constexpr int kFwdRows = 4, kBwdRows = 2;  // rows whose loads a group has in flight
+
+// Heads per item: two rounds of `rows` where the rows fill the GPU many times
+// over, so that the token's angles and the weights (as many load instructions
+// as four bf16 rows) are paid once for both; one round otherwise.  Measured,
+// forward B8 S4096 of 40 heads, 1 / 2 / 4 / 8 rounds: 120 / 109 / 140 / 127 us
+// (few, short-lived items keep the reads of a CTA close together); backward
+// B2 S4096, 1 / 2 / 3 / 16 rounds: 53 / 51 / 55 / 65 us; fp32 B3 S1001 of 16
+// heads, 1 / 2 rounds: 4.8 / 5.0 us.
+int heads_per_item(int64_t tokens, int64_t heads, int64_t lanes, int rows) {
+  return tokens * heads * lanes >= 16 * 512ll * num_sms() ? 2 * rows : rows;
+}
+
+template <typename T, int D, int U, bool kAppend>
+kda_status launch_fwd_u(FwdParams& p, int hp, cudaStream_t st) {
+  constexpr int LPR = D / (2 * Vec<T>::kN);
+  p.hp = hp;
+  p.cq = static_cast<unsigned>((p.QH + hp - 1) / hp);
+  p.ck = static_cast<unsigned>((p.KH + hp - 1) / hp);
+  const int64_t items = static_cast<int64_t>(p.B) * p.S * (p.cq + p.ck * (kAppend ? 2 : 1));
+  KDA_CHECK_SUPPORTED(items * LPR < (1ll << 32), "qk_norm_rope: too many rows (%lld tokens)", (long long)p.B * p.S);
+  const int64_t grid = (items * LPR + kThreads - 1) / kThreads;
+  norm_rope_kernel<T, D, U, kAppend><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p, kda_err_ptr_qk_norm());
+  return launch_status(kAppend ? "qk_norm_rope_append" : "qk_norm_rope");
+}
 
 template <typename T, int D, bool kAppend>
 kda_status launch_fwd_d(FwdParams& p, cudaStream_t st) {
   constexpr int LPR = D / (2 * Vec<T>::kN);
-  p.cq = (p.QH + kFwdHeads - 1) / kFwdHeads;
-  p.ck = (p.KH + kFwdHeads - 1) / kFwdHeads;
-  const int64_t items = static_cast<int64_t>(p.B) * p.S * (p.cq + p.ck * (kAppend ? 2 : 1));
-  const int64_t grid = (items * LPR + kThreads - 1) / kThreads;
-  norm_rope_kernel<T, D, kFwdHeads, kAppend>
-      <<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p, kda_err_ptr_qk_norm());
-  return launch_status(kAppend ? "qk_norm_rope_append" : "qk_norm_rope");
+  const int64_t tokens = static_cast<int64_t>(p.B) * p.S;
+  // few rows: one per group of lanes, so that all of them load at once
+  if (tokens * (p.QH + p.KH) * LPR <= 512ll * num_sms()) return launch_fwd_u<T, D, 1, kAppend>(p, 1, st);
+  return launch_fwd_u<T, D, kFwdRows, kAppend>(
+      p, heads_per_item(tokens, p.QH + p.KH, LPR, kFwdRows), st);
 }
 
 template <typename T, bool kAppend>
@@ -376,27 +435,47 @@ kda_status launch_fwd(FwdParams& p, int64_t D, cudaStream_t st) {
   }
 }
 
-// CTAs of the backward: four per SM, shared between queries and keys in
-// proportion to their rows, no more than there are rounds of work.
-void bwd_blocks(int64_t tokens, int64_t QH, int64_t KH, int64_t D, bool f32, int (&blocks)[2]) {
-  const int64_t groups = kThreads / (D / (f32 ? 8 : 16));
-  const int64_t total = 4ll * num_sms();
+// The backward's items and CTAs: one CTA per round of work up to four per SM;
+// beyond that the two that are resident on each SM, shared between queries and
+// keys in proportion to their rows (a CTA that walks many rounds leaves fewer
+// shares of dg to join: 51 against 53 us at B2 S4096 of 40 heads; a short call
+// gains from the parallelism: 6.7 against 8.1 us at 777 tokens of 9 heads).
+void bwd_split(int64_t tokens, int64_t QH, int64_t KH, int64_t D, bool f32, int (&hp)[2], int (&blocks)[2]) {
+  const int64_t lanes = D / (f32 ? 8 : 16);
+  const int64_t groups = kThreads / lanes;
   const int64_t heads[2] = {QH, KH};
+  int64_t rounds[2];
   for (int w = 0; w < 2; ++w) {
-    const int64_t rounds = (tokens * ((heads[w] + kBwdHeads - 1) / kBwdHeads) + groups - 1) / groups;
-    int64_t n = total * heads[w] / (QH + KH);
-    if (n < 1) n = 1;
-    blocks[w] = static_cast<int>(rounds < n ? rounds : n);
+    hp[w] = heads_per_item(tokens, QH + KH, lanes, kBwdRows);
+    rounds[w] = (tokens * ((heads[w] + hp[w] - 1) / hp[w]) + groups - 1) / groups;
+  }
+  const bool few = rounds[0] + rounds[1] <= 4ll * num_sms();
+  for (int w = 0; w < 2; ++w) {
+    const int64_t share = std::max<int64_t>(1, 2ll * num_sms() * heads[w] / (QH + KH));
+    blocks[w] = static_cast<int>(few ? rounds[w] : std::min(rounds[w], share));
   }
 }
 
 template <typename T, int D>
 kda_status launch_bwd_d(const BwdParams& p, float* dgq, float* dgk, cudaStream_t st) {
-  norm_rope_bwd_kernel<T, D, kBwdHeads>
+  const int64_t most = static_cast<int64_t>(p.B) * p.S *
+                       std::max((p.H[0] + p.hp[0] - 1) / p.hp[0], (p.H[1] + p.hp[1] - 1) / p.hp[1]);
+  KDA_CHECK_SUPPORTED(most < (1ll << 31), "qk_norm_rope_backward: too many rows (%lld tokens)", (long long)p.B * p.S);
+  norm_rope_bwd_kernel<T, D, kBwdRows>
       <<<static_cast<unsigned>(p.blocks[0] + p.blocks[1]), kThreads, 0, st>>>(p, kda_err_ptr_qk_norm());
   const kda_status s = launch_status("qk_norm_rope_backward");
   if (s != KDA_OK) return s;
-  dg_join_kernel<<<dim3(D / 32, 2), 1024, 0, st>>>(p.partial, dgq, dgk, D, p.blocks[0], p.blocks[1]);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(D / 32, 2);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, dg_join_kernel, static_cast<const float*>(p.partial), dgq, dgk, D, p.blocks[0],
+                     p.blocks[1]);
   return launch_status("qk_norm_rope_backward: dg");
 }
 
@@ -421,8 +500,7 @@ kda_status common_check(const char* op, int64_t B, int64_t S, int64_t QH, int64_
   KDA_CHECK_ARG(eps >= 0.f, "%s: eps must not be negative", op);
   KDA_CHECK_SUPPORTED(D == 64 || D == 128 || D == 256, "%s: head_dim must be 64, 128 or 256, got %lld", op,
                       (long long)D);
-  KDA_CHECK_SUPPORTED(B <= (1ll << 31) - 1 && S <= (1ll << 31) - 1 && QH <= 65535 && KH <= 65535 &&
-                          B * S <= (1ll << 36) / (QH + 2 * KH),
+  KDA_CHECK_SUPPORTED(B < (1ll << 31) && S < (1ll << 31) && B * S < (1ll << 31) && QH <= 65535 && KH <= 65535,
                       "%s: too many rows (B=%lld S=%lld QH=%lld KH=%lld)", op, (long long)B, (long long)S,
                       (long long)QH, (long long)KH);
   return KDA_OK;
@@ -524,8 +602,8 @@ extern "C" kda_status kda_qk_norm_rope_append_bf16(const void* q, const void* k,
 extern "C" size_t kda_qk_norm_rope_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
                                                            int f32) {
   if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || (D != 64 && D != 128 && D != 256)) return 0;
-  int blocks[2];
-  bwd_blocks(B * S, QH, KH, D, f32 != 0, blocks);
+  int hp[2], blocks[2];
+  bwd_split(B * S, QH, KH, D, f32 != 0, hp, blocks);
   return static_cast<size_t>(blocks[0] + blocks[1]) * D * 4;
 }
 
@@ -569,7 +647,7 @@ extern "C" kda_status kda_qk_norm_rope_backward(const void* dq_out, const void* 
   p.eps = eps;
   p.B = static_cast<int>(B);
   p.S = static_cast<int>(S);
-  bwd_blocks(B * S, QH, KH, D, f32 != 0, p.blocks);
+  bwd_split(B * S, QH, KH, D, f32 != 0, p.hp, p.blocks);
   p.partial = static_cast<float*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return f32 ? launch_bwd<float>(p, D, dgq, dgk, st) : launch_bwd<__nv_bfloat16>(p, D, dgq, dgk, st);
