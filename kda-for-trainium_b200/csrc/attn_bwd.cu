@@ -45,6 +45,8 @@
 // All mbarrier waits are bounded (common.cuh); every TMA load targets one CTA.
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 
 KDA_DEFINE_ERROR_WORD(attn_bwd)
@@ -82,6 +84,11 @@ struct BwdParams {
   int causal;
   int window, sinks;  // sliding window (kWindow): keys [0, sinks) and the `window` keys up to the query
   int row_stride;     // rows per (b, h) of lse and di: S, or (kWindow) S rounded up to whole blocks
+  // kWindow: the walk of each of the first `sink_blocks` key blocks, which every
+  // later query visits, is cut into sink_parts CTAs, that of the others into
+  // `parts`; where there are several, their dV_j and dK_j go to `partial`
+  int sink_blocks, sink_parts, parts;
+  float* partial;     // [item][2][128][128] fp32: dV_j, dK_j (unscaled) of an item's walk
   float sl2;        // softmax scale * log2(e)
   float scale;      // softmax scale (applied to dK here, to dQ by the conversion)
   const float* lse;  // [B][QH][row_stride]
@@ -111,7 +118,27 @@ template <bool kWindow>
 __device__ __forceinline__ void q_range(const BwdParams& p, int j, int& q0, int& nq) {
   q0 = kWindow || p.causal ? j : 0;
   nq = p.nkb - q0;
-  if (kWindow && j * kBlk >= p.sinks) nq = min(nq, (kBlk - 1 + p.window - 1) / kBlk + 1);
+  if (kWindow && j >= p.sink_blocks) nq = min(nq, (kBlk - 1 + p.window - 1) / kBlk + 1);
+}
+
+// What a CTA works on: the key block j of (batch, kv head) bg, and with a
+// window the part of the block's walk and its slot in `partial` (-1: the whole
+// walk, written as it is).  Heaviest key blocks first.
+struct Item {
+  int bg, j, part, parts, slot;
+};
+template <bool kWindow>
+__device__ __forceinline__ Item cta_item(const BwdParams& p) {
+  const int heads = p.B * p.KH;
+  int x = static_cast<int>(blockIdx.x);
+  if (!kWindow) return {x % heads, x / heads, 0, 1, -1};
+  const int sinks = p.sink_blocks * p.sink_parts * heads;
+  const bool sink = x < sinks;
+  const int parts = sink ? p.sink_parts : p.parts;
+  const int y = sink ? x : x - sinks;
+  const int slot = parts == 1 ? -1 : sink || p.sink_parts > 1 ? x : y;
+  const int bg = y % heads, r = y / heads;
+  return {bg, (sink ? 0 : p.sink_blocks) + r / parts, r % parts, parts, slot};
 }
 
 // Query block of step `it` (head it / nq of the group): each key block starts
@@ -168,12 +195,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   // heaviest key blocks first (causal: block j visits nkb - j query blocks)
-  const int bg = static_cast<int>(blockIdx.x) % (p.B * p.KH);
-  const int j = static_cast<int>(blockIdx.x) / (p.B * p.KH);
+  const Item item = cta_item<kWindow>(p);
+  const int bg = item.bg, j = item.j;
   const int b = bg / p.KH, g = bg - (bg / p.KH) * p.KH;
   int q0, nq;
   q_range<kWindow>(p, j, q0, nq);
-  const int n_iter = p.rep * nq;
+  int n_iter = p.rep * nq;  // steps of the walk ...
+  int it0 = 0;              // ... from this one on
+  if (kWindow) {
+    it0 = static_cast<int>(static_cast<int64_t>(n_iter) * item.part / item.parts);
+    n_iter = static_cast<int>(static_cast<int64_t>(n_iter) * (item.part + 1) / item.parts) - it0;
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -226,8 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t q_issued = 0;  // Q buffers with a load in flight at the end
       for (int it = 0; it < n_iter && ok; ++it) {
         const uint32_t pprev = static_cast<uint32_t>(it - 1) & 1u;
-        const int h = g * p.rep + it / nq;
-        const int s0 = q_block(j, q0, nq, it) * kBlk;
+        const int h = g * p.rep + (it0 + it) / nq;
+        const int s0 = q_block(j, q0, nq, it0 + it) * kBlk;
         const int qb = it & 1;
         const int64_t drow = (static_cast<int64_t>(b) * p.QH + h) * p.row_stride + s0;  // lse / di (dout) row
         const int valid = !kWindow && p.S - s0 < kBlk ? p.S - s0 : kBlk;  // query rows of the block that lse, di have
@@ -419,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int it = 0; it < n_iter && ok; ++it) {
       const uint32_t par = static_cast<uint32_t>(it) & 1u;
-      const int s0 = q_block(j, q0, nq, it) * kBlk;
+      const int s0 = q_block(j, q0, nq, it0 + it) * kBlk;
       ok = mbar_wait(s_ready, par, err, kErrWaitAccum) && mbar_wait(lse_full, par, err, kErrWaitFull);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -526,8 +558,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_warp(ds_ready);
     }
     // dV_j (group 0), dK_j (group 1; bf16, dK times the softmax scale) once
-    // every MMA is done (every key block visits at least one query block)
-    if (ok) ok = mbar_wait(dkv_ready, 0u, err, kErrWaitAccum);
+    // every MMA is done (every key block visits at least one query block; a
+    // part of its walk may be empty)
+    const bool some = !kWindow || n_iter > 0;
+    if (ok && some) ok = mbar_wait(dkv_ready, 0u, err, kErrWaitAccum);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
@@ -535,13 +569,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int which = grp;
         __nv_bfloat16* dst = (which == 0 ? p.dv : p.dk) +
                              ((static_cast<int64_t>(b) * p.S + kpos) * p.KH + g) * kD;
+        float* part = kWindow && item.slot >= 0
+                          ? p.partial + ((static_cast<int64_t>(item.slot) * 2 + which) * kBlk + kr) * kD
+                          : nullptr;
         const float f = which == 0 ? 1.f : p.scale;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t r[32];
-          tmem_ld_32x32b_x32(tmem + lane_base + 256 + which * 128 + c * 32, r);
-          tmem_ld_wait();
-          if (kpos < p.S) {
+          if (some) {
+            tmem_ld_32x32b_x32(tmem + lane_base + 256 + which * 128 + c * 32, r);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
+          }
+          if (kWindow && part) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              reinterpret_cast<uint4*>(part + c * 32)[q] =
+                  make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+          } else if (kpos < p.S) {
             uint4* o = reinterpret_cast<uint4*>(dst + c * 32);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -565,8 +612,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int it = 0; it < n_iter && ok; ++it) {
       const uint32_t par = static_cast<uint32_t>(it) & 1u;
-      const int h = g * p.rep + it / nq;
-      const int s0 = q_block(j, q0, nq, it) * kBlk;
+      const int h = g * p.rep + (it0 + it) / nq;
+      const int s0 = q_block(j, q0, nq, it0 + it) * kBlk;
       ok = mbar_wait(dq_ready, par, err, kErrWaitAccum);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -626,13 +673,11 @@ kda_status tmap_bshd(CUtensorMap* m, const void* base, int64_t B, int64_t S, int
   return make_tmap_bf16(m, base, 4, dims, strides, box);
 }
 
-// Opt-ins of one instantiation (once per device), the zeroed fp32 dq, the
-// kernel, and dq's conversion.
+// Opt-ins of one instantiation (once per device), the kernel on a zeroed fp32
+// dq, and dq's conversion.
 template <bool kWindow>
 kda_status launch_bwd(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CUtensorMap& tdo,
-                      const BwdParams& p, __nv_bfloat16* dq, cudaStream_t st) {
-  if (cudaMemsetAsync(p.dq, 0, attn_backward_scratch_bytes(p.B, p.S, p.QH), st) != cudaSuccess)
-    return launch_status("attn_backward: memset");
+                      const BwdParams& p, __nv_bfloat16* dq, unsigned grid, cudaStream_t st) {
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -649,7 +694,6 @@ kda_status launch_bwd(const CUtensorMap& tk, const CUtensorMap& tv, const CUtens
       return launch_status("attn_backward: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  const unsigned grid = static_cast<unsigned>(p.B * p.KH * p.nkb);
   attn_bwd_kernel<kWindow><<<grid, kThreads, Smem::kBytes, st>>>(tk, tv, tq, tdo, p, kda_err_ptr_attn_bwd());
   KDA_BWD_TRY(launch_status("attn_bwd_kernel"));
   const int64_t n8 = static_cast<int64_t>(p.B) * p.S * p.QH * kD / 8;
@@ -697,7 +741,9 @@ kda_status attn_backward_flash(const __nv_bfloat16* q, const __nv_bfloat16* k, c
   p.dq = dq32;
   p.dk = dk;
   p.dv = dv;
-  return launch_bwd<false>(tk, tv, tq, tdo, p, dq, st);
+  if (cudaMemsetAsync(dq32, 0, attn_backward_scratch_bytes(B, S, QH), st) != cudaSuccess)
+    return launch_status("attn_backward: memset");
+  return launch_bwd<false>(tk, tv, tq, tdo, p, dq, static_cast<unsigned>(B * KH * p.nkb), st);
 }
 
 }  // namespace kda
@@ -709,11 +755,13 @@ namespace kda {
 namespace {
 // di[b][h][s] = sum_d dout * out (fp32) and a copy of lse, both with rows
 // padded to whole query blocks (zeros) so that every block's 512 bytes load
-// aligned.  dout, out [B][S][QH][128]; 16 lanes per row, 8 values each.
+// aligned; and the zeros that dq's shares are added to.  dout, out
+// [B][S][QH][128]; 16 lanes per row, 8 values each.
 __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* __restrict__ dout,
                                                           const __nv_bfloat16* __restrict__ out,
                                                           const float* __restrict__ lse, float* __restrict__ di,
-                                                          float* __restrict__ lse_pad, int S, int SP, int QH) {
+                                                          float* __restrict__ lse_pad, float* __restrict__ dq, int S,
+                                                          int SP, int QH) {
   const int lane = threadIdx.x & 15;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);  // (s, h) of batch entry blockIdx.y
   const int b = blockIdx.y;
@@ -728,6 +776,8 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* _
     unpack_bf16x8(reinterpret_cast<const uint4*>(out + row * kD)[lane], fb);
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fb[e], acc);
+    float4* z = reinterpret_cast<float4*>(dq + ((static_cast<int64_t>(b) * QH + h) * S + s) * kD);
+    z[lane] = z[lane + 16] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
@@ -738,15 +788,73 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* _
   }
 }
 
+// dk, dv of the key blocks whose walk was cut: the parts' fp32 sums added in
+// order, to bf16.  `first` is the slot of the first block's first part, the
+// parts of block `jb` and (batch, kv head) bg are heads slots apart.  Grid
+// (blocks x 8, heads, 2: dv, dk); 16 lanes per key row.
+__global__ void __launch_bounds__(256) join_parts_kernel(const BwdParams p, int j0, int first, int parts) {
+  const int heads = p.B * p.KH;
+  const int jb = blockIdx.x >> 3;
+  const int row = (blockIdx.x & 7) * 16 + (threadIdx.x >> 4);
+  const int bg = blockIdx.y, which = blockIdx.z;
+  const int lane = threadIdx.x & 15;
+  const int kpos = (j0 + jb) * kBlk + row;
+  if (kpos >= p.S) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
+  for (int i = 0; i < parts; ++i) {
+    const int64_t slot = first + (static_cast<int64_t>(jb) * parts + i) * heads + bg;
+    const float4* src = reinterpret_cast<const float4*>(p.partial + ((slot * 2 + which) * kBlk + row) * kD) + 2 * lane;
+    const float4 u = src[0], v = src[1];
+    a = make_float4(a.x + u.x, a.y + u.y, a.z + u.z, a.w + u.w);
+    c = make_float4(c.x + v.x, c.y + v.y, c.z + v.z, c.w + v.w);
+  }
+  const float f = which == 0 ? 1.f : p.scale;
+  const int b = bg / p.KH, g = bg - b * p.KH;
+  uint4* dst = reinterpret_cast<uint4*>((which == 0 ? p.dv : p.dk) +
+                                        ((static_cast<int64_t>(b) * p.S + kpos) * p.KH + g) * kD);
+  dst[lane] = make_uint4(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(a.z * f, a.w * f), pack_bf16x2(c.x * f, c.y * f),
+                         pack_bf16x2(c.z * f, c.w * f));
+}
+
 size_t al256(size_t n) { return (n + 255) & ~size_t(255); }
 int64_t padded_rows(int64_t S) { return (S + kBlk - 1) / kBlk * kBlk; }
+
+// How the key blocks' walks are cut.  A walk takes rep x (query blocks that see
+// the block) steps: the same few for most blocks, up to the whole sequence for
+// those with sinks.  With `fair` = the steps of all walks / SMs, no CTA should
+// take much more: sink walks are cut to the length of the others (8 steps at
+// least: a part costs its 128 KB of partial sums), and all walks to `fair`
+// where there are too few of them to fill the GPU.
+struct Cut {
+  int64_t nkb, sink_blocks, sink_parts, parts, slots, grid;
+};
+Cut cut_walks(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t window, int64_t sinks) {
+  Cut c{};
+  const int64_t rep = QH / KH, heads = B * KH;
+  c.nkb = padded_rows(S) / kBlk;
+  const int64_t nq = std::min(c.nkb, (kBlk - 1 + std::min(window, S) - 1) / kBlk + 1);
+  c.sink_blocks = nq == c.nkb ? 0 : std::min(c.nkb, (std::min(sinks, S) + kBlk - 1) / kBlk);
+  const int64_t rest = c.nkb - c.sink_blocks;  // their walks: nq, and nq - 1 .. 1 at the sequence's end
+  int64_t steps = c.sink_blocks * c.nkb - c.sink_blocks * (c.sink_blocks - 1) / 2;
+  steps += rest >= nq ? rest * nq - nq * (nq - 1) / 2 : rest * (rest + 1) / 2;
+  const int64_t fair = std::max<int64_t>(4, (steps * rep * heads + num_sms() - 1) / num_sms());
+  const int64_t usual = rep * nq;
+  c.parts = usual <= fair ? 1 : (usual + fair - 1) / fair;
+  const int64_t len = std::min(fair, std::max<int64_t>(8, usual));
+  c.sink_parts = c.sink_blocks ? (rep * c.nkb + len - 1) / len : 1;
+  const int64_t sink_items = c.sink_blocks * c.sink_parts * heads, items = rest * c.parts * heads;
+  c.grid = sink_items + items;
+  c.slots = (c.sink_parts > 1 ? sink_items : 0) + (c.parts > 1 ? items : 0);
+  return c;
+}
 }  // namespace
 }  // namespace kda
 
 extern "C" size_t kda_gqa_window_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
                                                          int64_t window, int64_t sinks) {
-  if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || D != kD || window <= 0 || sinks < 0) return 0;
-  return 2 * al256(static_cast<size_t>(B) * QH * padded_rows(S) * 4) + attn_backward_scratch_bytes(B, S, QH);
+  if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || QH % KH || D != kD || window <= 0 || sinks < 0) return 0;
+  return 2 * al256(static_cast<size_t>(B) * QH * padded_rows(S) * 4) + attn_backward_scratch_bytes(B, S, QH) +
+         static_cast<size_t>(cut_walks(B, S, QH, KH, window, sinks).slots) * 2 * kBlk * kD * 4;
 }
 
 extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void* q, const void* k, const void* v,
@@ -759,6 +867,7 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   KDA_BWD_TRY(gqa_window_check(op, B, S, QH, KH, D, window, sinks));
   KDA_CHECK_ARG(dout && q && k && v && out && lse && dq && dk && dv && q_strides && k_strides && v_strides,
                 "%s: null pointer", op);
+  KDA_CHECK_SUPPORTED(B * KH <= 65535, "%s: too many kv heads (%lld)", op, (long long)(B * KH));
   const int64_t dense_q[3] = {S * QH * kD, QH * kD, kD}, dense_k[3] = {S * KH * kD, KH * kD, kD};
   KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
                           head_rows_ok(dout, dense_q) && head_rows_ok(out, dense_q) && head_rows_ok(dq, dense_q) &&
@@ -778,7 +887,7 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   float* lse_pad = reinterpret_cast<float*>(w + rows);
   p.dq = reinterpret_cast<float*>(w + 2 * rows);
   window_rows_kernel<<<dim3(static_cast<unsigned>((SP * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
-      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, di, lse_pad,
+      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, di, lse_pad, p.dq,
       static_cast<int>(S), static_cast<int>(SP), static_cast<int>(QH));
   KDA_BWD_TRY(launch_status("gqa_window_backward: rows"));
   CUtensorMap tk, tv, tq, tdo;
@@ -791,7 +900,13 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   p.QH = static_cast<int>(QH);
   p.KH = static_cast<int>(KH);
   p.rep = static_cast<int>(QH / KH);
-  p.nkb = static_cast<int>(SP / kBlk);
+  const Cut cut = cut_walks(B, S, QH, KH, window, sinks);
+  KDA_CHECK_SUPPORTED(cut.grid < (1ll << 31), "%s: too many key blocks (%lld)", op, (long long)cut.grid);
+  p.nkb = static_cast<int>(cut.nkb);
+  p.sink_blocks = static_cast<int>(cut.sink_blocks);
+  p.sink_parts = static_cast<int>(cut.sink_parts);
+  p.parts = static_cast<int>(cut.parts);
+  p.partial = p.dq + attn_backward_scratch_bytes(B, S, QH) / 4;
   p.causal = 1;
   p.window = static_cast<int>(window < S ? window : S);
   p.sinks = static_cast<int>(sinks < S ? sinks : S);
@@ -802,5 +917,13 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   p.di = di;
   p.dk = static_cast<__nv_bfloat16*>(dk);
   p.dv = static_cast<__nv_bfloat16*>(dv);
-  return launch_bwd<true>(tk, tv, tq, tdo, p, static_cast<__nv_bfloat16*>(dq), st);
+  KDA_BWD_TRY(launch_bwd<true>(tk, tv, tq, tdo, p, static_cast<__nv_bfloat16*>(dq), static_cast<unsigned>(cut.grid),
+                               st));
+  const unsigned heads = static_cast<unsigned>(B * KH);
+  if (p.sink_parts > 1)
+    join_parts_kernel<<<dim3(static_cast<unsigned>(p.sink_blocks) * 8, heads, 2), 256, 0, st>>>(p, 0, 0, p.sink_parts);
+  if (p.parts > 1)
+    join_parts_kernel<<<dim3(static_cast<unsigned>(p.nkb - p.sink_blocks) * 8, heads, 2), 256, 0, st>>>(
+        p, p.sink_blocks, p.sink_parts > 1 ? p.sink_blocks * p.sink_parts * static_cast<int>(heads) : 0, p.parts);
+  return launch_status("gqa_window_backward: join");
 }
