@@ -45,8 +45,6 @@
 // All mbarrier waits are bounded (common.cuh); every TMA load targets one CTA.
 #include <math.h>
 
-#include <algorithm>
-
 #include "common.cuh"
 
 KDA_DEFINE_ERROR_WORD(attn_bwd)
@@ -82,17 +80,10 @@ struct BwdParams {
   int B, S, QH, KH, rep;
   int nkb;          // key (and query) blocks per sequence
   int causal;
-  int window, sinks;  // sliding window (kWindow): keys [0, sinks) and the `window` keys up to the query
-  int row_stride;     // rows per (b, h) of lse and di: S, or (kWindow) S rounded up to whole blocks
-  // kWindow: the walk of each of the first `sink_blocks` key blocks, which every
-  // later query visits, is cut into sink_parts CTAs, that of the others into
-  // `parts`; where there are several, their dV_j and dK_j go to `partial`
-  int sink_blocks, sink_parts, parts;
-  float* partial;     // [item][2][128][128] fp32: dV_j, dK_j (unscaled) of an item's walk
   float sl2;        // softmax scale * log2(e)
   float scale;      // softmax scale (applied to dK here, to dQ by the conversion)
-  const float* lse;  // [B][QH][row_stride]
-  const float* di;   // [B][QH][row_stride]
+  const float* lse;  // [B][QH][S]
+  const float* di;   // [B][QH][S]
   float* dq;         // fp32 [B][QH][S][128] (the transposed dQ), zeroed before the launch, unscaled
   __nv_bfloat16* dk;  // [B][S][KH][128]
   __nv_bfloat16* dv;
@@ -112,33 +103,10 @@ struct Smem {
 };
 
 // Query blocks a key block visits (per head of its group): causal keeps the
-// blocks at or after it (128-row blocks on both sides), a window those up to
-// the last query that sees the block's last key, unless the block holds sinks.
-template <bool kWindow>
+// blocks at or after it (128-row blocks on both sides).
 __device__ __forceinline__ void q_range(const BwdParams& p, int j, int& q0, int& nq) {
-  q0 = kWindow || p.causal ? j : 0;
+  q0 = p.causal ? j : 0;
   nq = p.nkb - q0;
-  if (kWindow && j >= p.sink_blocks) nq = min(nq, (kBlk - 1 + p.window - 1) / kBlk + 1);
-}
-
-// What a CTA works on: the key block j of (batch, kv head) bg, and with a
-// window the part of the block's walk and its slot in `partial` (-1: the whole
-// walk, written as it is).  Heaviest key blocks first.
-struct Item {
-  int bg, j, part, parts, slot;
-};
-template <bool kWindow>
-__device__ __forceinline__ Item cta_item(const BwdParams& p) {
-  const int heads = p.B * p.KH;
-  int x = static_cast<int>(blockIdx.x);
-  if (!kWindow) return {x % heads, x / heads, 0, 1, -1};
-  const int sinks = p.sink_blocks * p.sink_parts * heads;
-  const bool sink = x < sinks;
-  const int parts = sink ? p.sink_parts : p.parts;
-  const int y = sink ? x : x - sinks;
-  const int slot = parts == 1 ? -1 : sink || p.sink_parts > 1 ? x : y;
-  const int bg = y % heads, r = y / heads;
-  return {bg, (sink ? 0 : p.sink_blocks) + r / parts, r % parts, parts, slot};
 }
 
 // Query block of step `it` (head it / nq of the group): each key block starts
@@ -168,7 +136,6 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   return v;
 }
 
-template <bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -195,17 +162,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   // heaviest key blocks first (causal: block j visits nkb - j query blocks)
-  const Item item = cta_item<kWindow>(p);
-  const int bg = item.bg, j = item.j;
+  const int bg = static_cast<int>(blockIdx.x) % (p.B * p.KH);
+  const int j = static_cast<int>(blockIdx.x) / (p.B * p.KH);
   const int b = bg / p.KH, g = bg - (bg / p.KH) * p.KH;
   int q0, nq;
-  q_range<kWindow>(p, j, q0, nq);
-  int n_iter = p.rep * nq;  // steps of the walk ...
-  int it0 = 0;              // ... from this one on
-  if (kWindow) {
-    it0 = static_cast<int>(static_cast<int64_t>(n_iter) * item.part / item.parts);
-    n_iter = static_cast<int>(static_cast<int64_t>(n_iter) * (item.part + 1) / item.parts) - it0;
-  }
+  q_range(p, j, q0, nq);
+  const int n_iter = p.rep * nq;
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -258,11 +220,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t q_issued = 0;  // Q buffers with a load in flight at the end
       for (int it = 0; it < n_iter && ok; ++it) {
         const uint32_t pprev = static_cast<uint32_t>(it - 1) & 1u;
-        const int h = g * p.rep + (it0 + it) / nq;
-        const int s0 = q_block(j, q0, nq, it0 + it) * kBlk;
+        const int h = g * p.rep + it / nq;
+        const int s0 = q_block(j, q0, nq, it) * kBlk;
         const int qb = it & 1;
-        const int64_t drow = (static_cast<int64_t>(b) * p.QH + h) * p.row_stride + s0;  // lse / di (dout) row
-        const int valid = !kWindow && p.S - s0 < kBlk ? p.S - s0 : kBlk;  // query rows of the block that lse, di have
+        const int64_t drow = (static_cast<int64_t>(b) * p.QH + h) * p.S + s0;  // dout / lse / di row
+        const int valid = p.S - s0 < kBlk ? p.S - s0 : kBlk;  // query rows of the block inside S
         const uint32_t vbytes = static_cast<uint32_t>(valid) * 4u;
         // Q_i into buffer i % 2 once dK of block i - 2 is done
         if (it >= 2) ok = mbar_wait(&q_free[qb], static_cast<uint32_t>((it >> 1) - 1) & 1u, err, kErrWaitEmpty);
@@ -281,10 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         mbar_arrive_expect_tx(do_full, kTile);
         for (int hh = 0; hh < 2; ++hh)
-          if (kWindow)
-            tma_load_4d(smem + Smem::kDO + hh * kHalf, &tmDO, do_full, hh * 64, h, s0, b);
-          else
-            tma_load_2d(smem + Smem::kDO + hh * kHalf, &tmDO, do_full, hh * 64, static_cast<int>(drow));
+          tma_load_2d(smem + Smem::kDO + hh * kHalf, &tmDO, do_full, hh * 64, static_cast<int>(drow));
         // di_i once the row warps are done with dS(i - 1)
         if (it >= 1) ok = mbar_wait(ds_ready, pprev, err, kErrWaitEmpty);
         if (!ok) break;
@@ -443,15 +402,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t prow = smem_u32(smem + Smem::kP) + static_cast<uint32_t>(kr * 128);
     const uint32_t dsrow = smem_u32(smem + Smem::kDS) + static_cast<uint32_t>(kr * 128);
     const uint32_t rsw = static_cast<uint32_t>(kr & 7);
-    // live queries of this key row: [qlo, qhi) -- from the key itself when causal,
-    // up to S or (a window, not a sink) the last query that sees it; none when
-    // the key is past S
-    const int qlo = kpos >= p.S ? p.S : (kWindow || p.causal ? kpos : 0);
-    const int qhi = kWindow && kpos >= p.sinks ? min(p.S, kpos + p.window) : p.S;
+    // live queries of this key row: [qlo, S) -- from the key itself when causal,
+    // none when the key is past S
+    const int qlo = kpos >= p.S ? p.S : (p.causal ? kpos : 0);
     bool ok = true;
     for (int it = 0; it < n_iter && ok; ++it) {
       const uint32_t par = static_cast<uint32_t>(it) & 1u;
-      const int s0 = q_block(j, q0, nq, it0 + it) * kBlk;
+      const int s0 = q_block(j, q0, nq, it) * kBlk;
       ok = mbar_wait(s_ready, par, err, kErrWaitAccum) && mbar_wait(lse_full, par, err, kErrWaitFull);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -464,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // [8u, 8u + 8) of a 64-query half = unit u).
       auto p_chunk = [&](const int k, const int odd, const uint32_t (&sv)[32]) {
         const int c = 2 * k + odd;
-        const uint32_t live = range_mask(qlo - s0 - c * 32, qhi - s0 - c * 32);
+        const uint32_t live = range_mask(qlo - s0 - c * 32, p.S - s0 - c * 32);
         float e[32];
 #pragma unroll
         for (int i4 = 0; i4 < 8; ++i4) {
@@ -507,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // masked entry (P = 0) stays 0 whatever di holds past S
       auto ds_chunk = [&](const int k, const int odd, const uint32_t (&dv)[32]) {
         const int c = 2 * k + odd;
-        const uint32_t live = range_mask(qlo - s0 - c * 32, qhi - s0 - c * 32);
+        const uint32_t live = range_mask(qlo - s0 - c * 32, p.S - s0 - c * 32);
         float w[32];
 #pragma unroll
         for (int u4 = 0; u4 < 4; ++u4) {
@@ -558,10 +515,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_warp(ds_ready);
     }
     // dV_j (group 0), dK_j (group 1; bf16, dK times the softmax scale) once
-    // every MMA is done (every key block visits at least one query block; a
-    // part of its walk may be empty)
-    const bool some = !kWindow || n_iter > 0;
-    if (ok && some) ok = mbar_wait(dkv_ready, 0u, err, kErrWaitAccum);
+    // every MMA is done (every key block visits at least one query block)
+    if (ok) ok = mbar_wait(dkv_ready, 0u, err, kErrWaitAccum);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
@@ -569,26 +524,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int which = grp;
         __nv_bfloat16* dst = (which == 0 ? p.dv : p.dk) +
                              ((static_cast<int64_t>(b) * p.S + kpos) * p.KH + g) * kD;
-        float* part = kWindow && item.slot >= 0
-                          ? p.partial + ((static_cast<int64_t>(item.slot) * 2 + which) * kBlk + kr) * kD
-                          : nullptr;
         const float f = which == 0 ? 1.f : p.scale;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t r[32];
-          if (some) {
-            tmem_ld_32x32b_x32(tmem + lane_base + 256 + which * 128 + c * 32, r);
-            tmem_ld_wait();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = 0u;
-          }
-          if (kWindow && part) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              reinterpret_cast<uint4*>(part + c * 32)[q] =
-                  make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-          } else if (kpos < p.S) {
+          tmem_ld_32x32b_x32(tmem + lane_base + 256 + which * 128 + c * 32, r);
+          tmem_ld_wait();
+          if (kpos < p.S) {
             uint4* o = reinterpret_cast<uint4*>(dst + c * 32);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -612,8 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int it = 0; it < n_iter && ok; ++it) {
       const uint32_t par = static_cast<uint32_t>(it) & 1u;
-      const int h = g * p.rep + (it0 + it) / nq;
-      const int s0 = q_block(j, q0, nq, it0 + it) * kBlk;
+      const int h = g * p.rep + it / nq;
+      const int s0 = q_block(j, q0, nq, it) * kBlk;
       ok = mbar_wait(dq_ready, par, err, kErrWaitAccum);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -673,34 +615,6 @@ kda_status tmap_bshd(CUtensorMap* m, const void* base, int64_t B, int64_t S, int
   return make_tmap_bf16(m, base, 4, dims, strides, box);
 }
 
-// Opt-ins of one instantiation (once per device), the kernel on a zeroed fp32
-// dq, and dq's conversion.
-template <bool kWindow>
-kda_status launch_bwd(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CUtensorMap& tdo,
-                      const BwdParams& p, __nv_bfloat16* dq, unsigned grid, cudaStream_t st) {
-  static std::atomic<bool> attr_set[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, attn_bwd_kernel<kWindow>) != cudaSuccess) return launch_status("attn_backward: attributes");
-    if (fa.numRegs < kRegsNeeded) {
-      set_error("attn_backward: kernel compiled to %d registers/thread, its register split needs %d", fa.numRegs,
-                kRegsNeeded);
-      return KDA_UNSUPPORTED;
-    }
-    if (cudaFuncSetAttribute(attn_bwd_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(Smem::kBytes)) != cudaSuccess)
-      return launch_status("attn_backward: cudaFuncSetAttribute");
-    attr_set[dev].store(true, std::memory_order_release);
-  }
-  attn_bwd_kernel<kWindow><<<grid, kThreads, Smem::kBytes, st>>>(tk, tv, tq, tdo, p, kda_err_ptr_attn_bwd());
-  KDA_BWD_TRY(launch_status("attn_bwd_kernel"));
-  const int64_t n8 = static_cast<int64_t>(p.B) * p.S * p.QH * kD / 8;
-  dq_to_bf16_kernel<<<static_cast<unsigned>((n8 + 255) / 256), 256, 0, st>>>(p.dq, dq, n8, p.S, p.QH, p.scale);
-  return launch_status("attn_backward: dq to bf16");
-}
-
 }  // namespace
 
 size_t attn_backward_scratch_bytes(int64_t B, int64_t S, int64_t QH) {
@@ -725,6 +639,8 @@ kda_status attn_backward_flash(const __nv_bfloat16* q, const __nv_bfloat16* k, c
     const uint32_t box[2] = {64, static_cast<uint32_t>(kBlk)};
     KDA_BWD_TRY(make_tmap_bf16(&tdo, dout, 2, dims, strides, box));
   }
+  if (cudaMemsetAsync(dq32, 0, attn_backward_scratch_bytes(B, S, QH), st) != cudaSuccess)
+    return launch_status("attn_backward: memset");
   BwdParams p{};
   p.B = static_cast<int>(B);
   p.S = static_cast<int>(S);
@@ -733,7 +649,6 @@ kda_status attn_backward_flash(const __nv_bfloat16* q, const __nv_bfloat16* k, c
   p.rep = static_cast<int>(QH / KH);
   p.nkb = static_cast<int>((S + kBlk - 1) / kBlk);
   p.causal = causal ? 1 : 0;
-  p.row_stride = p.S;
   p.scale = 1.0f / sqrtf(static_cast<float>(kD));
   p.sl2 = p.scale * 1.4426950408889634f;
   p.lse = lse;
@@ -741,189 +656,28 @@ kda_status attn_backward_flash(const __nv_bfloat16* q, const __nv_bfloat16* k, c
   p.dq = dq32;
   p.dk = dk;
   p.dv = dv;
-  if (cudaMemsetAsync(dq32, 0, attn_backward_scratch_bytes(B, S, QH), st) != cudaSuccess)
-    return launch_status("attn_backward: memset");
-  return launch_bwd<false>(tk, tv, tq, tdo, p, dq, static_cast<unsigned>(B * KH * p.nkb), st);
+  static std::atomic<bool> attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, attn_bwd_kernel) != cudaSuccess) return launch_status("attn_backward: attributes");
+    if (fa.numRegs < kRegsNeeded) {
+      set_error("attn_backward: kernel compiled to %d registers/thread, its register split needs %d", fa.numRegs,
+                kRegsNeeded);
+      return KDA_UNSUPPORTED;
+    }
+    if (cudaFuncSetAttribute(attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Smem::kBytes)) != cudaSuccess)
+      return launch_status("attn_backward: cudaFuncSetAttribute");
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  const unsigned grid = static_cast<unsigned>(B * KH * p.nkb);
+  attn_bwd_kernel<<<grid, kThreads, Smem::kBytes, st>>>(tk, tv, tq, tdo, p, kda_err_ptr_attn_bwd());
+  KDA_BWD_TRY(launch_status("attn_bwd_kernel"));
+  const int64_t n8 = B * S * QH * kD / 8;
+  dq_to_bf16_kernel<<<static_cast<unsigned>((n8 + 255) / 256), 256, 0, st>>>(dq32, dq, n8, p.S, p.QH, p.scale);
+  return launch_status("attn_backward: dq to bf16");
 }
 
 }  // namespace kda
-
-using namespace kda;
-
-// ------------------------------------------------- sliding window with sinks
-namespace kda {
-namespace {
-// di[b][h][s] = sum_d dout * out (fp32) and a copy of lse, both with rows
-// padded to whole query blocks (zeros) so that every block's 512 bytes load
-// aligned; and the zeros that dq's shares are added to.  dout, out
-// [B][S][QH][128]; 16 lanes per row, 8 values each.
-__global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* __restrict__ dout,
-                                                          const __nv_bfloat16* __restrict__ out,
-                                                          const float* __restrict__ lse, float* __restrict__ di,
-                                                          float* __restrict__ lse_pad, float* __restrict__ dq, int S,
-                                                          int SP, int QH) {
-  const int lane = threadIdx.x & 15;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);  // (s, h) of batch entry blockIdx.y
-  const int b = blockIdx.y;
-  const int h = static_cast<int>(i % QH);
-  const int s = static_cast<int>(i / QH);
-  const bool in = s < S;
-  float acc = 0.f;
-  if (in) {
-    const int64_t row = (static_cast<int64_t>(b) * S + s) * QH + h;
-    float fa[8], fb[8];
-    unpack_bf16x8(reinterpret_cast<const uint4*>(dout + row * kD)[lane], fa);
-    unpack_bf16x8(reinterpret_cast<const uint4*>(out + row * kD)[lane], fb);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fb[e], acc);
-    float4* z = reinterpret_cast<float4*>(dq + ((static_cast<int64_t>(b) * QH + h) * S + s) * kD);
-    z[lane] = z[lane + 16] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane == 0 && s < SP) {
-    const int64_t bh = static_cast<int64_t>(b) * QH + h;
-    di[bh * SP + s] = acc;
-    lse_pad[bh * SP + s] = in ? lse[bh * S + s] : 0.f;
-  }
-}
-
-// dk, dv of the key blocks whose walk was cut: the parts' fp32 sums added in
-// order, to bf16.  `first` is the slot of the first block's first part, the
-// parts of block `jb` and (batch, kv head) bg are heads slots apart.  Grid
-// (blocks x 8, heads, 2: dv, dk); 16 lanes per key row.
-__global__ void __launch_bounds__(256) join_parts_kernel(const BwdParams p, int j0, int first, int parts) {
-  const int heads = p.B * p.KH;
-  const int jb = blockIdx.x >> 3;
-  const int row = (blockIdx.x & 7) * 16 + (threadIdx.x >> 4);
-  const int bg = blockIdx.y, which = blockIdx.z;
-  const int lane = threadIdx.x & 15;
-  const int kpos = (j0 + jb) * kBlk + row;
-  if (kpos >= p.S) return;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
-  for (int i = 0; i < parts; ++i) {
-    const int64_t slot = first + (static_cast<int64_t>(jb) * parts + i) * heads + bg;
-    const float4* src = reinterpret_cast<const float4*>(p.partial + ((slot * 2 + which) * kBlk + row) * kD) + 2 * lane;
-    const float4 u = src[0], v = src[1];
-    a = make_float4(a.x + u.x, a.y + u.y, a.z + u.z, a.w + u.w);
-    c = make_float4(c.x + v.x, c.y + v.y, c.z + v.z, c.w + v.w);
-  }
-  const float f = which == 0 ? 1.f : p.scale;
-  const int b = bg / p.KH, g = bg - b * p.KH;
-  uint4* dst = reinterpret_cast<uint4*>((which == 0 ? p.dv : p.dk) +
-                                        ((static_cast<int64_t>(b) * p.S + kpos) * p.KH + g) * kD);
-  dst[lane] = make_uint4(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(a.z * f, a.w * f), pack_bf16x2(c.x * f, c.y * f),
-                         pack_bf16x2(c.z * f, c.w * f));
-}
-
-size_t al256(size_t n) { return (n + 255) & ~size_t(255); }
-int64_t padded_rows(int64_t S) { return (S + kBlk - 1) / kBlk * kBlk; }
-
-// How the key blocks' walks are cut.  A walk takes rep x (query blocks that see
-// the block) steps: the same few for most blocks, up to the whole sequence for
-// those with sinks.  With `fair` = the steps of all walks / SMs, no CTA should
-// take much more: sink walks are cut to the length of the others (8 steps at
-// least: a part costs its 128 KB of partial sums), and all walks to `fair`
-// where there are too few of them to fill the GPU.
-struct Cut {
-  int64_t nkb, sink_blocks, sink_parts, parts, slots, grid;
-};
-Cut cut_walks(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t window, int64_t sinks) {
-  Cut c{};
-  const int64_t rep = QH / KH, heads = B * KH;
-  c.nkb = padded_rows(S) / kBlk;
-  const int64_t nq = std::min(c.nkb, (kBlk - 1 + std::min(window, S) - 1) / kBlk + 1);
-  c.sink_blocks = nq == c.nkb ? 0 : std::min(c.nkb, (std::min(sinks, S) + kBlk - 1) / kBlk);
-  const int64_t rest = c.nkb - c.sink_blocks;  // their walks: nq, and nq - 1 .. 1 at the sequence's end
-  int64_t steps = c.sink_blocks * c.nkb - c.sink_blocks * (c.sink_blocks - 1) / 2;
-  steps += rest >= nq ? rest * nq - nq * (nq - 1) / 2 : rest * (rest + 1) / 2;
-  const int64_t fair = std::max<int64_t>(4, (steps * rep * heads + num_sms() - 1) / num_sms());
-  const int64_t usual = rep * nq;
-  c.parts = usual <= fair ? 1 : (usual + fair - 1) / fair;
-  const int64_t len = std::min(fair, std::max<int64_t>(8, usual));
-  c.sink_parts = c.sink_blocks ? (rep * c.nkb + len - 1) / len : 1;
-  const int64_t sink_items = c.sink_blocks * c.sink_parts * heads, items = rest * c.parts * heads;
-  c.grid = sink_items + items;
-  c.slots = (c.sink_parts > 1 ? sink_items : 0) + (c.parts > 1 ? items : 0);
-  return c;
-}
-}  // namespace
-}  // namespace kda
-
-extern "C" size_t kda_gqa_window_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
-                                                         int64_t window, int64_t sinks) {
-  if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || QH % KH || D != kD || window <= 0 || sinks < 0) return 0;
-  return 2 * al256(static_cast<size_t>(B) * QH * padded_rows(S) * 4) + attn_backward_scratch_bytes(B, S, QH) +
-         static_cast<size_t>(cut_walks(B, S, QH, KH, window, sinks).slots) * 2 * kBlk * kD * 4;
-}
-
-extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void* q, const void* k, const void* v,
-                                                   const void* out, const float* lse, void* dq, void* dk, void* dv,
-                                                   int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
-                                                   int64_t window, int64_t sinks, const int64_t* q_strides,
-                                                   const int64_t* k_strides, const int64_t* v_strides,
-                                                   void* workspace, size_t workspace_bytes, void* stream) {
-  const char* op = "gqa_window_backward";
-  KDA_BWD_TRY(gqa_window_check(op, B, S, QH, KH, D, window, sinks));
-  KDA_CHECK_ARG(dout && q && k && v && out && lse && dq && dk && dv && q_strides && k_strides && v_strides,
-                "%s: null pointer", op);
-  KDA_CHECK_SUPPORTED(B * KH <= 65535, "%s: too many kv heads (%lld)", op, (long long)(B * KH));
-  const int64_t dense_q[3] = {S * QH * kD, QH * kD, kD}, dense_k[3] = {S * KH * kD, KH * kD, kD};
-  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
-                          head_rows_ok(dout, dense_q) && head_rows_ok(out, dense_q) && head_rows_ok(dq, dense_q) &&
-                          head_rows_ok(dk, dense_k) && head_rows_ok(dv, dense_k),
-                      "%s: pointers and rows must be 16-byte aligned", op);
-  const size_t need = kda_gqa_window_backward_workspace_size(B, S, QH, KH, D, window, sinks);
-  KDA_CHECK_ARG(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes required, got %zu", op, need,
-                workspace_bytes);
-  KDA_CHECK_SUPPORTED((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "%s: workspace must be 16-byte aligned",
-                      op);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t SP = padded_rows(S);
-  uint8_t* w = static_cast<uint8_t*>(workspace);
-  const size_t rows = al256(static_cast<size_t>(B) * QH * SP * 4);
-  BwdParams p{};
-  float* di = reinterpret_cast<float*>(w);
-  float* lse_pad = reinterpret_cast<float*>(w + rows);
-  p.dq = reinterpret_cast<float*>(w + 2 * rows);
-  window_rows_kernel<<<dim3(static_cast<unsigned>((SP * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
-      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, di, lse_pad, p.dq,
-      static_cast<int>(S), static_cast<int>(SP), static_cast<int>(QH));
-  KDA_BWD_TRY(launch_status("gqa_window_backward: rows"));
-  CUtensorMap tk, tv, tq, tdo;
-  KDA_BWD_TRY(tmap_head_rows(&tk, k, B, S, KH, k_strides[0], k_strides[1], k_strides[2]));
-  KDA_BWD_TRY(tmap_head_rows(&tv, v, B, S, KH, v_strides[0], v_strides[1], v_strides[2]));
-  KDA_BWD_TRY(tmap_head_rows(&tq, q, B, S, QH, q_strides[0], q_strides[1], q_strides[2]));
-  KDA_BWD_TRY(tmap_head_rows(&tdo, dout, B, S, QH, dense_q[0], dense_q[1], dense_q[2]));
-  p.B = static_cast<int>(B);
-  p.S = static_cast<int>(S);
-  p.QH = static_cast<int>(QH);
-  p.KH = static_cast<int>(KH);
-  p.rep = static_cast<int>(QH / KH);
-  const Cut cut = cut_walks(B, S, QH, KH, window, sinks);
-  KDA_CHECK_SUPPORTED(cut.grid < (1ll << 31), "%s: too many key blocks (%lld)", op, (long long)cut.grid);
-  p.nkb = static_cast<int>(cut.nkb);
-  p.sink_blocks = static_cast<int>(cut.sink_blocks);
-  p.sink_parts = static_cast<int>(cut.sink_parts);
-  p.parts = static_cast<int>(cut.parts);
-  p.partial = p.dq + attn_backward_scratch_bytes(B, S, QH) / 4;
-  p.causal = 1;
-  p.window = static_cast<int>(window < S ? window : S);
-  p.sinks = static_cast<int>(sinks < S ? sinks : S);
-  p.row_stride = static_cast<int>(SP);
-  p.scale = 1.0f / sqrtf(static_cast<float>(kD));
-  p.sl2 = p.scale * 1.4426950408889634f;
-  p.lse = lse_pad;
-  p.di = di;
-  p.dk = static_cast<__nv_bfloat16*>(dk);
-  p.dv = static_cast<__nv_bfloat16*>(dv);
-  KDA_BWD_TRY(launch_bwd<true>(tk, tv, tq, tdo, p, static_cast<__nv_bfloat16*>(dq), static_cast<unsigned>(cut.grid),
-                               st));
-  const unsigned heads = static_cast<unsigned>(B * KH);
-  if (p.sink_parts > 1)
-    join_parts_kernel<<<dim3(static_cast<unsigned>(p.sink_blocks) * 8, heads, 2), 256, 0, st>>>(p, 0, 0, p.sink_parts);
-  if (p.parts > 1)
-    join_parts_kernel<<<dim3(static_cast<unsigned>(p.nkb - p.sink_blocks) * 8, heads, 2), 256, 0, st>>>(
-        p, p.sink_blocks, p.sink_parts > 1 ? p.sink_blocks * p.sink_parts * static_cast<int>(heads) : 0, p.parts);
-  return launch_status("gqa_window_backward: join");
-}

@@ -1,0 +1,1136 @@
+// Backward of the sliding-window attention with sinks (head_dim 128, bf16) on
+// tcgen05: P and dS live on chip, one 128 x 128 block at a time.
+//
+// Query i sees key j <= i where i - j < window or j < sinks.  With
+//   P = 2^(Q K^T scale log2e - lse),  dP = dO V^T,  dS = P (dP - di),
+//   di = rowsum(dO * O)
+// two kernels compute, block by block,
+//   window_dkv_kernel  dV_j = sum P^T dO, dK_j = scale sum dS^T Q over the query
+//                      blocks (of all heads of the group) that see key block j
+//   window_dq_kernel   dQ_i = scale sum dS K over the key blocks that query
+//                      block i sees
+// Each sum stays in TMEM until it is whole, so nothing is added through global
+// memory, and the results do not depend on timing.  S and dP are computed twice
+// (7 products a block pair instead of 5): with one kernel that adds dQ into an
+// fp32 buffer the L2 took the additions at 2.3 TB/s (64 KB a block pair,
+// red.global and bulk reductions alike), which bound it: 172 us at S4096 W1024
+// of 16 heads, 189 us with bulk reductions, against the figure at the launch.
+//
+// Both kernels: 640 threads -- warp 0 TMA producer, warp 1 TMEM allocator + MMA
+// issuer, warp 2 scheduler (performs every mbarrier wait the issuer needs and
+// releases it group by group at a named barrier: an mbarrier wait in the
+// issuing thread would stall behind its queued MMAs), warp 3 idle, warps 4-19
+// row warps: warp w reads TMEM lanes 32 (w % 4), columns 32 ((w - 4) / 4), i.e.
+// 32 values of one row per thread, four warps on each SM partition to cover
+// each other's latencies.  Operand tiles are two 16 KB halves of 64 columns,
+// 128-byte rows, 128-byte swizzle, loaded once and read K-major where their rows
+// index M or N and MN-major where their rows index K.  Both are bound by shared memory: 64 KB of MMA operands per
+// product at 128 B/clk.
+// All mbarrier waits are bounded (common.cuh); every TMA load targets one CTA.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+KDA_DEFINE_ERROR_WORD(window_bwd)
+
+#define KDA_WB_TRY(expr)                  \
+  do {                                    \
+    const kda_status s_ = (expr);         \
+    if (s_ != KDA_OK) return s_;          \
+  } while (0)
+
+namespace kda {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kBlk = 128;
+constexpr uint32_t kTile = kBlk * kD * 2;  // 32 KB
+constexpr uint32_t kHalf = kTile / 2;
+constexpr int kRowWarps = 16;
+constexpr int kThreads = 128 + 32 * kRowWarps;
+constexpr int kRowThreads = 32 * kRowWarps;
+constexpr int kGoBarrier = 1;   // named barrier: scheduler warp + MMA warp
+constexpr int kRowsBarrier = 6;  // all row warps; 2 .. 5: the four warps of one column group
+
+struct BwdParams {
+  int B, S, QH, KH, rep;
+  int nkb;            // key (and query) blocks per sequence
+  int nq;             // query blocks that see a key block without sinks (fewer at the sequence's end)
+  int window, sinks;
+  int sink_blocks;    // key blocks that hold sinks: every later query block visits them
+  int sp;             // rows per (b, h) of nlse and ndi: S rounded up to whole blocks
+  int64_t steps;      // dkv: steps of the walks of one (batch, kv head)
+  int64_t total;      // of all
+  float sl2;          // softmax scale * log2(e)
+  float scale;
+  const float* nlse;  // [B][QH][sp]: -lse
+  const float* ndi;   // [B][QH][sp]: -rowsum(dout * out)
+  float* partial;     // [2 x CTAs][2][128 d][128 keys] fp32: dV_j, dK_j (unscaled) of cut walks
+  int4* pieces;       // [2 x CTAs] beside them: (batch, kv head), j, steps of the share, of the walk
+  __nv_bfloat16* dk;  // [B][S][KH][128], for the join
+  __nv_bfloat16* dv;
+};
+
+// Seven tiles, then small things.
+struct Smem {
+  // dkv: K_j | V_j | Q (two buffers) | dO | P^T | dS^T
+  // dq:  Q | dO | K (three buffers) | V | dS
+  static constexpr uint32_t kLse = 7 * kTile;             // dkv: 128 floats
+  static constexpr uint32_t kDi = kLse + 512;             // dkv: 128 floats
+  static constexpr uint32_t kBars = kDi + 512;
+  static constexpr uint32_t kNumBars = 24;
+  static constexpr uint32_t kFirst = kBars + kNumBars * 8;  // dkv: the run's first piece and its length
+  static constexpr size_t kBytes = 1024 + kFirst + 32;
+  static_assert(kBytes > 116 * 1024 && kBytes <= 227 * 1024, "shared memory budget");
+};
+
+// Steps before key block j's walk in its (batch, kv head).
+__host__ __device__ __forceinline__ int64_t steps_before(int64_t nkb, int64_t sink_blocks, int64_t nq, int64_t rep,
+                                                         int64_t j) {
+  const int64_t a = j < sink_blocks ? j : sink_blocks;          // walks of nkb - j blocks
+  int64_t n = a * nkb - a * (a - 1) / 2;
+  int64_t full = nkb - nq + 1 - sink_blocks;                    // walks of nq blocks
+  if (full < 0) full = 0;
+  const int64_t r = j - a, r1 = r < full ? r : full, r2 = r - r1;
+  n += r1 * nq + r2 * (nkb - sink_blocks - full) - r2 * (r2 - 1) / 2;  // the last ones: to the sequence's end
+  return n * rep;
+}
+
+// A piece of a CTA's run: steps [it0, it0 + n) of the walk of key block j of
+// (batch, kv head) bg, which has `walk` steps, nq for each head.
+struct Piece {
+  int bg, j, it0, n, walk, nq;
+};
+__device__ __forceinline__ int blocks_that_see(const BwdParams& p, int j) {
+  return j < p.sink_blocks ? p.nkb - j : min(p.nq, p.nkb - j);
+}
+// The piece at step x of the concatenated walks (x < total), of at most `most` steps.
+__device__ __forceinline__ Piece piece_at(const BwdParams& p, int64_t x, int64_t most) {
+  Piece c;
+  c.bg = static_cast<int>(x / p.steps);
+  const int64_t y = x - c.bg * p.steps;
+  int lo = 0, hi = p.nkb;  // the last key block whose walk starts at or before y
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (steps_before(p.nkb, p.sink_blocks, p.nq, p.rep, mid) <= y) lo = mid;
+    else hi = mid;
+  }
+  c.j = lo;
+  c.nq = blocks_that_see(p, lo);
+  c.walk = p.rep * c.nq;
+  c.it0 = static_cast<int>(y - steps_before(p.nkb, p.sink_blocks, p.nq, p.rep, lo));
+  c.n = static_cast<int>(min(most, static_cast<int64_t>(c.walk - c.it0)));
+  return c;
+}
+// The piece after c, of at most `most` steps: the next walk from its start.
+__device__ __forceinline__ Piece piece_after(const BwdParams& p, const Piece& c, int most) {
+  Piece d;
+  d.j = c.j + 1;
+  d.bg = c.bg;
+  if (d.j == p.nkb) {
+    d.j = 0;
+    ++d.bg;
+  }
+  d.nq = blocks_that_see(p, d.j);
+  d.walk = p.rep * d.nq;
+  d.it0 = 0;
+  d.n = min(most, d.walk);
+  return d;
+}
+__device__ __forceinline__ int64_t run_start(const BwdParams& p, int cta, int ctas) { return p.total * cta / ctas; }
+// Head and query block of step `it` of a walk.
+__device__ __forceinline__ int step_head(const BwdParams& p, int g, const Piece& c, int it) {
+  return g * p.rep + it / c.nq;
+}
+__device__ __forceinline__ int step_block(const Piece& c, int it) { return c.j + it % c.nq; }
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// 32 values of a row as bf16 into a K-major, 128-byte-swizzled half tile: columns
+// [8u, 8u + 8) of the half = 16-byte unit u, at u ^ (row % 8); u0 the first unit.
+__device__ __forceinline__ void store32(uint32_t row, int u0, uint32_t rsw, const float2 (&e)[16]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    st_shared_v4(row + ((static_cast<uint32_t>(u0 + u) ^ rsw) << 4), pack_bf16x2(e[4 * u].x, e[4 * u].y),
+                 pack_bf16x2(e[4 * u + 1].x, e[4 * u + 1].y), pack_bf16x2(e[4 * u + 2].x, e[4 * u + 2].y),
+                 pack_bf16x2(e[4 * u + 3].x, e[4 * u + 3].y));
+}
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// The same, returning the AND of every thread's `ok`.  Named barriers have no
+// time limit, so a warp whose bounded wait expired still joins the next one of
+// its group, with false, and all of them stop there together.
+__device__ __forceinline__ bool bar_and(int id, int threads, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.and.pred p, %2, %3, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(ok ? 1u : 0u), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+// Every committed bulk store of this thread has read its shared memory.
+__device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, const void* src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+
+// Bits [a, b) of a 32-bit word (empty when a >= b); a, b may lie outside [0, 32].
+__device__ __forceinline__ uint32_t range_mask(int a, int b) {
+  a = a < 0 ? 0 : a;
+  b = b > 32 ? 32 : b;
+  if (a >= b) return 0u;
+  const uint32_t hi = b >= 32 ? 0xffffffffu : ((1u << b) - 1u);
+  return hi & ~((1u << a) - 1u);
+}
+
+// Bounded wait at the end, also after an error elsewhere: what is in flight
+// must land before shared memory and TMEM go.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > kWaitLimitNs) return;
+}
+
+// Values of hidden pairs become exactly zero: pair i of e is live where bits
+// 2i and 2i + 1 of `live` are set.
+__device__ __forceinline__ void keep_live(uint32_t live, float2 (&e)[16]) {
+  if (live != 0xffffffffu) {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      e[q].x = (live >> (2 * q)) & 1u ? e[q].x : 0.f;
+      e[q].y = (live >> (2 * q + 1)) & 1u ? e[q].y : 0.f;
+    }
+  }
+}
+
+constexpr uint32_t kIdKK = idesc_bf16_f32(kBlk, kBlk, 0, 0);  // K-major A, K-major B
+constexpr uint32_t kIdKM = idesc_bf16_f32(kBlk, kBlk, 0, 1);  // K-major A, MN-major B
+// Descriptors of a tile read K-major (rows = M or N, 64-element halves along K:
+// K step kk at (kk / 4) halves + (kk % 4) x 32 bytes) and MN-major (rows = K: K
+// step kk at kk x 16 rows x 128 bytes, the two 64-element MN atoms 16 KB apart).
+__device__ __forceinline__ uint64_t kmajor(uint32_t tile) { return smem_desc_sw128(tile, 16, 1024); }
+__device__ __forceinline__ uint64_t mnmajor(uint32_t tile) { return smem_desc_sw128(tile, kHalf, 1024); }
+__device__ __forceinline__ uint64_t kmajor_step(int kk) {
+  return static_cast<uint64_t>(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4);
+}
+__device__ __forceinline__ uint64_t mnmajor_step(int kk) { return static_cast<uint64_t>(kk * 128); }
+// D (+)= A B^T with both read K-major, and D (+)= A B with A K-major, B MN-major: 128 x 128 x 128
+__device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t b) {
+  const uint64_t da = kmajor(a), db = kmajor(b);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) umma_bf16(d, da + kmajor_step(kk), db + kmajor_step(kk), kIdKK, kk != 0 ? 1u : 0u);
+}
+__device__ __forceinline__ void mma_km(uint32_t d, uint32_t a, uint32_t b, bool first) {
+  const uint64_t da = kmajor(a), db = mnmajor(b);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    umma_bf16(d, da + kmajor_step(kk), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
+}
+// 128 rows x 128 columns as two halves
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int head, int row, int b) {
+  tma_load_4d(dst, m, bar, 0, head, row, b);
+  tma_load_4d(dst + kHalf, m, bar, 64, head, row, b);
+}
+
+// One thread of the scheduler waits for up to three barriers, then both warps
+// meet; false once any wait has expired.
+__device__ __forceinline__ bool sched_wait(unsigned* err, uint64_t* b1, uint32_t p1, uint64_t* b2 = nullptr,
+                                           uint32_t p2 = 0u, uint64_t* b3 = nullptr, uint32_t p3 = 0u) {
+  bool good = true;
+  if ((threadIdx.x & 31) == 0) {
+    good = mbar_wait(b1, p1, err, kErrWaitFull);
+    if (good && b2) good = mbar_wait(b2, p2, err, kErrWaitFull);
+    if (good && b3) good = mbar_wait(b3, p3, err, kErrWaitAccumFree);
+  }
+  return go_barrier64<kGoBarrier>(__shfl_sync(0xffffffffu, good, 0));
+}
+
+// ---------------------------------------------------------------- dK and dV
+// A step is one (head, query block) of a key block's walk.  A walk is short for
+// most blocks (rep x the blocks of the window) and as long as the sequence for
+// those with sinks, and there may be few walks, so the CTAs (one per SM,
+// persistent) each take an equal run of the concatenated walks.  Where a run
+// cuts a walk, its dV_j and dK_j are fp32 partial sums that window_join_kernel
+// adds in order.
+//   S^T = K_j Q^T, P^T (row warps, key rows; 32 queries per thread, kept in
+//   registers as fp32, bf16 into a tile), dP^T = V_j dO^T, dV_j += P^T dO,
+//   dS^T = P^T (dP^T - di) (from the unrounded P^T, into a tile of its own),
+//   dK_j += dS^T Q
+// Issue order per step n: dV(n) S(n+1) | dK(n) | dP(n+1), the first two groups
+// released when the row warps have written their operand and read their
+// columns, the last when dO has been replaced.
+// TMEM columns: S^T [0,128), dP^T [128,256), dV [256,384), dK [384,512).
+__global__ void __launch_bounds__(kThreads, 1)
+    window_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                      const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV,
+                      const BwdParams p, unsigned* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kDO = 4 * kTile, kP = 5 * kTile, kDS = 6 * kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
+  // one phase per piece
+  uint64_t* k_full = bars + 0;      // K_j landed
+  uint64_t* v_full = bars + 1;      // V_j landed
+  uint64_t* dkv_ready = bars + 2;   // every MMA of the piece done: dV_j, dK_j final
+  uint64_t* acc_free = bars + 3;    // dV_j, dK_j read out of TMEM (16 warps)
+  // one phase per step n of the run ([2]: per use of buffer n % 2)
+  uint64_t* q_full = bars + 4;      // [2] Q landed
+  uint64_t* q_free = bars + 6;      // [2] dK(n) done: Q and dS^T read
+  uint64_t* do_full = bars + 8;     // dO landed
+  uint64_t* do_free = bars + 9;     // dV(n) done: dO and P^T read
+  uint64_t* lse_full = bars + 12;   // nlse landed (loaded once the row warps wrote P(n - 1))
+  uint64_t* di_full = bars + 13;    // ndi landed (loaded once the row warps wrote dS(n - 1))
+  uint64_t* s_ready = bars + 14;    // S^T(n) in TMEM
+  uint64_t* dp_ready = bars + 15;   // dP^T(n) in TMEM
+  uint64_t* p_ready = bars + 16;    // P^T(n) in its tile, S^T(n) read out (16 warps)
+  uint64_t* ds_ready = bars + 17;   // dS^T(n) in its tile, dP^T(n) read out (16 warps)
+  uint64_t* drain = bars + 18;      // once
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 19);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 19; ++i)
+      mbar_init(bars + i, i == 3 || i == 16 || i == 17 ? kRowWarps : 1);
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmDO);
+    tma_prefetch_desc(&tmDK);
+    tma_prefetch_desc(&tmDV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  int* first_s = reinterpret_cast<int*>(smem + Smem::kFirst);
+  if (warp == 3 && lane == 0) {
+    const int64_t x = run_start(p, blockIdx.x, gridDim.x), end = run_start(p, blockIdx.x + 1, gridDim.x);
+    const Piece c = piece_at(p, x, end - x);
+    first_s[0] = c.bg, first_s[1] = c.j, first_s[2] = c.it0, first_s[3] = c.n, first_s[4] = c.walk, first_s[5] = c.nq;
+    first_s[6] = static_cast<int>(end - x);
+    // no cut walk starts here, unless the row warps say so
+    if (c.it0 > 0 || c.n == c.walk) p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  // every role walks the run's pieces; n0: steps of the earlier ones
+  Piece c = {first_s[0], first_s[1], first_s[2], first_s[3], first_s[4], first_s[5]};
+  const int run = first_s[6];
+  int n0 = 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      bool ok = true;
+      int ks = 0, vs = 0, qs = 0, dos = 0, lses = 0, dis = 0;  // loads issued
+      while (ok) {
+        const int b = c.bg / p.KH, g = c.bg - b * p.KH;
+        for (int i = 0; i < c.n; ++i) {
+          const int n = n0 + i;
+          const uint32_t pprev = static_cast<uint32_t>(n - 1) & 1u;
+          const uint32_t use = static_cast<uint32_t>((n >> 1) - 1) & 1u;  // phase of step n - 2 in its buffer
+          const int h = step_head(p, g, c, c.it0 + i);
+          const int s0 = step_block(c, c.it0 + i) * kBlk;
+          const int nb = n & 1;
+          const int64_t row = (static_cast<int64_t>(b) * p.QH + h) * p.sp + s0;
+          if (n >= 2) ok = mbar_wait(&q_free[nb], use, err, kErrWaitEmpty);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&q_full[nb], kTile);
+          load_tile(smem + kQ + nb * kTile, &tmQ, &q_full[nb], h, s0, b);
+          ++qs;
+          if (i == 0) {
+            // K_j once the previous piece's last S is done, V_j once its last dP is
+            if (n > 0) ok = mbar_wait(s_ready, pprev, err, kErrWaitEmpty);
+            if (!ok) break;
+            mbar_arrive_expect_tx(k_full, kTile);
+            load_tile(smem + kK, &tmK, k_full, g, c.j * kBlk, b);
+            ++ks;
+            if (n > 0) ok = mbar_wait(dp_ready, pprev, err, kErrWaitEmpty);
+            if (!ok) break;
+            mbar_arrive_expect_tx(v_full, kTile);
+            load_tile(smem + kV, &tmV, v_full, g, c.j * kBlk, b);
+            ++vs;
+          }
+          if (n == 0) pdl_wait();  // nlse, ndi are written by the launch before this one
+          if (n >= 1) ok = mbar_wait(p_ready, pprev, err, kErrWaitEmpty);
+          if (!ok) break;
+          mbar_arrive_expect_tx(lse_full, kBlk * 4);
+          bulk_load_1d(smem + Smem::kLse, p.nlse + row, kBlk * 4, lse_full);
+          ++lses;
+          if (n >= 1) ok = mbar_wait(do_free, pprev, err, kErrWaitEmpty);
+          if (!ok) break;
+          mbar_arrive_expect_tx(do_full, kTile);
+          load_tile(smem + kDO, &tmDO, do_full, h, s0, b);
+          ++dos;
+          if (n >= 1) ok = mbar_wait(ds_ready, pprev, err, kErrWaitEmpty);
+          if (!ok) break;
+          mbar_arrive_expect_tx(di_full, kBlk * 4);
+          bulk_load_1d(smem + Smem::kDi, p.ndi + row, kBlk * 4, di_full);
+          ++dis;
+        }
+        n0 += c.n;
+        if (n0 >= run) break;
+        c = piece_after(p, c, run - n0);
+      }
+      // no copy may still be writing shared memory when the CTA exits
+      if (ks > 0) mbar_drain(k_full, static_cast<uint32_t>(ks - 1) & 1u);
+      if (vs > 0) mbar_drain(v_full, static_cast<uint32_t>(vs - 1) & 1u);
+      if (lses > 0) mbar_drain(lse_full, static_cast<uint32_t>(lses - 1) & 1u);
+      if (dis > 0) mbar_drain(di_full, static_cast<uint32_t>(dis - 1) & 1u);
+      if (dos > 0) mbar_drain(do_full, static_cast<uint32_t>(dos - 1) & 1u);
+      for (int t = 0; t < 2; ++t) {
+        const int uses = (qs + 1 - t) >> 1;
+        if (uses > 0) mbar_drain(&q_full[t], static_cast<uint32_t>(uses - 1) & 1u);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1 || warp == 2) {
+    // ------------------------------------------------ MMA issuer / scheduler
+    // Both warps walk the same groups and meet at the go barrier before each.
+    const bool sched = warp == 2;
+    const uint32_t base = smem_u32(smem);
+    bool ok = true, any = false;
+    int pieces = 0;
+    while (ok) {
+      // S^T and dP^T of the piece's first step (their columns were read before
+      // the last piece's dK was issued)
+      {
+        const uint32_t pp = static_cast<uint32_t>(pieces) & 1u, nb = static_cast<uint32_t>(n0) & 1u;
+        const uint32_t use = static_cast<uint32_t>(n0 >> 1) & 1u;
+        ok = sched ? sched_wait(err, k_full, pp, &q_full[nb], use) : go_barrier64<kGoBarrier>(true);
+        if (!ok) break;
+        if (!sched && lane == 0) {
+          tc_fence_after();
+          mma_kk(tmem, base + kK, base + kQ + nb * kTile);
+          umma_commit(s_ready);
+          any = true;
+        }
+        __syncwarp();
+        ok = sched ? sched_wait(err, v_full, pp, do_full, nb) : go_barrier64<kGoBarrier>(true);
+        if (!ok) break;
+        if (!sched && lane == 0) {
+          tc_fence_after();
+          mma_kk(tmem + 128, base + kV, base + kDO);
+          umma_commit(dp_ready);
+        }
+        __syncwarp();
+      }
+      for (int i = 0; i < c.n; ++i) {
+        const int n = n0 + i;
+        const uint32_t par = static_cast<uint32_t>(n) & 1u, nb = par, ob = par ^ 1u;
+        const uint32_t use = static_cast<uint32_t>((n + 1) >> 1) & 1u;
+        const bool more = i + 1 < c.n;
+        // dV_j += P^T(n) dO(n) (the first of a piece once the last piece's sums
+        // are read), S^T(n + 1)
+        ok = sched ? sched_wait(err, p_ready, par, more ? &q_full[ob] : nullptr, use,
+                                i == 0 && pieces > 0 ? acc_free : nullptr, static_cast<uint32_t>(pieces - 1) & 1u)
+                   : go_barrier64<kGoBarrier>(true);
+        if (!ok) break;
+        if (!sched && lane == 0) {
+          tc_fence_after();
+          mma_km(tmem + 256, base + kP, base + kDO, i == 0);
+          umma_commit(do_free);
+          if (more) {
+            mma_kk(tmem, base + kK, base + kQ + ob * kTile);
+            umma_commit(s_ready);
+          }
+        }
+        __syncwarp();
+        // dK_j += dS^T(n) Q(n)
+        ok = sched ? sched_wait(err, ds_ready, par) : go_barrier64<kGoBarrier>(true);
+        if (!ok) break;
+        if (!sched && lane == 0) {
+          tc_fence_after();
+          mma_km(tmem + 384, base + kDS, base + kQ + nb * kTile, i == 0);
+          umma_commit(&q_free[nb]);
+          if (!more) umma_commit(dkv_ready);
+        }
+        __syncwarp();
+        // dP^T(n + 1)
+        if (more) {
+          ok = sched ? sched_wait(err, do_full, ob) : go_barrier64<kGoBarrier>(true);
+          if (!ok) break;
+          if (!sched && lane == 0) {
+            tc_fence_after();
+            mma_kk(tmem + 128, base + kV, base + kDO);
+            umma_commit(dp_ready);
+          }
+          __syncwarp();
+        }
+      }
+      n0 += c.n;
+      ++pieces;
+      if (n0 >= run) break;
+      c = piece_after(p, c, run - n0);
+    }
+    if (!sched && lane == 0 && any) {
+      // every issued MMA must finish before TMEM is released
+      umma_commit(drain);
+      mbar_drain(drain, 0u);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------- row warps
+    const int grp = (warp - 4) >> 2;        // queries [32 grp, + 32) of the block
+    const int kr = (warp & 3) * 32 + lane;  // key row of this thread (TMEM lane)
+    const uint32_t col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float4* nlse_s = reinterpret_cast<const float4*>(smem + Smem::kLse) + 8 * grp;
+    const float4* ndi_s = reinterpret_cast<const float4*>(smem + Smem::kDi) + 8 * grp;
+    const uint32_t prow = smem_u32(smem + kP) + static_cast<uint32_t>(kr * 128) + (grp >> 1) * kHalf;
+    const uint32_t dsrow = smem_u32(smem + kDS) + static_cast<uint32_t>(kr * 128) + (grp >> 1) * kHalf;
+    const int u0 = (grp & 1) * 4;
+    const uint32_t rsw = static_cast<uint32_t>(kr & 7);
+    const float2 sl2 = make_float2(p.sl2, p.sl2);
+    bool ok = true;
+    int pieces = 0;
+    while (ok) {
+      const int kpos = c.j * kBlk + kr;
+      // live queries of this key row: from the key itself up to the last that
+      // sees it; none when the key is past S
+      const int qlo = kpos >= p.S ? p.S : kpos;
+      const int qhi = kpos < p.sinks ? p.S : min(p.S, kpos + p.window);
+      for (int i = 0; i < c.n; ++i) {
+        const int n = n0 + i;
+        const uint32_t par = static_cast<uint32_t>(n) & 1u;
+        const int s0 = step_block(c, c.it0 + i) * kBlk + 32 * grp;  // this thread's first query
+        const uint32_t live = range_mask(qlo - s0, qhi - s0);
+        ok = mbar_wait(s_ready, par, err, kErrWaitAccum) && mbar_wait(lse_full, par, err, kErrWaitFull);
+        if (i == 0 && pieces > 0) {  // the last piece's dV, dK have left the tile
+          if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
+          ok = bar_and(kRowsBarrier, kRowThreads, ok);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        float2 e[16];  // P^T: 2^(s scale log2e - lse[q])
+        {
+          uint32_t s[32];
+          tmem_ld_32x32b_x32(col + 32 * grp, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 l = nlse_s[q];
+            const float2 a = __ffma2_rn(make_float2(__uint_as_float(s[4 * q]), __uint_as_float(s[4 * q + 1])), sl2,
+                                        make_float2(l.x, l.y));
+            const float2 b = __ffma2_rn(make_float2(__uint_as_float(s[4 * q + 2]), __uint_as_float(s[4 * q + 3])), sl2,
+                                        make_float2(l.z, l.w));
+            e[2 * q] = make_float2(exp2_approx(a.x), exp2_approx(a.y));
+            e[2 * q + 1] = make_float2(exp2_approx(b.x), exp2_approx(b.y));
+          }
+        }
+        keep_live(live, e);
+        // the tile is free once dV(n - 1) is done
+        if (n > 0) ok = mbar_wait(do_free, par ^ 1u, err, kErrWaitEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        store32(prow, u0, rsw, e);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive_warp(p_ready);
+        // dS^T = P^T (dP^T - di[q])
+        ok = mbar_wait(dp_ready, par, err, kErrWaitAccum) && mbar_wait(di_full, par, err, kErrWaitFull);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        {
+          uint32_t d[32];
+          tmem_ld_32x32b_x32(col + 128 + 32 * grp, d);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 l = ndi_s[q];
+            e[2 * q] = __fmul2_rn(e[2 * q], __fadd2_rn(make_float2(__uint_as_float(d[4 * q]), __uint_as_float(d[4 * q + 1])),
+                                                       make_float2(l.x, l.y)));
+            e[2 * q + 1] =
+                __fmul2_rn(e[2 * q + 1], __fadd2_rn(make_float2(__uint_as_float(d[4 * q + 2]), __uint_as_float(d[4 * q + 3])),
+                                                    make_float2(l.z, l.w)));
+          }
+        }
+        keep_live(live, e);
+        // the tile is free once dK(n - 1) is done
+        if (n > 0) ok = mbar_wait(&q_free[par ^ 1u], static_cast<uint32_t>((n - 1) >> 1) & 1u, err, kErrWaitEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        store32(dsrow, u0, rsw, e);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive_warp(ds_ready);
+      }
+      // dV_j (groups 0, 1) and dK_j (2, 3), 64 columns a thread, once the piece's
+      // MMAs are done: bf16 (dK times the softmax scale), or the fp32 share of a
+      // cut walk
+      if (ok) ok = mbar_wait(dkv_ready, static_cast<uint32_t>(pieces) & 1u, err, kErrWaitAccum);
+      ok = bar_and(kRowsBarrier, kRowThreads, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const bool cut = c.n < c.walk;
+      const int which = grp >> 1;
+      const int slot = 2 * static_cast<int>(blockIdx.x) + (c.it0 == 0 ? 1 : 0);
+      // [slot][dV, dK][d][key]: a warp writes 32 keys of one d, a 128-byte line
+      float* part = p.partial + ((static_cast<int64_t>(slot) * 2 + which) * kD + (grp & 1) * 64) * kBlk + kr;
+      if (cut && warp == 4 && lane == 0) p.pieces[slot] = make_int4(c.bg, c.j, c.n, c.walk);
+      const float f1 = which == 0 ? 1.f : p.scale;
+      const float2 f = make_float2(f1, f1);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(col + 256 + grp * 64 + half * 32, r);
+        tmem_ld_wait();
+        if (half == 1) {
+          tc_fence_before();
+          mbar_arrive_warp(acc_free);
+        }
+        if (cut) {
+#pragma unroll
+          for (int q = 0; q < 32; ++q) part[(half * 32 + q) * kBlk] = __uint_as_float(r[q]);
+        } else {
+          // 32 columns at a time through this group's quarter of P^T's tile (64-byte
+          // rows, 64-byte swizzle), whose MMAs are done, and out by TMA (rows past
+          // S are not written)
+          if (half == 1) {
+            if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
+            bar_sync(2 + grp, 128);
+          }
+          const uint32_t out = smem_u32(smem + kP) + grp * (kTile / 4) + static_cast<uint32_t>(kr * 64);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 v = __fmul2_rn(
+                  make_float2(__uint_as_float(r[8 * u + 2 * k]), __uint_as_float(r[8 * u + 2 * k + 1])), f);
+              w[k] = pack_bf16x2(v.x, v.y);
+            }
+            st_shared_v4(out + ((static_cast<uint32_t>(u) ^ ((kr >> 1) & 3u)) << 4), w[0], w[1], w[2], w[3]);
+          }
+          fence_proxy_async_smem();
+          bar_sync(2 + grp, 128);
+          if ((threadIdx.x & 127) == 0) {
+            const int b = c.bg / p.KH, g = c.bg - b * p.KH;
+            tma_store_4d(which == 0 ? &tmDV : &tmDK, smem + kP + grp * (kTile / 4), (grp & 1) * 64 + half * 32,
+                         g, c.j * kBlk, b);
+            bulk_commit();
+          }
+        }
+      }
+      n0 += c.n;
+      ++pieces;
+      if (n0 >= run) break;
+      c = piece_after(p, c, run - n0);
+    }
+    if ((threadIdx.x & 127) == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// ----------------------------------------------------------------------- dQ
+// Unit = (batch, query head, query block); one persistent CTA per SM.  Per key
+// block the unit sees: S = Q K^T, dP = dO V^T, dS = P (dP - di) (row warps, query
+// rows; 32 keys per thread, lse and di one register each), dQ += dS K.
+// Issue order: dP(n + 1) as soon as the row warps have copied step n out of TMEM,
+// S(n + 2) (two column sets), dQ(n).  V's buffer is
+// free after dP, K's (one of three) after dQ.
+// TMEM columns: S [0,128) and [384,512), dP [128,256), dQ [256,384).
+struct Unit {
+  int b, h, i;         // batch, query head, query block
+  int n, ns, skip;     // key blocks: [0, ns) (sinks), then [ns + skip, n + skip)
+};
+__device__ __forceinline__ Unit dq_unit(const BwdParams& p, int u) {
+  const int heads = p.B * p.QH;
+  Unit c;
+  c.i = p.nkb - 1 - u / heads;  // the last query blocks, which see the most, first
+  const int bh = u % heads;
+  c.b = bh / p.QH;
+  c.h = bh - c.b * p.QH;
+  const int first = max(0, c.i * kBlk - p.window + 1) / kBlk;
+  c.ns = min((p.sinks + kBlk - 1) / kBlk, first);
+  c.n = c.ns + c.i + 1 - first;
+  c.skip = first - c.ns;
+  return c;
+}
+__device__ __forceinline__ int unit_block(const Unit& c, int j) { return j < c.ns ? j : j + c.skip; }
+
+__global__ void __launch_bounds__(kThreads, 1)
+    window_dq_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                     const __grid_constant__ CUtensorMap tmDQ, const BwdParams p, unsigned* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr uint32_t kQ = 0, kDO = kTile, kK = 2 * kTile, kV = 5 * kTile, kDS = 6 * kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
+  // one phase per unit
+  uint64_t* qdo_full = bars + 0;    // Q, dO landed
+  uint64_t* dq_ready = bars + 1;    // every MMA of the unit done: dQ final
+  uint64_t* dq_free = bars + 2;     // dQ read out of TMEM (16 warps)
+  // one phase per step n of the CTA ([3]: per use of buffer n % 3)
+  uint64_t* k_full = bars + 3;      // [3] K landed
+  uint64_t* k_free = bars + 6;      // [3] dQ(n) done: K and the tile's dS read
+  uint64_t* v_full = bars + 9;      // V landed
+  uint64_t* sp_ready = bars + 11;   // S(n), dP(n) in TMEM, V read
+  uint64_t* sp_free = bars + 12;    // S(n), dP(n) read out (16 warps)
+  uint64_t* ds_ready = bars + 13;   // dS(n) in the tile (16 warps)
+  uint64_t* drain = bars + 14;      // once
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 15);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 15; ++i) mbar_init(bars + i, i == 2 || i == 12 || i == 13 ? kRowWarps : 1);
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmDO);
+    tma_prefetch_desc(&tmDQ);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  const int units = p.B * p.QH * p.nkb;
+  int n0 = 0;  // steps of earlier units
+  int uc = 0;  // earlier units
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      bool ok = true;
+      int qs = 0, vs = 0, ks = 0;  // loads issued
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit c = dq_unit(p, u);
+        const int g = c.h / p.rep;
+        // Q, dO once the last unit's last S, dP are done
+        if (n0 > 0) ok = mbar_wait(sp_ready, static_cast<uint32_t>(n0 - 1) & 1u, err, kErrWaitEmpty);
+        if (!ok) break;
+        mbar_arrive_expect_tx(qdo_full, 2 * kTile);
+        load_tile(smem + kQ, &tmQ, qdo_full, c.h, c.i * kBlk, c.b);
+        load_tile(smem + kDO, &tmDO, qdo_full, c.h, c.i * kBlk, c.b);
+        ++qs;
+        for (int j = 0; j < c.n; ++j) {
+          const int n = n0 + j, kb = n % 3;
+          const int k0 = unit_block(c, j) * kBlk;
+          if (n >= 3) ok = mbar_wait(&k_free[kb], static_cast<uint32_t>(n / 3 - 1) & 1u, err, kErrWaitEmpty);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&k_full[kb], kTile);
+          load_tile(smem + kK + kb * kTile, &tmK, &k_full[kb], g, k0, c.b);
+          ++ks;
+          if (j > 0) ok = mbar_wait(sp_ready, static_cast<uint32_t>(n - 1) & 1u, err, kErrWaitEmpty);
+          if (!ok) break;
+          mbar_arrive_expect_tx(v_full, kTile);
+          load_tile(smem + kV, &tmV, v_full, g, k0, c.b);
+          ++vs;
+        }
+        n0 += c.n;
+      }
+      // no copy may still be writing shared memory when the CTA exits
+      if (qs > 0) mbar_drain(qdo_full, static_cast<uint32_t>(qs - 1) & 1u);
+      if (vs > 0) mbar_drain(v_full, static_cast<uint32_t>(vs - 1) & 1u);
+      for (int t = 0; t < 3; ++t) {
+        const int uses = (ks + 2 - t) / 3;
+        if (uses > 0) mbar_drain(&k_full[t], static_cast<uint32_t>(uses - 1) & 1u);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1 || warp == 2) {
+    // ------------------------------------------------ MMA issuer / scheduler
+    const bool sched = warp == 2;
+    const uint32_t base = smem_u32(smem);
+    bool ok = true, any = false;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
+      const Unit c = dq_unit(p, u);
+      auto s_group = [&](int n, bool first) -> bool {  // S(n): its columns were copied before dP(n - 1) was issued
+        const int kb = n % 3;
+        const bool good = sched ? sched_wait(err, &k_full[kb], static_cast<uint32_t>(n / 3) & 1u,
+                                             first ? qdo_full : nullptr, static_cast<uint32_t>(uc) & 1u)
+                                : go_barrier64<kGoBarrier>(true);
+        if (good && !sched && lane == 0) {
+          tc_fence_after();
+          mma_kk(tmem + (n & 1) * 384, base + kQ, base + kK + kb * kTile);
+          any = true;
+        }
+        __syncwarp();
+        return good;
+      };
+      ok = s_group(n0, true);
+      if (!ok) break;
+      // step -1 issues the first dP alone
+      for (int j = -1; j < c.n; ++j) {
+        const int n = n0 + j;
+        if (j + 1 < c.n) {
+          // dP(n + 1) into the columns that the row warps have copied
+          const uint32_t nb = static_cast<uint32_t>(n + 1) & 1u;
+          ok = sched ? sched_wait(err, v_full, nb, n + 1 > 0 ? sp_free : nullptr, nb ^ 1u)
+                     : go_barrier64<kGoBarrier>(true);
+          if (!ok) break;
+          if (!sched && lane == 0) {
+            tc_fence_after();
+            mma_kk(tmem + 128, base + kDO, base + kV);
+            umma_commit(sp_ready);
+          }
+          __syncwarp();
+          if (j + 2 < c.n) ok = s_group(n + 2, false);
+          if (!ok) break;
+        }
+        if (j >= 0) {
+          // dQ += dS(n) K (the first of a unit once the last unit's dQ is read)
+          const int kb = n % 3;
+          ok = sched ? sched_wait(err, ds_ready, static_cast<uint32_t>(n) & 1u, j == 0 && uc > 0 ? dq_free : nullptr,
+                                  static_cast<uint32_t>(uc - 1) & 1u)
+                     : go_barrier64<kGoBarrier>(true);
+          if (!ok) break;
+          if (!sched && lane == 0) {
+            tc_fence_after();
+            mma_km(tmem + 256, base + kDS, base + kK + kb * kTile, j == 0);
+            umma_commit(&k_free[kb]);
+            if (j + 1 == c.n) umma_commit(dq_ready);
+          }
+          __syncwarp();
+        }
+      }
+      n0 += c.n;
+    }
+    if (!sched && lane == 0 && any) {
+      // every issued MMA must finish before TMEM is released
+      umma_commit(drain);
+      mbar_drain(drain, 0u);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------- row warps
+    const int grp = (warp - 4) >> 2;       // keys (and columns of dQ) [32 grp, + 32)
+    const int r = (warp & 3) * 32 + lane;  // query row of this thread (TMEM lane)
+    const uint32_t col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 32 * grp;
+    const uint32_t row = smem_u32(smem + kDS) + static_cast<uint32_t>(r * 128) + (grp >> 1) * kHalf;
+    const uint32_t out = smem_u32(smem + kDS) + grp * (kTile / 4) + static_cast<uint32_t>(r * 64);
+    const int u0 = (grp & 1) * 4;
+    const uint32_t rsw = static_cast<uint32_t>(r & 7);
+    const float2 sl2 = make_float2(p.sl2, p.sl2);
+    bool ok = true;
+    pdl_wait();  // nlse, ndi: written two launches before
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
+      const Unit c = dq_unit(p, u);
+      const int qpos = c.i * kBlk + r;
+      const int64_t at = (static_cast<int64_t>(c.b) * p.QH + c.h) * p.sp + qpos;
+      const float nl = p.nlse[at], nd = p.ndi[at];
+      const float2 nlse = make_float2(nl, nl), ndi = make_float2(nd, nd);
+      for (int j = 0; j < c.n; ++j) {
+        const int n = n0 + j;
+        const uint32_t par = static_cast<uint32_t>(n) & 1u;
+        const int k0 = unit_block(c, j) * kBlk + 32 * grp;  // this thread's first key
+        const int hi = qpos < p.S ? qpos + 1 - k0 : 0;      // keys [k0, k0 + hi) are not after the query
+        const uint32_t live = range_mask(qpos + 1 - p.window - k0, hi) | range_mask(0, min(hi, p.sinks - k0));
+        ok = mbar_wait(sp_ready, par, err, kErrWaitAccum);
+        if (j == 0 && uc > 0) {  // the last unit's dQ has left the tile
+          if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
+          ok = bar_and(kRowsBarrier, kRowThreads, ok);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[32], d[32];
+        tmem_ld_32x32b_x32(col + par * 384, s);
+        tmem_ld_32x32b_x32(col + 128, d);
+        tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive_warp(sp_free);
+        float2 e[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float2 a = __ffma2_rn(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), sl2, nlse);
+          const float2 t = __fadd2_rn(make_float2(__uint_as_float(d[2 * q]), __uint_as_float(d[2 * q + 1])), ndi);
+          e[q] = __fmul2_rn(make_float2(exp2_approx(a.x), exp2_approx(a.y)), t);
+        }
+        keep_live(live, e);
+        // the tile is free once dQ(n - 1) is done
+        if (n > 0) ok = mbar_wait(&k_free[(n - 1) % 3], static_cast<uint32_t>((n - 1) / 3) & 1u, err, kErrWaitEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        store32(row, u0, rsw, e);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive_warp(ds_ready);
+      }
+      n0 += c.n;
+      if (ok) ok = mbar_wait(dq_ready, static_cast<uint32_t>(uc) & 1u, err, kErrWaitAccum);
+      ok = bar_and(kRowsBarrier, kRowThreads, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t o[32];
+      tmem_ld_32x32b_x32(col + 256, o);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive_warp(dq_free);
+      // 32 columns through this group's quarter of dS's tile (64-byte rows, 64-byte
+      // swizzle), whose MMAs are done, and out by TMA (rows past S are not written)
+      const float2 f = make_float2(p.scale, p.scale);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 t =
+              __fmul2_rn(make_float2(__uint_as_float(o[8 * v + 2 * k]), __uint_as_float(o[8 * v + 2 * k + 1])), f);
+          w[k] = pack_bf16x2(t.x, t.y);
+        }
+        st_shared_v4(out + ((static_cast<uint32_t>(v) ^ ((r >> 1) & 3u)) << 4), w[0], w[1], w[2], w[3]);
+      }
+      fence_proxy_async_smem();
+      bar_sync(2 + grp, 128);
+      if ((threadIdx.x & 127) == 0) {
+        tma_store_4d(&tmDQ, smem + kDS + grp * (kTile / 4), 32 * grp, c.h, c.i * kBlk, c.b);
+        bulk_commit();
+      }
+    }
+    if ((threadIdx.x & 127) == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Before the products: -rowsum(dout * out) and -lse of every query row, padded
+// to whole query blocks (zeros) so that a block's 512 bytes load aligned.  dout,
+// out [B][S][QH][128]; 16 lanes per row, 8 values each.
+__global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* __restrict__ dout,
+                                                          const __nv_bfloat16* __restrict__ out,
+                                                          const float* __restrict__ lse, float* __restrict__ ndi,
+                                                          float* __restrict__ nlse, int S, int SP, int QH) {
+  pdl_trigger();
+  const int lane = threadIdx.x & 15;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);  // (s, h) of batch entry blockIdx.y
+  const int b = blockIdx.y;
+  const int s = static_cast<int>(i / QH);
+  const int h = static_cast<int>(i - static_cast<int64_t>(s) * QH);
+  const bool in = s < S;
+  float acc = 0.f;
+  if (in) {
+    const int64_t row = (static_cast<int64_t>(b) * S + s) * QH + h;
+    float fa[8], fb[8];
+    unpack_bf16x8(reinterpret_cast<const uint4*>(dout + row * kD)[lane], fa);
+    unpack_bf16x8(reinterpret_cast<const uint4*>(out + row * kD)[lane], fb);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fb[e], acc);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0 && s < SP) {
+    const int64_t bh = static_cast<int64_t>(b) * QH + h;
+    ndi[bh * SP + s] = -acc;
+    nlse[bh * SP + s] = in ? -lse[bh * S + s] : 0.f;
+  }
+}
+
+// dk and dv of the walks that were cut.  8 blocks for each CTA of the products
+// (4 x 32 key rows of dV, then of dK): if a cut walk starts in its run, the
+// shares of that walk (this CTA's and the next ones') added in order, and
+// transposed ([d][key] to rows) through shared memory.
+__global__ void __launch_bounds__(256) window_join_kernel(const BwdParams p) {
+  __shared__ float tile[32][kD + 1];
+  pdl_wait();
+  const int cta = static_cast<int>(blockIdx.x) >> 3, which = (blockIdx.x >> 2) & 1, k0 = (blockIdx.x & 3) * 32;
+  const int4 w = p.pieces[2 * cta + 1];
+  if (w.z == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float v[kD / 8];  // d = warp + 8 e, key k0 + lane
+#pragma unroll
+  for (int e = 0; e < kD / 8; ++e) v[e] = 0.f;
+  int64_t slot = 2 * cta + 1;
+  for (int steps = w.z;; steps += p.pieces[slot].z) {
+    const float* src = p.partial + (slot * 2 + which) * kD * kBlk + k0 + lane;
+#pragma unroll
+    for (int e = 0; e < kD / 8; ++e) v[e] += src[(warp + 8 * e) * kBlk];
+    if (steps >= w.w) break;
+    slot = (slot | 1) + 1;
+  }
+  const float f = which == 0 ? 1.f : p.scale;
+#pragma unroll
+  for (int e = 0; e < kD / 8; ++e) tile[lane][warp + 8 * e] = v[e] * f;
+  __syncthreads();
+  const int b = w.x / p.KH, g = w.x - b * p.KH;
+  for (int i = threadIdx.x; i < 32 * 16; i += 256) {
+    const int r = i >> 4, u = i & 15;
+    const int kpos = w.y * kBlk + k0 + r;
+    if (kpos < p.S) {
+      const float* t = &tile[r][8 * u];
+      reinterpret_cast<uint4*>((which == 0 ? p.dv : p.dk) + ((static_cast<int64_t>(b) * p.S + kpos) * p.KH + g) * kD)[u] =
+          make_uint4(pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]), pack_bf16x2(t[4], t[5]),
+                     pack_bf16x2(t[6], t[7]));
+    }
+  }
+}
+
+inline size_t al256(size_t n) { return (n + 255) & ~size_t(255); }
+inline int64_t padded_rows(int64_t S) { return (S + kBlk - 1) / kBlk * kBlk; }
+
+// dq, dk, dv [B][S][H][128] as the kernels write them: 32-column boxes.
+kda_status tmap_out(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(H), static_cast<uint64_t>(S),
+                            static_cast<uint64_t>(B)};
+  const uint64_t strides[3] = {kD * 2, static_cast<uint64_t>(H) * kD * 2, static_cast<uint64_t>(S) * H * kD * 2};
+  const uint32_t box[4] = {32, 1, static_cast<uint32_t>(kBlk), 1};
+  return make_tmap_bf16_sw(m, base, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// How the walks lie and over how many CTAs they are spread.
+struct Plan {
+  int64_t nkb, nq, sink_blocks, steps, total, ctas;
+};
+Plan make_plan(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t window, int64_t sinks) {
+  Plan c;
+  c.nkb = padded_rows(S) / kBlk;
+  c.nq = std::min(c.nkb, (kBlk - 1 + std::min(window, S) - 1) / kBlk + 1);
+  c.sink_blocks = c.nq == c.nkb ? 0 : (std::min(sinks, S) + kBlk - 1) / kBlk;
+  c.steps = steps_before(c.nkb, c.sink_blocks, c.nq, QH / KH, c.nkb);
+  c.total = c.steps * B * KH;
+  c.ctas = std::min<int64_t>(num_sms(), c.total);
+  return c;
+}
+
+// `args...` launched so that its CTAs may take their places while the launch
+// before it drains; the kernels wait (griddepcontrol.wait) before they read
+// what that launch wrote.
+template <typename... P, typename... A>
+kda_status launch_after(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                        A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return launch_status(what);
+}
+
+}  // namespace
+}  // namespace kda
+
+using namespace kda;
+
+extern "C" size_t kda_gqa_window_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
+                                                         int64_t window, int64_t sinks) {
+  if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || QH % KH || D != kD || window <= 0 || sinks < 0) return 0;
+  return 2 * al256(static_cast<size_t>(B) * QH * padded_rows(S) * 4) +
+         static_cast<size_t>(make_plan(B, S, QH, KH, window, sinks).ctas) * (4 * kBlk * kD * 4 + 32);
+}
+
+extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void* q, const void* k, const void* v,
+                                                   const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                                   int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
+                                                   int64_t window, int64_t sinks, const int64_t* q_strides,
+                                                   const int64_t* k_strides, const int64_t* v_strides,
+                                                   void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "gqa_window_backward";
+  KDA_WB_TRY(gqa_window_check(op, B, S, QH, KH, D, window, sinks));
+  KDA_CHECK_ARG(dout && q && k && v && out && lse && dq && dk && dv && q_strides && k_strides && v_strides,
+                "%s: null pointer", op);
+  const int64_t dense_q[3] = {S * QH * kD, QH * kD, kD}, dense_k[3] = {S * KH * kD, KH * kD, kD};
+  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
+                          head_rows_ok(dout, dense_q) && head_rows_ok(out, dense_q) && head_rows_ok(dq, dense_q) &&
+                          head_rows_ok(dk, dense_k) && head_rows_ok(dv, dense_k),
+                      "%s: pointers and rows must be 16-byte aligned", op);
+  const size_t need = kda_gqa_window_backward_workspace_size(B, S, QH, KH, D, window, sinks);
+  KDA_CHECK_ARG(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes required, got %zu", op, need,
+                workspace_bytes);
+  KDA_CHECK_SUPPORTED((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "%s: workspace must be 16-byte aligned",
+                      op);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const Plan plan = make_plan(B, S, QH, KH, window, sinks);
+  KDA_CHECK_SUPPORTED(plan.total < (1ll << 31) * plan.ctas, "%s: too many steps (%lld)", op, (long long)plan.total);
+  const int64_t SP = padded_rows(S);
+  const size_t rows = al256(static_cast<size_t>(B) * QH * SP * 4);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  float* ndi = reinterpret_cast<float*>(w);
+  float* nlse = reinterpret_cast<float*>(w + rows);
+  BwdParams p{};
+  p.B = static_cast<int>(B);
+  p.S = static_cast<int>(S);
+  p.QH = static_cast<int>(QH);
+  p.KH = static_cast<int>(KH);
+  p.rep = static_cast<int>(QH / KH);
+  p.nkb = static_cast<int>(plan.nkb);
+  p.nq = static_cast<int>(plan.nq);
+  p.window = static_cast<int>(std::min(window, S));
+  p.sinks = static_cast<int>(std::min(sinks, S));
+  p.sink_blocks = static_cast<int>(plan.sink_blocks);
+  p.sp = static_cast<int>(SP);
+  p.steps = plan.steps;
+  p.total = plan.total;
+  p.scale = 1.0f / sqrtf(static_cast<float>(kD));
+  p.sl2 = p.scale * 1.4426950408889634f;
+  p.nlse = nlse;
+  p.ndi = ndi;
+  p.partial = reinterpret_cast<float*>(w + 2 * rows);
+  p.pieces = reinterpret_cast<int4*>(p.partial + plan.ctas * 4 * kBlk * kD);
+  p.dk = static_cast<__nv_bfloat16*>(dk);
+  p.dv = static_cast<__nv_bfloat16*>(dv);
+  static std::atomic<bool> attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    constexpr int bytes = static_cast<int>(Smem::kBytes);
+    if (cudaFuncSetAttribute(window_dkv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+        cudaFuncSetAttribute(window_dq_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return launch_status("gqa_window_backward: cudaFuncSetAttribute");
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  window_rows_kernel<<<dim3(static_cast<unsigned>((SP * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
+      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi, nlse, p.S, p.sp, p.QH);
+  KDA_WB_TRY(launch_status("gqa_window_backward: rows"));
+  // after a launch, which makes the device's context current in a thread that
+  // has not used it yet (autograd's); the encoder is a driver call and needs one
+  CUtensorMap tk, tv, tq, tdo, tdq, tdk, tdv;
+  KDA_WB_TRY(tmap_head_rows(&tk, k, B, S, KH, k_strides[0], k_strides[1], k_strides[2]));
+  KDA_WB_TRY(tmap_head_rows(&tv, v, B, S, KH, v_strides[0], v_strides[1], v_strides[2]));
+  KDA_WB_TRY(tmap_head_rows(&tq, q, B, S, QH, q_strides[0], q_strides[1], q_strides[2]));
+  KDA_WB_TRY(tmap_head_rows(&tdo, dout, B, S, QH, dense_q[0], dense_q[1], dense_q[2]));
+  KDA_WB_TRY(tmap_out(&tdq, dq, B, S, QH));
+  KDA_WB_TRY(tmap_out(&tdk, dk, B, S, KH));
+  KDA_WB_TRY(tmap_out(&tdv, dv, B, S, KH));
+  const unsigned ctas = static_cast<unsigned>(plan.ctas);
+  KDA_WB_TRY(launch_after("gqa_window_backward: dk, dv", window_dkv_kernel, dim3(ctas), kThreads, Smem::kBytes, st, tk,
+                          tv, tq, tdo, tdk, tdv, p, kda_err_ptr_window_bwd()));
+  const int64_t units = B * QH * plan.nkb;
+  KDA_WB_TRY(launch_after("gqa_window_backward: dq", window_dq_kernel,
+                          dim3(static_cast<unsigned>(std::min<int64_t>(units, num_sms()))), kThreads, Smem::kBytes, st,
+                          tk, tv, tq, tdo, tdq, p, kda_err_ptr_window_bwd()));
+  return launch_after("gqa_window_backward: join", window_join_kernel, dim3(8 * ctas), 256, 0, st, p);
+}
