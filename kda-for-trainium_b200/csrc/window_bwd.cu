@@ -269,9 +269,9 @@ __device__ __forceinline__ bool sched_wait(unsigned* err, uint64_t* b1, uint32_t
 //   registers as fp32, bf16 into a tile), dP^T = V_j dO^T, dV_j += P^T dO,
 //   dS^T = P^T (dP^T - di) (from the unrounded P^T, into a tile of its own),
 //   dK_j += dS^T Q
-// Issue order per step n: dV(n) S(n+1) | dK(n) | dP(n+1), the first two groups
-// released when the row warps have written their operand and read their
-// columns, the last when dO has been replaced.
+// Issue order per step n: S(n+1) as soon as the row warps have copied S(n) out of
+// TMEM, dV(n) and dK(n) as soon as they have written P^T(n) and dS^T(n), dP(n+1)
+// when dO has been replaced.
 // TMEM columns: S^T [0,128), dP^T [128,256), dV [256,384), dK [384,512).
 __global__ void __launch_bounds__(kThreads, 1)
     window_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* di_full = bars + 13;    // ndi landed (loaded once the row warps wrote dS(n - 1))
   uint64_t* s_ready = bars + 14;    // S^T(n) in TMEM
   uint64_t* dp_ready = bars + 15;   // dP^T(n) in TMEM
-  uint64_t* p_ready = bars + 16;    // P^T(n) in its tile, S^T(n) read out (16 warps)
+  uint64_t* s_free = bars + 10;     // S^T(n) read out (16 warps)
+  uint64_t* p_ready = bars + 16;    // P^T(n) in its tile (16 warps)
   uint64_t* ds_ready = bars + 17;   // dS^T(n) in its tile, dP^T(n) read out (16 warps)
   uint64_t* drain = bars + 18;      // once
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 19);
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 19; ++i)
-      mbar_init(bars + i, i == 3 || i == 16 || i == 17 ? kRowWarps : 1);
+      mbar_init(bars + i, i == 3 || i == 10 || i == 16 || i == 17 ? kRowWarps : 1);
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -441,20 +442,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t par = static_cast<uint32_t>(n) & 1u, nb = par, ob = par ^ 1u;
         const uint32_t use = static_cast<uint32_t>((n + 1) >> 1) & 1u;
         const bool more = i + 1 < c.n;
-        // dV_j += P^T(n) dO(n) (the first of a piece once the last piece's sums
-        // are read), S^T(n + 1)
-        ok = sched ? sched_wait(err, p_ready, par, more ? &q_full[ob] : nullptr, use,
-                                i == 0 && pieces > 0 ? acc_free : nullptr, static_cast<uint32_t>(pieces - 1) & 1u)
+        // S^T(n + 1)
+        if (more) {
+          ok = sched ? sched_wait(err, &q_full[ob], use, s_free, par) : go_barrier64<kGoBarrier>(true);
+          if (!ok) break;
+          if (!sched && lane == 0) {
+            tc_fence_after();
+            mma_kk(tmem, base + kK, base + kQ + ob * kTile);
+            umma_commit(s_ready);
+          }
+          __syncwarp();
+        }
+        // dV_j += P^T(n) dO(n) (the first of a piece once the last piece's sums are read)
+        ok = sched ? sched_wait(err, p_ready, par, i == 0 && pieces > 0 ? acc_free : nullptr,
+                                static_cast<uint32_t>(pieces - 1) & 1u)
                    : go_barrier64<kGoBarrier>(true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
           mma_km(tmem + 256, base + kP, base + kDO, i == 0);
           umma_commit(do_free);
-          if (more) {
-            mma_kk(tmem, base + kK, base + kQ + ob * kTile);
-            umma_commit(s_ready);
-          }
         }
         __syncwarp();
         // dK_j += dS^T(n) Q(n)
@@ -528,6 +535,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t s[32];
           tmem_ld_32x32b_x32(col + 32 * grp, s);
           tmem_ld_wait();
+          tc_fence_before();
+          mbar_arrive_warp(s_free);
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const float4 l = nlse_s[q];
@@ -924,33 +933,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Before the products: -rowsum(dout * out) and -lse of every query row, padded
 // to whole query blocks (zeros) so that a block's 512 bytes load aligned.  dout,
-// out [B][S][QH][128]; 16 lanes per row, 8 values each.
+// out [B][S][QH][128]; 16 lanes take four consecutive rows of a head, 8 values
+// of each per lane, all loads issued first.
+constexpr int kRowsEach = 4;
 __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* __restrict__ dout,
                                                           const __nv_bfloat16* __restrict__ out,
                                                           const float* __restrict__ lse, float* __restrict__ ndi,
                                                           float* __restrict__ nlse, int S, int SP, int QH) {
   pdl_trigger();
   const int lane = threadIdx.x & 15;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);  // (s, h) of batch entry blockIdx.y
-  const int b = blockIdx.y;
-  const int s = static_cast<int>(i / QH);
-  const int h = static_cast<int>(i - static_cast<int64_t>(s) * QH);
-  const bool in = s < S;
-  float acc = 0.f;
-  if (in) {
-    const int64_t row = (static_cast<int64_t>(b) * S + s) * QH + h;
-    float fa[8], fb[8];
-    unpack_bf16x8(reinterpret_cast<const uint4*>(dout + row * kD)[lane], fa);
-    unpack_bf16x8(reinterpret_cast<const uint4*>(out + row * kD)[lane], fb);
+  const int i = blockIdx.x * 16 + (threadIdx.x >> 4);  // (rows s .. s + 3, h) of batch entry blockIdx.y
+  const int64_t b = blockIdx.y;
+  const int h = i % QH;
+  const int s = i / QH * kRowsEach;
+  uint4 a[kRowsEach], o[kRowsEach];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc = fmaf(fa[e], fb[e], acc);
+  for (int k = 0; k < kRowsEach; ++k) {
+    a[k] = o[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (s + k < S) {
+      const int64_t row = (b * S + s + k) * QH + h;
+      a[k] = __ldg(reinterpret_cast<const uint4*>(dout + row * kD) + lane);
+      o[k] = __ldg(reinterpret_cast<const uint4*>(out + row * kD) + lane);
+    }
   }
+  const int64_t bh = b * QH + h;
+  const float l = lane < kRowsEach && s + lane < S ? -lse[bh * S + s + lane] : 0.f;
+  float acc[kRowsEach];
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane == 0 && s < SP) {
-    const int64_t bh = static_cast<int64_t>(b) * QH + h;
-    ndi[bh * SP + s] = -acc;
-    nlse[bh * SP + s] = in ? -lse[bh * S + s] : 0.f;
+  for (int k = 0; k < kRowsEach; ++k) {
+    float fa[8], fo[8];
+    unpack_bf16x8(a[k], fa);
+    unpack_bf16x8(o[k], fo);
+    acc[k] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[k] = fmaf(fa[e], fo[e], acc[k]);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], d);
+  }
+  if (lane < kRowsEach && s < SP) {  // SP is a multiple of kRowsEach
+    const float v = lane == 0 ? acc[0] : lane == 1 ? acc[1] : lane == 2 ? acc[2] : acc[3];
+    ndi[bh * SP + s + lane] = -v;
+    nlse[bh * SP + s + lane] = l;
   }
 }
 
@@ -1112,7 +1135,7 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
       return launch_status("gqa_window_backward: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  window_rows_kernel<<<dim3(static_cast<unsigned>((SP * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
+  window_rows_kernel<<<dim3(static_cast<unsigned>((SP / kRowsEach * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
       static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi, nlse, p.S, p.sp, p.QH);
   KDA_WB_TRY(launch_status("gqa_window_backward: rows"));
   // after a launch, which makes the device's context current in a thread that
