@@ -493,12 +493,11 @@ kda_status kda_qk_norm_rope_backward(const void* dq_out, const void* dk_out, con
 /* gqa_window (bf16, D 128): causal attention in which query i sees key j <= i
  * where i - j < window or j < sinks; scores scaled by 1/sqrt(D).  out
  * (B,S,QH,D) contiguous; lse, if not NULL, [B][QH][S] fp32: each row's
- * log2-sum-exp of the scaled scores, for the backward. */
-size_t kda_gqa_window_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D);
+ * log2-sum-exp of the scaled scores, for the backward.  No workspace. */
 kda_status kda_gqa_window_bf16(const void* q, const void* k, const void* v, void* out, float* lse, int64_t B,
                                int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window, int64_t sinks,
                                const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                               void* workspace, size_t workspace_bytes, void* stream);
+                               void* stream);
 
 /* Gradients of gqa_window given dout and the forward's out (B,S,QH,D,
  * contiguous) and lse: dq, dk, dv bf16, contiguous. */

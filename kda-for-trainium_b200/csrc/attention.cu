@@ -86,7 +86,6 @@ struct AttnParams {
   int B, S, QH, KH, n_rep;
   int npairs;       // 256-row query units per head
   int causal;
-  int window, sinks;  // sliding window (kWindow): keys [0, sinks) and the `window` keys up to the query
   float scale_log2;  // softmax scale * log2(e)
   void* out;
   int64_t out_row_stride;   // elements between consecutive query rows
@@ -117,26 +116,12 @@ __device__ __forceinline__ void unit_coords(int u, const AttnParams& p, int& b, 
   h = bh - b * p.QH;
 }
 
-// K/V blocks a unit visits, in order: `nb` blocks for both tiles (tile 0 sees
-// its last block fully masked when causal).  With a sliding window they are
-// the blocks that hold sinks, [0, ns), then those from the first query's
-// window on, [ns + skip, nb + skip).
-struct Walk {
-  int nb, ns, skip;
-};
-template <bool kWindow>
-__device__ __forceinline__ Walk unit_walk(const AttnParams& p, int qp) {
+// K/V blocks a unit visits: both tiles share the count; tile 0 sees its last
+// block fully masked when causal.
+__device__ __forceinline__ int num_kv_blocks(const AttnParams& p, int qp) {
   const int all = (p.S + kBlk - 1) / kBlk;
   const int need = 2 * qp + 2;
-  if (!kWindow) return {p.causal ? (need < all ? need : all) : all, 0, 0};
-  const int last = need < all ? need : all;
-  const int first = max(0, qp * 2 * kBlk - p.window + 1) / kBlk;
-  const int ns = min((p.sinks + kBlk - 1) / kBlk, first);
-  return {ns + last - first, ns, first - ns};
-}
-template <bool kWindow>
-__device__ __forceinline__ int key_block(const Walk& w, int j) {
-  return kWindow && j >= w.ns ? j + w.skip : j;
+  return p.causal ? (need < all ? need : all) : all;
 }
 
 // Ring items of a unit with nb blocks, in load order K_0, K_1, V_0, K_2, V_1,
@@ -152,7 +137,6 @@ __device__ __forceinline__ uint32_t item_v(uint32_t base, int j, int nb) {
 __device__ __forceinline__ uint32_t item_slot(uint32_t x) { return x % kSlots; }
 __device__ __forceinline__ uint32_t item_par(uint32_t x) { return (x / kSlots) & 1u; }
 
-template <bool kWindow>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const AttnParams p, unsigned* err) {
@@ -229,8 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int b, h, qp;
       unit_coords(u, p, b, h, qp);
       const int kvh = h / p.n_rep;
-      const Walk walk = unit_walk<kWindow>(p, qp);
-      const int nb = walk.nb;
+      const int nb = num_kv_blocks(p, qp);
       // Q is free once the previous unit's last QK group (which read its
       // last K item) is done
       if (!first && lane == 0) ok = mbar_wait(&slot_free[item_slot(prev_qk_last)], item_par(prev_qk_last), err,
@@ -246,10 +229,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_4d(smem + Smem::kQ + t * kTile + kHalf, &tmQ, q_full, 64, h, row, b);
         }
       }
-      ok = load_item(item_k(base, 0), false, kvh, key_block<kWindow>(walk, 0), b);
+      ok = load_item(item_k(base, 0), false, kvh, 0, b);
       for (int j = 0; j < nb && ok; ++j) {
-        if (j + 1 < nb) ok = load_item(item_k(base, j + 1), false, kvh, key_block<kWindow>(walk, j + 1), b);
-        if (ok) ok = load_item(item_v(base, j, nb), true, kvh, key_block<kWindow>(walk, j), b);
+        if (j + 1 < nb) ok = load_item(item_k(base, j + 1), false, kvh, j + 1, b);
+        if (ok) ok = load_item(item_v(base, j, nb), true, kvh, j, b);
       }
       prev_qk_last = item_k(base, nb - 1);
       base += 2u * static_cast<uint32_t>(nb);
@@ -319,8 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
       int b, h, qp;
       unit_coords(u, p, b, h, qp);
-      const Walk walk = unit_walk<kWindow>(p, qp);
-      const int nb = walk.nb;
+      const int nb = num_kv_blocks(p, qp);
       // group: S = Q K_0^T (needs Q, K_0, and S released by the softmax of
       // the previous block, if any)
       {
@@ -392,8 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       int b, h, qp;
       unit_coords(u, p, b, h, qp);
-      const Walk walk = unit_walk<kWindow>(p, qp);
-      const int nb = walk.nb;
+      const int nb = num_kv_blocks(p, qp);
       const int q0 = qp * 2 * kBlk + t * kBlk;  // first query row of this tile
       const int qpos = q0 + r;
       float m_run = -INFINITY, l_run = 0.f;
@@ -413,21 +394,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_wait();
         tc_fence_before();
         mbar_arrive_warp(s_free);
-        const int k0 = key_block<kWindow>(walk, j) * kBlk;
+        const int k0 = j * kBlk;
         // masks only touch the diagonal / ragged blocks (block-uniform branch)
-        // and, with a window, those that start before the last row's window
-        const bool causal = kWindow || p.causal;
-        const bool masked_blk = (causal && k0 + kBlk - 1 > q0) || (k0 + kBlk > p.S) ||
-                                (kWindow && k0 + p.window < q0 + kBlk && k0 + kBlk > p.sinks);
+        const bool masked_blk = (p.causal && k0 + kBlk - 1 > q0) || (k0 + kBlk > p.S);
         if (masked_blk) {
-          const int lim_c = causal ? qpos - k0 + 1 : kBlk;
+          const int lim_c = p.causal ? qpos - k0 + 1 : kBlk;
           const int lim_s = p.S - k0;
           const int lim = lim_c < lim_s ? lim_c : lim_s;  // keys [k0, k0 + lim) are visible
-          const int old = qpos - p.window + 1 - k0;       // kWindow: of those, keys before k0 + old only as sinks
-          const int sink = p.sinks - k0;
 #pragma unroll
           for (int i = 0; i < kBlk; ++i)
-            if (i >= lim || (kWindow && i < old && i >= sink)) sv[i] = 0xff800000u;  // -inf
+            if (i >= lim) sv[i] = 0xff800000u;  // -inf
         }
         // raw row max (the scale is positive): 3-input max, eight chains
         float mxa[8];
@@ -460,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < kBlk / 2; ++i) {
           const float2 v = make_float2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1]));
           const float2 a = __ffma2_rn(v, sc2, nm2);
-          const float2 e = (((kWindow ? 0u : kPolyPairs) >> (i & 15)) & 1u) ? exp2_poly2_lp(a)
+          const float2 e = ((kPolyPairs >> (i & 15)) & 1u) ? exp2_poly2_lp(a)
                                                             : make_float2(exp2_approx(a.x), exp2_approx(a.y));
           sum2[i & 3] = __fadd2_rn(sum2[i & 3], e);
           pk[i] = pack_bf16x2(e.x, e.y);
@@ -591,14 +567,13 @@ __global__ void rope_rotate_kernel(const __nv_bfloat16* __restrict__ x, __nv_bfl
 }
 
 // ------------------------------------------------------------- V^T copy
-// v [B][S][KH][128] (element strides vb, vs, vh) -> vt [B][KH][128][S8] (S8 = S rounded up to 8 so rows
+// v [B][S][KH][128] -> vt [B][KH][128][S8] (S8 = S rounded up to 8 so rows
 // are 16-byte aligned for TMA; keys [S, S8) are written as zeros).  One CTA
 // per (64 keys, kv head, batch): the tile goes through padded shared memory
 // so both the reads and the writes are 16-byte coalesced.
 constexpr int kTrKeys = 64;
 __global__ void __launch_bounds__(256) v_transpose_kernel(const __nv_bfloat16* __restrict__ v,
-                                                          __nv_bfloat16* __restrict__ vt, int S, int S8, int KH,
-                                                          int64_t vb, int64_t vs, int64_t vh) {
+                                                          __nv_bfloat16* __restrict__ vt, int S, int S8, int KH) {
   __shared__ __align__(16) __nv_bfloat16 tile[kTrKeys][kD + 8];
   const int s0 = blockIdx.x * kTrKeys;
   const int kvh = blockIdx.y, b = blockIdx.z;
@@ -607,7 +582,7 @@ __global__ void __launch_bounds__(256) v_transpose_kernel(const __nv_bfloat16* _
     const int row = i >> 4, unit = i & 15;
     uint4 val = make_uint4(0u, 0u, 0u, 0u);
     if (s0 + row < S)
-      val = *reinterpret_cast<const uint4*>(v + b * vb + (s0 + row) * vs + kvh * vh + unit * 8);
+      val = *reinterpret_cast<const uint4*>(v + ((static_cast<int64_t>(b) * S + s0 + row) * KH + kvh) * kD + unit * 8);
     *reinterpret_cast<uint4*>(&tile[row][unit * 8]) = val;
   }
   __syncthreads();
@@ -627,9 +602,15 @@ __global__ void __launch_bounds__(256) v_transpose_kernel(const __nv_bfloat16* _
 inline size_t al256(size_t n) { return (n + 255) & ~size_t(255); }
 inline int64_t keys8(int64_t S) { return (S + 7) & ~int64_t(7); }
 
-// Dense [B][S][H][128].
+// [B][S][H][128] as a 4-D map {128, H, S, B} (rows past S read as zeros);
+// box {64, 1, 128, 1}.
 kda_status tmap_heads(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H) {
-  return tmap_head_rows(m, base, B, S, H, S * H * kD, H * kD, kD);
+  const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(H), static_cast<uint64_t>(S),
+                            static_cast<uint64_t>(B)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(kD) * 2, static_cast<uint64_t>(H) * kD * 2,
+                               static_cast<uint64_t>(S) * H * kD * 2};
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(kBlk), 1};
+  return make_tmap_bf16(m, base, 4, dims, strides, box);
 }
 
 // V^T [B][KH][128][S8] as a 4-D map {S8, 128, KH, B}; box {64, 128, 1, 1}
@@ -643,46 +624,7 @@ kda_status tmap_vt(CUtensorMap* m, const void* base, int64_t B, int64_t S8, int6
   return make_tmap_bf16(m, base, 4, dims, strides, box);
 }
 
-// Opt-ins of one instantiation (once per device), then its persistent launch.
-template <bool kWindow>
-kda_status launch_attn(const char* op, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                       const AttnParams& p, cudaStream_t st) {
-  static std::atomic<bool> attr_set[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    // the setmaxnreg split only balances when the kernel launches with
-    // exactly kRegsLaunch registers per thread
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, attn_kernel<kWindow>) != cudaSuccess) return launch_status("attn_kernel: attributes");
-    KDA_CHECK_SUPPORTED(fa.numRegs == kRegsLaunch,
-                        "%s: attention kernel compiled to %d registers/thread, its register split needs %d",
-                        op, fa.numRegs, kRegsLaunch);
-    if (cudaFuncSetAttribute(attn_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(Smem::kBytes)) != cudaSuccess)
-      return launch_status("attn_kernel: cudaFuncSetAttribute");
-    attr_set[dev].store(true, std::memory_order_release);
-  }
-  const long long units = static_cast<long long>(p.B) * p.QH * p.npairs;
-  const int grid = static_cast<int>(units < num_sms() ? units : num_sms());
-  attn_kernel<kWindow><<<grid, kThreads, Smem::kBytes, st>>>(tq, tk, tv, p, kda_err_ptr_attn());
-  return launch_status("attn_kernel");
-}
-
 }  // namespace
-
-// [B][S][H][128] rows with element strides sb, ss, sh as a 4-D map
-// {128, H, S, B} (rows past S read as zeros); box {64, 1, 128, 1}.  An axis of
-// one entry may have any stride.
-kda_status tmap_head_rows(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H, int64_t sb, int64_t ss,
-                          int64_t sh) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(H), static_cast<uint64_t>(S),
-                            static_cast<uint64_t>(B)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(H > 1 ? sh : kD) * 2, static_cast<uint64_t>(S > 1 ? ss : kD) * 2,
-                               static_cast<uint64_t>(B > 1 ? sb : kD) * 2};
-  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(kBlk), 1};
-  return make_tmap_bf16(m, base, 4, dims, strides, box);
-}
 
 // RoPE for the attention backward in another translation unit: the table of
 // S positions x 64 frequencies (cos, sin) and the rotation of [rows][128]
@@ -761,7 +703,7 @@ kda_status kda::gqa_forward(const void* q, const void* k, const void* v, void* o
   v_transpose_kernel<<<dim3(static_cast<unsigned>((S + kTrKeys - 1) / kTrKeys), static_cast<unsigned>(KH),
                            static_cast<unsigned>(B)),
                        256, 0, st>>>(static_cast<const __nv_bfloat16*>(v), vt, static_cast<int>(S),
-                                     static_cast<int>(S8), static_cast<int>(KH), S * KH * kD, KH * kD, kD);
+                                     static_cast<int>(S8), static_cast<int>(KH));
   if (launch_status("gqa_full v transpose") != KDA_OK) return KDA_CUDA_ERROR;
   const void* qs = q;
   const void* ks = k;
@@ -806,79 +748,24 @@ kda_status kda::gqa_forward(const void* q, const void* k, const void* v, void* o
     p.out_head_stride = S * kD;
     p.out_batch_stride = QH * S * kD;
   }
-  return launch_attn<false>("gqa_full", tq, tk, tv, p, st);
-}
-
-// ------------------------------------------------- sliding window with sinks
-// Causal attention in which query i sees key j <= i where i - j < window or
-// j < sinks: attn_kernel<true> on operands as stored (strided rows, no RoPE).
-extern "C" size_t kda_gqa_window_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D) {
-  if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || D != kD) return 0;
-  return al256(static_cast<size_t>(B) * KH * kD * keys8(S) * 2);  // V^T
-}
-
-kda_status kda::gqa_window_check(const char* op, int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D,
-                                 int64_t window, int64_t sinks) {
-  KDA_CHECK_ARG(B > 0 && S > 0 && QH > 0 && KH > 0 && QH % KH == 0, "%s: bad sizes B=%lld S=%lld QH=%lld KH=%lld", op,
-                (long long)B, (long long)S, (long long)QH, (long long)KH);
-  KDA_CHECK_ARG(window > 0 && sinks >= 0, "%s: window must be positive and sinks not negative, got %lld and %lld", op,
-                (long long)window, (long long)sinks);
-  KDA_CHECK_SUPPORTED(D == kD, "%s: head_dim must be 128, got %lld", op, (long long)D);
-  KDA_CHECK_SUPPORTED(S < (1ll << 24) && QH <= 65535 && B <= 65535 && B * S < (1ll << 31) / QH,
-                      "%s: too many rows (B=%lld S=%lld QH=%lld)", op, (long long)B, (long long)S, (long long)QH);
-  return KDA_OK;
-}
-
-bool kda::head_rows_ok(const void* p, const int64_t* s) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 &&
-         s[0] >= 0 && s[1] >= 0 && s[2] >= 0;
-}
-
-extern "C" kda_status kda_gqa_window_bf16(const void* q, const void* k, const void* v, void* out, float* lse,
-                                          int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window,
-                                          int64_t sinks, const int64_t* q_strides, const int64_t* k_strides,
-                                          const int64_t* v_strides, void* workspace, size_t workspace_bytes,
-                                          void* stream) {
-  const char* op = "gqa_window";
-  kda_status s;
-  if ((s = kda::gqa_window_check(op, B, S, QH, KH, D, window, sinks)) != KDA_OK) return s;
-  KDA_CHECK_ARG(q && k && v && out && q_strides && k_strides && v_strides, "%s: null pointer", op);
-  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
-                          (reinterpret_cast<uintptr_t>(out) & 15u) == 0,
-                      "%s: pointers and rows must be 16-byte aligned", op);
-  const size_t need = kda_gqa_window_workspace_size(B, S, QH, KH, D);
-  KDA_CHECK_ARG(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes required, got %zu", op, need,
-                workspace_bytes);
-  KDA_CHECK_SUPPORTED((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "%s: workspace must be 16-byte aligned",
-                      op);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t S8 = keys8(S);
-  auto* vt = static_cast<__nv_bfloat16*>(workspace);
-  v_transpose_kernel<<<dim3(static_cast<unsigned>((S + kTrKeys - 1) / kTrKeys), static_cast<unsigned>(KH),
-                           static_cast<unsigned>(B)),
-                       256, 0, st>>>(static_cast<const __nv_bfloat16*>(v), vt, static_cast<int>(S),
-                                     static_cast<int>(S8), static_cast<int>(KH), v_strides[0], v_strides[1],
-                                     v_strides[2]);
-  if (launch_status("gqa_window v transpose") != KDA_OK) return KDA_CUDA_ERROR;
-  CUtensorMap tq, tk, tv;
-  if ((s = tmap_head_rows(&tq, q, B, S, QH, q_strides[0], q_strides[1], q_strides[2])) != KDA_OK) return s;
-  if ((s = tmap_head_rows(&tk, k, B, S, KH, k_strides[0], k_strides[1], k_strides[2])) != KDA_OK) return s;
-  if ((s = tmap_vt(&tv, vt, B, S8, KH)) != KDA_OK) return s;
-  AttnParams p{};
-  p.B = static_cast<int>(B);
-  p.S = static_cast<int>(S);
-  p.QH = static_cast<int>(QH);
-  p.KH = static_cast<int>(KH);
-  p.n_rep = static_cast<int>(QH / KH);
-  p.npairs = static_cast<int>((S + 2 * kBlk - 1) / (2 * kBlk));
-  p.causal = 1;
-  p.window = static_cast<int>(window < S ? window : S);
-  p.sinks = static_cast<int>(sinks < S ? sinks : S);
-  p.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(kD)));
-  p.out = out;
-  p.lse = lse;
-  p.out_row_stride = QH * kD;
-  p.out_head_stride = kD;
-  p.out_batch_stride = S * QH * kD;
-  return launch_attn<true>(op, tq, tk, tv, p, st);
+  static std::atomic<bool> attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    // the setmaxnreg split only balances when the kernel launches with
+    // exactly kRegsLaunch registers per thread
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, attn_kernel) != cudaSuccess) return launch_status("gqa_full: attributes");
+    KDA_CHECK_SUPPORTED(fa.numRegs == kRegsLaunch,
+                        "gqa_full: attention kernel compiled to %d registers/thread, its register split needs %d",
+                        fa.numRegs, kRegsLaunch);
+    if (cudaFuncSetAttribute(attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Smem::kBytes)) != cudaSuccess)
+      return launch_status("gqa_full: cudaFuncSetAttribute");
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  const long long units = static_cast<long long>(B) * QH * p.npairs;
+  const int grid = static_cast<int>(units < num_sms() ? units : num_sms());
+  attn_kernel<<<grid, kThreads, Smem::kBytes, st>>>(tq, tk, tv, p, kda_err_ptr_attn());
+  return launch_status("attn_kernel");
 }

@@ -224,18 +224,15 @@ WindowArgs window_args(const Tensor& q, const Tensor& k, const Tensor& v) {
 }
 
 std::tuple<Tensor, OptTensor> gqa_window(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window,
-                                         int64_t sinks, const OptTensor& out, bool with_lse,
-                                         const OptTensor& workspace) {
+                                         int64_t sinks, const OptTensor& out, bool with_lse) {
   const WindowArgs a = window_args(q, k, v);
   const c10::cuda::CUDAGuard guard(a.dev);
   Tensor y = out_or_empty(out, "out", {a.B, a.S, a.QH, a.D}, kBf16, a.dev);
   OptTensor lse;
   if (with_lse) lse = empty({a.B, a.QH, a.S}, kF32, a.dev);
-  const size_t nb = kda_gqa_window_workspace_size(a.B, a.S, a.QH, a.KH, a.D);
-  Tensor ws = workspace_or_empty(workspace, nb, a.dev);
   done("kda_gqa_window_bf16",
        kda_gqa_window_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(), ptr<float>(lse), a.B, a.S, a.QH,
-                           a.KH, a.D, window, sinks, a.q.s, a.k.s, a.v.s, ws.data_ptr(), nb, stream(a.dev)));
+                           a.KH, a.D, window, sinks, a.q.s, a.k.s, a.v.s, stream(a.dev)));
   return {y, lse};
 }
 

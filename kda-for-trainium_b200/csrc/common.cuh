@@ -502,15 +502,6 @@ kda_status gqa_forward(const void* q, const void* k, const void* v, void* out, i
                        int64_t KH, int64_t D, int causal, float rope_theta, int out_bshd, void* workspace,
                        size_t workspace_bytes, float* lse, cudaStream_t st);
 
-// Shared by the sliding-window entry points: the size checks, whether strided
-// head rows start on 16 bytes, and the TMA map of [B][S][H][128] rows with
-// element strides (128-row boxes of 64 columns).
-kda_status gqa_window_check(const char* op, int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window,
-                            int64_t sinks);
-bool head_rows_ok(const void* p, const int64_t* strides);
-kda_status tmap_head_rows(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H, int64_t sb, int64_t ss,
-                          int64_t sh);
-
 }  // namespace kda
 
 // Define a per-TU device error word plus its host reader.

@@ -31,7 +31,7 @@
 
 #include <algorithm>
 
-#include "common.cuh"
+#include "window.cuh"
 
 KDA_DEFINE_ERROR_WORD(window_bwd)
 
@@ -44,14 +44,9 @@ KDA_DEFINE_ERROR_WORD(window_bwd)
 namespace kda {
 namespace {
 
-constexpr int kD = 128;
-constexpr int kBlk = 128;
-constexpr uint32_t kTile = kBlk * kD * 2;  // 32 KB
-constexpr uint32_t kHalf = kTile / 2;
 constexpr int kRowWarps = 16;
 constexpr int kThreads = 128 + 32 * kRowWarps;
 constexpr int kRowThreads = 32 * kRowWarps;
-constexpr int kGoBarrier = 1;   // named barrier: scheduler warp + MMA warp
 constexpr int kRowsBarrier = 6;  // all row warps; 2 .. 5: the four warps of one column group
 
 struct BwdParams {
@@ -146,10 +141,6 @@ __device__ __forceinline__ int step_head(const BwdParams& p, int g, const Piece&
 }
 __device__ __forceinline__ int step_block(const Piece& c, int it) { return c.j + it % c.nq; }
 
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
 // 32 values of a row as bf16 into a K-major, 128-byte-swizzled half tile: columns
 // [8u, 8u + 8) of the half = 16-byte unit u, at u ^ (row % 8); u0 the first unit.
 __device__ __forceinline__ void store32(uint32_t row, int u0, uint32_t rsw, const float2 (&e)[16]) {
@@ -158,50 +149,6 @@ __device__ __forceinline__ void store32(uint32_t row, int u0, uint32_t rsw, cons
     st_shared_v4(row + ((static_cast<uint32_t>(u0 + u) ^ rsw) << 4), pack_bf16x2(e[4 * u].x, e[4 * u].y),
                  pack_bf16x2(e[4 * u + 1].x, e[4 * u + 1].y), pack_bf16x2(e[4 * u + 2].x, e[4 * u + 2].y),
                  pack_bf16x2(e[4 * u + 3].x, e[4 * u + 3].y));
-}
-
-__device__ __forceinline__ void bar_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-// The same, returning the AND of every thread's `ok`.  Named barriers have no
-// time limit, so a warp whose bounded wait expired still joins the next one of
-// its group, with false, and all of them stop there together.
-__device__ __forceinline__ bool bar_and(int id, int threads, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %1, 0;\n\t"
-      "bar.red.and.pred p, %2, %3, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r)
-      : "r"(ok ? 1u : 0u), "r"(id), "r"(threads)
-      : "memory");
-  return r != 0;
-}
-// Every committed bulk store of this thread has read its shared memory.
-__device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, const void* src, int x, int y, int z, int w) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(m)),
-               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
-               : "memory");
-}
-
-// Bits [a, b) of a 32-bit word (empty when a >= b); a, b may lie outside [0, 32].
-__device__ __forceinline__ uint32_t range_mask(int a, int b) {
-  a = a < 0 ? 0 : a;
-  b = b > 32 ? 32 : b;
-  if (a >= b) return 0u;
-  const uint32_t hi = b >= 32 ? 0xffffffffu : ((1u << b) - 1u);
-  return hi & ~((1u << a) - 1u);
-}
-
-// Bounded wait at the end, also after an error elsewhere: what is in flight
-// must land before shared memory and TMEM go.
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
-  const unsigned long long t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity))
-    if (globaltimer_ns() - t0 > kWaitLimitNs) return;
 }
 
 // Values of hidden pairs become exactly zero: pair i of e is live where bits
@@ -214,48 +161,6 @@ __device__ __forceinline__ void keep_live(uint32_t live, float2 (&e)[16]) {
       e[q].y = (live >> (2 * q + 1)) & 1u ? e[q].y : 0.f;
     }
   }
-}
-
-constexpr uint32_t kIdKK = idesc_bf16_f32(kBlk, kBlk, 0, 0);  // K-major A, K-major B
-constexpr uint32_t kIdKM = idesc_bf16_f32(kBlk, kBlk, 0, 1);  // K-major A, MN-major B
-// Descriptors of a tile read K-major (rows = M or N, 64-element halves along K:
-// K step kk at (kk / 4) halves + (kk % 4) x 32 bytes) and MN-major (rows = K: K
-// step kk at kk x 16 rows x 128 bytes, the two 64-element MN atoms 16 KB apart).
-__device__ __forceinline__ uint64_t kmajor(uint32_t tile) { return smem_desc_sw128(tile, 16, 1024); }
-__device__ __forceinline__ uint64_t mnmajor(uint32_t tile) { return smem_desc_sw128(tile, kHalf, 1024); }
-__device__ __forceinline__ uint64_t kmajor_step(int kk) {
-  return static_cast<uint64_t>(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4);
-}
-__device__ __forceinline__ uint64_t mnmajor_step(int kk) { return static_cast<uint64_t>(kk * 128); }
-// D (+)= A B^T with both read K-major, and D (+)= A B with A K-major, B MN-major: 128 x 128 x 128
-__device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t b) {
-  const uint64_t da = kmajor(a), db = kmajor(b);
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk) umma_bf16(d, da + kmajor_step(kk), db + kmajor_step(kk), kIdKK, kk != 0 ? 1u : 0u);
-}
-__device__ __forceinline__ void mma_km(uint32_t d, uint32_t a, uint32_t b, bool first) {
-  const uint64_t da = kmajor(a), db = mnmajor(b);
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
-    umma_bf16(d, da + kmajor_step(kk), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
-}
-// 128 rows x 128 columns as two halves
-__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int head, int row, int b) {
-  tma_load_4d(dst, m, bar, 0, head, row, b);
-  tma_load_4d(dst + kHalf, m, bar, 64, head, row, b);
-}
-
-// One thread of the scheduler waits for up to three barriers, then both warps
-// meet; false once any wait has expired.
-__device__ __forceinline__ bool sched_wait(unsigned* err, uint64_t* b1, uint32_t p1, uint64_t* b2 = nullptr,
-                                           uint32_t p2 = 0u, uint64_t* b3 = nullptr, uint32_t p3 = 0u) {
-  bool good = true;
-  if ((threadIdx.x & 31) == 0) {
-    good = mbar_wait(b1, p1, err, kErrWaitFull);
-    if (good && b2) good = mbar_wait(b2, p2, err, kErrWaitFull);
-    if (good && b3) good = mbar_wait(b3, p3, err, kErrWaitAccumFree);
-  }
-  return go_barrier64<kGoBarrier>(__shfl_sync(0xffffffffu, good, 0));
 }
 
 // ---------------------------------------------------------------- dK and dV
@@ -1141,10 +1046,10 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   // after a launch, which makes the device's context current in a thread that
   // has not used it yet (autograd's); the encoder is a driver call and needs one
   CUtensorMap tk, tv, tq, tdo, tdq, tdk, tdv;
-  KDA_WB_TRY(tmap_head_rows(&tk, k, B, S, KH, k_strides[0], k_strides[1], k_strides[2]));
-  KDA_WB_TRY(tmap_head_rows(&tv, v, B, S, KH, v_strides[0], v_strides[1], v_strides[2]));
-  KDA_WB_TRY(tmap_head_rows(&tq, q, B, S, QH, q_strides[0], q_strides[1], q_strides[2]));
-  KDA_WB_TRY(tmap_head_rows(&tdo, dout, B, S, QH, dense_q[0], dense_q[1], dense_q[2]));
+  KDA_WB_TRY(tmap_head_rows(&tk, k, B, S, KH, k_strides));
+  KDA_WB_TRY(tmap_head_rows(&tv, v, B, S, KH, v_strides));
+  KDA_WB_TRY(tmap_head_rows(&tq, q, B, S, QH, q_strides));
+  KDA_WB_TRY(tmap_head_rows(&tdo, dout, B, S, QH, dense_q));
   KDA_WB_TRY(tmap_out(&tdq, dq, B, S, QH));
   KDA_WB_TRY(tmap_out(&tdk, dk, B, S, KH));
   KDA_WB_TRY(tmap_out(&tdv, dv, B, S, KH));

@@ -23,14 +23,13 @@
 // shared memory: one launch, no workspace, one fixed order of summation.
 #include <math.h>
 
-#include "common.cuh"
+#include "window.cuh"
 
 KDA_DEFINE_ERROR_WORD(window_decode)
 
 namespace kda {
 namespace {
 
-constexpr int kD = 128;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 3;

@@ -1,0 +1,512 @@
+// Forward of the sliding-window attention with sinks (head_dim 128, bf16) on
+// tcgen05.  Query i sees key j <= i where i - j < window or j < sinks:
+//   S = Q K^T,  P = 2^(S scale log2e - m),  O = P V / rowsum(P)
+// with m a running reference of each row's scores: it only moves when a score
+// exceeds it by more than 2^8, because weights up to 256 are as exact in bf16
+// and their sum in fp32 as weights up to 1.
+//
+// Work unit = (batch, query head, 256 query rows as two 128-row tiles); one
+// persistent CTA per SM.  Per unit the K and V blocks of its window (and those
+// with sinks before it) pass through a 3-slot TMA ring, K_0, K_1, V_0, K_2, V_1,
+// ..., and serve both tiles.  A tile skips the blocks that none of its rows sees.
+//
+// 640 threads: warp 0 TMA producer, warp 1 TMEM allocator + MMA issuer, warp 2
+// scheduler (performs every mbarrier wait the issuer needs and releases it group
+// by group at a named barrier: an mbarrier wait in the issuing thread would stall
+// behind its queued MMAs), warp 3 idle, warps 4-11 / 12-19 softmax of tile 0 / 1:
+// warp w reads TMEM lanes 32 (w % 4), 64 of a row's 128 keys per thread.  The two
+// tiles run half a step apart (issue order S_0(j+1) PV_0(j) S_1(j+1) PV_1(j)), so
+// one exponentiates while the other stores; S's columns are handed back as soon
+// as they are copied, so S(j+1) is there before P(j) is done.
+// The two warps that share a row agree on its reference with one bar.red a step
+// (did a score exceed it?) and exchange maxima only when one did.
+// V is read as stored (MN-major B), P from shared memory.
+// TMEM columns: S_0 [0,128), S_1 [128,256), O_0 [256,384), O_1 [384,512).
+// Shared memory: Q_0 | Q_1 | P_0 | P_1 | ring (3 x 32 KB) | row exchange.
+// Bound by the 128 B/clk of shared memory: 256 KB of MMA operands, 64 KB of loads
+// and 64 KB of P a step of two tiles, about 3,000 cycles.
+// All mbarrier waits are bounded (common.cuh); every TMA load targets one CTA.
+#include <math.h>
+
+#include "window.cuh"
+
+KDA_DEFINE_ERROR_WORD(window_fwd)
+
+namespace kda {
+namespace {
+
+constexpr int kSlots = 3;
+constexpr int kRowWarps = 16;
+constexpr int kThreads = 128 + 32 * kRowWarps;
+constexpr int kPairBarrier = 2;  // named barriers 2 .. 9: the two warps of a (tile, 32 rows)
+constexpr int kHalfBarrier = 10;  // 10 .. 13: the four warps of a (tile, 64 columns)
+
+struct FwdParams {
+  int B, S, QH, KH, rep;
+  int npairs;  // 256-row units per head
+  int window, sinks;
+  float scale_log2;  // softmax scale * log2(e)
+  float* lse;        // [B][QH][S] or null: each row's log2-sum-exp of the scaled scores
+};
+
+struct Smem {
+  static constexpr uint32_t kQ = 0, kP = 2 * kTile, kRing = 4 * kTile;
+  static constexpr uint32_t kExchange = 7 * kTile;  // 1 KB, fp32 [tile][row]: maxima and sums of two warps' halves
+  static constexpr uint32_t kBars = kExchange + 1024;
+  static constexpr uint32_t kNumBars = 24;
+  static constexpr size_t kBytes = 1024 + kBars + kNumBars * 8;
+  static_assert(kBytes > 116 * 1024 && kBytes <= 227 * 1024, "shared memory budget");
+};
+
+// A unit and the key blocks it visits: [0, ns) (sinks), then [ns + skip, nb + skip).
+struct Unit {
+  int b, h, q0;
+  int nb, ns, skip;
+};
+__device__ __forceinline__ Unit unit_at(const FwdParams& p, int u) {
+  const int heads = p.B * p.QH;
+  const int level = u / heads, bh = u - level * heads;
+  const int qp = p.npairs - 1 - level;  // the last units, which see the most, first
+  Unit c;
+  c.b = bh / p.QH;
+  c.h = bh - c.b * p.QH;
+  c.q0 = qp * 2 * kBlk;
+  const int all = (p.S + kBlk - 1) / kBlk;
+  const int last = min(2 * qp + 2, all);
+  const int first = max(0, c.q0 - p.window + 1) / kBlk;
+  c.ns = min((p.sinks + kBlk - 1) / kBlk, first);
+  c.nb = c.ns + last - first;
+  c.skip = first - c.ns;
+  return c;
+}
+__device__ __forceinline__ int key_block(const Unit& c, int j) { return j < c.ns ? j : j + c.skip; }
+// Whether any row of tile t sees a key of the unit's block j.
+__device__ __forceinline__ bool tile_sees(const FwdParams& p, const Unit& c, int t, int j) {
+  const int q0 = c.q0 + t * kBlk, k0 = key_block(c, j) * kBlk;
+  return q0 < p.S && k0 < q0 + kBlk && (k0 + kBlk > q0 - p.window + 1 || k0 < p.sinks);
+}
+
+// Ring items of a unit: K_0, K_1, V_0, K_2, V_1, ..., K_{nb-1}, V_{nb-2}, V_{nb-1};
+// `base` counts the items of earlier units.  Item x lives in slot x % 3.
+__device__ __forceinline__ uint32_t item_k(uint32_t base, int j) {
+  return base + (j == 0 ? 0u : 2u * static_cast<uint32_t>(j) - 1u);
+}
+__device__ __forceinline__ uint32_t item_v(uint32_t base, int j, int nb) {
+  return base + (j == nb - 1 ? 2u * static_cast<uint32_t>(nb) - 1u : 2u * static_cast<uint32_t>(j) + 2u);
+}
+__device__ __forceinline__ uint32_t item_slot(uint32_t x) { return x % kSlots; }
+__device__ __forceinline__ uint32_t item_par(uint32_t x) { return (x / kSlots) & 1u; }
+
+__global__ void __launch_bounds__(kThreads, 1)
+    window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                      const FwdParams p, unsigned* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
+  uint64_t* slot_full = bars;      // [3] an item landed
+  uint64_t* slot_free = bars + 3;  // [3] both tiles' MMAs that read it are done (or skip it)
+  uint64_t* q_full = bars + 6;     // one phase per unit: both Q tiles landed
+  // [2], per tile; one phase per block that the tile sees
+  uint64_t* s_ready = bars + 7;    // S in TMEM
+  uint64_t* s_free = bars + 9;     // S copied out (8 warps)
+  uint64_t* p_ready = bars + 11;   // P in its tile (8 warps)
+  uint64_t* pv_done = bars + 13;   // O += P V done
+  // [2], one phase per unit in which the tile has rows
+  uint64_t* o_free = bars + 15;    // O read out (8 warps)
+  uint64_t* drain = bars + 17;     // once
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 18);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 18; ++i) {
+      const bool rows = (i >= 9 && i <= 12) || i == 15 || i == 16;
+      mbar_init(bars + i, rows ? kRowWarps / 2 : i >= 3 && i < 6 ? 2 : 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmO);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  const int units = p.B * p.QH * p.npairs;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t base = 0, items = 0;  // items of earlier units; loads issued
+      int qs = 0;
+      uint32_t seen[2] = {0u, 0u};   // blocks each tile has seen
+      auto load_item = [&](uint32_t x, const CUtensorMap* m, int g, int j, int b) -> bool {
+        const uint32_t s = item_slot(x);
+        if (x >= kSlots && !mbar_wait(&slot_free[s], item_par(x) ^ 1u, err, kErrWaitEmpty)) return false;
+        mbar_arrive_expect_tx(&slot_full[s], kTile);
+        load_tile(smem + Smem::kRing + s * kTile, m, &slot_full[s], g, j * kBlk, b);
+        ++items;
+        return true;
+      };
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit c = unit_at(p, u);
+        const int g = c.h / p.rep;
+        // Q once the last S of both tiles is done
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && seen[t] > 0) ok = mbar_wait(&s_ready[t], (seen[t] - 1u) & 1u, err, kErrWaitEmpty);
+        if (!ok) break;
+        mbar_arrive_expect_tx(q_full, 2 * kTile);
+        for (int t = 0; t < 2; ++t) load_tile(smem + Smem::kQ + t * kTile, &tmQ, q_full, c.h, c.q0 + t * kBlk, c.b);
+        ++qs;
+        ok = load_item(item_k(base, 0), &tmK, g, key_block(c, 0), c.b);
+        for (int j = 0; j < c.nb && ok; ++j) {
+          if (j + 1 < c.nb) ok = load_item(item_k(base, j + 1), &tmK, g, key_block(c, j + 1), c.b);
+          if (ok) ok = load_item(item_v(base, j, c.nb), &tmV, g, key_block(c, j), c.b);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) seen[t] += tile_sees(p, c, t, j) ? 1u : 0u;
+        }
+        base += 2u * static_cast<uint32_t>(c.nb);
+      }
+      // no copy may still be writing shared memory when the CTA exits
+      if (qs > 0) mbar_drain(q_full, static_cast<uint32_t>(qs - 1) & 1u);
+      for (uint32_t s = 0; s < kSlots; ++s) {
+        const uint32_t uses = (items + kSlots - 1u - s) / kSlots;
+        if (uses > 0) mbar_drain(&slot_full[s], (uses - 1u) & 1u);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1 || warp == 2) {
+    // ------------------------------------------------ MMA issuer / scheduler
+    // Both warps walk the same groups and meet at the go barrier before each.
+    const bool sched = warp == 2;
+    const uint32_t sbase = smem_u32(smem);
+    uint32_t base = 0;
+    uint32_t ns[2] = {0u, 0u}, np[2] = {0u, 0u}, uo[2] = {0u, 0u};  // S, PV groups and units of each tile so far
+    int uc = 0;
+    bool ok = true, any = false;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
+      const Unit c = unit_at(p, u);
+      bool first[2] = {true, true};
+      // a tile that does not see the block releases its item (once it has landed:
+      // the slot's earlier phase is over then)
+      auto skip = [&](uint32_t x) -> bool {
+        const uint32_t s = item_slot(x);
+        const bool good = sched ? sched_wait(err, &slot_full[s], item_par(x)) : go_barrier64<kGoBarrier>(true);
+        if (good && sched && lane == 0) mbar_arrive(&slot_free[s]);
+        return good;
+      };
+      // S_t = Q_t K_j^T into the columns that the softmax warps have copied
+      auto s_group = [&](int t, int j) -> bool {
+        const uint32_t x = item_k(base, j), s = item_slot(x);
+        if (!tile_sees(p, c, t, j)) return skip(x);
+        const bool good = sched ? sched_wait(err, &slot_full[s], item_par(x), j == 0 ? q_full : nullptr,
+                                             static_cast<uint32_t>(uc) & 1u, ns[t] > 0 ? &s_free[t] : nullptr,
+                                             (ns[t] - 1u) & 1u)
+                                : go_barrier64<kGoBarrier>(true);
+        if (good && !sched && lane == 0) {
+          tc_fence_after();
+          mma_kk(tmem + t * kBlk, sbase + Smem::kQ + t * kTile, sbase + Smem::kRing + s * kTile);
+          umma_commit(&s_ready[t]);
+          umma_commit(&slot_free[s]);
+          any = true;
+        }
+        __syncwarp();
+        ++ns[t];
+        return good;
+      };
+      // O_t (+)= P_t V_j (the first of a unit once the last unit's O is read)
+      auto pv_group = [&](int t, int j) -> bool {
+        const uint32_t x = item_v(base, j, c.nb), s = item_slot(x);
+        if (!tile_sees(p, c, t, j)) return skip(x);
+        const bool good = sched ? sched_wait(err, &slot_full[s], item_par(x), &p_ready[t], np[t] & 1u,
+                                             first[t] && uo[t] > 0 ? &o_free[t] : nullptr, (uo[t] - 1u) & 1u)
+                                : go_barrier64<kGoBarrier>(true);
+        if (good && !sched && lane == 0) {
+          tc_fence_after();
+          mma_km(tmem + 256 + t * kBlk, sbase + Smem::kP + t * kTile, sbase + Smem::kRing + s * kTile, first[t]);
+          umma_commit(&pv_done[t]);
+          umma_commit(&slot_free[s]);
+        }
+        __syncwarp();
+        ++np[t];
+        first[t] = false;
+        return good;
+      };
+      ok = s_group(0, 0) && s_group(1, 0);
+      for (int j = 0; j < c.nb && ok; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (ok && j + 1 < c.nb) ok = s_group(t, j + 1);
+          if (ok) ok = pv_group(t, j);
+        }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) uo[t] += first[t] ? 0u : 1u;
+      base += 2u * static_cast<uint32_t>(c.nb);
+    }
+    if (!sched && lane == 0 && any) {
+      // every issued MMA must finish before TMEM is released
+      umma_commit(drain);
+      mbar_drain(drain, 0u);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------- softmax
+    const int t = (warp - 4) >> 3;          // tile
+    const int half = ((warp - 4) >> 2) & 1;  // keys (and columns of O) [64 half, + 64)
+    const int quad = warp & 3;
+    const int r = quad * 32 + lane;  // query row of this thread (TMEM lane)
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t scol = lanes + t * kBlk + 64 * half;
+    const uint32_t ocol = lanes + 256 + t * kBlk + 64 * half;
+    uint8_t* tile = smem + Smem::kP + t * kTile + half * kHalf;
+    const uint32_t row = smem_u32(tile) + static_cast<uint32_t>(r * 128);
+    const uint32_t rsw = static_cast<uint32_t>(r & 7);
+    float* xch = reinterpret_cast<float*>(smem + Smem::kExchange) + t * kBlk + r;
+    const int pair = kPairBarrier + t * 4 + quad, quarter = kHalfBarrier + t * 2 + half;
+    const bool elected = quad == 0 && lane == 0;  // issues this (tile, half)'s output
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+    uint32_t n = 0;  // blocks seen so far
+    bool ok = true, stored = false;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const Unit c = unit_at(p, u);
+      const int qpos = c.q0 + t * kBlk + r;
+      if (c.q0 + t * kBlk >= p.S) continue;  // no rows (both halves alike)
+      if (stored) {  // the last unit's output has left P's tile
+        if (elected) bulk_wait_read_all();
+        ok = bar_and(quarter, 128, ok);
+        if (!ok) break;
+      }
+      float m = -INFINITY, l = 0.f;
+      bool first = true;
+      // A wait that expires does not leave the loop by itself: its warp meets its
+      // partner at the next pair barrier (or the unit's end) and both leave there.
+      for (int j = 0; j < c.nb; ++j) {
+        if (!tile_sees(p, c, t, j)) continue;
+        const uint32_t par = n & 1u;
+        const int k0 = key_block(c, j) * kBlk + 64 * half;  // this thread's first key
+        if (ok) ok = mbar_wait(&s_ready[t], par, err, kErrWaitAccum);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        uint32_t s[64];
+        tmem_ld_32x32b_x32(scol, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_ld_32x32b_x32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+        tmem_ld_wait();
+        tc_fence_before();
+        if (ok) mbar_arrive_warp(&s_free[t]);
+        // keys [k0, k0 + hi) are not after the query; of those, keys before k0 + old
+        // only as sinks.  The test is on the tile's first and last row: most blocks
+        // are visible whole.
+        const int q0 = c.q0 + t * kBlk;
+        if (k0 + 63 > q0 || (k0 + p.window < q0 + kBlk && k0 + 64 > p.sinks)) {
+          const int hi = qpos + 1 - k0, old = qpos + 1 - p.window - k0, sink = min(hi, p.sinks - k0);
+          const uint32_t live0 = range_mask(old, hi) | range_mask(0, sink);
+          const uint32_t live1 = range_mask(old - 32, hi - 32) | range_mask(-32, sink - 32);
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            s[i] = ((i < 32 ? live0 : live1) >> (i & 31)) & 1u ? s[i] : 0xff800000u;  // -inf
+        }
+        float mx;
+        {
+          float a[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) a[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 4]));
+#pragma unroll
+          for (int i = 8; i < 64; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] = fmax3(a[k], __uint_as_float(s[i + k]), __uint_as_float(s[i + 4 + k]));
+          mx = fmaxf(fmax3(a[0], a[1], a[2]), a[3]) * p.scale_log2;
+        }
+        // a score above the reference by 2^8 anywhere in these 32 rows (or a wait
+        // that expired): both warps exchange their maxima and move the reference
+        if (bar_or(pair, 64, !ok || mx > m + 8.f)) {
+          if (half == 1) *xch = mx;
+          ok = bar_and(pair, 64, ok);
+          if (!ok) break;
+          if (half == 0) *xch = fmaxf(m, fmaxf(mx, *xch));
+          bar_sync(pair, 64);
+          const float m_new = *xch;
+          const float f = m_new == -INFINITY ? 1.f : exp2_approx(m - m_new);
+          m = m_new;
+          l *= f;
+          if (!first) {
+            // O += P V of the last block must be done before O is rescaled
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], par ^ 1u, err, kErrWaitAccum));
+            if (ok) {
+              tc_fence_after();
+#pragma unroll 1
+              for (int k = 0; k < 64; k += 16) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(ocol + k, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st_32x32b_x16(ocol + k, o);
+              }
+              tmem_st_wait();
+              tc_fence_before();
+            }
+          }
+        }
+        const float mb = m == -INFINITY ? 0.f : m;
+        const float2 nm2 = make_float2(-mb, -mb);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 a = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, nm2);
+          const float2 e = make_float2(exp2_approx(a.x), exp2_approx(a.y));
+          sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+          s[i] = pack_bf16x2(e.x, e.y);  // the weights meet V as bf16, the tensor core's operand type
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        // P's tile is free once O += P V of the last block is done
+        if (ok && !first) ok = mbar_wait(&pv_done[t], par ^ 1u, err, kErrWaitAccum);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            st_shared_v4(row + ((static_cast<uint32_t>(v) ^ rsw) << 4), s[4 * v], s[4 * v + 1], s[4 * v + 2],
+                         s[4 * v + 3]);
+          fence_proxy_async_smem();
+          tc_fence_before();
+          mbar_arrive_warp(&p_ready[t]);
+        }
+        first = false;
+        ++n;
+      }
+      // O / l to bf16, through P's tile, out by TMA (rows past S are not written)
+      if (ok) ok = mbar_wait(&pv_done[t], (n - 1u) & 1u, err, kErrWaitAccum);
+      ok = bar_and(quarter, 128, ok);
+      // the two halves' sums: half 1 hands its over, half 0 answers with the whole
+      if (half == 1) *xch = l;
+      ok = bar_and(pair, 64, ok);
+      if (!ok) break;
+      if (half == 0) {
+        l += *xch;
+        *xch = l;
+        if (p.lse && qpos < p.S)
+          p.lse[(static_cast<int64_t>(c.b) * p.QH + c.h) * p.S + qpos] = (m == -INFINITY ? 0.f : m) + __log2f(l);
+      }
+      bar_sync(pair, 64);
+      if (half == 1) l = *xch;
+      tc_fence_after();
+      const float inv = 1.0f / l;
+      uint32_t o[64];
+      tmem_ld_32x32b_x32(ocol, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+      tmem_ld_32x32b_x32(ocol + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive_warp(&o_free[t]);
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * k]) * inv, __uint_as_float(o[8 * v + 2 * k + 1]) * inv);
+        st_shared_v4(row + ((static_cast<uint32_t>(v) ^ rsw) << 4), w[0], w[1], w[2], w[3]);
+      }
+      fence_proxy_async_smem();
+      bar_sync(quarter, 128);
+      if (elected) {
+        tma_store_4d(&tmO, tile, 64 * half, c.h, c.q0 + t * kBlk, c.b);
+        bulk_commit();
+      }
+      stored = true;
+    }
+    if (elected) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace
+
+kda_status gqa_window_check(const char* op, int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window,
+                            int64_t sinks) {
+  KDA_CHECK_ARG(B > 0 && S > 0 && QH > 0 && KH > 0 && QH % KH == 0, "%s: bad sizes B=%lld S=%lld QH=%lld KH=%lld", op,
+                (long long)B, (long long)S, (long long)QH, (long long)KH);
+  KDA_CHECK_ARG(window > 0 && sinks >= 0, "%s: window must be positive and sinks not negative, got %lld and %lld", op,
+                (long long)window, (long long)sinks);
+  KDA_CHECK_SUPPORTED(D == kD, "%s: head_dim must be 128, got %lld", op, (long long)D);
+  KDA_CHECK_SUPPORTED(S < (1ll << 24) && QH <= 65535 && B <= 65535 && B * S < (1ll << 31) / QH,
+                      "%s: too many rows (B=%lld S=%lld QH=%lld)", op, (long long)B, (long long)S, (long long)QH);
+  return KDA_OK;
+}
+
+bool head_rows_ok(const void* p, const int64_t* s) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 &&
+         s[0] >= 0 && s[1] >= 0 && s[2] >= 0;
+}
+
+kda_status tmap_head_rows(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H, const int64_t* strides) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(H), static_cast<uint64_t>(S),
+                            static_cast<uint64_t>(B)};
+  const uint64_t st[3] = {static_cast<uint64_t>(H > 1 ? strides[2] : kD) * 2,
+                          static_cast<uint64_t>(S > 1 ? strides[1] : kD) * 2,
+                          static_cast<uint64_t>(B > 1 ? strides[0] : kD) * 2};
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(kBlk), 1};
+  return make_tmap_bf16(m, base, 4, dims, st, box);
+}
+
+}  // namespace kda
+
+using namespace kda;
+
+extern "C" kda_status kda_gqa_window_bf16(const void* q, const void* k, const void* v, void* out, float* lse,
+                                          int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window,
+                                          int64_t sinks, const int64_t* q_strides, const int64_t* k_strides,
+                                          const int64_t* v_strides, void* stream) {
+  const char* op = "gqa_window";
+  kda_status s;
+  if ((s = gqa_window_check(op, B, S, QH, KH, D, window, sinks)) != KDA_OK) return s;
+  KDA_CHECK_ARG(q && k && v && out && q_strides && k_strides && v_strides, "%s: null pointer", op);
+  const int64_t dense[3] = {S * QH * kD, QH * kD, kD};
+  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
+                          head_rows_ok(out, dense),
+                      "%s: pointers and rows must be 16-byte aligned", op);
+  FwdParams p{};
+  p.B = static_cast<int>(B);
+  p.S = static_cast<int>(S);
+  p.QH = static_cast<int>(QH);
+  p.KH = static_cast<int>(KH);
+  p.rep = static_cast<int>(QH / KH);
+  p.npairs = static_cast<int>((S + 2 * kBlk - 1) / (2 * kBlk));
+  p.window = static_cast<int>(window < S ? window : S);
+  p.sinks = static_cast<int>(sinks < S ? sinks : S);
+  p.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(kD)));
+  p.lse = lse;
+  static std::atomic<bool> attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(window_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(Smem::kBytes)) != cudaSuccess)
+      return launch_status("gqa_window: cudaFuncSetAttribute");
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  // the encoder is a driver call that needs a current context: a thread that has
+  // not used the device yet (autograd's) gets it here
+  cudaSetDevice(dev);
+  CUtensorMap tq, tk, tv, to;
+  if ((s = tmap_head_rows(&tq, q, B, S, QH, q_strides)) != KDA_OK) return s;
+  if ((s = tmap_head_rows(&tk, k, B, S, KH, k_strides)) != KDA_OK) return s;
+  if ((s = tmap_head_rows(&tv, v, B, S, KH, v_strides)) != KDA_OK) return s;
+  if ((s = tmap_head_rows(&to, out, B, S, QH, dense)) != KDA_OK) return s;
+  const int64_t units = B * QH * p.npairs;
+  const int grid = static_cast<int>(units < num_sms() ? units : num_sms());
+  window_fwd_kernel<<<grid, kThreads, Smem::kBytes, static_cast<cudaStream_t>(stream)>>>(tq, tk, tv, to, p,
+                                                                                         kda_err_ptr_window_fwd());
+  return launch_status("gqa_window");
+}

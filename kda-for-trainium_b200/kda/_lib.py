@@ -101,8 +101,7 @@ PROTOTYPES = {
     "kda_qk_norm_rope_backward_workspace_size": (SZ, [I64, I64, I64, I64, I64, INT]),
     "kda_qk_norm_rope_backward": (INT, [P, P, P, P, P, P, P, I64, P, F, P, P, P, P, I64, I64, I64, I64, I64, P, P,
                                         INT, P, SZ, P]),
-    "kda_gqa_window_workspace_size": (SZ, [I64, I64, I64, I64, I64]),
-    "kda_gqa_window_bf16": (INT, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P, SZ, P]),
+    "kda_gqa_window_bf16": (INT, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P]),
     "kda_gqa_window_backward_workspace_size": (SZ, [I64, I64, I64, I64, I64, I64, I64]),
     "kda_gqa_window_backward_bf16": (INT, [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P,
                                            SZ, P]),

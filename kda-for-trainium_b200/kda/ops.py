@@ -663,18 +663,18 @@ def qk_norm_rope_append(q, k, v, gq, gk, table, k_cache, v_cache, lengths, *, ep
     return _native.qk_norm_rope_append(q, k, v, gq, gk, table, k_cache, v_cache, lengths, eps, q_out)
 
 
-def gqa_window(q, k, v, window, sinks=0, *, out=None, workspace=None):
+def gqa_window(q, k, v, window, sinks=0, *, out=None):
     """Causal grouped-query attention inside a sliding window with sinks: query i
     sees key j <= i where i - j < window or j < sinks.  q (B,S,QH,128), k, v
     (B,S,KH,128) bf16, views are fine; returns (B,S,QH,128).  No rotation (see
     ``qk_norm_rope``); scores scaled by 1 / sqrt(128)."""
-    return _native.gqa_window(q, k, v, window, sinks, out, False, workspace)[0]
+    return _native.gqa_window(q, k, v, window, sinks, out, False)[0]
 
 
-def gqa_window_lse(q, k, v, window, sinks=0, *, workspace=None):
+def gqa_window_lse(q, k, v, window, sinks=0):
     """``gqa_window`` that also returns each query row's log2-sum-exp of the
     scaled scores, (B, QH, S) fp32: the forward of a training step."""
-    return _native.gqa_window(q, k, v, window, sinks, None, True, workspace)
+    return _native.gqa_window(q, k, v, window, sinks, None, True)
 
 
 def gqa_window_backward(dout, q, k, v, out, lse, window, sinks=0, *, workspace=None):

@@ -122,8 +122,8 @@ def test_c_entries_reject_bad_arguments(kda):
     def norm(B=1, S=2, D=128, eps=1e-6, q=16, st=s3, tab=2):
         _lib.call("kda_qk_norm_rope", q, 16, 16, 16, 16, tab, None, eps, 16, 16, B, S, 4, 1, D, st, s3, 0, None)
 
-    def window(S=2, D=128, QH=4, w=1, sinks=0, q=16, st=s3, ws=16, nb=1 << 20):
-        _lib.call("kda_gqa_window_bf16", q, 16, 16, 16, None, 1, S, QH, 1, D, w, sinks, st, s3, s3, ws, nb, None)
+    def window(S=2, D=128, QH=4, w=1, sinks=0, q=16, st=s3):
+        _lib.call("kda_gqa_window_bf16", q, 16, 16, 16, None, 1, S, QH, 1, D, w, sinks, st, s3, s3, None)
 
     def decode(T=2, D=128, QH=4, w=1, sinks=0, q=16, st=s3):
         _lib.call("kda_gqa_window_decode_bf16", q, 16, 16, 16, 16, 1, T, QH, 1, D, w, sinks, s3, st, s3, None)
@@ -134,8 +134,7 @@ def test_c_entries_reject_bad_arguments(kda):
 
     for bad in (lambda: norm(B=0), lambda: norm(S=0), lambda: norm(eps=-1.0), lambda: norm(q=None),
                 lambda: norm(tab=1), lambda: window(S=0), lambda: window(w=0), lambda: window(sinks=-1),
-                lambda: window(q=None), lambda: window(nb=1), lambda: window(ws=None), lambda: decode(T=0),
-                lambda: decode(w=0), lambda: decode(q=None), lambda: backward(S=0), lambda: backward(w=0),
+                lambda: window(q=None), lambda: decode(T=0), lambda: decode(w=0), lambda: decode(q=None), lambda: backward(S=0), lambda: backward(w=0),
                 lambda: backward(nb=8)):
         with pytest.raises(ValueError):
             bad()
@@ -546,7 +545,8 @@ def test_refusals(kda):
         lambda: kda.gqa_window(q, wide[..., 4:], kv, 4),          # rows off 16 bytes
         lambda: kda.gqa_window(q, kv[:, :, :1].expand(-1, -1, 2, -1), kv, 4),
         lambda: kda.gqa_window(q, kv, kv.transpose(2, 3).contiguous().transpose(2, 3), 4),
-        lambda: kda.gqa_window(q, kv, kv, 4, workspace=torch.empty(8, dtype=torch.uint8, device="cuda")),
+        lambda: kda.gqa_window_backward(q, q, kv, kv, q, torch.zeros(1, 4, 4, device="cuda"), 4,
+                                        workspace=torch.empty(8, dtype=torch.uint8, device="cuda")),
         lambda: kda.gqa_window_backward(q, q, kv, kv, q, torch.zeros(1, 4, 5, device="cuda"), 4),
         lambda: kda.qk_norm_rope(q, kv, g[:64], g, table), lambda: kda.qk_norm_rope(q, kv, g, g.to(BF16), table),
         lambda: kda.qk_norm_rope(q, kv, g, g, table[:3]), lambda: kda.qk_norm_rope(q, kv, g, g, table[:, :32]),
