@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       {
         const uint32_t pp = static_cast<uint32_t>(pieces) & 1u, nb = static_cast<uint32_t>(n0) & 1u;
         const uint32_t use = static_cast<uint32_t>(n0 >> 1) & 1u;
-        ok = sched ? sched_wait(err, k_full, pp, &q_full[nb], use) : go_barrier64<kGoBarrier>(true);
+        ok = sched ? sched_wait(kGoBarrier, err, k_full, pp, &q_full[nb], use) : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           any = true;
         }
         __syncwarp();
-        ok = sched ? sched_wait(err, v_full, pp, do_full, nb) : go_barrier64<kGoBarrier>(true);
+        ok = sched ? sched_wait(kGoBarrier, err, v_full, pp, do_full, nb) : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool more = i + 1 < c.n;
         // S^T(n + 1)
         if (more) {
-          ok = sched ? sched_wait(err, &q_full[ob], use, s_free, par) : go_barrier64<kGoBarrier>(true);
+          ok = sched ? sched_wait(kGoBarrier, err, &q_full[ob], use, s_free, par) : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
           if (!sched && lane == 0) {
             tc_fence_after();
@@ -359,9 +359,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         // dV_j += P^T(n) dO(n) (the first of a piece once the last piece's sums are read)
-        ok = sched ? sched_wait(err, p_ready, par, i == 0 && pieces > 0 ? acc_free : nullptr,
+        ok = sched ? sched_wait(kGoBarrier, err, p_ready, par, i == 0 && pieces > 0 ? acc_free : nullptr,
                                 static_cast<uint32_t>(pieces - 1) & 1u)
-                   : go_barrier64<kGoBarrier>(true);
+                   : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         // dK_j += dS^T(n) Q(n)
-        ok = sched ? sched_wait(err, ds_ready, par) : go_barrier64<kGoBarrier>(true);
+        ok = sched ? sched_wait(kGoBarrier, err, ds_ready, par) : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         // dP^T(n + 1)
         if (more) {
-          ok = sched ? sched_wait(err, do_full, ob) : go_barrier64<kGoBarrier>(true);
+          ok = sched ? sched_wait(kGoBarrier, err, do_full, ob) : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
           if (!sched && lane == 0) {
             tc_fence_after();
@@ -686,9 +686,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit c = dq_unit(p, u);
       auto s_group = [&](int n, bool first) -> bool {  // S(n): its columns were copied before dP(n - 1) was issued
         const int kb = n % 3;
-        const bool good = sched ? sched_wait(err, &k_full[kb], static_cast<uint32_t>(n / 3) & 1u,
+        const bool good = sched ? sched_wait(kGoBarrier, err, &k_full[kb], static_cast<uint32_t>(n / 3) & 1u,
                                              first ? qdo_full : nullptr, static_cast<uint32_t>(uc) & 1u)
-                                : go_barrier64<kGoBarrier>(true);
+                                : bar_and(kGoBarrier, 64, true);
         if (good && !sched && lane == 0) {
           tc_fence_after();
           mma_kk(tmem + (n & 1) * 384, base + kQ, base + kK + kb * kTile);
@@ -705,8 +705,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j + 1 < c.n) {
           // dP(n + 1) into the columns that the row warps have copied
           const uint32_t nb = static_cast<uint32_t>(n + 1) & 1u;
-          ok = sched ? sched_wait(err, v_full, nb, n + 1 > 0 ? sp_free : nullptr, nb ^ 1u)
-                     : go_barrier64<kGoBarrier>(true);
+          ok = sched ? sched_wait(kGoBarrier, err, v_full, nb, n + 1 > 0 ? sp_free : nullptr, nb ^ 1u)
+                     : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
           if (!sched && lane == 0) {
             tc_fence_after();
@@ -720,9 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j >= 0) {
           // dQ += dS(n) K (the first of a unit once the last unit's dQ is read)
           const int kb = n % 3;
-          ok = sched ? sched_wait(err, ds_ready, static_cast<uint32_t>(n) & 1u, j == 0 && uc > 0 ? dq_free : nullptr,
+          ok = sched ? sched_wait(kGoBarrier, err, ds_ready, static_cast<uint32_t>(n) & 1u, j == 0 && uc > 0 ? dq_free : nullptr,
                                   static_cast<uint32_t>(uc - 1) & 1u)
-                     : go_barrier64<kGoBarrier>(true);
+                     : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
           if (!sched && lane == 0) {
             tc_fence_after();

@@ -10,14 +10,17 @@
 // with sinks before it) pass through a 3-slot TMA ring, K_0, K_1, V_0, K_2, V_1,
 // ..., and serve both tiles.  A tile skips the blocks that none of its rows sees.
 //
-// 640 threads: warp 0 TMA producer, warp 1 TMEM allocator + MMA issuer, warp 2
-// scheduler (performs every mbarrier wait the issuer needs and releases it group
-// by group at a named barrier: an mbarrier wait in the issuing thread would stall
-// behind its queued MMAs), warp 3 idle, warps 4-11 / 12-19 softmax of tile 0 / 1:
-// warp w reads TMEM lanes 32 (w % 4), 64 of a row's 128 keys per thread.  The two
-// tiles run half a step apart (issue order S_0(j+1) PV_0(j) S_1(j+1) PV_1(j)), so
-// one exponentiates while the other stores; S's columns are handed back as soon
-// as they are copied, so S(j+1) is there before P(j) is done.
+// 640 threads: warp 0 TMA producer, warps 1 and 3 MMA issuers of tile 0 and 1
+// (warp 1 allocates TMEM), warp 2 scheduler, warps 4-11 / 12-19 softmax of tile
+// 0 / 1: warp w reads TMEM lanes 32 (w % 4), 64 of a row's 128 keys per thread.
+// The scheduler performs every mbarrier wait the issuers need and releases them
+// round by round at a named barrier: an mbarrier wait in an issuing thread would
+// stall behind its queued MMAs.  A round has an S of one tile and a P V of the
+// other, S_0(j+1) | PV_1(j-1), then PV_0(j) | S_1(j+1): the tiles run half a step
+// apart, one exponentiates while the other stores, and the tensor core always has
+// two groups queued (with one issuer and four groups a step, a step of both tiles
+// took 4,560 cycles, 1,700 of them between groups).  S's columns are handed back
+// as soon as they are copied, so S(j+1) is there before P(j) is done.
 // The two warps that share a row agree on its reference with one bar.red a step
 // (did a score exceed it?) and exchange maxima only when one did.
 // V is read as stored (MN-major B), P from shared memory.
@@ -80,10 +83,19 @@ __device__ __forceinline__ Unit unit_at(const FwdParams& p, int u) {
   return c;
 }
 __device__ __forceinline__ int key_block(const Unit& c, int j) { return j < c.ns ? j : j + c.skip; }
-// Whether any row of tile t sees a key of the unit's block j.
-__device__ __forceinline__ bool tile_sees(const FwdParams& p, const Unit& c, int t, int j) {
-  const int q0 = c.q0 + t * kBlk, k0 = key_block(c, j) * kBlk;
-  return q0 < p.S && k0 < q0 + kBlk && (k0 + kBlk > q0 - p.window + 1 || k0 < p.sinks);
+// The unit's blocks that any row of a tile sees: j < sinks and from <= j < to.
+struct Seen {
+  int sinks, from, to;
+  __device__ __forceinline__ bool at(int j) const { return j < sinks || (j >= from && j < to); }
+};
+__device__ __forceinline__ Seen tile_sees(const FwdParams& p, const Unit& c, int t) {
+  const int q0 = c.q0 + t * kBlk;
+  if (q0 >= p.S) return {0, 0, 0};
+  const int first = max(0, q0 - p.window + 1) / kBlk;  // >= the unit's, which goes by tile 0
+  // blocks [0, sink blocks) of key order that lie in the walk: those before ns, and
+  // where the window reaches down to them, the ones from ns on
+  const int sinks = (p.sinks + kBlk - 1) / kBlk, to = q0 / kBlk + 1 - c.skip;
+  return {min(max(c.ns, sinks - c.skip), to), max(first, c.ns + c.skip) - c.skip, to};
 }
 
 // Ring items of a unit: K_0, K_1, V_0, K_2, V_1, ..., K_{nb-1}, V_{nb-2}, V_{nb-1};
@@ -106,7 +118,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
   uint64_t* slot_full = bars;      // [3] an item landed
   uint64_t* slot_free = bars + 3;  // [3] both tiles' MMAs that read it are done (or skip it)
-  uint64_t* q_full = bars + 6;     // one phase per unit: both Q tiles landed
   // [2], per tile; one phase per block that the tile sees
   uint64_t* s_ready = bars + 7;    // S in TMEM
   uint64_t* s_free = bars + 9;     // S copied out (8 warps)
@@ -114,13 +125,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* pv_done = bars + 13;   // O += P V done
   // [2], one phase per unit in which the tile has rows
   uint64_t* o_free = bars + 15;    // O read out (8 warps)
+  uint64_t* q_full = bars + 19;    // Q landed
   uint64_t* drain = bars + 17;     // once
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 18);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 21);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 18; ++i) {
+    for (int i = 0; i < 21; ++i) {
       const bool rows = (i >= 9 && i <= 12) || i == 15 || i == 16;
       mbar_init(bars + i, rows ? kRowWarps / 2 : i >= 3 && i < 6 ? 2 : 1);
     }
@@ -147,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       bool ok = true;
       uint32_t base = 0, items = 0;  // items of earlier units; loads issued
-      int qs = 0;
+      int qs[2] = {0, 0};
       uint32_t seen[2] = {0u, 0u};   // blocks each tile has seen
       auto load_item = [&](uint32_t x, const CUtensorMap* m, int g, int j, int b) -> bool {
         const uint32_t s = item_slot(x);
@@ -160,106 +172,148 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
         const Unit c = unit_at(p, u);
         const int g = c.h / p.rep;
-        // Q once the last S of both tiles is done
+        const Seen sees[2] = {tile_sees(p, c, 0), tile_sees(p, c, 1)};
+        // Q of a tile that has rows, once its last S is done
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (ok && seen[t] > 0) ok = mbar_wait(&s_ready[t], (seen[t] - 1u) & 1u, err, kErrWaitEmpty);
+          if (sees[t].to > 0) {
+            if (ok && seen[t] > 0) ok = mbar_wait(&s_ready[t], (seen[t] - 1u) & 1u, err, kErrWaitEmpty);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&q_full[t], kTile);
+            load_tile(smem + Smem::kQ + t * kTile, &tmQ, &q_full[t], c.h, c.q0 + t * kBlk, c.b);
+            ++qs[t];
+          }
         if (!ok) break;
-        mbar_arrive_expect_tx(q_full, 2 * kTile);
-        for (int t = 0; t < 2; ++t) load_tile(smem + Smem::kQ + t * kTile, &tmQ, q_full, c.h, c.q0 + t * kBlk, c.b);
-        ++qs;
         ok = load_item(item_k(base, 0), &tmK, g, key_block(c, 0), c.b);
         for (int j = 0; j < c.nb && ok; ++j) {
           if (j + 1 < c.nb) ok = load_item(item_k(base, j + 1), &tmK, g, key_block(c, j + 1), c.b);
           if (ok) ok = load_item(item_v(base, j, c.nb), &tmV, g, key_block(c, j), c.b);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) seen[t] += tile_sees(p, c, t, j) ? 1u : 0u;
+          for (int t = 0; t < 2; ++t) seen[t] += sees[t].at(j) ? 1u : 0u;
         }
         base += 2u * static_cast<uint32_t>(c.nb);
       }
       // no copy may still be writing shared memory when the CTA exits
-      if (qs > 0) mbar_drain(q_full, static_cast<uint32_t>(qs - 1) & 1u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (qs[t] > 0) mbar_drain(&q_full[t], static_cast<uint32_t>(qs[t] - 1) & 1u);
       for (uint32_t s = 0; s < kSlots; ++s) {
         const uint32_t uses = (items + kSlots - 1u - s) / kSlots;
         if (uses > 0) mbar_drain(&slot_full[s], (uses - 1u) & 1u);
       }
     }
     __syncwarp();
-  } else if (warp == 1 || warp == 2) {
-    // ------------------------------------------------ MMA issuer / scheduler
-    // Both warps walk the same groups and meet at the go barrier before each.
+  } else if (warp < 4) {
+    // ------------------------------------------- MMA issuers and scheduler
+    // The three warps walk the same rounds and meet before each.
     const bool sched = warp == 2;
+    const int mine = warp == 3 ? 1 : 0;  // an issuer's tile
     const uint32_t sbase = smem_u32(smem);
-    uint32_t base = 0;
-    uint32_t ns[2] = {0u, 0u}, np[2] = {0u, 0u}, uo[2] = {0u, 0u};  // S, PV groups and units of each tile so far
-    int uc = 0;
+    // The units' blocks one after the other.  A round has blocks of different
+    // units where one ends, so that the tensor core is not drained there.
+    struct Block {
+      bool valid;
+      uint32_t k, v;                 // its ring items
+      bool sees0, sees1, new0, new1;  // whether a tile sees it, and as its unit's first
+    };
+    int u = blockIdx.x, j = -1;
+    uint32_t base = 0;  // ring items of earlier units
+    Unit c = u < units ? unit_at(p, u) : Unit{};
+    Seen see0 = tile_sees(p, c, 0), see1 = tile_sees(p, c, 1);
+    bool open0 = true, open1 = true;
+    auto next_block = [&]() -> Block {
+      if (u >= units) return {false, 0u, 0u, false, false, false, false};
+      if (++j == c.nb) {
+        base += 2u * static_cast<uint32_t>(c.nb);
+        u += gridDim.x;
+        if (u >= units) return {false, 0u, 0u, false, false, false, false};
+        c = unit_at(p, u);
+        see0 = tile_sees(p, c, 0);
+        see1 = tile_sees(p, c, 1);
+        open0 = open1 = true;
+        j = 0;
+      }
+      const bool a = see0.at(j), b = see1.at(j);
+      const Block blk = {true, item_k(base, j), item_v(base, j, c.nb), a, b, a && open0, b && open1};
+      open0 = open0 && !a;
+      open1 = open1 && !b;
+      return blk;
+    };
+    uint32_t ns[2] = {0u, 0u}, np[2] = {0u, 0u}, qn[2] = {0u, 0u}, on[2] = {0u, 0u};  // S, PV groups, units begun by each
     bool ok = true, any = false;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
-      const Unit c = unit_at(p, u);
-      bool first[2] = {true, true};
-      // a tile that does not see the block releases its item (once it has landed:
-      // the slot's earlier phase is over then)
-      auto skip = [&](uint32_t x) -> bool {
-        const uint32_t s = item_slot(x);
-        const bool good = sched ? sched_wait(err, &slot_full[s], item_par(x)) : go_barrier64<kGoBarrier>(true);
-        if (good && sched && lane == 0) mbar_arrive(&slot_free[s]);
-        return good;
-      };
-      // S_t = Q_t K_j^T into the columns that the softmax warps have copied
-      auto s_group = [&](int t, int j) -> bool {
-        const uint32_t x = item_k(base, j), s = item_slot(x);
-        if (!tile_sees(p, c, t, j)) return skip(x);
-        const bool good = sched ? sched_wait(err, &slot_full[s], item_par(x), j == 0 ? q_full : nullptr,
-                                             static_cast<uint32_t>(uc) & 1u, ns[t] > 0 ? &s_free[t] : nullptr,
-                                             (ns[t] - 1u) & 1u)
-                                : go_barrier64<kGoBarrier>(true);
-        if (good && !sched && lane == 0) {
+    // One thread's waits for S_t: K (and Q) landed, the columns copied out.  A tile
+    // that does not see the block releases its item (once it has landed: the
+    // slot's earlier phase is over then).
+    auto wait_s = [&](int t, uint32_t x, bool sees, bool begins) -> bool {
+      const uint32_t s = item_slot(x);
+      if (!mbar_wait(&slot_full[s], item_par(x), err, kErrWaitFull)) return false;
+      if (!sees) {
+        mbar_arrive(&slot_free[s]);
+        return true;
+      }
+      if (begins && !mbar_wait(&q_full[t], qn[t] & 1u, err, kErrWaitFull)) return false;
+      return ns[t] == 0 || mbar_wait(&s_free[t], (ns[t] - 1u) & 1u, err, kErrWaitAccumFree);
+    };
+    // and for O_t (+)= P_t V: V landed, P written, the last unit's O read
+    auto wait_pv = [&](int t, uint32_t x, bool sees, bool begins) -> bool {
+      const uint32_t s = item_slot(x);
+      if (!mbar_wait(&slot_full[s], item_par(x), err, kErrWaitFull)) return false;
+      if (!sees) {
+        mbar_arrive(&slot_free[s]);
+        return true;
+      }
+      if (!mbar_wait(&p_ready[t], np[t] & 1u, err, kErrWaitFull)) return false;
+      return !begins || on[t] == 0 || mbar_wait(&o_free[t], (on[t] - 1u) & 1u, err, kErrWaitAccumFree);
+    };
+    // S of tile ts, P V of the other
+    auto round = [&](const int ts, const Block& sb, const Block& pb) -> bool {
+      const int tp = 1 - ts;
+      const bool s_sees = ts == 0 ? sb.sees0 : sb.sees1, s_new = ts == 0 ? sb.new0 : sb.new1;
+      const bool p_sees = tp == 0 ? pb.sees0 : pb.sees1, p_new = tp == 0 ? pb.new0 : pb.new1;
+      bool good = true;
+      if (sched && lane == 0) {
+        if (sb.valid) good = wait_s(ts, sb.k, s_sees, s_new);
+        if (good && pb.valid) good = wait_pv(tp, pb.v, p_sees, p_new);
+      }
+      good = bar_and(kGoBarrier, 96, __shfl_sync(0xffffffffu, good, 0));
+      if (good && !sched && lane == 0) {
+        if (s_sees && mine == ts) {
+          const uint32_t s = item_slot(sb.k);
           tc_fence_after();
-          mma_kk(tmem + t * kBlk, sbase + Smem::kQ + t * kTile, sbase + Smem::kRing + s * kTile);
-          umma_commit(&s_ready[t]);
+          mma_kk(tmem + ts * kBlk, sbase + Smem::kQ + ts * kTile, sbase + Smem::kRing + s * kTile);
+          umma_commit(&s_ready[ts]);
           umma_commit(&slot_free[s]);
           any = true;
         }
-        __syncwarp();
-        ++ns[t];
-        return good;
-      };
-      // O_t (+)= P_t V_j (the first of a unit once the last unit's O is read)
-      auto pv_group = [&](int t, int j) -> bool {
-        const uint32_t x = item_v(base, j, c.nb), s = item_slot(x);
-        if (!tile_sees(p, c, t, j)) return skip(x);
-        const bool good = sched ? sched_wait(err, &slot_full[s], item_par(x), &p_ready[t], np[t] & 1u,
-                                             first[t] && uo[t] > 0 ? &o_free[t] : nullptr, (uo[t] - 1u) & 1u)
-                                : go_barrier64<kGoBarrier>(true);
-        if (good && !sched && lane == 0) {
+        if (p_sees && mine == tp) {
+          const uint32_t s = item_slot(pb.v);
           tc_fence_after();
-          mma_km(tmem + 256 + t * kBlk, sbase + Smem::kP + t * kTile, sbase + Smem::kRing + s * kTile, first[t]);
-          umma_commit(&pv_done[t]);
+          mma_km(tmem + 256 + tp * kBlk, sbase + Smem::kP + tp * kTile, sbase + Smem::kRing + s * kTile, p_new);
+          umma_commit(&pv_done[tp]);
           umma_commit(&slot_free[s]);
         }
-        __syncwarp();
-        ++np[t];
-        first[t] = false;
-        return good;
-      };
-      ok = s_group(0, 0) && s_group(1, 0);
-      for (int j = 0; j < c.nb && ok; ++j)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (ok && j + 1 < c.nb) ok = s_group(t, j + 1);
-          if (ok) ok = pv_group(t, j);
-        }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) uo[t] += first[t] ? 0u : 1u;
-      base += 2u * static_cast<uint32_t>(c.nb);
+      }
+      __syncwarp();
+      ns[ts] += s_sees ? 1u : 0u;
+      qn[ts] += s_new ? 1u : 0u;
+      np[tp] += p_sees ? 1u : 0u;
+      on[tp] += p_new ? 1u : 0u;
+      return good;
+    };
+    Block b2 = {false, 0u, 0u, false, false, false, false}, b1 = b2, b0 = next_block();  // blocks k - 1, k, k + 1
+    while (ok && (b0.valid || b1.valid || b2.valid)) {
+      ok = round(0, b0, b2) && round(1, b0, b1);
+      b2 = b1;
+      b1 = b0;
+      b0 = next_block();
     }
     if (!sched && lane == 0 && any) {
       // every issued MMA must finish before TMEM is released
-      umma_commit(drain);
-      mbar_drain(drain, 0u);
+      umma_commit(&drain[mine]);
+      mbar_drain(&drain[mine], 0u);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------------------- softmax
     const int t = (warp - 4) >> 3;          // tile
     const int half = ((warp - 4) >> 2) & 1;  // keys (and columns of O) [64 half, + 64)
@@ -281,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit c = unit_at(p, u);
       const int qpos = c.q0 + t * kBlk + r;
       if (c.q0 + t * kBlk >= p.S) continue;  // no rows (both halves alike)
+      const Seen sees = tile_sees(p, c, t);
       if (stored) {  // the last unit's output has left P's tile
         if (elected) bulk_wait_read_all();
         ok = bar_and(quarter, 128, ok);
@@ -291,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A wait that expires does not leave the loop by itself: its warp meets its
       // partner at the next pair barrier (or the unit's end) and both leave there.
       for (int j = 0; j < c.nb; ++j) {
-        if (!tile_sees(p, c, t, j)) continue;
+        if (!sees.at(j)) continue;
         const uint32_t par = n & 1u;
         const int k0 = key_block(c, j) * kBlk + 64 * half;  // this thread's first key
         if (ok) ok = mbar_wait(&s_ready[t], par, err, kErrWaitAccum);
@@ -309,11 +364,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int q0 = c.q0 + t * kBlk;
         if (k0 + 63 > q0 || (k0 + p.window < q0 + kBlk && k0 + 64 > p.sinks)) {
           const int hi = qpos + 1 - k0, old = qpos + 1 - p.window - k0, sink = min(hi, p.sinks - k0);
-          const uint32_t live0 = range_mask(old, hi) | range_mask(0, sink);
-          const uint32_t live1 = range_mask(old - 32, hi - 32) | range_mask(-32, sink - 32);
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            s[i] = ((i < 32 ? live0 : live1) >> (i & 31)) & 1u ? s[i] : 0xff800000u;  // -inf
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t live = range_mask(old - 32 * w, hi - 32 * w) | range_mask(0, sink - 32 * w);
+            if (live != 0xffffffffu)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[32 * w + i] = (live >> i) & 1u ? s[32 * w + i] : 0xff800000u;  // -inf
+          }
         }
         float mx;
         {
