@@ -11,7 +11,7 @@ constexpr int kD = 128;                    // head dim
 constexpr int kBlk = 128;                  // rows of a block of queries or keys
 constexpr uint32_t kTile = kBlk * kD * 2;  // 32 KB: two halves of 64 columns, 128-byte rows, 128-byte swizzle
 constexpr uint32_t kHalf = kTile / 2;
-constexpr int kGoBarrier = 1;              // named barrier: scheduler warp + MMA issuer's warp
+constexpr int kGoBarrier = 1;              // named barrier: the scheduler's and the MMA issuers' warps
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -121,8 +121,8 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, ui
 }
 
 // One thread of the scheduler waits for up to three barriers, then its warp and
-// the issuer's meet at named barrier `id`; false once any wait has expired.
-__device__ __forceinline__ bool sched_wait(int id, unsigned* err, uint64_t* b1, uint32_t p1, uint64_t* b2 = nullptr,
+// the issuers' (`threads` in all) meet; false once any wait has expired.
+__device__ __forceinline__ bool sched_wait(int threads, unsigned* err, uint64_t* b1, uint32_t p1, uint64_t* b2 = nullptr,
                                            uint32_t p2 = 0u, uint64_t* b3 = nullptr, uint32_t p3 = 0u) {
   bool good = true;
   if ((threadIdx.x & 31) == 0) {
@@ -130,7 +130,7 @@ __device__ __forceinline__ bool sched_wait(int id, unsigned* err, uint64_t* b1, 
     if (good && b2) good = mbar_wait(b2, p2, err, kErrWaitFull);
     if (good && b3) good = mbar_wait(b3, p3, err, kErrWaitAccumFree);
   }
-  return bar_and(id, 64, __shfl_sync(0xffffffffu, good, 0));
+  return bar_and(kGoBarrier, threads, __shfl_sync(0xffffffffu, good, 0));
 }
 
 // The entry points' size checks; whether strided head rows start on 16 bytes; the

@@ -135,12 +135,6 @@ __device__ __forceinline__ Piece piece_after(const BwdParams& p, const Piece& c,
   return d;
 }
 __device__ __forceinline__ int64_t run_start(const BwdParams& p, int cta, int ctas) { return p.total * cta / ctas; }
-// Head and query block of step `it` of a walk.
-__device__ __forceinline__ int step_head(const BwdParams& p, int g, const Piece& c, int it) {
-  return g * p.rep + it / c.nq;
-}
-__device__ __forceinline__ int step_block(const Piece& c, int it) { return c.j + it % c.nq; }
-
 // 32 values of a row as bf16 into a K-major, 128-byte-swizzled half tile: columns
 // [8u, 8u + 8) of the half = 16-byte unit u, at u ^ (row % 8); u0 the first unit.
 __device__ __forceinline__ void store32(uint32_t row, int u0, uint32_t rsw, const float2 (&e)[16]) {
@@ -252,12 +246,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       int ks = 0, vs = 0, qs = 0, dos = 0, lses = 0, dis = 0;  // loads issued
       while (ok) {
         const int b = c.bg / p.KH, g = c.bg - b * p.KH;
+        int h = g * p.rep + c.it0 / c.nq, q = c.it0 % c.nq;  // head; query block of the walk
         for (int i = 0; i < c.n; ++i) {
           const int n = n0 + i;
           const uint32_t pprev = static_cast<uint32_t>(n - 1) & 1u;
           const uint32_t use = static_cast<uint32_t>((n >> 1) - 1) & 1u;  // phase of step n - 2 in its buffer
-          const int h = step_head(p, g, c, c.it0 + i);
-          const int s0 = step_block(c, c.it0 + i) * kBlk;
+          const int s0 = (c.j + q) * kBlk;
           const int nb = n & 1;
           const int64_t row = (static_cast<int64_t>(b) * p.QH + h) * p.sp + s0;
           if (n >= 2) ok = mbar_wait(&q_free[nb], use, err, kErrWaitEmpty);
@@ -294,6 +288,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(di_full, kBlk * 4);
           bulk_load_1d(smem + Smem::kDi, p.ndi + row, kBlk * 4, di_full);
           ++dis;
+          if (++q == c.nq) {
+            q = 0;
+            ++h;
+          }
         }
         n0 += c.n;
         if (n0 >= run) break;
@@ -324,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       {
         const uint32_t pp = static_cast<uint32_t>(pieces) & 1u, nb = static_cast<uint32_t>(n0) & 1u;
         const uint32_t use = static_cast<uint32_t>(n0 >> 1) & 1u;
-        ok = sched ? sched_wait(kGoBarrier, err, k_full, pp, &q_full[nb], use) : bar_and(kGoBarrier, 64, true);
+        ok = sched ? sched_wait(64, err, k_full, pp, &q_full[nb], use) : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
@@ -333,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           any = true;
         }
         __syncwarp();
-        ok = sched ? sched_wait(kGoBarrier, err, v_full, pp, do_full, nb) : bar_and(kGoBarrier, 64, true);
+        ok = sched ? sched_wait(64, err, v_full, pp, do_full, nb) : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
@@ -349,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool more = i + 1 < c.n;
         // S^T(n + 1)
         if (more) {
-          ok = sched ? sched_wait(kGoBarrier, err, &q_full[ob], use, s_free, par) : bar_and(kGoBarrier, 64, true);
+          ok = sched ? sched_wait(64, err, &q_full[ob], use, s_free, par) : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
           if (!sched && lane == 0) {
             tc_fence_after();
@@ -359,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         // dV_j += P^T(n) dO(n) (the first of a piece once the last piece's sums are read)
-        ok = sched ? sched_wait(kGoBarrier, err, p_ready, par, i == 0 && pieces > 0 ? acc_free : nullptr,
+        ok = sched ? sched_wait(64, err, p_ready, par, i == 0 && pieces > 0 ? acc_free : nullptr,
                                 static_cast<uint32_t>(pieces - 1) & 1u)
                    : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
@@ -370,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         // dK_j += dS^T(n) Q(n)
-        ok = sched ? sched_wait(kGoBarrier, err, ds_ready, par) : bar_and(kGoBarrier, 64, true);
+        ok = sched ? sched_wait(64, err, ds_ready, par) : bar_and(kGoBarrier, 64, true);
         if (!ok) break;
         if (!sched && lane == 0) {
           tc_fence_after();
@@ -381,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         // dP^T(n + 1)
         if (more) {
-          ok = sched ? sched_wait(kGoBarrier, err, do_full, ob) : bar_and(kGoBarrier, 64, true);
+          ok = sched ? sched_wait(64, err, do_full, ob) : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
           if (!sched && lane == 0) {
             tc_fence_after();
@@ -422,11 +420,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       // sees it; none when the key is past S
       const int qlo = kpos >= p.S ? p.S : kpos;
       const int qhi = kpos < p.sinks ? p.S : min(p.S, kpos + p.window);
+      int q = c.it0 % c.nq;  // query block of the walk
       for (int i = 0; i < c.n; ++i) {
         const int n = n0 + i;
         const uint32_t par = static_cast<uint32_t>(n) & 1u;
-        const int s0 = step_block(c, c.it0 + i) * kBlk + 32 * grp;  // this thread's first query
+        const int s0 = (c.j + q) * kBlk + 32 * grp;  // this thread's first query
         const uint32_t live = range_mask(qlo - s0, qhi - s0);
+        q = q + 1 == c.nq ? 0 : q + 1;
         ok = mbar_wait(s_ready, par, err, kErrWaitAccum) && mbar_wait(lse_full, par, err, kErrWaitFull);
         if (i == 0 && pieces > 0) {  // the last piece's dV, dK have left the tile
           if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Unit c = dq_unit(p, u);
       auto s_group = [&](int n, bool first) -> bool {  // S(n): its columns were copied before dP(n - 1) was issued
         const int kb = n % 3;
-        const bool good = sched ? sched_wait(kGoBarrier, err, &k_full[kb], static_cast<uint32_t>(n / 3) & 1u,
+        const bool good = sched ? sched_wait(64, err, &k_full[kb], static_cast<uint32_t>(n / 3) & 1u,
                                              first ? qdo_full : nullptr, static_cast<uint32_t>(uc) & 1u)
                                 : bar_and(kGoBarrier, 64, true);
         if (good && !sched && lane == 0) {
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j + 1 < c.n) {
           // dP(n + 1) into the columns that the row warps have copied
           const uint32_t nb = static_cast<uint32_t>(n + 1) & 1u;
-          ok = sched ? sched_wait(kGoBarrier, err, v_full, nb, n + 1 > 0 ? sp_free : nullptr, nb ^ 1u)
+          ok = sched ? sched_wait(64, err, v_full, nb, n + 1 > 0 ? sp_free : nullptr, nb ^ 1u)
                      : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
           if (!sched && lane == 0) {
@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j >= 0) {
           // dQ += dS(n) K (the first of a unit once the last unit's dQ is read)
           const int kb = n % 3;
-          ok = sched ? sched_wait(kGoBarrier, err, ds_ready, static_cast<uint32_t>(n) & 1u, j == 0 && uc > 0 ? dq_free : nullptr,
+          ok = sched ? sched_wait(64, err, ds_ready, static_cast<uint32_t>(n) & 1u, j == 0 && uc > 0 ? dq_free : nullptr,
                                   static_cast<uint32_t>(uc - 1) & 1u)
                      : bar_and(kGoBarrier, 64, true);
           if (!ok) break;
