@@ -563,3 +563,12 @@ def test_refusals(kda):
     ):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.gpu
+def test_example_runs():
+    import runpy
+
+    from conftest import REPO
+    worst = runpy.run_path(str(REPO / "examples" / "local_attention.py"))["main"]()
+    assert worst <= 4 * 2.0 ** -8
