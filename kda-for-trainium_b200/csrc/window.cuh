@@ -48,6 +48,19 @@ __device__ __forceinline__ bool bar_or(int id, int threads, bool v) {
       : "memory");
   return r != 0;
 }
+// Whether a phase is complete, without waiting: asked early, so that the answer's
+// latency (200 cycles and more beside the tensor core's operand reads) is hidden.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return r != 0;
+}
 // Every committed bulk store of this thread has read its shared memory.
 __device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, const void* src, int x, int y, int z, int w) {
@@ -102,6 +115,16 @@ __device__ __forceinline__ uint64_t kmajor_step(int kk) {
   return static_cast<uint64_t>(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4);
 }
 __device__ __forceinline__ uint64_t mnmajor_step(int kk) { return static_cast<uint64_t>(kk * 128); }
+// D (+)= A B with A in TMEM: lane = row of A, 32-bit column = two of its columns
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // D (+)= A B^T with both read K-major, and D (+)= A B with A K-major, B MN-major: 128 x 128 x 128
 __device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t b) {
   const uint64_t da = kmajor(a), db = kmajor(b);
@@ -113,6 +136,12 @@ __device__ __forceinline__ void mma_km(uint32_t d, uint32_t a, uint32_t b, bool 
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
     umma_bf16(d, da + kmajor_step(kk), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
+}
+// D (+)= A B with A (bf16 pairs, 64 columns) in TMEM and B MN-major
+__device__ __forceinline__ void mma_tm(uint32_t d, uint32_t a, uint32_t b, bool first) {
+  const uint64_t db = mnmajor(b);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) umma_bf16_ts(d, a + 8 * kk, db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
 }
 // 128 rows x 128 columns as two halves
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int head, int row, int b) {

@@ -41,6 +41,10 @@ namespace {
 constexpr int kSlots = 3;
 constexpr int kRowWarps = 16;
 constexpr int kThreads = 128 + 32 * kRowWarps;
+// Registers per thread: at launch (what the compiler reports for 640 threads), and
+// after the control warpgroup has given some to the four of row warps.
+constexpr int kRegsLaunch = 96, kRegsCtl = 64, kRegsRow = 104;
+static_assert(128 * kRegsCtl + 32 * kRowWarps * kRegsRow <= kThreads * kRegsLaunch, "register split");
 constexpr int kPairBarrier = 2;  // named barriers 2 .. 9: the two warps of a (tile, 32 rows)
 constexpr int kHalfBarrier = 10;  // 10 .. 13: the four warps of a (tile, 64 columns)
 
@@ -117,11 +121,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
   uint64_t* slot_full = bars;      // [3] an item landed
-  uint64_t* slot_free = bars + 3;  // [3] both tiles' MMAs that read it are done (or skip it)
+  uint64_t* slot_free = bars + 3;  // [3] the MMAs that read it are done
+  uint64_t* s_free = bars + 9;     // S copied out (8 warps); one phase per S, of either tile
   // [2], per tile; one phase per block that the tile sees
   uint64_t* s_ready = bars + 7;    // S in TMEM
-  uint64_t* s_free = bars + 9;     // S copied out (8 warps)
-  uint64_t* p_ready = bars + 11;   // P in its tile (8 warps)
+  uint64_t* p_ready = bars + 11;   // P in TMEM (8 warps)
   uint64_t* pv_done = bars + 13;   // O += P V done
   // [2], one phase per unit in which the tile has rows
   uint64_t* o_free = bars + 15;    // O read out (8 warps)
@@ -133,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 21; ++i) {
-      const bool rows = (i >= 9 && i <= 12) || i == 15 || i == 16;
-      mbar_init(bars + i, rows ? kRowWarps / 2 : i >= 3 && i < 6 ? 2 : 1);
+      const bool rows = i == 9 || i == 11 || i == 12 || i == 15 || i == 16;
+      mbar_init(bars + i, rows ? kRowWarps / 2 : 1);
     }
     fence_mbar_init();
   }
@@ -154,6 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_holder;
   const int units = p.B * p.QH * p.npairs;
 
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -204,123 +209,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp < 4) {
-    // ------------------------------------------- MMA issuers and scheduler
-    // The three warps walk the same rounds and meet before each.
-    const bool sched = warp == 2;
-    const int mine = warp == 3 ? 1 : 0;  // an issuer's tile
-    const uint32_t sbase = smem_u32(smem);
-    // The units' blocks one after the other.  A round has blocks of different
-    // units where one ends, so that the tensor core is not drained there.
-    struct Block {
-      bool valid;
-      uint32_t k, v;                 // its ring items
-      bool sees0, sees1, new0, new1;  // whether a tile sees it, and as its unit's first
-    };
-    int u = blockIdx.x, j = -1;
-    uint32_t base = 0;  // ring items of earlier units
-    Unit c = u < units ? unit_at(p, u) : Unit{};
-    Seen see0 = tile_sees(p, c, 0), see1 = tile_sees(p, c, 1);
-    bool open0 = true, open1 = true;
-    auto next_block = [&]() -> Block {
-      if (u >= units) return {false, 0u, 0u, false, false, false, false};
-      if (++j == c.nb) {
+    // ------------------------------- MMA issuers: S (warp 1) and P V (warp 3)
+    if ((warp == 1 || warp == 3) && lane == 0) {
+      const uint32_t ring = smem_u32(smem) + Smem::kRing, qs = smem_u32(smem) + Smem::kQ;
+      const bool is_s = warp == 1;
+      uint32_t base = 0;           // ring items of earlier units
+      uint32_t ns = 0;             // S so far, of both tiles
+      uint32_t np[2] = {0u, 0u};   // a tile's P V so far
+      uint32_t un[2] = {0u, 0u};   // and its units
+      bool ok = true, any = false;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit c = unit_at(p, u);
+        const Seen sees[2] = {tile_sees(p, c, 0), tile_sees(p, c, 1)};
+        bool begins[2] = {true, true};
+        for (int j = 0; j < c.nb && ok; ++j) {
+          const uint32_t x = is_s ? item_k(base, j) : item_v(base, j, c.nb), slot = item_slot(x);
+          const uint32_t tile = ring + slot * kTile;
+          bool seen = false;
+          ok = mbar_wait(&slot_full[slot], item_par(x), err, kErrWaitFull);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || !sees[t].at(j)) continue;
+            if (is_s) {  // Q landed, the last S copied out
+              if (begins[t]) ok = mbar_wait(&q_full[t], un[t] & 1u, err, kErrWaitFull);
+              if (ok && ns > 0) ok = mbar_wait(s_free, (ns - 1u) & 1u, err, kErrWaitAccumFree);
+              if (!ok) continue;
+              tc_fence_after();
+              mma_kk(tmem, qs + t * kTile, tile);
+              umma_commit(&s_ready[t]);
+              ++ns;
+            } else {  // P written, the last unit's O read
+              ok = mbar_wait(&p_ready[t], np[t] & 1u, err, kErrWaitFull);
+              if (ok && begins[t] && un[t] > 0) ok = mbar_wait(&o_free[t], (un[t] - 1u) & 1u, err, kErrWaitAccumFree);
+              if (!ok) continue;
+              tc_fence_after();
+              mma_tm(tmem + 256 + t * kBlk, tmem + 128 + t * 64, tile, begins[t]);
+              umma_commit(&pv_done[t]);
+              ++np[t];
+            }
+            un[t] += begins[t] ? 1u : 0u;
+            begins[t] = false;
+            seen = any = true;
+          }
+          if (seen) umma_commit(&slot_free[slot]);  // once this thread's MMAs have read the item
+          else if (ok) mbar_arrive(&slot_free[slot]);
+        }
         base += 2u * static_cast<uint32_t>(c.nb);
-        u += gridDim.x;
-        if (u >= units) return {false, 0u, 0u, false, false, false, false};
-        c = unit_at(p, u);
-        see0 = tile_sees(p, c, 0);
-        see1 = tile_sees(p, c, 1);
-        open0 = open1 = true;
-        j = 0;
       }
-      const bool a = see0.at(j), b = see1.at(j);
-      const Block blk = {true, item_k(base, j), item_v(base, j, c.nb), a, b, a && open0, b && open1};
-      open0 = open0 && !a;
-      open1 = open1 && !b;
-      return blk;
-    };
-    uint32_t ns[2] = {0u, 0u}, np[2] = {0u, 0u}, qn[2] = {0u, 0u}, on[2] = {0u, 0u};  // S, PV groups, units begun by each
-    bool ok = true, any = false;
-    // One thread's waits for S_t: K (and Q) landed, the columns copied out.  A tile
-    // that does not see the block releases its item (once it has landed: the
-    // slot's earlier phase is over then).
-    auto wait_s = [&](int t, uint32_t x, bool sees, bool begins) -> bool {
-      const uint32_t s = item_slot(x);
-      if (!mbar_wait(&slot_full[s], item_par(x), err, kErrWaitFull)) return false;
-      if (!sees) {
-        mbar_arrive(&slot_free[s]);
-        return true;
+      if (any) {
+        // every issued MMA must finish before TMEM is released
+        umma_commit(&drain[is_s ? 0 : 1]);
+        mbar_drain(&drain[is_s ? 0 : 1], 0u);
       }
-      if (begins && !mbar_wait(&q_full[t], qn[t] & 1u, err, kErrWaitFull)) return false;
-      return ns[t] == 0 || mbar_wait(&s_free[t], (ns[t] - 1u) & 1u, err, kErrWaitAccumFree);
-    };
-    // and for O_t (+)= P_t V: V landed, P written, the last unit's O read
-    auto wait_pv = [&](int t, uint32_t x, bool sees, bool begins) -> bool {
-      const uint32_t s = item_slot(x);
-      if (!mbar_wait(&slot_full[s], item_par(x), err, kErrWaitFull)) return false;
-      if (!sees) {
-        mbar_arrive(&slot_free[s]);
-        return true;
-      }
-      if (!mbar_wait(&p_ready[t], np[t] & 1u, err, kErrWaitFull)) return false;
-      return !begins || on[t] == 0 || mbar_wait(&o_free[t], (on[t] - 1u) & 1u, err, kErrWaitAccumFree);
-    };
-    // S of tile ts, P V of the other
-    auto round = [&](const int ts, const Block& sb, const Block& pb) -> bool {
-      const int tp = 1 - ts;
-      const bool s_sees = ts == 0 ? sb.sees0 : sb.sees1, s_new = ts == 0 ? sb.new0 : sb.new1;
-      const bool p_sees = tp == 0 ? pb.sees0 : pb.sees1, p_new = tp == 0 ? pb.new0 : pb.new1;
-      bool good = true;
-      if (sched && lane == 0) {
-        if (sb.valid) good = wait_s(ts, sb.k, s_sees, s_new);
-        if (good && pb.valid) good = wait_pv(tp, pb.v, p_sees, p_new);
-      }
-      good = bar_and(kGoBarrier, 96, __shfl_sync(0xffffffffu, good, 0));
-      if (good && !sched && lane == 0) {
-        if (s_sees && mine == ts) {
-          const uint32_t s = item_slot(sb.k);
-          tc_fence_after();
-          mma_kk(tmem + ts * kBlk, sbase + Smem::kQ + ts * kTile, sbase + Smem::kRing + s * kTile);
-          umma_commit(&s_ready[ts]);
-          umma_commit(&slot_free[s]);
-          any = true;
-        }
-        if (p_sees && mine == tp) {
-          const uint32_t s = item_slot(pb.v);
-          tc_fence_after();
-          mma_km(tmem + 256 + tp * kBlk, sbase + Smem::kP + tp * kTile, sbase + Smem::kRing + s * kTile, p_new);
-          umma_commit(&pv_done[tp]);
-          umma_commit(&slot_free[s]);
-        }
-      }
-      __syncwarp();
-      ns[ts] += s_sees ? 1u : 0u;
-      qn[ts] += s_new ? 1u : 0u;
-      np[tp] += p_sees ? 1u : 0u;
-      on[tp] += p_new ? 1u : 0u;
-      return good;
-    };
-    Block b2 = {false, 0u, 0u, false, false, false, false}, b1 = b2, b0 = next_block();  // blocks k - 1, k, k + 1
-    while (ok && (b0.valid || b1.valid || b2.valid)) {
-      ok = round(0, b0, b2) && round(1, b0, b1);
-      b2 = b1;
-      b1 = b0;
-      b0 = next_block();
-    }
-    if (!sched && lane == 0 && any) {
-      // every issued MMA must finish before TMEM is released
-      umma_commit(&drain[mine]);
-      mbar_drain(&drain[mine], 0u);
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsRow));
     const int t = (warp - 4) >> 3;          // tile
     const int half = ((warp - 4) >> 2) & 1;  // keys (and columns of O) [64 half, + 64)
     const int quad = warp & 3;
     const int r = quad * 32 + lane;  // query row of this thread (TMEM lane)
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t scol = lanes + t * kBlk + 64 * half;
+    const uint32_t scol = lanes + 64 * half;
+    const uint32_t pcol = lanes + 128 + 64 * t + 32 * half;
     const uint32_t ocol = lanes + 256 + t * kBlk + 64 * half;
     uint8_t* tile = smem + Smem::kP + t * kTile + half * kHalf;
     const uint32_t row = smem_u32(tile) + static_cast<uint32_t>(r * 128);
@@ -329,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int pair = kPairBarrier + t * 4 + quad, quarter = kHalfBarrier + t * 2 + half;
     const bool elected = quad == 0 && lane == 0;  // issues this (tile, half)'s output
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-    uint32_t n = 0;  // blocks seen so far
+    uint32_t n = 0;   // blocks seen so far
     bool ok = true, stored = false;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const Unit c = unit_at(p, u);
@@ -345,11 +297,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool first = true;
       // A wait that expires does not leave the loop by itself: its warp meets its
       // partner at the next pair barrier (or the unit's end) and both leave there.
-      for (int j = 0; j < c.nb; ++j) {
-        if (!sees.at(j)) continue;
+      bool s_there = false;  // S is known to be ready
+      for (int j = sees.sinks > 0 ? 0 : sees.from; j < sees.to; j = j + 1 >= sees.sinks ? max(j + 1, sees.from) : j + 1) {
         const uint32_t par = n & 1u;
         const int k0 = key_block(c, j) * kBlk + 64 * half;  // this thread's first key
-        if (ok) ok = mbar_wait(&s_ready[t], par, err, kErrWaitAccum);
+        if (ok && !s_there) ok = mbar_wait(&s_ready[t], par, err, kErrWaitAccum);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         uint32_t s[64];
@@ -357,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_32x32b_x32(scol + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
         tmem_ld_wait();
         tc_fence_before();
-        if (ok) mbar_arrive_warp(&s_free[t]);
+        if (ok) mbar_arrive_warp(s_free);
         // keys [k0, k0 + hi) are not after the query; of those, keys before k0 + old
         // only as sinks.  The test is on the tile's first and last row: most blocks
         // are visible whole.
@@ -414,6 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        const bool p_free = first || mbar_test(&pv_done[t], par ^ 1u);
         const float mb = m == -INFINITY ? 0.f : m;
         const float2 nm2 = make_float2(-mb, -mb);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -425,15 +378,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           s[i] = pack_bf16x2(e.x, e.y);  // the weights meet V as bf16, the tensor core's operand type
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        // P's tile is free once O += P V of the last block is done
-        if (ok && !first) ok = mbar_wait(&pv_done[t], par ^ 1u, err, kErrWaitAccum);
+        // P's columns are free once O += P V of the last block is done
+        if (ok && !p_free) ok = mbar_wait(&pv_done[t], par ^ 1u, err, kErrWaitAccum);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
-#pragma unroll
-          for (int v = 0; v < 8; ++v)
-            st_shared_v4(row + ((static_cast<uint32_t>(v) ^ rsw) << 4), s[4 * v], s[4 * v + 1], s[4 * v + 2],
-                         s[4 * v + 3]);
-          fence_proxy_async_smem();
+          tmem_st_32x32b_x16(pcol, *reinterpret_cast<const uint32_t(*)[16]>(&s[0]));
+          tmem_st_32x32b_x16(pcol + 16, *reinterpret_cast<const uint32_t(*)[16]>(&s[16]));
+          s_there = mbar_test(&s_ready[t], par ^ 1u);
+          tmem_st_wait();
           tc_fence_before();
           mbar_arrive_warp(&p_ready[t]);
         }
@@ -548,6 +500,10 @@ extern "C" kda_status kda_gqa_window_bf16(const void* q, const void* k, const vo
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, window_fwd_kernel) != cudaSuccess) return launch_status("gqa_window: attributes");
+    KDA_CHECK_SUPPORTED(fa.numRegs == kRegsLaunch, "%s: kernel compiled to %d registers/thread, its split needs %d", op,
+                        fa.numRegs, kRegsLaunch);
     if (cudaFuncSetAttribute(window_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(Smem::kBytes)) != cudaSuccess)
       return launch_status("gqa_window: cudaFuncSetAttribute");
