@@ -48,6 +48,16 @@ __device__ __forceinline__ bool bar_or(int id, int threads, bool v) {
       : "memory");
   return r != 0;
 }
+// For warps that run as one and issue from one elected lane (uniform control flow
+// keeps descriptors in uniform registers: a product issues in fewer cycles).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
 // Whether a phase is complete, without waiting: asked early, so that the answer's
 // latency (200 cycles and more beside the tensor core's operand reads) is hidden.
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -142,6 +152,13 @@ __device__ __forceinline__ void mma_tm(uint32_t d, uint32_t a, uint32_t b, bool 
   const uint64_t db = mnmajor(b);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) umma_bf16_ts(d, a + 8 * kk, db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
+}
+// with A's K steps in pairs 32 columns apart: [0, 16), [32, 48), ... of 128
+__device__ __forceinline__ void mma_tm_pairs(uint32_t d, uint32_t a, uint32_t b, bool first) {
+  const uint64_t db = mnmajor(b);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    umma_bf16_ts(d, a + 32 * (kk >> 1) + 8 * (kk & 1), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
 }
 // 128 rows x 128 columns as two halves
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int head, int row, int b) {

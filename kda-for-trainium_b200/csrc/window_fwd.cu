@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp < 4) {
     // ------------------------------- MMA issuers: S (warp 1) and P V (warp 3)
-    if ((warp == 1 || warp == 3) && lane == 0) {
+    if (warp == 1 || warp == 3) {
+      const bool one = elect_one();
       const uint32_t ring = smem_u32(smem) + Smem::kRing, qs = smem_u32(smem) + Smem::kQ;
       const bool is_s = warp == 1;
       uint32_t base = 0;           // ring items of earlier units
@@ -226,37 +227,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t x = is_s ? item_k(base, j) : item_v(base, j, c.nb), slot = item_slot(x);
           const uint32_t tile = ring + slot * kTile;
           bool seen = false;
-          ok = mbar_wait(&slot_full[slot], item_par(x), err, kErrWaitFull);
+          ok = warp_wait(&slot_full[slot], item_par(x), err, kErrWaitFull);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || !sees[t].at(j)) continue;
             if (is_s) {  // Q landed, the last S copied out
-              if (begins[t]) ok = mbar_wait(&q_full[t], un[t] & 1u, err, kErrWaitFull);
-              if (ok && ns > 0) ok = mbar_wait(s_free, (ns - 1u) & 1u, err, kErrWaitAccumFree);
+              if (begins[t]) ok = warp_wait(&q_full[t], un[t] & 1u, err, kErrWaitFull);
+              if (ok && ns > 0) ok = warp_wait(s_free, (ns - 1u) & 1u, err, kErrWaitAccumFree);
               if (!ok) continue;
               tc_fence_after();
-              mma_kk(tmem, qs + t * kTile, tile);
-              umma_commit(&s_ready[t]);
+              if (one) {
+                mma_kk(tmem, qs + t * kTile, tile);
+                umma_commit(&s_ready[t]);
+              }
               ++ns;
             } else {  // P written, the last unit's O read
-              ok = mbar_wait(&p_ready[t], np[t] & 1u, err, kErrWaitFull);
-              if (ok && begins[t] && un[t] > 0) ok = mbar_wait(&o_free[t], (un[t] - 1u) & 1u, err, kErrWaitAccumFree);
+              ok = warp_wait(&p_ready[t], np[t] & 1u, err, kErrWaitFull);
+              if (ok && begins[t] && un[t] > 0) ok = warp_wait(&o_free[t], (un[t] - 1u) & 1u, err, kErrWaitAccumFree);
               if (!ok) continue;
               tc_fence_after();
-              mma_tm(tmem + 256 + t * kBlk, tmem + 128 + t * 64, tile, begins[t]);
-              umma_commit(&pv_done[t]);
+              if (one) {
+                mma_tm(tmem + 256 + t * kBlk, tmem + 128 + t * 64, tile, begins[t]);
+                umma_commit(&pv_done[t]);
+              }
               ++np[t];
             }
             un[t] += begins[t] ? 1u : 0u;
             begins[t] = false;
             seen = any = true;
           }
-          if (seen) umma_commit(&slot_free[slot]);  // once this thread's MMAs have read the item
-          else if (ok) mbar_arrive(&slot_free[slot]);
+          if (one && seen) umma_commit(&slot_free[slot]);  // once this thread's MMAs have read the item
+          else if (one && ok) mbar_arrive(&slot_free[slot]);
         }
         base += 2u * static_cast<uint32_t>(c.nb);
       }
-      if (any) {
+      if (one && any) {
         // every issued MMA must finish before TMEM is released
         umma_commit(&drain[is_s ? 0 : 1]);
         mbar_drain(&drain[is_s ? 0 : 1], 0u);
