@@ -70,14 +70,14 @@ struct BwdParams {
 
 // Seven tiles, then small things.
 struct Smem {
-  // dkv: K_j | V_j | Q (two buffers) | dO | P^T | dS^T
+  // dkv: K_j | V_j | Q (two buffers) | dO (two) | results on their way out
   // dq:  Q | dO | K (three buffers) | V | dS
-  static constexpr uint32_t kLse = 7 * kTile;             // dkv: 128 floats
-  static constexpr uint32_t kDi = kLse + 512;             // dkv: 128 floats
-  static constexpr uint32_t kBars = kDi + 512;
+  static constexpr uint32_t kLse = 7 * kTile;             // dkv: [2][128] floats
+  static constexpr uint32_t kDi = kLse + 1024;            // dkv: [2][128] floats
+  static constexpr uint32_t kBars = kDi + 1024;
   static constexpr uint32_t kNumBars = 24;
   static constexpr uint32_t kFirst = kBars + kNumBars * 8;  // dkv: the run's first piece and its length
-  static constexpr size_t kBytes = 1024 + kFirst + 32;
+  static constexpr size_t kBytes = kFirst + 32;
   static_assert(kBytes > 116 * 1024 && kBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -145,6 +145,11 @@ __device__ __forceinline__ void store32(uint32_t row, int u0, uint32_t rsw, cons
                  pack_bf16x2(e[4 * u + 3].x, e[4 * u + 3].y));
 }
 
+__device__ __forceinline__ void pack16(const float2 (&e)[16], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(e[i].x, e[i].y);
+}
+
 // Values of hidden pairs become exactly zero: pair i of e is live where bits
 // 2i and 2i + 1 of `live` are set.
 __device__ __forceinline__ void keep_live(uint32_t live, float2 (&e)[16]) {
@@ -177,28 +182,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                       const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV,
                       const BwdParams p, unsigned* err) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kDO = 4 * kTile, kP = 5 * kTile, kDS = 6 * kTile;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kDO = 4 * kTile, kOut = 6 * kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
   // one phase per piece
   uint64_t* k_full = bars + 0;      // K_j landed
   uint64_t* v_full = bars + 1;      // V_j landed
-  uint64_t* dkv_ready = bars + 2;   // every MMA of the piece done: dV_j, dK_j final
+  uint64_t* dkv_ready = bars + 2;   // every MMA of the piece done: dV_j, dK_j final (2 issuers)
   uint64_t* acc_free = bars + 3;    // dV_j, dK_j read out of TMEM (16 warps)
-  // one phase per step n of the run ([2]: per use of buffer n % 2)
-  uint64_t* q_full = bars + 4;      // [2] Q landed
-  uint64_t* q_free = bars + 6;      // [2] dK(n) done: Q and dS^T read
+  // [2] one phase per use of the buffers of step n, n % 2
+  uint64_t* q_full = bars + 4;      // Q, nlse, ndi landed
+  uint64_t* q_free = bars + 6;      // dK(n) done: Q read, dS^T read, and the rows are past nlse, ndi
   uint64_t* do_full = bars + 8;     // dO landed
-  uint64_t* do_free = bars + 9;     // dV(n) done: dO and P^T read
-  uint64_t* lse_full = bars + 12;   // nlse landed (loaded once the row warps wrote P(n - 1))
-  uint64_t* di_full = bars + 13;    // ndi landed (loaded once the row warps wrote dS(n - 1))
-  uint64_t* s_ready = bars + 14;    // S^T(n) in TMEM
-  uint64_t* dp_ready = bars + 15;   // dP^T(n) in TMEM
-  uint64_t* s_free = bars + 10;     // S^T(n) read out (16 warps)
-  uint64_t* p_ready = bars + 16;    // P^T(n) in its tile (16 warps)
-  uint64_t* ds_ready = bars + 17;   // dS^T(n) in its tile, dP^T(n) read out (16 warps)
-  uint64_t* drain = bars + 18;      // once
+  uint64_t* do_free = bars + 10;    // dV(n) done: P^T read
+  // one phase per step n of the run
+  uint64_t* s_ready = bars + 12;    // S^T(n) in TMEM
+  uint64_t* dp_ready = bars + 13;   // dP^T(n) in TMEM
+  uint64_t* dp_free = bars + 14;    // dP^T(n) read out (16 warps)
+  uint64_t* p_ready = bars + 15;    // P^T(n) in TMEM (16 warps)
+  uint64_t* ds_ready = bars + 16;   // dS^T(n) in TMEM (16 warps)
+  uint64_t* drain = bars + 17;      // [2] once
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 19);
 
   const int warp = threadIdx.x >> 5;
@@ -206,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 19; ++i)
-      mbar_init(bars + i, i == 3 || i == 10 || i == 16 || i == 17 ? kRowWarps : 1);
+      mbar_init(bars + i, i == 3 || (i >= 14 && i <= 16) ? kRowWarps : i == 2 ? 2 : 1);
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -243,21 +246,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       bool ok = true;
-      int ks = 0, vs = 0, qs = 0, dos = 0, lses = 0, dis = 0;  // loads issued
+      int ks = 0, vs = 0, qs = 0, dos = 0;  // loads issued
       while (ok) {
         const int b = c.bg / p.KH, g = c.bg - b * p.KH;
         int h = g * p.rep + c.it0 / c.nq, q = c.it0 % c.nq;  // head; query block of the walk
         for (int i = 0; i < c.n; ++i) {
           const int n = n0 + i;
           const uint32_t pprev = static_cast<uint32_t>(n - 1) & 1u;
-          const uint32_t use = static_cast<uint32_t>((n >> 1) - 1) & 1u;  // phase of step n - 2 in its buffer
+          const uint32_t use = static_cast<uint32_t>((n >> 1) - 1) & 1u;  // phase of step n - 2 in its buffers
           const int s0 = (c.j + q) * kBlk;
           const int nb = n & 1;
           const int64_t row = (static_cast<int64_t>(b) * p.QH + h) * p.sp + s0;
           if (n >= 2) ok = mbar_wait(&q_free[nb], use, err, kErrWaitEmpty);
           if (!ok) break;
-          mbar_arrive_expect_tx(&q_full[nb], kTile);
+          mbar_arrive_expect_tx(&q_full[nb], kTile + 2 * kBlk * 4);
           load_tile(smem + kQ + nb * kTile, &tmQ, &q_full[nb], h, s0, b);
+          if (n == 0) pdl_wait();  // nlse, ndi are written by the launch before this one
+          bulk_load_1d(smem + Smem::kLse + nb * kBlk * 4, p.nlse + row, kBlk * 4, &q_full[nb]);
+          bulk_load_1d(smem + Smem::kDi + nb * kBlk * 4, p.ndi + row, kBlk * 4, &q_full[nb]);
           ++qs;
           if (i == 0) {
             // K_j once the previous piece's last S is done, V_j once its last dP is
@@ -272,22 +278,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             load_tile(smem + kV, &tmV, v_full, g, c.j * kBlk, b);
             ++vs;
           }
-          if (n == 0) pdl_wait();  // nlse, ndi are written by the launch before this one
-          if (n >= 1) ok = mbar_wait(p_ready, pprev, err, kErrWaitEmpty);
+          // dO(n - 2) has been read: by dV, and by dP before the dK of above
+          if (n >= 2) ok = mbar_wait(&do_free[nb], use, err, kErrWaitEmpty);
           if (!ok) break;
-          mbar_arrive_expect_tx(lse_full, kBlk * 4);
-          bulk_load_1d(smem + Smem::kLse, p.nlse + row, kBlk * 4, lse_full);
-          ++lses;
-          if (n >= 1) ok = mbar_wait(do_free, pprev, err, kErrWaitEmpty);
-          if (!ok) break;
-          mbar_arrive_expect_tx(do_full, kTile);
-          load_tile(smem + kDO, &tmDO, do_full, h, s0, b);
+          mbar_arrive_expect_tx(&do_full[nb], kTile);
+          load_tile(smem + kDO + nb * kTile, &tmDO, &do_full[nb], h, s0, b);
           ++dos;
-          if (n >= 1) ok = mbar_wait(ds_ready, pprev, err, kErrWaitEmpty);
-          if (!ok) break;
-          mbar_arrive_expect_tx(di_full, kBlk * 4);
-          bulk_load_1d(smem + Smem::kDi, p.ndi + row, kBlk * 4, di_full);
-          ++dis;
           if (++q == c.nq) {
             q = 0;
             ++h;
@@ -300,104 +296,112 @@ __global__ void __launch_bounds__(kThreads, 1)
       // no copy may still be writing shared memory when the CTA exits
       if (ks > 0) mbar_drain(k_full, static_cast<uint32_t>(ks - 1) & 1u);
       if (vs > 0) mbar_drain(v_full, static_cast<uint32_t>(vs - 1) & 1u);
-      if (lses > 0) mbar_drain(lse_full, static_cast<uint32_t>(lses - 1) & 1u);
-      if (dis > 0) mbar_drain(di_full, static_cast<uint32_t>(dis - 1) & 1u);
-      if (dos > 0) mbar_drain(do_full, static_cast<uint32_t>(dos - 1) & 1u);
       for (int t = 0; t < 2; ++t) {
-        const int uses = (qs + 1 - t) >> 1;
+        const int uses = (qs + 1 - t) >> 1, douses = (dos + 1 - t) >> 1;
         if (uses > 0) mbar_drain(&q_full[t], static_cast<uint32_t>(uses - 1) & 1u);
+        if (douses > 0) mbar_drain(&do_full[t], static_cast<uint32_t>(douses - 1) & 1u);
       }
     }
     __syncwarp();
-  } else if (warp == 1 || warp == 2) {
-    // ------------------------------------------------ MMA issuer / scheduler
-    // Both warps walk the same groups and meet at the go barrier before each.
-    const bool sched = warp == 2;
+  } else if (warp == 1) {
+    // -------------------------------------------------- issuer of dK and dP^T
+    const bool one = elect_one();
     const uint32_t base = smem_u32(smem);
     bool ok = true, any = false;
     int pieces = 0;
+    // dP^T(n) into the columns of step n - 1's S^T, once dV(n - 1) and dK(n - 1) have
+    // read the P^T and dS^T there
+    auto issue_dp = [&](int n, bool first) -> bool {
+      const uint32_t nb = static_cast<uint32_t>(n) & 1u, ob = nb ^ 1u;
+      const uint32_t prev = static_cast<uint32_t>((n - 1) >> 1) & 1u;
+      if (first && !warp_wait(v_full, static_cast<uint32_t>(pieces) & 1u, err, kErrWaitFull)) return false;
+      if (!warp_wait(&do_full[nb], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitFull)) return false;
+      if (n > 0 && !(warp_wait(&do_free[ob], prev, err, kErrWaitAccumFree) &&
+                     warp_wait(&q_free[ob], prev, err, kErrWaitAccumFree)))
+        return false;
+      tc_fence_after();
+      if (one) {
+        mma_kk(tmem + ob * 128, base + kV, base + kDO + nb * kTile);
+        umma_commit(dp_ready);
+      }
+      __syncwarp();
+      return any = true;
+    };
     while (ok) {
-      // S^T and dP^T of the piece's first step (their columns were read before
-      // the last piece's dK was issued)
-      {
-        const uint32_t pp = static_cast<uint32_t>(pieces) & 1u, nb = static_cast<uint32_t>(n0) & 1u;
-        const uint32_t use = static_cast<uint32_t>(n0 >> 1) & 1u;
-        ok = sched ? sched_wait(64, err, k_full, pp, &q_full[nb], use) : bar_and(kGoBarrier, 64, true);
-        if (!ok) break;
-        if (!sched && lane == 0) {
-          tc_fence_after();
-          mma_kk(tmem, base + kK, base + kQ + nb * kTile);
-          umma_commit(s_ready);
-          any = true;
-        }
-        __syncwarp();
-        ok = sched ? sched_wait(64, err, v_full, pp, do_full, nb) : bar_and(kGoBarrier, 64, true);
-        if (!ok) break;
-        if (!sched && lane == 0) {
-          tc_fence_after();
-          mma_kk(tmem + 128, base + kV, base + kDO);
-          umma_commit(dp_ready);
-        }
-        __syncwarp();
-      }
-      for (int i = 0; i < c.n; ++i) {
+      for (int i = 0; i < c.n && ok; ++i) {
         const int n = n0 + i;
-        const uint32_t par = static_cast<uint32_t>(n) & 1u, nb = par, ob = par ^ 1u;
-        const uint32_t use = static_cast<uint32_t>((n + 1) >> 1) & 1u;
-        const bool more = i + 1 < c.n;
-        // S^T(n + 1)
-        if (more) {
-          ok = sched ? sched_wait(64, err, &q_full[ob], use, s_free, par) : bar_and(kGoBarrier, 64, true);
-          if (!ok) break;
-          if (!sched && lane == 0) {
-            tc_fence_after();
-            mma_kk(tmem, base + kK, base + kQ + ob * kTile);
-            umma_commit(s_ready);
-          }
-          __syncwarp();
-        }
-        // dV_j += P^T(n) dO(n) (the first of a piece once the last piece's sums are read)
-        ok = sched ? sched_wait(64, err, p_ready, par, i == 0 && pieces > 0 ? acc_free : nullptr,
-                                static_cast<uint32_t>(pieces - 1) & 1u)
-                   : bar_and(kGoBarrier, 64, true);
+        const uint32_t nb = static_cast<uint32_t>(n) & 1u;
+        ok = issue_dp(n, i == 0);
+        // dK_j += dS^T(n) Q(n) (the first of a piece once the last piece's sums are read)
+        if (ok && i == 0 && pieces > 0)
+          ok = warp_wait(acc_free, static_cast<uint32_t>(pieces - 1) & 1u, err, kErrWaitAccumFree);
+        if (ok) ok = warp_wait(ds_ready, nb, err, kErrWaitFull);
         if (!ok) break;
-        if (!sched && lane == 0) {
-          tc_fence_after();
-          mma_km(tmem + 256, base + kP, base + kDO, i == 0);
-          umma_commit(do_free);
-        }
-        __syncwarp();
-        // dK_j += dS^T(n) Q(n)
-        ok = sched ? sched_wait(64, err, ds_ready, par) : bar_and(kGoBarrier, 64, true);
-        if (!ok) break;
-        if (!sched && lane == 0) {
-          tc_fence_after();
-          mma_km(tmem + 384, base + kDS, base + kQ + nb * kTile, i == 0);
+        tc_fence_after();
+        if (one) {
+          mma_tm_pairs(tmem + 384, tmem + nb * 128 + 16, base + kQ + nb * kTile, i == 0);
           umma_commit(&q_free[nb]);
-          if (!more) umma_commit(dkv_ready);
+          if (i + 1 == c.n) umma_commit(dkv_ready);
         }
         __syncwarp();
-        // dP^T(n + 1)
-        if (more) {
-          ok = sched ? sched_wait(64, err, do_full, ob) : bar_and(kGoBarrier, 64, true);
-          if (!ok) break;
-          if (!sched && lane == 0) {
-            tc_fence_after();
-            mma_kk(tmem + 128, base + kV, base + kDO);
-            umma_commit(dp_ready);
-          }
-          __syncwarp();
-        }
       }
+      if (!ok) break;
       n0 += c.n;
       ++pieces;
       if (n0 >= run) break;
       c = piece_after(p, c, run - n0);
     }
-    if (!sched && lane == 0 && any) {
+    if (one && any) {
       // every issued MMA must finish before TMEM is released
-      umma_commit(drain);
-      mbar_drain(drain, 0u);
+      umma_commit(&drain[0]);
+      mbar_drain(&drain[0], 0u);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // --------------------------------------------------- issuer of S^T and dV
+    const bool one = elect_one();
+    const uint32_t base = smem_u32(smem);
+    bool ok = true, any = false;
+    int pieces = 0;
+    while (ok) {
+      for (int i = 0; i < c.n && ok; ++i) {
+        const int n = n0 + i;
+        const uint32_t nb = static_cast<uint32_t>(n) & 1u, use = static_cast<uint32_t>(n >> 1) & 1u;
+        // S^T(n) into the columns that dP^T(n - 1) has been read from
+        if (i == 0) ok = warp_wait(k_full, static_cast<uint32_t>(pieces) & 1u, err, kErrWaitFull);
+        if (ok) ok = warp_wait(&q_full[nb], use, err, kErrWaitFull);
+        if (ok && n > 0) ok = warp_wait(dp_free, nb ^ 1u, err, kErrWaitAccumFree);
+        if (!ok) break;
+        tc_fence_after();
+        if (one) {
+          mma_kk(tmem + nb * 128, base + kK, base + kQ + nb * kTile);
+          umma_commit(s_ready);
+        }
+        __syncwarp();
+        any = true;
+        // dV_j += P^T(n) dO(n)
+        if (i == 0 && pieces > 0)
+          ok = warp_wait(acc_free, static_cast<uint32_t>(pieces - 1) & 1u, err, kErrWaitAccumFree);
+        if (ok) ok = warp_wait(&do_full[nb], use, err, kErrWaitFull);
+        if (ok) ok = warp_wait(p_ready, nb, err, kErrWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+        if (one) {
+          mma_tm_pairs(tmem + 256, tmem + nb * 128, base + kDO + nb * kTile, i == 0);
+          umma_commit(&do_free[nb]);
+          if (i + 1 == c.n) umma_commit(dkv_ready);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      n0 += c.n;
+      ++pieces;
+      if (n0 >= run) break;
+      c = piece_after(p, c, run - n0);
+    }
+    if (one && any) {
+      umma_commit(&drain[1]);
+      mbar_drain(&drain[1], 0u);
     }
     __syncwarp();
   } else if (warp >= 4) {
@@ -405,12 +409,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int grp = (warp - 4) >> 2;        // queries [32 grp, + 32) of the block
     const int kr = (warp & 3) * 32 + lane;  // key row of this thread (TMEM lane)
     const uint32_t col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const float4* nlse_s = reinterpret_cast<const float4*>(smem + Smem::kLse) + 8 * grp;
-    const float4* ndi_s = reinterpret_cast<const float4*>(smem + Smem::kDi) + 8 * grp;
-    const uint32_t prow = smem_u32(smem + kP) + static_cast<uint32_t>(kr * 128) + (grp >> 1) * kHalf;
-    const uint32_t dsrow = smem_u32(smem + kDS) + static_cast<uint32_t>(kr * 128) + (grp >> 1) * kHalf;
-    const int u0 = (grp & 1) * 4;
-    const uint32_t rsw = static_cast<uint32_t>(kr & 7);
     const float2 sl2 = make_float2(p.sl2, p.sl2);
     bool ok = true;
     int pieces = 0;
@@ -426,22 +424,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t par = static_cast<uint32_t>(n) & 1u;
         const int s0 = (c.j + q) * kBlk + 32 * grp;  // this thread's first query
         const uint32_t live = range_mask(qlo - s0, qhi - s0);
+        // S^T(n) here, overwritten by P^T(n) and dS^T(n); dP^T(n) in the other region
+        const uint32_t scol = col + par * 128 + 32 * grp, dpcol = col + (par ^ 1u) * 128 + 32 * grp;
+        const float4* nlse_s = reinterpret_cast<const float4*>(smem + Smem::kLse) + par * 32 + 8 * grp;
+        const float4* ndi_s = reinterpret_cast<const float4*>(smem + Smem::kDi) + par * 32 + 8 * grp;
         q = q + 1 == c.nq ? 0 : q + 1;
-        ok = mbar_wait(s_ready, par, err, kErrWaitAccum) && mbar_wait(lse_full, par, err, kErrWaitFull);
-        if (i == 0 && pieces > 0) {  // the last piece's dV, dK have left the tile
-          if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
-          ok = bar_and(kRowsBarrier, kRowThreads, ok);
-        }
+        ok = mbar_wait(s_ready, par, err, kErrWaitAccum) &&
+             mbar_wait(&q_full[par], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitFull);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         float2 e[16];  // P^T: 2^(s scale log2e - lse[q])
+        uint32_t w[16];
         {
           uint32_t s[32];
-          tmem_ld_32x32b_x32(col + 32 * grp, s);
+          tmem_ld_32x32b_x32(scol, s);
           tmem_ld_wait();
-          tc_fence_before();
-          mbar_arrive_warp(s_free);
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const float4 l = nlse_s[q];
@@ -454,23 +452,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         keep_live(live, e);
-        // the tile is free once dV(n - 1) is done
-        if (n > 0) ok = mbar_wait(do_free, par ^ 1u, err, kErrWaitEmpty);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        store32(prow, u0, rsw, e);
-        fence_proxy_async_smem();
+        pack16(e, w);
+        tmem_st_32x32b_x16(scol, w);
+        tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(p_ready);
         // dS^T = P^T (dP^T - di[q])
-        ok = mbar_wait(dp_ready, par, err, kErrWaitAccum) && mbar_wait(di_full, par, err, kErrWaitFull);
+        ok = mbar_wait(dp_ready, par, err, kErrWaitAccum);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         {
           uint32_t d[32];
-          tmem_ld_32x32b_x32(col + 128 + 32 * grp, d);
+          tmem_ld_32x32b_x32(dpcol, d);
           tmem_ld_wait();
+          tc_fence_before();
+          mbar_arrive_warp(dp_free);
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const float4 l = ndi_s[q];
@@ -482,12 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         keep_live(live, e);
-        // the tile is free once dK(n - 1) is done
-        if (n > 0) ok = mbar_wait(&q_free[par ^ 1u], static_cast<uint32_t>((n - 1) >> 1) & 1u, err, kErrWaitEmpty);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        store32(dsrow, u0, rsw, e);
-        fence_proxy_async_smem();
+        pack16(e, w);
+        tmem_st_32x32b_x16(scol + 16, w);
+        tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(ds_ready);
       }
@@ -495,6 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // MMAs are done: bf16 (dK times the softmax scale), or the fp32 share of a
       // cut walk
       if (ok) ok = mbar_wait(dkv_ready, static_cast<uint32_t>(pieces) & 1u, err, kErrWaitAccum);
+      if ((threadIdx.x & 127) == 0) bulk_wait_read_all();  // the last piece's have left the tile
       ok = bar_and(kRowsBarrier, kRowThreads, ok);
       if (!ok) break;
       tc_fence_after();
@@ -519,14 +514,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int q = 0; q < 32; ++q) part[(half * 32 + q) * kBlk] = __uint_as_float(r[q]);
         } else {
-          // 32 columns at a time through this group's quarter of P^T's tile (64-byte
-          // rows, 64-byte swizzle), whose MMAs are done, and out by TMA (rows past
-          // S are not written)
+          // 32 columns at a time through this group's quarter of a tile (64-byte rows,
+          // 64-byte swizzle), and out by TMA (rows past S are not written)
           if (half == 1) {
             if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
             bar_sync(2 + grp, 128);
           }
-          const uint32_t out = smem_u32(smem + kP) + grp * (kTile / 4) + static_cast<uint32_t>(kr * 64);
+          const uint32_t out = smem_u32(smem + kOut) + grp * (kTile / 4) + static_cast<uint32_t>(kr * 64);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             uint32_t w[4];
@@ -542,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bar_sync(2 + grp, 128);
           if ((threadIdx.x & 127) == 0) {
             const int b = c.bg / p.KH, g = c.bg - b * p.KH;
-            tma_store_4d(which == 0 ? &tmDV : &tmDK, smem + kP + grp * (kTile / 4), (grp & 1) * 64 + half * 32,
+            tma_store_4d(which == 0 ? &tmDV : &tmDK, smem + kOut + grp * (kTile / 4), (grp & 1) * 64 + half * 32,
                          g, c.j * kBlk, b);
             bulk_commit();
           }
@@ -593,8 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     window_dq_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                      const __grid_constant__ CUtensorMap tmDQ, const BwdParams p, unsigned* err) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   constexpr uint32_t kQ = 0, kDO = kTile, kK = 2 * kTile, kV = 5 * kTile, kDS = 6 * kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
   // one phase per unit
