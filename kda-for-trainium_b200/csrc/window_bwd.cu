@@ -201,14 +201,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* dp_free = bars + 14;    // dP^T(n) read out (16 warps)
   uint64_t* p_ready = bars + 15;    // P^T(n) in TMEM (16 warps)
   uint64_t* ds_ready = bars + 16;   // dS^T(n) in TMEM (16 warps)
-  uint64_t* drain = bars + 17;      // [2] once
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* drain = bars + 17;      // [3] once
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 20);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 19; ++i)
+    for (int i = 0; i < 20; ++i)
       mbar_init(bars + i, i == 3 || (i >= 14 && i <= 16) ? kRowWarps : i == 2 ? 2 : 1);
     fence_mbar_init();
   }
@@ -357,8 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_drain(&drain[0], 0u);
     }
     __syncwarp();
-  } else if (warp == 3) {
-    // --------------------------------------------------- issuer of S^T and dV
+  } else if (warp < 4) {
+    // ------------------------------------ issuers of dV (warp 2) and S^T (warp 3)
     const bool one = elect_one();
     const uint32_t base = smem_u32(smem);
     bool ok = true, any = false;
@@ -367,31 +367,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < c.n && ok; ++i) {
         const int n = n0 + i;
         const uint32_t nb = static_cast<uint32_t>(n) & 1u, use = static_cast<uint32_t>(n >> 1) & 1u;
-        // S^T(n) into the columns that dP^T(n - 1) has been read from
-        if (i == 0) ok = warp_wait(k_full, static_cast<uint32_t>(pieces) & 1u, err, kErrWaitFull);
-        if (ok) ok = warp_wait(&q_full[nb], use, err, kErrWaitFull);
-        if (ok && n > 0) ok = warp_wait(dp_free, nb ^ 1u, err, kErrWaitAccumFree);
-        if (!ok) break;
-        tc_fence_after();
-        if (one) {
-          mma_kk(tmem + nb * 128, base + kK, base + kQ + nb * kTile);
-          umma_commit(s_ready);
+        if (warp == 3) {
+          // S^T(n) into the columns that dP^T(n - 1) has been read from
+          if (i == 0) ok = warp_wait(k_full, static_cast<uint32_t>(pieces) & 1u, err, kErrWaitFull);
+          if (ok) ok = warp_wait(&q_full[nb], use, err, kErrWaitFull);
+          if (ok && n > 0) ok = warp_wait(dp_free, nb ^ 1u, err, kErrWaitAccumFree);
+          if (!ok) break;
+          tc_fence_after();
+          if (one) {
+            mma_kk(tmem + nb * 128, base + kK, base + kQ + nb * kTile);
+            umma_commit(s_ready);
+          }
+        } else {
+          // dV_j += P^T(n) dO(n) (the first of a piece once the last piece's sums are read)
+          if (i == 0 && pieces > 0)
+            ok = warp_wait(acc_free, static_cast<uint32_t>(pieces - 1) & 1u, err, kErrWaitAccumFree);
+          if (ok) ok = warp_wait(&do_full[nb], use, err, kErrWaitFull);
+          if (ok) ok = warp_wait(p_ready, nb, err, kErrWaitFull);
+          if (!ok) break;
+          tc_fence_after();
+          if (one) {
+            mma_tm_pairs(tmem + 256, tmem + nb * 128, base + kDO + nb * kTile, i == 0);
+            umma_commit(&do_free[nb]);
+            if (i + 1 == c.n) umma_commit(dkv_ready);
+          }
         }
         __syncwarp();
         any = true;
-        // dV_j += P^T(n) dO(n)
-        if (i == 0 && pieces > 0)
-          ok = warp_wait(acc_free, static_cast<uint32_t>(pieces - 1) & 1u, err, kErrWaitAccumFree);
-        if (ok) ok = warp_wait(&do_full[nb], use, err, kErrWaitFull);
-        if (ok) ok = warp_wait(p_ready, nb, err, kErrWaitFull);
-        if (!ok) break;
-        tc_fence_after();
-        if (one) {
-          mma_tm_pairs(tmem + 256, tmem + nb * 128, base + kDO + nb * kTile, i == 0);
-          umma_commit(&do_free[nb]);
-          if (i + 1 == c.n) umma_commit(dkv_ready);
-        }
-        __syncwarp();
       }
       if (!ok) break;
       n0 += c.n;
@@ -400,11 +402,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       c = piece_after(p, c, run - n0);
     }
     if (one && any) {
-      umma_commit(&drain[1]);
-      mbar_drain(&drain[1], 0u);
+      umma_commit(&drain[warp - 1]);
+      mbar_drain(&drain[warp - 1], 0u);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else {
     // ---------------------------------------------------------- row warps
     const int grp = (warp - 4) >> 2;        // queries [32 grp, + 32) of the block
     const int kr = (warp & 3) * 32 + lane;  // key row of this thread (TMEM lane)
