@@ -64,6 +64,9 @@ struct BwdParams {
   const float* ndi;   // [B][QH][sp]: -rowsum(dout * out)
   float* partial;     // [2 x CTAs][2][128 d][128 keys] fp32: dV_j, dK_j (unscaled) of cut walks
   int4* pieces;       // [2 x CTAs] beside them: (batch, kv head), j, steps of the share, of the walk
+  unsigned* counter;  // join items taken
+  int ctas;           // of dkv
+  __nv_bfloat16* dq;  // [B][S][QH][128]
   __nv_bfloat16* dk;  // [B][S][KH][128], for the join
   __nv_bfloat16* dv;
 };
@@ -71,7 +74,7 @@ struct BwdParams {
 // Seven tiles, then small things.
 struct Smem {
   // dkv: K_j | V_j | Q (two buffers) | dO (two) | results on their way out
-  // dq:  Q | dO | K (three buffers) | V | dS
+  // dq:  Q | dO | K (three buffers) | V (two)
   static constexpr uint32_t kLse = 7 * kTile;             // dkv: [2][128] floats
   static constexpr uint32_t kDi = kLse + 1024;            // dkv: [2][128] floats
   static constexpr uint32_t kBars = kDi + 1024;
@@ -135,16 +138,6 @@ __device__ __forceinline__ Piece piece_after(const BwdParams& p, const Piece& c,
   return d;
 }
 __device__ __forceinline__ int64_t run_start(const BwdParams& p, int cta, int ctas) { return p.total * cta / ctas; }
-// 32 values of a row as bf16 into a K-major, 128-byte-swizzled half tile: columns
-// [8u, 8u + 8) of the half = 16-byte unit u, at u ^ (row % 8); u0 the first unit.
-__device__ __forceinline__ void store32(uint32_t row, int u0, uint32_t rsw, const float2 (&e)[16]) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    st_shared_v4(row + ((static_cast<uint32_t>(u0 + u) ^ rsw) << 4), pack_bf16x2(e[4 * u].x, e[4 * u].y),
-                 pack_bf16x2(e[4 * u + 1].x, e[4 * u + 1].y), pack_bf16x2(e[4 * u + 2].x, e[4 * u + 2].y),
-                 pack_bf16x2(e[4 * u + 3].x, e[4 * u + 3].y));
-}
-
 __device__ __forceinline__ void pack16(const float2 (&e)[16], uint32_t (&w)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(e[i].x, e[i].y);
@@ -562,10 +555,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Unit = (batch, query head, query block); one persistent CTA per SM.  Per key
 // block the unit sees: S = Q K^T, dP = dO V^T, dS = P (dP - di) (row warps, query
 // rows; 32 keys per thread, lse and di one register each), dQ += dS K.
-// Issue order: dP(n + 1) as soon as the row warps have copied step n out of TMEM,
-// S(n + 2) (two column sets), dQ(n).  V's buffer is
-// free after dP, K's (one of three) after dQ.
-// TMEM columns: S [0,128) and [384,512), dP [128,256), dQ [256,384).
+// dS(n), in bf16, takes the columns of the S(n) that its thread has read, and is
+// dQ's operand there.  dP(n + 1) is issued as soon as the rows have copied step n,
+// S(n + 2) (two regions) when dQ(n) has read dS(n); units follow one another
+// without a gap.
+// TMEM columns: S [0,128) and [256,384), dP [128,256), dQ [384,512).
 struct Unit {
   int b, h, i;         // batch, query head, query block
   int n, ns, skip;     // key blocks: [0, ns) (sinks), then [ns + skip, n + skip)
@@ -585,32 +579,74 @@ __device__ __forceinline__ Unit dq_unit(const BwdParams& p, int u) {
 }
 __device__ __forceinline__ int unit_block(const Unit& c, int j) { return j < c.ns ? j : j + c.skip; }
 
+// dk and dv of the walks that were cut: the shares of a walk (one at the start
+// of its run's CTA and the next ones'), added in order.  The row warps that have no
+// unit left take the items -- (CTA, dV or dK, 32 keys, 32 of d) -- one by one from
+// a counter, so the CTAs that had one unit fewer do most of it; which warp takes an
+// item makes no difference to its sum.
+__device__ __forceinline__ void join_cut_walks(const BwdParams& p) {
+  const int lane = threadIdx.x & 31;
+  for (;;) {
+    unsigned item = 0;
+    if (lane == 0) item = atomicAdd(p.counter, 1u);
+    item = __shfl_sync(0xffffffffu, item, 0);
+    if (item >= 32u * static_cast<unsigned>(p.ctas)) return;
+    const int cta = static_cast<int>(item >> 5), which = (item >> 4) & 1, k0 = ((item >> 2) & 3) * 32, d0 = (item & 3) * 32;
+    const int4 w = p.pieces[2 * cta + 1];
+    if (w.z == 0) continue;
+    float v[32];  // d0 + e of key k0 + lane
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = 0.f;
+    int64_t slot = 2 * cta + 1;
+    for (int steps = w.z;; steps += p.pieces[slot].z) {
+      const float* src = p.partial + ((slot * 2 + which) * kD + d0) * kBlk + k0 + lane;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] += src[e * kBlk];
+      if (steps >= w.w) break;
+      slot = (slot | 1) + 1;
+    }
+    const float f = which == 0 ? 1.f : p.scale;
+    const int b = w.x / p.KH, g = w.x - b * p.KH;
+    const int kpos = w.y * kBlk + k0 + lane;
+    if (kpos >= p.S) continue;
+    uint4* dst = reinterpret_cast<uint4*>((which == 0 ? p.dv : p.dk) +
+                                          ((static_cast<int64_t>(b) * p.S + kpos) * p.KH + g) * kD + d0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      dst[u] = make_uint4(pack_bf16x2(v[8 * u] * f, v[8 * u + 1] * f), pack_bf16x2(v[8 * u + 2] * f, v[8 * u + 3] * f),
+                          pack_bf16x2(v[8 * u + 4] * f, v[8 * u + 5] * f), pack_bf16x2(v[8 * u + 6] * f, v[8 * u + 7] * f));
+  }
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     window_dq_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
-                     const __grid_constant__ CUtensorMap tmDQ, const BwdParams p, unsigned* err) {
+                     const BwdParams p, unsigned* err) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  constexpr uint32_t kQ = 0, kDO = kTile, kK = 2 * kTile, kV = 5 * kTile, kDS = 6 * kTile;
+  constexpr uint32_t kQ = 0, kDO = kTile, kK = 2 * kTile, kV = 5 * kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
   // one phase per unit
-  uint64_t* qdo_full = bars + 0;    // Q, dO landed
-  uint64_t* dq_ready = bars + 1;    // every MMA of the unit done: dQ final
-  uint64_t* dq_free = bars + 2;     // dQ read out of TMEM (16 warps)
-  // one phase per step n of the CTA ([3]: per use of buffer n % 3)
-  uint64_t* k_full = bars + 3;      // [3] K landed
-  uint64_t* k_free = bars + 6;      // [3] dQ(n) done: K and the tile's dS read
-  uint64_t* v_full = bars + 9;      // V landed
-  uint64_t* sp_ready = bars + 11;   // S(n), dP(n) in TMEM, V read
-  uint64_t* sp_free = bars + 12;    // S(n), dP(n) read out (16 warps)
-  uint64_t* ds_ready = bars + 13;   // dS(n) in the tile (16 warps)
-  uint64_t* drain = bars + 14;      // once
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* q_full = bars + 0;      // Q landed
+  uint64_t* do_full = bars + 1;     // dO landed
+  uint64_t* dq_ready = bars + 2;    // dQ final
+  uint64_t* dq_free = bars + 3;     // dQ read out of TMEM (16 warps)
+  // one phase per step n of the CTA ([m]: per use of buffer n % m)
+  uint64_t* k_full = bars + 4;      // [3] K landed
+  uint64_t* k_free = bars + 7;      // [3] dQ(n) done: K and dS read
+  uint64_t* v_full = bars + 10;     // [2] V landed
+  uint64_t* s_ready = bars + 12;    // [2] S(n) in TMEM
+  uint64_t* dp_ready = bars + 14;   // dP(n) in TMEM
+  uint64_t* sp_free = bars + 15;    // S(n), dP(n) read out (16 warps)
+  uint64_t* ds_ready = bars + 16;   // dS(n) in TMEM (16 warps)
+  uint64_t* v_free = bars + 17;     // [2] dP(n) done: V read
+  uint64_t* drain = bars + 19;      // [2] once
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 21);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 15; ++i) mbar_init(bars + i, i == 2 || i == 12 || i == 13 ? kRowWarps : 1);
+    for (int i = 0; i < 21; ++i) mbar_init(bars + i, i == 3 || i == 15 || i == 16 ? kRowWarps : 1);
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -618,7 +654,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmV);
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmDO);
-    tma_prefetch_desc(&tmDQ);
   }
   if (warp == 1) {
     tmem_alloc(tmem_holder, 512);
@@ -629,111 +664,136 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const int units = p.B * p.QH * p.nkb;
-  int n0 = 0;  // steps of earlier units
-  int uc = 0;  // earlier units
+  int n = 0;   // steps so far
+  int uc = 0;  // units so far
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       bool ok = true;
-      int qs = 0, vs = 0, ks = 0;  // loads issued
+      int qs = 0, dos = 0, vs = 0, ks = 0;  // loads issued
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
         const Unit c = dq_unit(p, u);
         const int g = c.h / p.rep;
-        // Q, dO once the last unit's last S, dP are done
-        if (n0 > 0) ok = mbar_wait(sp_ready, static_cast<uint32_t>(n0 - 1) & 1u, err, kErrWaitEmpty);
-        if (!ok) break;
-        mbar_arrive_expect_tx(qdo_full, 2 * kTile);
-        load_tile(smem + kQ, &tmQ, qdo_full, c.h, c.i * kBlk, c.b);
-        load_tile(smem + kDO, &tmDO, qdo_full, c.h, c.i * kBlk, c.b);
-        ++qs;
-        for (int j = 0; j < c.n; ++j) {
-          const int n = n0 + j, kb = n % 3;
+        for (int j = 0; j < c.n && ok; ++j, ++n) {
+          const int kb = n % 3, vb = n & 1;
           const int k0 = unit_block(c, j) * kBlk;
+          if (j == 0) {  // Q once the last unit's last S is done
+            if (n > 0) ok = mbar_wait(&s_ready[vb ^ 1], static_cast<uint32_t>((n - 1) >> 1) & 1u, err, kErrWaitEmpty);
+            if (!ok) break;
+            mbar_arrive_expect_tx(q_full, kTile);
+            load_tile(smem + kQ, &tmQ, q_full, c.h, c.i * kBlk, c.b);
+            ++qs;
+          }
           if (n >= 3) ok = mbar_wait(&k_free[kb], static_cast<uint32_t>(n / 3 - 1) & 1u, err, kErrWaitEmpty);
           if (!ok) break;
           mbar_arrive_expect_tx(&k_full[kb], kTile);
           load_tile(smem + kK + kb * kTile, &tmK, &k_full[kb], g, k0, c.b);
           ++ks;
-          if (j > 0) ok = mbar_wait(sp_ready, static_cast<uint32_t>(n - 1) & 1u, err, kErrWaitEmpty);
+          if (j == 0) {  // dO once the last unit's last dP is done
+            if (n > 0) ok = mbar_wait(dp_ready, static_cast<uint32_t>(n - 1) & 1u, err, kErrWaitEmpty);
+            if (!ok) break;
+            mbar_arrive_expect_tx(do_full, kTile);
+            load_tile(smem + kDO, &tmDO, do_full, c.h, c.i * kBlk, c.b);
+            ++dos;
+          }
+          if (n >= 2) ok = mbar_wait(&v_free[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty);
           if (!ok) break;
-          mbar_arrive_expect_tx(v_full, kTile);
-          load_tile(smem + kV, &tmV, v_full, g, k0, c.b);
+          mbar_arrive_expect_tx(&v_full[vb], kTile);
+          load_tile(smem + kV + vb * kTile, &tmV, &v_full[vb], g, k0, c.b);
           ++vs;
         }
-        n0 += c.n;
       }
       // no copy may still be writing shared memory when the CTA exits
-      if (qs > 0) mbar_drain(qdo_full, static_cast<uint32_t>(qs - 1) & 1u);
-      if (vs > 0) mbar_drain(v_full, static_cast<uint32_t>(vs - 1) & 1u);
+      if (qs > 0) mbar_drain(q_full, static_cast<uint32_t>(qs - 1) & 1u);
+      if (dos > 0) mbar_drain(do_full, static_cast<uint32_t>(dos - 1) & 1u);
       for (int t = 0; t < 3; ++t) {
-        const int uses = (ks + 2 - t) / 3;
+        const int uses = (ks + 2 - t) / 3, vuses = (vs + 1 - t) >> 1;
         if (uses > 0) mbar_drain(&k_full[t], static_cast<uint32_t>(uses - 1) & 1u);
+        if (t < 2 && vuses > 0) mbar_drain(&v_full[t], static_cast<uint32_t>(vuses - 1) & 1u);
       }
     }
     __syncwarp();
-  } else if (warp == 1 || warp == 2) {
-    // ------------------------------------------------ MMA issuer / scheduler
-    const bool sched = warp == 2;
+  } else if (warp == 1) {
+    // -------------------------------------------------------- issuer of dP
+    const bool one = elect_one();
     const uint32_t base = smem_u32(smem);
-    bool ok = true, any = false;
+    bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
       const Unit c = dq_unit(p, u);
-      auto s_group = [&](int n, bool first) -> bool {  // S(n): its columns were copied before dP(n - 1) was issued
-        const int kb = n % 3;
-        const bool good = sched ? sched_wait(64, err, &k_full[kb], static_cast<uint32_t>(n / 3) & 1u,
-                                             first ? qdo_full : nullptr, static_cast<uint32_t>(uc) & 1u)
-                                : bar_and(kGoBarrier, 64, true);
-        if (good && !sched && lane == 0) {
-          tc_fence_after();
-          mma_kk(tmem + (n & 1) * 384, base + kQ, base + kK + kb * kTile);
-          any = true;
+      for (int j = 0; j < c.n; ++j, ++n) {
+        const uint32_t nb = static_cast<uint32_t>(n) & 1u;
+        if (j == 0) ok = warp_wait(do_full, static_cast<uint32_t>(uc) & 1u, err, kErrWaitFull);
+        if (ok) ok = warp_wait(&v_full[nb], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitFull);
+        if (ok && n > 0) ok = warp_wait(sp_free, nb ^ 1u, err, kErrWaitAccumFree);
+        if (!ok) break;
+        tc_fence_after();
+        if (one) {
+          mma_kk(tmem + 128, base + kDO, base + kV + nb * kTile);
+          umma_commit(dp_ready);
+          umma_commit(&v_free[nb]);
         }
         __syncwarp();
-        return good;
-      };
-      ok = s_group(n0, true);
-      if (!ok) break;
-      // step -1 issues the first dP alone
-      for (int j = -1; j < c.n; ++j) {
-        const int n = n0 + j;
-        if (j + 1 < c.n) {
-          // dP(n + 1) into the columns that the row warps have copied
-          const uint32_t nb = static_cast<uint32_t>(n + 1) & 1u;
-          ok = sched ? sched_wait(64, err, v_full, nb, n + 1 > 0 ? sp_free : nullptr, nb ^ 1u)
-                     : bar_and(kGoBarrier, 64, true);
-          if (!ok) break;
-          if (!sched && lane == 0) {
-            tc_fence_after();
-            mma_kk(tmem + 128, base + kDO, base + kV);
-            umma_commit(sp_ready);
-          }
-          __syncwarp();
-          if (j + 2 < c.n) ok = s_group(n + 2, false);
-          if (!ok) break;
-        }
-        if (j >= 0) {
-          // dQ += dS(n) K (the first of a unit once the last unit's dQ is read)
-          const int kb = n % 3;
-          ok = sched ? sched_wait(64, err, ds_ready, static_cast<uint32_t>(n) & 1u, j == 0 && uc > 0 ? dq_free : nullptr,
-                                  static_cast<uint32_t>(uc - 1) & 1u)
-                     : bar_and(kGoBarrier, 64, true);
-          if (!ok) break;
-          if (!sched && lane == 0) {
-            tc_fence_after();
-            mma_km(tmem + 256, base + kDS, base + kK + kb * kTile, j == 0);
-            umma_commit(&k_free[kb]);
-            if (j + 1 == c.n) umma_commit(dq_ready);
-          }
-          __syncwarp();
-        }
       }
-      n0 += c.n;
     }
-    if (!sched && lane == 0 && any) {
+    if (one && n > 0) {
       // every issued MMA must finish before TMEM is released
-      umma_commit(drain);
-      mbar_drain(drain, 0u);
+      umma_commit(&drain[0]);
+      mbar_drain(&drain[0], 0u);
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // --------------------------------------------------- issuer of dQ and S
+    // dQ(n), then S(n + 2) into the columns of its dS; S runs two steps ahead.
+    const bool one = elect_one();
+    const uint32_t base = smem_u32(smem);
+    bool ok = true;
+    int su = blockIdx.x, sj = 0, sn = 0, sc = 0;  // the next S: its unit, step in it, step and unit of the CTA
+    int slen = su < units ? dq_unit(p, su).n : 0;
+    auto issue_s = [&]() -> bool {
+      if (su >= units) return true;
+      const int kb = sn % 3;
+      if (sj == 0 && !warp_wait(q_full, static_cast<uint32_t>(sc) & 1u, err, kErrWaitFull)) return false;
+      if (!warp_wait(&k_full[kb], static_cast<uint32_t>(sn / 3) & 1u, err, kErrWaitFull)) return false;
+      if (sn >= 2 && !warp_wait(&k_free[(sn - 2) % 3], static_cast<uint32_t>((sn - 2) / 3) & 1u, err, kErrWaitAccumFree))
+        return false;
+      tc_fence_after();
+      if (one) {
+        mma_kk(tmem + (sn & 1) * 256, base + kQ, base + kK + kb * kTile);
+        umma_commit(&s_ready[sn & 1]);
+      }
+      __syncwarp();
+      ++sn;
+      if (++sj == slen) {
+        sj = 0;
+        ++sc;
+        su += gridDim.x;
+        slen = su < units ? dq_unit(p, su).n : 0;
+      }
+      return true;
+    };
+    ok = issue_s() && issue_s();
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
+      const Unit c = dq_unit(p, u);
+      for (int j = 0; j < c.n && ok; ++j, ++n) {
+        // dQ += dS(n) K (the first of a unit once the last unit's dQ is read)
+        const int kb = n % 3;
+        if (j == 0 && uc > 0) ok = warp_wait(dq_free, static_cast<uint32_t>(uc - 1) & 1u, err, kErrWaitAccumFree);
+        if (ok) ok = warp_wait(ds_ready, static_cast<uint32_t>(n) & 1u, err, kErrWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+        if (one) {
+          mma_tm_pairs(tmem + 384, tmem + (n & 1) * 256, base + kK + kb * kTile, j == 0);
+          umma_commit(&k_free[kb]);
+          if (j + 1 == c.n) umma_commit(dq_ready);
+        }
+        __syncwarp();
+        ok = issue_s();
+      }
+    }
+    if (one && sn > 0) {
+      umma_commit(&drain[1]);
+      mbar_drain(&drain[1], 0u);
     }
     __syncwarp();
   } else if (warp >= 4) {
@@ -741,35 +801,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int grp = (warp - 4) >> 2;       // keys (and columns of dQ) [32 grp, + 32)
     const int r = (warp & 3) * 32 + lane;  // query row of this thread (TMEM lane)
     const uint32_t col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 32 * grp;
-    const uint32_t row = smem_u32(smem + kDS) + static_cast<uint32_t>(r * 128) + (grp >> 1) * kHalf;
-    const uint32_t out = smem_u32(smem + kDS) + grp * (kTile / 4) + static_cast<uint32_t>(r * 64);
-    const int u0 = (grp & 1) * 4;
-    const uint32_t rsw = static_cast<uint32_t>(r & 7);
     const float2 sl2 = make_float2(p.sl2, p.sl2);
     bool ok = true;
-    pdl_wait();  // nlse, ndi: written two launches before
+    pdl_wait();  // nlse, ndi: written two launches before; the shares to join: by the last one
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
       const Unit c = dq_unit(p, u);
       const int qpos = c.i * kBlk + r;
       const int64_t at = (static_cast<int64_t>(c.b) * p.QH + c.h) * p.sp + qpos;
       const float nl = p.nlse[at], nd = p.ndi[at];
       const float2 nlse = make_float2(nl, nl), ndi = make_float2(nd, nd);
-      for (int j = 0; j < c.n; ++j) {
-        const int n = n0 + j;
+      for (int j = 0; j < c.n; ++j, ++n) {
         const uint32_t par = static_cast<uint32_t>(n) & 1u;
         const int k0 = unit_block(c, j) * kBlk + 32 * grp;  // this thread's first key
         const int hi = qpos < p.S ? qpos + 1 - k0 : 0;      // keys [k0, k0 + hi) are not after the query
         const uint32_t live = range_mask(qpos + 1 - p.window - k0, hi) | range_mask(0, min(hi, p.sinks - k0));
-        ok = mbar_wait(sp_ready, par, err, kErrWaitAccum);
-        if (j == 0 && uc > 0) {  // the last unit's dQ has left the tile
-          if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
-          ok = bar_and(kRowsBarrier, kRowThreads, ok);
-        }
+        ok = mbar_wait(&s_ready[par], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitAccum) &&
+             mbar_wait(dp_ready, par, err, kErrWaitAccum);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         uint32_t s[32], d[32];
-        tmem_ld_32x32b_x32(col + par * 384, s);
+        tmem_ld_32x32b_x32(col + par * 256, s);
         tmem_ld_32x32b_x32(col + 128, d);
         tmem_ld_wait();
         tc_fence_before();
@@ -782,47 +834,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           e[q] = __fmul2_rn(make_float2(exp2_approx(a.x), exp2_approx(a.y)), t);
         }
         keep_live(live, e);
-        // the tile is free once dQ(n - 1) is done
-        if (n > 0) ok = mbar_wait(&k_free[(n - 1) % 3], static_cast<uint32_t>((n - 1) / 3) & 1u, err, kErrWaitEmpty);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        store32(row, u0, rsw, e);
-        fence_proxy_async_smem();
+        uint32_t w[16];
+        pack16(e, w);
+        tmem_st_32x32b_x16(col + par * 256, w);
+        tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(ds_ready);
       }
-      n0 += c.n;
       if (ok) ok = mbar_wait(dq_ready, static_cast<uint32_t>(uc) & 1u, err, kErrWaitAccum);
-      ok = bar_and(kRowsBarrier, kRowThreads, ok);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       uint32_t o[32];
-      tmem_ld_32x32b_x32(col + 256, o);
+      tmem_ld_32x32b_x32(col + 384, o);
       tmem_ld_wait();
       tc_fence_before();
       mbar_arrive_warp(dq_free);
-      // 32 columns through this group's quarter of dS's tile (64-byte rows, 64-byte
-      // swizzle), whose MMAs are done, and out by TMA (rows past S are not written)
-      const float2 f = make_float2(p.scale, p.scale);
+      if (qpos < p.S) {
+        uint4* dst = reinterpret_cast<uint4*>(
+            p.dq + ((static_cast<int64_t>(c.b) * p.S + qpos) * p.QH + c.h) * kD + 32 * grp);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        uint32_t w[4];
+        for (int v = 0; v < 4; ++v) {
+          uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 t =
-              __fmul2_rn(make_float2(__uint_as_float(o[8 * v + 2 * k]), __uint_as_float(o[8 * v + 2 * k + 1])), f);
-          w[k] = pack_bf16x2(t.x, t.y);
+          for (int k = 0; k < 4; ++k)
+            w[k] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * k]) * p.scale, __uint_as_float(o[8 * v + 2 * k + 1]) * p.scale);
+          dst[v] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        st_shared_v4(out + ((static_cast<uint32_t>(v) ^ ((r >> 1) & 3u)) << 4), w[0], w[1], w[2], w[3]);
-      }
-      fence_proxy_async_smem();
-      bar_sync(2 + grp, 128);
-      if ((threadIdx.x & 127) == 0) {
-        tma_store_4d(&tmDQ, smem + kDS + grp * (kTile / 4), 32 * grp, c.h, c.i * kBlk, c.b);
-        bulk_commit();
       }
     }
-    if ((threadIdx.x & 127) == 0) bulk_wait_all();
+    if (ok) join_cut_walks(p);
   }
 
   tc_fence_before();
@@ -839,8 +880,10 @@ constexpr int kRowsEach = 4;
 __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* __restrict__ dout,
                                                           const __nv_bfloat16* __restrict__ out,
                                                           const float* __restrict__ lse, float* __restrict__ ndi,
-                                                          float* __restrict__ nlse, int S, int SP, int QH) {
+                                                          float* __restrict__ nlse, unsigned* __restrict__ counter,
+                                                          int S, int SP, int QH) {
   pdl_trigger();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *counter = 0u;
   const int lane = threadIdx.x & 15;
   const int i = blockIdx.x * 16 + (threadIdx.x >> 4);  // (rows s .. s + 3, h) of batch entry blockIdx.y
   const int64_t b = blockIdx.y;
@@ -877,49 +920,10 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* _
   }
 }
 
-// dk and dv of the walks that were cut.  8 blocks for each CTA of the products
-// (4 x 32 key rows of dV, then of dK): if a cut walk starts in its run, the
-// shares of that walk (this CTA's and the next ones') added in order, and
-// transposed ([d][key] to rows) through shared memory.
-__global__ void __launch_bounds__(256) window_join_kernel(const BwdParams p) {
-  __shared__ float tile[32][kD + 1];
-  pdl_wait();
-  const int cta = static_cast<int>(blockIdx.x) >> 3, which = (blockIdx.x >> 2) & 1, k0 = (blockIdx.x & 3) * 32;
-  const int4 w = p.pieces[2 * cta + 1];
-  if (w.z == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float v[kD / 8];  // d = warp + 8 e, key k0 + lane
-#pragma unroll
-  for (int e = 0; e < kD / 8; ++e) v[e] = 0.f;
-  int64_t slot = 2 * cta + 1;
-  for (int steps = w.z;; steps += p.pieces[slot].z) {
-    const float* src = p.partial + (slot * 2 + which) * kD * kBlk + k0 + lane;
-#pragma unroll
-    for (int e = 0; e < kD / 8; ++e) v[e] += src[(warp + 8 * e) * kBlk];
-    if (steps >= w.w) break;
-    slot = (slot | 1) + 1;
-  }
-  const float f = which == 0 ? 1.f : p.scale;
-#pragma unroll
-  for (int e = 0; e < kD / 8; ++e) tile[lane][warp + 8 * e] = v[e] * f;
-  __syncthreads();
-  const int b = w.x / p.KH, g = w.x - b * p.KH;
-  for (int i = threadIdx.x; i < 32 * 16; i += 256) {
-    const int r = i >> 4, u = i & 15;
-    const int kpos = w.y * kBlk + k0 + r;
-    if (kpos < p.S) {
-      const float* t = &tile[r][8 * u];
-      reinterpret_cast<uint4*>((which == 0 ? p.dv : p.dk) + ((static_cast<int64_t>(b) * p.S + kpos) * p.KH + g) * kD)[u] =
-          make_uint4(pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3]), pack_bf16x2(t[4], t[5]),
-                     pack_bf16x2(t[6], t[7]));
-    }
-  }
-}
-
 inline size_t al256(size_t n) { return (n + 255) & ~size_t(255); }
 inline int64_t padded_rows(int64_t S) { return (S + kBlk - 1) / kBlk * kBlk; }
 
-// dq, dk, dv [B][S][H][128] as the kernels write them: 32-column boxes.
+// dk, dv [B][S][H][128] as window_dkv_kernel writes them: 32-column boxes.
 kda_status tmap_out(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H) {
   const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(H), static_cast<uint64_t>(S),
                             static_cast<uint64_t>(B)};
@@ -972,7 +976,7 @@ extern "C" size_t kda_gqa_window_backward_workspace_size(int64_t B, int64_t S, i
                                                          int64_t window, int64_t sinks) {
   if (B <= 0 || S <= 0 || QH <= 0 || KH <= 0 || QH % KH || D != kD || window <= 0 || sinks < 0) return 0;
   return 2 * al256(static_cast<size_t>(B) * QH * padded_rows(S) * 4) +
-         static_cast<size_t>(make_plan(B, S, QH, KH, window, sinks).ctas) * (4 * kBlk * kD * 4 + 32);
+         static_cast<size_t>(make_plan(B, S, QH, KH, window, sinks).ctas) * (4 * kBlk * kD * 4 + 32) + 16;
 }
 
 extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void* q, const void* k, const void* v,
@@ -1023,6 +1027,9 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   p.ndi = ndi;
   p.partial = reinterpret_cast<float*>(w + 2 * rows);
   p.pieces = reinterpret_cast<int4*>(p.partial + plan.ctas * 4 * kBlk * kD);
+  p.counter = reinterpret_cast<unsigned*>(p.pieces + 2 * plan.ctas);
+  p.ctas = static_cast<int>(plan.ctas);
+  p.dq = static_cast<__nv_bfloat16*>(dq);
   p.dk = static_cast<__nv_bfloat16*>(dk);
   p.dv = static_cast<__nv_bfloat16*>(dv);
   static std::atomic<bool> attr_set[64] = {};
@@ -1036,24 +1043,23 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
     attr_set[dev].store(true, std::memory_order_release);
   }
   window_rows_kernel<<<dim3(static_cast<unsigned>((SP / kRowsEach * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
-      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi, nlse, p.S, p.sp, p.QH);
+      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi, nlse, p.counter, p.S,
+      p.sp, p.QH);
   KDA_WB_TRY(launch_status("gqa_window_backward: rows"));
   // after a launch, which makes the device's context current in a thread that
   // has not used it yet (autograd's); the encoder is a driver call and needs one
-  CUtensorMap tk, tv, tq, tdo, tdq, tdk, tdv;
+  CUtensorMap tk, tv, tq, tdo, tdk, tdv;
   KDA_WB_TRY(tmap_head_rows(&tk, k, B, S, KH, k_strides));
   KDA_WB_TRY(tmap_head_rows(&tv, v, B, S, KH, v_strides));
   KDA_WB_TRY(tmap_head_rows(&tq, q, B, S, QH, q_strides));
   KDA_WB_TRY(tmap_head_rows(&tdo, dout, B, S, QH, dense_q));
-  KDA_WB_TRY(tmap_out(&tdq, dq, B, S, QH));
   KDA_WB_TRY(tmap_out(&tdk, dk, B, S, KH));
   KDA_WB_TRY(tmap_out(&tdv, dv, B, S, KH));
   const unsigned ctas = static_cast<unsigned>(plan.ctas);
   KDA_WB_TRY(launch_after("gqa_window_backward: dk, dv", window_dkv_kernel, dim3(ctas), kThreads, Smem::kBytes, st, tk,
                           tv, tq, tdo, tdk, tdv, p, kda_err_ptr_window_bwd()));
   const int64_t units = B * QH * plan.nkb;
-  KDA_WB_TRY(launch_after("gqa_window_backward: dq", window_dq_kernel,
-                          dim3(static_cast<unsigned>(std::min<int64_t>(units, num_sms()))), kThreads, Smem::kBytes, st,
-                          tk, tv, tq, tdo, tdq, p, kda_err_ptr_window_bwd()));
-  return launch_after("gqa_window_backward: join", window_join_kernel, dim3(8 * ctas), 256, 0, st, p);
+  return launch_after("gqa_window_backward: dq", window_dq_kernel,
+                      dim3(static_cast<unsigned>(std::min<int64_t>(units, num_sms()))), kThreads, Smem::kBytes, st, tk,
+                      tv, tq, tdo, p, kda_err_ptr_window_bwd());
 }
