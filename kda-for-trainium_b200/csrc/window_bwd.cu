@@ -47,7 +47,6 @@ namespace {
 constexpr int kRowWarps = 16;
 constexpr int kThreads = 128 + 32 * kRowWarps;
 constexpr int kRowThreads = 32 * kRowWarps;
-constexpr int kRowsBarrier = 6;  // all row warps; 2 .. 5: the four warps of one column group
 
 struct BwdParams {
   int B, S, QH, KH, rep;
@@ -67,13 +66,13 @@ struct BwdParams {
   unsigned* counter;  // join items taken
   int ctas;           // of dkv
   __nv_bfloat16* dq;  // [B][S][QH][128]
-  __nv_bfloat16* dk;  // [B][S][KH][128], for the join
+  __nv_bfloat16* dk;  // [B][S][KH][128]
   __nv_bfloat16* dv;
 };
 
 // Seven tiles, then small things.
 struct Smem {
-  // dkv: K_j | V_j | Q (two buffers) | dO (two) | results on their way out
+  // dkv: K_j | V_j | Q (two buffers) | dO (two)
   // dq:  Q | dO | K (three buffers) | V (two)
   static constexpr uint32_t kLse = 7 * kTile;             // dkv: [2][128] floats
   static constexpr uint32_t kDi = kLse + 1024;            // dkv: [2][128] floats
@@ -143,6 +142,32 @@ __device__ __forceinline__ void pack16(const float2 (&e)[16], uint32_t (&w)[16])
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(e[i].x, e[i].y);
 }
 
+// A warp's 32 rows x 32 columns of bf16 results, a row per lane (w: its 64 bytes),
+// to rows of global memory: first the four lanes of a quad exchange 16-byte pieces
+// (lane i gets piece i of the quad's four rows), so that a quad's stores fill whole
+// sectors of a row.  dst: row 0, `stride` elements between rows; rows from `rows`
+// on are not written.
+__device__ __forceinline__ void store_rows(uint32_t (&w)[16], __nv_bfloat16* dst, int64_t stride, int rows) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d <= 2; d *= 2) {
+    const bool up = (lane & d) != 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((i / 4) & d) continue;  // pieces i / 4 and i / 4 + d
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[i] : w[i + 4 * d], d);
+      w[i] = up ? got : w[i];
+      w[i + 4 * d] = up ? w[i + 4 * d] : got;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = (lane & ~3) + r;
+    if (row < rows)
+      reinterpret_cast<uint4*>(dst + row * stride)[lane & 3] = make_uint4(w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]);
+  }
+}
+
 // Values of hidden pairs become exactly zero: pair i of e is live where bits
 // 2i and 2i + 1 of `live` are set.
 __device__ __forceinline__ void keep_live(uint32_t live, float2 (&e)[16]) {
@@ -173,10 +198,9 @@ __device__ __forceinline__ void keep_live(uint32_t live, float2 (&e)[16]) {
 __global__ void __launch_bounds__(kThreads, 1)
     window_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
-                      const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV,
                       const BwdParams p, unsigned* err) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kDO = 4 * kTile, kOut = 6 * kTile;
+  constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kDO = 4 * kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
   // one phase per piece
   uint64_t* k_full = bars + 0;      // K_j landed
@@ -210,8 +234,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmV);
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmDO);
-    tma_prefetch_desc(&tmDK);
-    tma_prefetch_desc(&tmDV);
   }
   if (warp == 1) {
     tmem_alloc(tmem_holder, 512);
@@ -405,8 +427,47 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kr = (warp & 3) * 32 + lane;  // key row of this thread (TMEM lane)
     const uint32_t col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float2 sl2 = make_float2(p.sl2, p.sl2);
+    // dV_j (groups 0, 1) and dK_j (2, 3) of a piece, 64 columns a thread, once its
+    // MMAs are done: bf16 (dK times the softmax scale), or the fp32 share of a cut
+    // walk.  Called after the next piece's first step, whose MMAs run meanwhile.
+    auto finish = [&](const Piece& c, int piece) -> bool {
+      if (!warp_wait(dkv_ready, static_cast<uint32_t>(piece) & 1u, err, kErrWaitAccum)) return false;
+      tc_fence_after();
+      const bool cut = c.n < c.walk;
+      const int which = grp >> 1;
+      const int slot = 2 * static_cast<int>(blockIdx.x) + (c.it0 == 0 ? 1 : 0);
+      // [slot][dV, dK][d][key]: a warp writes 32 keys of one d, a 128-byte line
+      float* part = p.partial + ((static_cast<int64_t>(slot) * 2 + which) * kD + (grp & 1) * 64) * kBlk + kr;
+      if (cut && warp == 4 && lane == 0) p.pieces[slot] = make_int4(c.bg, c.j, c.n, c.walk);
+      const float f = which == 0 ? 1.f : p.scale;
+      const int b = c.bg / p.KH, g = c.bg - b * p.KH;
+      const int k0 = c.j * kBlk + (warp & 3) * 32;
+      __nv_bfloat16* dst = (which == 0 ? p.dv : p.dk) +
+                           ((static_cast<int64_t>(b) * p.S + k0) * p.KH + g) * kD + (grp & 1) * 64;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(col + 256 + grp * 64 + half * 32, r);
+        tmem_ld_wait();
+        if (half == 1) {
+          tc_fence_before();
+          mbar_arrive_warp(acc_free);
+        }
+        if (cut) {
+#pragma unroll
+          for (int q = 0; q < 32; ++q) part[(half * 32 + q) * kBlk] = __uint_as_float(r[q]);
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) w[q] = pack_bf16x2(__uint_as_float(r[2 * q]) * f, __uint_as_float(r[2 * q + 1]) * f);
+          store_rows(w, dst + 32 * half, static_cast<int64_t>(p.KH) * kD, p.S - k0);
+        }
+      }
+      return true;
+    };
     bool ok = true;
     int pieces = 0;
+    Piece last = c;  // the piece before this one
     while (ok) {
       const int kpos = c.j * kBlk + kr;
       // live queries of this key row: from the key itself up to the last that
@@ -479,70 +540,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(ds_ready);
-      }
-      // dV_j (groups 0, 1) and dK_j (2, 3), 64 columns a thread, once the piece's
-      // MMAs are done: bf16 (dK times the softmax scale), or the fp32 share of a
-      // cut walk
-      if (ok) ok = mbar_wait(dkv_ready, static_cast<uint32_t>(pieces) & 1u, err, kErrWaitAccum);
-      if ((threadIdx.x & 127) == 0) bulk_wait_read_all();  // the last piece's have left the tile
-      ok = bar_and(kRowsBarrier, kRowThreads, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const bool cut = c.n < c.walk;
-      const int which = grp >> 1;
-      const int slot = 2 * static_cast<int>(blockIdx.x) + (c.it0 == 0 ? 1 : 0);
-      // [slot][dV, dK][d][key]: a warp writes 32 keys of one d, a 128-byte line
-      float* part = p.partial + ((static_cast<int64_t>(slot) * 2 + which) * kD + (grp & 1) * 64) * kBlk + kr;
-      if (cut && warp == 4 && lane == 0) p.pieces[slot] = make_int4(c.bg, c.j, c.n, c.walk);
-      const float f1 = which == 0 ? 1.f : p.scale;
-      const float2 f = make_float2(f1, f1);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(col + 256 + grp * 64 + half * 32, r);
-        tmem_ld_wait();
-        if (half == 1) {
-          tc_fence_before();
-          mbar_arrive_warp(acc_free);
-        }
-        if (cut) {
-#pragma unroll
-          for (int q = 0; q < 32; ++q) part[(half * 32 + q) * kBlk] = __uint_as_float(r[q]);
-        } else {
-          // 32 columns at a time through this group's quarter of a tile (64-byte rows,
-          // 64-byte swizzle), and out by TMA (rows past S are not written)
-          if (half == 1) {
-            if ((threadIdx.x & 127) == 0) bulk_wait_read_all();
-            bar_sync(2 + grp, 128);
-          }
-          const uint32_t out = smem_u32(smem + kOut) + grp * (kTile / 4) + static_cast<uint32_t>(kr * 64);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 v = __fmul2_rn(
-                  make_float2(__uint_as_float(r[8 * u + 2 * k]), __uint_as_float(r[8 * u + 2 * k + 1])), f);
-              w[k] = pack_bf16x2(v.x, v.y);
-            }
-            st_shared_v4(out + ((static_cast<uint32_t>(u) ^ ((kr >> 1) & 3u)) << 4), w[0], w[1], w[2], w[3]);
-          }
-          fence_proxy_async_smem();
-          bar_sync(2 + grp, 128);
-          if ((threadIdx.x & 127) == 0) {
-            const int b = c.bg / p.KH, g = c.bg - b * p.KH;
-            tma_store_4d(which == 0 ? &tmDV : &tmDK, smem + kOut + grp * (kTile / 4), (grp & 1) * 64 + half * 32,
-                         g, c.j * kBlk, b);
-            bulk_commit();
-          }
-        }
+        if (i == 0 && pieces > 0) ok = finish(last, pieces - 1);
+        if (!ok) break;
       }
       n0 += c.n;
       ++pieces;
+      last = c;
       if (n0 >= run) break;
       c = piece_after(p, c, run - n0);
     }
-    if ((threadIdx.x & 127) == 0) bulk_wait_all();
+    if (ok) finish(last, pieces - 1);
   }
 
   tc_fence_before();
@@ -802,14 +809,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = (warp & 3) * 32 + lane;  // query row of this thread (TMEM lane)
     const uint32_t col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 32 * grp;
     const float2 sl2 = make_float2(p.sl2, p.sl2);
+    // dQ of a unit, once its MMAs are done.  Called after the next unit's first step,
+    // whose MMAs run meanwhile.
+    auto finish = [&](const Unit& c, int unit) -> bool {
+      if (!warp_wait(dq_ready, static_cast<uint32_t>(unit) & 1u, err, kErrWaitAccum)) return false;
+      tc_fence_after();
+      uint32_t o[32], w[16];
+      tmem_ld_32x32b_x32(col + 384, o);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive_warp(dq_free);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        w[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * p.scale, __uint_as_float(o[2 * i + 1]) * p.scale);
+      const int s0 = c.i * kBlk + (warp & 3) * 32;
+      store_rows(w, p.dq + ((static_cast<int64_t>(c.b) * p.S + s0) * p.QH + c.h) * kD + 32 * grp,
+                 static_cast<int64_t>(p.QH) * kD, p.S - s0);
+      return true;
+    };
+    auto row_at = [&](const Unit& c) -> int64_t {
+      return (static_cast<int64_t>(c.b) * p.QH + c.h) * p.sp + c.i * kBlk + r;
+    };
     bool ok = true;
     pdl_wait();  // nlse, ndi: written two launches before; the shares to join: by the last one
+    int64_t at = static_cast<int>(blockIdx.x) < units ? row_at(dq_unit(p, blockIdx.x)) : 0;
+    float nl = p.nlse[at], nd = p.ndi[at];  // of the next unit, so that it does not wait for them
+    Unit last = {};  // the unit before this one
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
       const Unit c = dq_unit(p, u);
       const int qpos = c.i * kBlk + r;
-      const int64_t at = (static_cast<int64_t>(c.b) * p.QH + c.h) * p.sp + qpos;
-      const float nl = p.nlse[at], nd = p.ndi[at];
       const float2 nlse = make_float2(nl, nl), ndi = make_float2(nd, nd);
+      if (u + static_cast<int>(gridDim.x) < units) {
+        at = row_at(dq_unit(p, u + gridDim.x));
+        nl = p.nlse[at];
+        nd = p.ndi[at];
+      }
       for (int j = 0; j < c.n; ++j, ++n) {
         const uint32_t par = static_cast<uint32_t>(n) & 1u;
         const int k0 = unit_block(c, j) * kBlk + 32 * grp;  // this thread's first key
@@ -840,29 +874,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive_warp(ds_ready);
+        if (j == 0 && uc > 0) ok = finish(last, uc - 1);
+        if (!ok) break;
       }
-      if (ok) ok = mbar_wait(dq_ready, static_cast<uint32_t>(uc) & 1u, err, kErrWaitAccum);
-      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      tc_fence_after();
-      uint32_t o[32];
-      tmem_ld_32x32b_x32(col + 384, o);
-      tmem_ld_wait();
-      tc_fence_before();
-      mbar_arrive_warp(dq_free);
-      if (qpos < p.S) {
-        uint4* dst = reinterpret_cast<uint4*>(
-            p.dq + ((static_cast<int64_t>(c.b) * p.S + qpos) * p.QH + c.h) * kD + 32 * grp);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = pack_bf16x2(__uint_as_float(o[8 * v + 2 * k]) * p.scale, __uint_as_float(o[8 * v + 2 * k + 1]) * p.scale);
-          dst[v] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+      last = c;
     }
+    if (ok && uc > 0) ok = finish(last, uc - 1);
     if (ok) join_cut_walks(p);
   }
 
@@ -922,15 +940,6 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* _
 
 inline size_t al256(size_t n) { return (n + 255) & ~size_t(255); }
 inline int64_t padded_rows(int64_t S) { return (S + kBlk - 1) / kBlk * kBlk; }
-
-// dk, dv [B][S][H][128] as window_dkv_kernel writes them: 32-column boxes.
-kda_status tmap_out(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(H), static_cast<uint64_t>(S),
-                            static_cast<uint64_t>(B)};
-  const uint64_t strides[3] = {kD * 2, static_cast<uint64_t>(H) * kD * 2, static_cast<uint64_t>(S) * H * kD * 2};
-  const uint32_t box[4] = {32, 1, static_cast<uint32_t>(kBlk), 1};
-  return make_tmap_bf16_sw(m, base, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
-}
 
 // How the walks lie and over how many CTAs they are spread.
 struct Plan {
@@ -1048,16 +1057,14 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   KDA_WB_TRY(launch_status("gqa_window_backward: rows"));
   // after a launch, which makes the device's context current in a thread that
   // has not used it yet (autograd's); the encoder is a driver call and needs one
-  CUtensorMap tk, tv, tq, tdo, tdk, tdv;
+  CUtensorMap tk, tv, tq, tdo;
   KDA_WB_TRY(tmap_head_rows(&tk, k, B, S, KH, k_strides));
   KDA_WB_TRY(tmap_head_rows(&tv, v, B, S, KH, v_strides));
   KDA_WB_TRY(tmap_head_rows(&tq, q, B, S, QH, q_strides));
   KDA_WB_TRY(tmap_head_rows(&tdo, dout, B, S, QH, dense_q));
-  KDA_WB_TRY(tmap_out(&tdk, dk, B, S, KH));
-  KDA_WB_TRY(tmap_out(&tdv, dv, B, S, KH));
   const unsigned ctas = static_cast<unsigned>(plan.ctas);
   KDA_WB_TRY(launch_after("gqa_window_backward: dk, dv", window_dkv_kernel, dim3(ctas), kThreads, Smem::kBytes, st, tk,
-                          tv, tq, tdo, tdk, tdv, p, kda_err_ptr_window_bwd()));
+                          tv, tq, tdo, p, kda_err_ptr_window_bwd()));
   const int64_t units = B * QH * plan.nkb;
   return launch_after("gqa_window_backward: dq", window_dq_kernel,
                       dim3(static_cast<unsigned>(std::min<int64_t>(units, num_sms()))), kThreads, Smem::kBytes, st, tk,
