@@ -223,7 +223,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 20; ++i)
       mbar_init(bars + i, i == 3 || (i >= 14 && i <= 16) ? kRowWarps : i == 2 ? 2 : 1);
@@ -276,7 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           mbar_arrive_expect_tx(&q_full[nb], kTile + 2 * kBlk * 4);
           load_tile(smem + kQ + nb * kTile, &tmQ, &q_full[nb], h, s0, b);
-          if (n == 0) pdl_wait();  // nlse, ndi are written by the launch before this one
+          if (n == 0) {
+            pdl_wait();     // nlse, ndi are written by the launch before this one
+            pdl_trigger();  // and complete before any CTA of the launch after this one starts
+          }
           bulk_load_1d(smem + Smem::kLse + nb * kBlk * 4, p.nlse + row, kBlk * 4, &q_full[nb]);
           bulk_load_1d(smem + Smem::kDi + nb * kBlk * 4, p.ndi + row, kBlk * 4, &q_full[nb]);
           ++qs;
@@ -831,9 +833,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       return (static_cast<int64_t>(c.b) * p.QH + c.h) * p.sp + c.i * kBlk + r;
     };
     bool ok = true;
-    pdl_wait();  // nlse, ndi: written two launches before; the shares to join: by the last one
     int64_t at = static_cast<int>(blockIdx.x) < units ? row_at(dq_unit(p, blockIdx.x)) : 0;
-    float nl = p.nlse[at], nd = p.ndi[at];  // of the next unit, so that it does not wait for them
+    // of the next unit, so that it does not wait for them.  They are complete: every CTA
+    // of the launch before this one waited for their launch before it let this one start.
+    float nl = __ldcg(p.nlse + at), nd = __ldcg(p.ndi + at);
     Unit last = {};  // the unit before this one
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
       const Unit c = dq_unit(p, u);
@@ -841,8 +844,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float2 nlse = make_float2(nl, nl), ndi = make_float2(nd, nd);
       if (u + static_cast<int>(gridDim.x) < units) {
         at = row_at(dq_unit(p, u + gridDim.x));
-        nl = p.nlse[at];
-        nd = p.ndi[at];
+        nl = __ldcg(p.nlse + at);
+        nd = __ldcg(p.ndi + at);
       }
       for (int j = 0; j < c.n; ++j, ++n) {
         const uint32_t par = static_cast<uint32_t>(n) & 1u;
@@ -881,6 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       last = c;
     }
     if (ok && uc > 0) ok = finish(last, uc - 1);
+    pdl_wait();  // the shares are written by the launch before this one
     if (ok) join_cut_walks(p);
   }
 
