@@ -216,16 +216,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_ready = bars + 12;    // S^T(n) in TMEM
   uint64_t* dp_ready = bars + 13;   // dP^T(n) in TMEM
   uint64_t* dp_free = bars + 14;    // dP^T(n) read out (16 warps)
-  uint64_t* p_ready = bars + 15;    // P^T(n) in TMEM (16 warps)
-  uint64_t* ds_ready = bars + 16;   // dS^T(n) in TMEM (16 warps)
-  uint64_t* drain = bars + 17;      // [3] once
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* p_ready = bars + 15;    // [2] P^T(n) in TMEM (16 warps): the rows may be a step ahead of dV
+  uint64_t* ds_ready = bars + 17;   // dS^T(n) in TMEM (16 warps)
+  uint64_t* drain = bars + 18;      // [3] once
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 21);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 20; ++i)
-      mbar_init(bars + i, i == 3 || (i >= 14 && i <= 16) ? kRowWarps : i == 2 ? 2 : 1);
+    for (int i = 0; i < 21; ++i)
+      mbar_init(bars + i, i == 3 || (i >= 14 && i <= 17) ? kRowWarps : i == 2 ? 2 : 1);
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (i == 0 && pieces > 0)
             ok = warp_wait(acc_free, static_cast<uint32_t>(pieces - 1) & 1u, err, kErrWaitAccumFree);
           if (ok) ok = warp_wait(&do_full[nb], use, err, kErrWaitFull);
-          if (ok) ok = warp_wait(p_ready, nb, err, kErrWaitFull);
+          if (ok) ok = warp_wait(&p_ready[nb], use, err, kErrWaitFull);
           if (!ok) break;
           tc_fence_after();
           if (one) {
@@ -446,22 +446,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int k0 = c.j * kBlk + (warp & 3) * 32;
       __nv_bfloat16* dst = (which == 0 ? p.dv : p.dk) +
                            ((static_cast<int64_t>(b) * p.S + k0) * p.KH + g) * kD + (grp & 1) * 64;
+      uint32_t r[64];
+      tmem_ld_32x32b_x32(col + 256 + grp * 64, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+      tmem_ld_32x32b_x32(col + 256 + grp * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive_warp(acc_free);
+      if (cut) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(col + 256 + grp * 64 + half * 32, r);
-        tmem_ld_wait();
-        if (half == 1) {
-          tc_fence_before();
-          mbar_arrive_warp(acc_free);
-        }
-        if (cut) {
+        for (int q = 0; q < 64; ++q) part[q * kBlk] = __uint_as_float(r[q]);
+      } else {
 #pragma unroll
-          for (int q = 0; q < 32; ++q) part[(half * 32 + q) * kBlk] = __uint_as_float(r[q]);
-        } else {
+        for (int half = 0; half < 2; ++half) {
           uint32_t w[16];
 #pragma unroll
-          for (int q = 0; q < 16; ++q) w[q] = pack_bf16x2(__uint_as_float(r[2 * q]) * f, __uint_as_float(r[2 * q + 1]) * f);
+          for (int q = 0; q < 16; ++q)
+            w[q] = pack_bf16x2(__uint_as_float(r[32 * half + 2 * q]) * f, __uint_as_float(r[32 * half + 2 * q + 1]) * f);
           store_rows(w, dst + 32 * half, static_cast<int64_t>(p.KH) * kD, p.S - k0);
         }
       }
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_32x32b_x16(scol, w);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive_warp(p_ready);
+        mbar_arrive_warp(&p_ready[par]);
         // dS^T = P^T (dP^T - di[q])
         ok = mbar_wait(dp_ready, par, err, kErrWaitAccum);
         ok = __all_sync(0xffffffffu, ok);
@@ -646,16 +646,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_ready = bars + 12;    // [2] S(n) in TMEM
   uint64_t* dp_ready = bars + 14;   // dP(n) in TMEM
   uint64_t* sp_free = bars + 15;    // S(n), dP(n) read out (16 warps)
-  uint64_t* ds_ready = bars + 16;   // dS(n) in TMEM (16 warps)
-  uint64_t* v_free = bars + 17;     // [2] dP(n) done: V read
-  uint64_t* drain = bars + 19;      // [2] once
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* ds_ready = bars + 16;   // [2] dS(n) in TMEM (16 warps): the rows may be a step ahead of dQ
+  uint64_t* v_free = bars + 18;     // [2] dP(n) done: V read
+  uint64_t* drain = bars + 20;      // [2] once
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 22);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 21; ++i) mbar_init(bars + i, i == 3 || i == 15 || i == 16 ? kRowWarps : 1);
+    for (int i = 0; i < 22; ++i) mbar_init(bars + i, i == 3 || (i >= 15 && i <= 17) ? kRowWarps : 1);
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // dQ += dS(n) K (the first of a unit once the last unit's dQ is read)
         const int kb = n % 3;
         if (j == 0 && uc > 0) ok = warp_wait(dq_free, static_cast<uint32_t>(uc - 1) & 1u, err, kErrWaitAccumFree);
-        if (ok) ok = warp_wait(ds_ready, static_cast<uint32_t>(n) & 1u, err, kErrWaitFull);
+        if (ok) ok = warp_wait(&ds_ready[n & 1], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitFull);
         if (!ok) break;
         tc_fence_after();
         if (one) {
@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_32x32b_x16(col + par * 256, w);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive_warp(ds_ready);
+        mbar_arrive_warp(&ds_ready[par]);
         if (j == 0 && uc > 0) ok = finish(last, uc - 1);
         if (!ok) break;
       }
