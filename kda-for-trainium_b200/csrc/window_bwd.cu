@@ -700,13 +700,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           load_tile(smem + kK + kb * kTile, &tmK, &k_full[kb], g, k0, c.b);
           ++ks;
           if (j == 0) {  // dO once the last unit's last dP is done
-            if (n > 0) ok = mbar_wait(dp_ready, static_cast<uint32_t>(n - 1) & 1u, err, kErrWaitEmpty);
+            if (n > 0) ok = mbar_wait(&v_free[vb ^ 1], static_cast<uint32_t>((n - 1) >> 1) & 1u, err, kErrWaitEmpty);
             if (!ok) break;
             mbar_arrive_expect_tx(do_full, kTile);
             load_tile(smem + kDO, &tmDO, do_full, c.h, c.i * kBlk, c.b);
             ++dos;
           }
-          if (n >= 2) ok = mbar_wait(&v_free[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty);
+          // (S(n - 2) too: a barrier tells phases apart by parity, so Q's wait for S above
+          // needs the ones before it to be known done)
+          if (n >= 2)
+            ok = mbar_wait(&v_free[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty) &&
+                 mbar_wait(&s_ready[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty);
           if (!ok) break;
           mbar_arrive_expect_tx(&v_full[vb], kTile);
           load_tile(smem + kV + vb * kTile, &tmV, &v_full[vb], g, k0, c.b);

@@ -572,3 +572,44 @@ def test_example_runs():
     from conftest import REPO
     worst = runpy.run_path(str(REPO / "examples" / "local_attention.py"))["main"]()
     assert worst <= 4 * 2.0 ** -8
+
+
+def _window64(q, k, v, window, sinks, dout):
+    """Output and gradients of one batch entry in 64 bits, on the GPU."""
+    S, QH, KH = q.shape[0], q.shape[1], k.shape[1]
+    q, k, v = (t.double().transpose(0, 1).requires_grad_() for t in (q, k, v))
+    i = torch.arange(S, device="cuda")
+    seen = (i[None] <= i[:, None]) & ((i[:, None] - i[None] < window) | (i[None] < sinks))
+    outs = []
+    for h in range(QH):
+        s = (q[h] @ k[h // (QH // KH)].T) * 128 ** -0.5
+        outs.append(torch.softmax(s.masked_fill(~seen, -torch.inf), dim=-1) @ v[h // (QH // KH)])
+    out = torch.stack(outs)
+    grads = torch.autograd.grad(out, (q, k, v), dout.double().transpose(0, 1))
+    return tuple(t.transpose(0, 1) for t in (out.detach(), *grads))
+
+
+# Many units per CTA, each of one or two key blocks: the pipelines run across the
+# units' ends all the time.  Every call has to give the same bits.
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,QH,KH,window,sinks", [(1, 4000, 8, 8, 62, 0), (3, 2724, 4, 4, 62, 0), (3, 971, 16, 8, 1, 64),
+                                                    (2, 3000, 8, 2, 128, 1), (1, 5000, 12, 4, 1, 0)])
+def test_gqa_window_short_units(kda, B, S, QH, KH, window, sinks):
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q, dout = (torch.randn(B, S, QH, 128, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2))
+    k, v = (torch.randn(B, S, KH, 128, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2))
+    first = None
+    for _ in range(20):
+        out, lse = kda.gqa_window_lse(q, k, v, window, sinks)
+        got = (out, *kda.gqa_window_backward(dout, q, k, v, out, lse, window, sinks))
+        if first is None:
+            first = got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+    b = B - 1
+    want = _window64(q[b], k[b], v[b], window, sinks, dout[b])
+    for name, g, w in zip(("out", "dq", "dk", "dv"), first, want):
+        if name in ("dq", "dk") and window + sinks == 1:  # zero up to rounding, as above
+            assert g[b].abs().max() < 1e-3
+            continue
+        # the output's own rounding, the weights' and, for the gradients, dS's and di's
+        assert (g[b].double() - w).norm() <= rounds(4) * w.norm(), name
