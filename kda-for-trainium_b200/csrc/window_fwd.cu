@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Smem::kBars);
-  uint64_t* slot_full = bars;      // [3] an item landed
-  uint64_t* slot_free = bars + 3;  // [3] the MMAs that read it are done
+  uint64_t* slot_full = bars;      // [2][2] the nth K, the nth V landed: at n % 2 (each issuer waits for its own in turn)
+  uint64_t* slot_free = bars + 4;  // [3] the MMAs that read it are done
   uint64_t* s_free = bars + 9;     // S copied out (8 warps); one phase per S, of either tile
   // [2], per tile; one phase per block that the tile sees
   uint64_t* s_ready = bars + 7;    // S in TMEM
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // [2], one phase per unit in which the tile has rows
   uint64_t* o_free = bars + 15;    // O read out (8 warps)
   uint64_t* q_full = bars + 19;    // Q landed
-  uint64_t* drain = bars + 17;     // once
+  uint64_t* drain = bars + 17;     // [2] once
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 21);
 
   const int warp = threadIdx.x >> 5;
@@ -163,15 +163,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       bool ok = true;
-      uint32_t base = 0, items = 0;  // items of earlier units; loads issued
+      uint32_t base = 0, loads[2] = {0u, 0u};  // items of earlier units; loads of K and V issued
       int qs[2] = {0, 0};
       uint32_t seen[2] = {0u, 0u};   // blocks each tile has seen
-      auto load_item = [&](uint32_t x, const CUtensorMap* m, int g, int j, int b) -> bool {
+      auto load_item = [&](const int kv, uint32_t x, const CUtensorMap* m, int g, int j, int b) -> bool {
         const uint32_t s = item_slot(x);
+        uint64_t* full = &slot_full[2 * kv + (loads[kv] & 1u)];
         if (x >= kSlots && !mbar_wait(&slot_free[s], item_par(x) ^ 1u, err, kErrWaitEmpty)) return false;
-        mbar_arrive_expect_tx(&slot_full[s], kTile);
-        load_tile(smem + Smem::kRing + s * kTile, m, &slot_full[s], g, j * kBlk, b);
-        ++items;
+        mbar_arrive_expect_tx(full, kTile);
+        load_tile(smem + Smem::kRing + s * kTile, m, full, g, j * kBlk, b);
+        ++loads[kv];
         return true;
       };
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
@@ -189,10 +190,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++qs[t];
           }
         if (!ok) break;
-        ok = load_item(item_k(base, 0), &tmK, g, key_block(c, 0), c.b);
+        ok = load_item(0, item_k(base, 0), &tmK, g, key_block(c, 0), c.b);
         for (int j = 0; j < c.nb && ok; ++j) {
-          if (j + 1 < c.nb) ok = load_item(item_k(base, j + 1), &tmK, g, key_block(c, j + 1), c.b);
-          if (ok) ok = load_item(item_v(base, j, c.nb), &tmV, g, key_block(c, j), c.b);
+          if (j + 1 < c.nb) ok = load_item(0, item_k(base, j + 1), &tmK, g, key_block(c, j + 1), c.b);
+          if (ok) ok = load_item(1, item_v(base, j, c.nb), &tmV, g, key_block(c, j), c.b);
 #pragma unroll
           for (int t = 0; t < 2; ++t) seen[t] += sees[t].at(j) ? 1u : 0u;
         }
@@ -202,9 +203,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         if (qs[t] > 0) mbar_drain(&q_full[t], static_cast<uint32_t>(qs[t] - 1) & 1u);
-      for (uint32_t s = 0; s < kSlots; ++s) {
-        const uint32_t uses = (items + kSlots - 1u - s) / kSlots;
-        if (uses > 0) mbar_drain(&slot_full[s], (uses - 1u) & 1u);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t uses = (loads[i >> 1] + 1u - (i & 1u)) >> 1;
+        if (uses > 0) mbar_drain(&slot_full[i], (uses - 1u) & 1u);
       }
     }
     __syncwarp();
@@ -215,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t ring = smem_u32(smem) + Smem::kRing, qs = smem_u32(smem) + Smem::kQ;
       const bool is_s = warp == 1;
       uint32_t base = 0;           // ring items of earlier units
+      uint32_t items = 0;          // K (or V) so far
       uint32_t ns = 0;             // S so far, of both tiles
       uint32_t np[2] = {0u, 0u};   // a tile's P V so far
       uint32_t un[2] = {0u, 0u};   // and its units
@@ -227,7 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t x = is_s ? item_k(base, j) : item_v(base, j, c.nb), slot = item_slot(x);
           const uint32_t tile = ring + slot * kTile;
           bool seen = false;
-          ok = warp_wait(&slot_full[slot], item_par(x), err, kErrWaitFull);
+          ok = warp_wait(&slot_full[(is_s ? 0 : 2) + (items & 1u)], (items >> 1) & 1u, err, kErrWaitFull);
+          ++items;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || !sees[t].at(j)) continue;
