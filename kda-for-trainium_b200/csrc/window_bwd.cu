@@ -687,6 +687,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < c.n && ok; ++j, ++n) {
           const int kb = n % 3, vb = n & 1;
           const int k0 = unit_block(c, j) * kBlk;
+          // A barrier tells phases apart by parity: every S is waited for in turn, before
+          // anything of step n is loaded, so that neither an earlier nor a later phase is
+          // taken for the one that Q waits for.
+          if (n >= 2) ok = mbar_wait(&s_ready[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty);
+          if (!ok) break;
           if (j == 0) {  // Q once the last unit's last S is done
             if (n > 0) ok = mbar_wait(&s_ready[vb ^ 1], static_cast<uint32_t>((n - 1) >> 1) & 1u, err, kErrWaitEmpty);
             if (!ok) break;
@@ -706,11 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             load_tile(smem + kDO, &tmDO, do_full, c.h, c.i * kBlk, c.b);
             ++dos;
           }
-          // (S(n - 2) too: a barrier tells phases apart by parity, so Q's wait for S above
-          // needs the ones before it to be known done)
-          if (n >= 2)
-            ok = mbar_wait(&v_free[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty) &&
-                 mbar_wait(&s_ready[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty);
+          if (n >= 2) ok = mbar_wait(&v_free[vb], static_cast<uint32_t>((n >> 1) - 1) & 1u, err, kErrWaitEmpty);
           if (!ok) break;
           mbar_arrive_expect_tx(&v_full[vb], kTile);
           load_tile(smem + kV + vb * kTile, &tmV, &v_full[vb], g, k0, c.b);
