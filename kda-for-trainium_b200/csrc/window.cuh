@@ -11,7 +11,6 @@ constexpr int kD = 128;                    // head dim
 constexpr int kBlk = 128;                  // rows of a block of queries or keys
 constexpr uint32_t kTile = kBlk * kD * 2;  // 32 KB: two halves of 64 columns, 128-byte rows, 128-byte swizzle
 constexpr uint32_t kHalf = kTile / 2;
-constexpr int kGoBarrier = 1;              // named barrier: the scheduler's and the MMA issuers' warps
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -135,17 +134,11 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, u
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D (+)= A B^T with both read K-major, and D (+)= A B with A K-major, B MN-major: 128 x 128 x 128
+// D = A B^T with both read K-major: 128 x 128 x 128
 __device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t b) {
   const uint64_t da = kmajor(a), db = kmajor(b);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) umma_bf16(d, da + kmajor_step(kk), db + kmajor_step(kk), kIdKK, kk != 0 ? 1u : 0u);
-}
-__device__ __forceinline__ void mma_km(uint32_t d, uint32_t a, uint32_t b, bool first) {
-  const uint64_t da = kmajor(a), db = mnmajor(b);
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
-    umma_bf16(d, da + kmajor_step(kk), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
 }
 // D (+)= A B with A (bf16 pairs, 64 columns) in TMEM and B MN-major
 __device__ __forceinline__ void mma_tm(uint32_t d, uint32_t a, uint32_t b, bool first) {
@@ -164,19 +157,6 @@ __device__ __forceinline__ void mma_tm_pairs(uint32_t d, uint32_t a, uint32_t b,
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int head, int row, int b) {
   tma_load_4d(dst, m, bar, 0, head, row, b);
   tma_load_4d(dst + kHalf, m, bar, 64, head, row, b);
-}
-
-// One thread of the scheduler waits for up to three barriers, then its warp and
-// the issuers' (`threads` in all) meet; false once any wait has expired.
-__device__ __forceinline__ bool sched_wait(int threads, unsigned* err, uint64_t* b1, uint32_t p1, uint64_t* b2 = nullptr,
-                                           uint32_t p2 = 0u, uint64_t* b3 = nullptr, uint32_t p3 = 0u) {
-  bool good = true;
-  if ((threadIdx.x & 31) == 0) {
-    good = mbar_wait(b1, p1, err, kErrWaitFull);
-    if (good && b2) good = mbar_wait(b2, p2, err, kErrWaitFull);
-    if (good && b3) good = mbar_wait(b3, p3, err, kErrWaitAccumFree);
-  }
-  return bar_and(kGoBarrier, threads, __shfl_sync(0xffffffffu, good, 0));
 }
 
 // The entry points' size checks; whether strided head rows start on 16 bytes; the

@@ -13,19 +13,25 @@
 // memory, and the results do not depend on timing.  S and dP are computed twice
 // (7 products a block pair instead of 5): with one kernel that adds dQ into an
 // fp32 buffer the L2 took the additions at 2.3 TB/s (64 KB a block pair,
-// red.global and bulk reductions alike), which bound it: 172 us at S4096 W1024
-// of 16 heads, 189 us with bulk reductions, against the figure at the launch.
+// red.global and bulk reductions alike), which bound it at 172 us for S4096 W1024
+// of 16 heads, where the whole call now takes 125.
 //
-// Both kernels: 640 threads -- warp 0 TMA producer, warp 1 TMEM allocator + MMA
-// issuer, warp 2 scheduler (performs every mbarrier wait the issuer needs and
-// releases it group by group at a named barrier: an mbarrier wait in the
-// issuing thread would stall behind its queued MMAs), warp 3 idle, warps 4-19
-// row warps: warp w reads TMEM lanes 32 (w % 4), columns 32 ((w - 4) / 4), i.e.
-// 32 values of one row per thread, four warps on each SM partition to cover
-// each other's latencies.  Operand tiles are two 16 KB halves of 64 columns,
-// 128-byte rows, 128-byte swizzle, loaded once and read K-major where their rows
-// index M or N and MN-major where their rows index K.  Both are bound by shared memory: 64 KB of MMA operands per
-// product at 128 B/clk.
+// P^T, dS^T and dS are written to TMEM as bf16, each thread's into the columns of S
+// that it has read, and are the A operand of their products there: through shared
+// memory (a 32 KB tile stored and read back for each) the same call took 179 us.
+//
+// Both kernels: 640 threads -- warp 0 TMA producer, warps 1-3 MMA issuers (warp 1
+// allocates TMEM), warps 4-19 row warps: warp w reads TMEM lanes 32 (w % 4), columns
+// 32 ((w - 4) / 4), i.e. 32 values of one row per thread, four warps on each SM
+// partition to cover each other's latencies.  An issuer's mbarrier wait stalls
+// behind its own queued MMAs, so products that wait for different things have
+// issuers of their own (S and dV from one warp: 9 % slower).
+// An mbarrier tells phases apart by parity only.  A barrier that may complete again
+// before a waiter has looked is one of a pair (p_ready, ds_ready, s_ready), and
+// every waiter waits for the phases in turn.
+// Operand tiles are two 16 KB halves of 64 columns, 128-byte rows, 128-byte swizzle,
+// loaded once and read K-major where their rows index M or N and MN-major where their
+// rows index K.
 // All mbarrier waits are bounded (common.cuh); every TMA load targets one CTA.
 #include <math.h>
 
@@ -185,16 +191,21 @@ __device__ __forceinline__ void keep_live(uint32_t live, float2 (&e)[16]) {
 // most blocks (rep x the blocks of the window) and as long as the sequence for
 // those with sinks, and there may be few walks, so the CTAs (one per SM,
 // persistent) each take an equal run of the concatenated walks.  Where a run
-// cuts a walk, its dV_j and dK_j are fp32 partial sums that window_join_kernel
-// adds in order.
+// cuts a walk, its dV_j and dK_j are fp32 partial sums, which the row warps of the
+// dQ kernel add in order.
 //   S^T = K_j Q^T, P^T (row warps, key rows; 32 queries per thread, kept in
-//   registers as fp32, bf16 into a tile), dP^T = V_j dO^T, dV_j += P^T dO,
-//   dS^T = P^T (dP^T - di) (from the unrounded P^T, into a tile of its own),
-//   dK_j += dS^T Q
-// Issue order per step n: S(n+1) as soon as the row warps have copied S(n) out of
-// TMEM, dV(n) and dK(n) as soon as they have written P^T(n) and dS^T(n), dP(n+1)
-// when dO has been replaced.
-// TMEM columns: S^T [0,128), dP^T [128,256), dV [256,384), dK [384,512).
+//   registers as fp32, bf16 for the product), dP^T = V_j dO^T, dV_j += P^T dO,
+//   dS^T = P^T (dP^T - di) (from the unrounded P^T), dK_j += dS^T Q
+// S^T(n) lies in region n % 2 and dP^T(n) in the other; P^T(n) and dS^T(n) replace
+// S^T(n) column by column.  S^T(n+1) is issued as soon as the row warps have copied
+// dP^T(n), dV(n) and dK(n) as soon as they have written P^T(n) and dS^T(n), and
+// dP^T(n+1) once both are done with the region it overwrites.
+// A step takes about 2,900 cycles, the row warps' chain: wait, TMEM load, 16,384
+// exponentials (1,024 cycles of their pipe), store, wait, load, store.  The tensor
+// core works 2,048 of them.  With the exponentials of one in four or eight pairs as
+// a polynomial, with nlse and ndi loaded ahead, or with the waits asked for early,
+// it stays within 1 %.  78 us at S4096 W1024 of 16 heads.
+// TMEM columns: regions [0,128), [128,256), dV [256,384), dK [384,512).
 __global__ void __launch_bounds__(kThreads, 1)
     window_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -568,6 +579,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // dQ's operand there.  dP(n + 1) is issued as soon as the rows have copied step n,
 // S(n + 2) (two regions) when dQ(n) has read dS(n); units follow one another
 // without a gap.
+// A step takes about 1,950 cycles, the row warps' chain again (1,024 of them the
+// exponentials' pipe); the tensor core works 1,536.  60 us at S4096 W1024 of 16
+// heads, cut walks joined: 512 units in 3.5 waves.
 // TMEM columns: S [0,128) and [256,384), dP [128,256), dQ [384,512).
 struct Unit {
   int b, h, i;         // batch, query head, query block

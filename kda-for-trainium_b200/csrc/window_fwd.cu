@@ -10,24 +10,30 @@
 // with sinks before it) pass through a 3-slot TMA ring, K_0, K_1, V_0, K_2, V_1,
 // ..., and serve both tiles.  A tile skips the blocks that none of its rows sees.
 //
-// 640 threads: warp 0 TMA producer, warps 1 and 3 MMA issuers of tile 0 and 1
-// (warp 1 allocates TMEM), warp 2 scheduler, warps 4-11 / 12-19 softmax of tile
-// 0 / 1: warp w reads TMEM lanes 32 (w % 4), 64 of a row's 128 keys per thread.
-// The scheduler performs every mbarrier wait the issuers need and releases them
-// round by round at a named barrier: an mbarrier wait in an issuing thread would
-// stall behind its queued MMAs.  A round has an S of one tile and a P V of the
-// other, S_0(j+1) | PV_1(j-1), then PV_0(j) | S_1(j+1): the tiles run half a step
-// apart, one exponentiates while the other stores, and the tensor core always has
-// two groups queued (with one issuer and four groups a step, a step of both tiles
-// took 4,560 cycles, 1,700 of them between groups).  S's columns are handed back
-// as soon as they are copied, so S(j+1) is there before P(j) is done.
+// 640 threads: warp 0 TMA producer, warp 1 MMA issuer of S (allocates TMEM), warp 3
+// of P V, warps 4-11 / 12-19 softmax of tile 0 / 1: warp w reads TMEM lanes
+// 32 (w % 4), 64 of a row's 128 keys per thread.
+// P stays in TMEM, as bf16, and is the P V product's A operand there: 64 KB a step
+// of two tiles that are neither stored to shared memory nor read back from it (the
+// TMEM operand beside shared-memory ones runs at the full rate: 2,048 cycles for
+// the step's four products).  With P's columns of their own, one region is left for
+// S, which the tiles take in turn: S_0(j), S_1(j), S_0(j+1), ...; a tile's S is
+// issued as soon as the other has copied its S into registers, so the tiles run
+// half a step apart and one exponentiates while the other stores.  An issuer's wait
+// stalls behind its own queued MMAs, hence one for S and one for P V: neither's next
+// wait ends before its last product anyway.
 // The two warps that share a row agree on its reference with one bar.red a step
 // (did a score exceed it?) and exchange maxima only when one did.
-// V is read as stored (MN-major B), P from shared memory.
-// TMEM columns: S_0 [0,128), S_1 [128,256), O_0 [256,384), O_1 [384,512).
-// Shared memory: Q_0 | Q_1 | P_0 | P_1 | ring (3 x 32 KB) | row exchange.
-// Bound by the 128 B/clk of shared memory: 256 KB of MMA operands, 64 KB of loads
-// and 64 KB of P a step of two tiles, about 3,000 cycles.
+// V is read as stored (MN-major B).
+// TMEM columns: S [0,128), P_0 [128,192), P_1 [192,256), O_0 [256,384), O_1 [384,512).
+// Shared memory: Q_0 | Q_1 | outgoing O_0 | O_1 | ring (3 x 32 KB) | row exchange.
+// 1.17 ms at S32768 W2048 of 32 heads (1.07 TFLOP on visible pairs: 910 TFLOP/s, 0.53
+// of the measured bf16 rate): a step of two tiles takes about 3,250 cycles, of
+// which the tensor core works 2,048 and the exponentials' pipe 2,048; the rest is the
+// latency of a tile's chain (wait, TMEM load, maximum, exponentials, store).  With P
+// through shared memory, S_t of each tile its own: 1.43 ms.  One of eight pairs by
+// a polynomial instead of ex2: 1 % faster, one of four 4 % slower; not kept.  One
+// tile a unit for calls that leave SMs idle: no faster.
 // All mbarrier waits are bounded (common.cuh); every TMA load targets one CTA.
 #include <math.h>
 
@@ -57,7 +63,7 @@ struct FwdParams {
 };
 
 struct Smem {
-  static constexpr uint32_t kQ = 0, kP = 2 * kTile, kRing = 4 * kTile;
+  static constexpr uint32_t kQ = 0, kOut = 2 * kTile, kRing = 4 * kTile;
   static constexpr uint32_t kExchange = 7 * kTile;  // 1 KB, fp32 [tile][row]: maxima and sums of two warps' halves
   static constexpr uint32_t kBars = kExchange + 1024;
   static constexpr uint32_t kNumBars = 24;
@@ -283,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t scol = lanes + 64 * half;
     const uint32_t pcol = lanes + 128 + 64 * t + 32 * half;
     const uint32_t ocol = lanes + 256 + t * kBlk + 64 * half;
-    uint8_t* tile = smem + Smem::kP + t * kTile + half * kHalf;
+    uint8_t* tile = smem + Smem::kOut + t * kTile + half * kHalf;
     const uint32_t row = smem_u32(tile) + static_cast<uint32_t>(r * 128);
     const uint32_t rsw = static_cast<uint32_t>(r & 7);
     float* xch = reinterpret_cast<float*>(smem + Smem::kExchange) + t * kBlk + r;
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int qpos = c.q0 + t * kBlk + r;
       if (c.q0 + t * kBlk >= p.S) continue;  // no rows (both halves alike)
       const Seen sees = tile_sees(p, c, t);
-      if (stored) {  // the last unit's output has left P's tile
+      if (stored) {  // the last unit's output has left its tile
         if (elected) bulk_wait_read_all();
         ok = bar_and(quarter, 128, ok);
         if (!ok) break;
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         first = false;
         ++n;
       }
-      // O / l to bf16, through P's tile, out by TMA (rows past S are not written)
+      // O / l to bf16, through shared memory, out by TMA (rows past S are not written)
       if (ok) ok = mbar_wait(&pv_done[t], (n - 1u) & 1u, err, kErrWaitAccum);
       ok = bar_and(quarter, 128, ok);
       // the two halves' sums: half 1 hands its over, half 0 answers with the whole
