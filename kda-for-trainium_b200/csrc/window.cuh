@@ -54,8 +54,18 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
 }
+// Their waits, every lane's: one lane's alone would diverge, which costs far more
+// (20 % of the backward).  warp_wait2: both barriers are asked before either answer
+// is needed.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+__device__ __forceinline__ bool warp_wait2(uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2, unsigned* err,
+                                           unsigned code) {
+  const bool a = mbar_try_wait(b1, p1), b = mbar_try_wait(b2, p2);
+  if (__all_sync(0xffffffffu, a && b)) return true;
+  return __all_sync(0xffffffffu, mbar_wait(b1, p1, err, code) && mbar_wait(b2, p2, err, code));
 }
 // Whether a phase is complete, without waiting: asked early, so that the answer's
 // latency (200 cycles and more beside the tensor core's operand reads) is hidden.

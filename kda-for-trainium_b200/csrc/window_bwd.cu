@@ -498,9 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float4* nlse_s = reinterpret_cast<const float4*>(smem + Smem::kLse) + par * 32 + 8 * grp;
         const float4* ndi_s = reinterpret_cast<const float4*>(smem + Smem::kDi) + par * 32 + 8 * grp;
         q = q + 1 == c.nq ? 0 : q + 1;
-        ok = mbar_wait(s_ready, par, err, kErrWaitAccum) &&
-             mbar_wait(&q_full[par], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitFull);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait2(s_ready, par, &q_full[par], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitAccum);
         if (!ok) break;
         tc_fence_after();
         float2 e[16];  // P^T: 2^(s scale log2e - lse[q])
@@ -527,8 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive_warp(&p_ready[par]);
         // dS^T = P^T (dP^T - di[q])
-        ok = mbar_wait(dp_ready, par, err, kErrWaitAccum);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait(dp_ready, par, err, kErrWaitAccum);
         if (!ok) break;
         tc_fence_after();
         {
@@ -871,9 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int k0 = unit_block(c, j) * kBlk + 32 * grp;  // this thread's first key
         const int hi = qpos < p.S ? qpos + 1 - k0 : 0;      // keys [k0, k0 + hi) are not after the query
         const uint32_t live = range_mask(qpos + 1 - p.window - k0, hi) | range_mask(0, min(hi, p.sinks - k0));
-        ok = mbar_wait(&s_ready[par], static_cast<uint32_t>(n >> 1) & 1u, err, kErrWaitAccum) &&
-             mbar_wait(dp_ready, par, err, kErrWaitAccum);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait2(&s_ready[par], static_cast<uint32_t>(n >> 1) & 1u, dp_ready, par, err, kErrWaitAccum);
         if (!ok) break;
         tc_fence_after();
         uint32_t s[32], d[32];

@@ -316,8 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = sees.sinks > 0 ? 0 : sees.from; j < sees.to; j = j + 1 >= sees.sinks ? max(j + 1, sees.from) : j + 1) {
         const uint32_t par = n & 1u;
         const int k0 = key_block(c, j) * kBlk + 64 * half;  // this thread's first key
-        if (ok && !s_there) ok = mbar_wait(&s_ready[t], par, err, kErrWaitAccum);
-        ok = __all_sync(0xffffffffu, ok);
+        if (ok && !s_there) ok = warp_wait(&s_ready[t], par, err, kErrWaitAccum);
         tc_fence_after();
         uint32_t s[64];
         tmem_ld_32x32b_x32(scol, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
@@ -381,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const bool p_free = first || mbar_test(&pv_done[t], par ^ 1u);
+        const bool p_free = first || __all_sync(0xffffffffu, mbar_test(&pv_done[t], par ^ 1u));
         const float mb = m == -INFINITY ? 0.f : m;
         const float2 nm2 = make_float2(-mb, -mb);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -394,12 +393,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         // P's columns are free once O += P V of the last block is done
-        if (ok && !p_free) ok = mbar_wait(&pv_done[t], par ^ 1u, err, kErrWaitAccum);
-        ok = __all_sync(0xffffffffu, ok);
+        if (ok && !p_free) ok = warp_wait(&pv_done[t], par ^ 1u, err, kErrWaitAccum);
         if (ok) {
           tmem_st_32x32b_x16(pcol, *reinterpret_cast<const uint32_t(*)[16]>(&s[0]));
           tmem_st_32x32b_x16(pcol + 16, *reinterpret_cast<const uint32_t(*)[16]>(&s[16]));
-          s_there = mbar_test(&s_ready[t], par ^ 1u);
+          s_there = __all_sync(0xffffffffu, mbar_test(&s_ready[t], par ^ 1u));
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive_warp(&p_ready[t]);
