@@ -79,7 +79,7 @@ def _build_binding(force: bool, verbose: bool) -> Path:
     inc = [*include_paths(), str(cuda_inc), sysconfig.get_paths()["include"], str(INCLUDE)]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(src), "-o", str(BINDING),
-           *(f"-I{p}" for p in inc), *(f"-L{p}" for p in library_paths()), "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           *(f"-I{p}" for p in inc), *(f"-L{p}" for p in library_paths()), "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            "-lc10", "-lc10_cuda", f"-L{LIB.parent}", "-l:libkda.so", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
