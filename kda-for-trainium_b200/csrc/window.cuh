@@ -144,11 +144,12 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, u
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D = A B^T with both read K-major: 128 x 128 x 128
-__device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t b) {
+// D = A B^T with both read K-major: 128 x (16 n16) x 128, from the first 16 n16 rows of B
+__device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t b, int n16 = 8) {
   const uint64_t da = kmajor(a), db = kmajor(b);
+  const uint32_t id = kIdKK - (static_cast<uint32_t>(8 - n16) << 18);  // bits 17 to 22: N / 8
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) umma_bf16(d, da + kmajor_step(kk), db + kmajor_step(kk), kIdKK, kk != 0 ? 1u : 0u);
+  for (int kk = 0; kk < 8; ++kk) umma_bf16(d, da + kmajor_step(kk), db + kmajor_step(kk), id, kk != 0 ? 1u : 0u);
 }
 // D (+)= A B with A (bf16 pairs, 64 columns) in TMEM and B MN-major
 __device__ __forceinline__ void mma_tm(uint32_t d, uint32_t a, uint32_t b, bool first) {
@@ -156,12 +157,14 @@ __device__ __forceinline__ void mma_tm(uint32_t d, uint32_t a, uint32_t b, bool 
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) umma_bf16_ts(d, a + 8 * kk, db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
 }
-// with A's K steps in pairs 32 columns apart: [0, 16), [32, 48), ... of 128
-__device__ __forceinline__ void mma_tm_pairs(uint32_t d, uint32_t a, uint32_t b, bool first) {
+// with A's K steps in pairs 32 columns apart, [0, 16), [32, 48), ... of 128; the first k16
+// of them
+__device__ __forceinline__ void mma_tm_pairs(uint32_t d, uint32_t a, uint32_t b, bool first, int k16 = 8) {
   const uint64_t db = mnmajor(b);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    umma_bf16_ts(d, a + 32 * (kk >> 1) + 8 * (kk & 1), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
+    if (kk < k16)
+      umma_bf16_ts(d, a + 32 * (kk >> 1) + 8 * (kk & 1), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
 }
 // 128 rows x 128 columns as two halves
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int head, int row, int b) {

@@ -598,6 +598,13 @@ __device__ __forceinline__ Unit dq_unit(const BwdParams& p, int u) {
   return c;
 }
 __device__ __forceinline__ int unit_block(const Unit& c, int j) { return j < c.ns ? j : j + c.skip; }
+// Keys of a unit's block j that are worked on: of one visited for its sinks alone,
+// only those; in 16s for the tensor core (4 sinks at S8192 of 16 heads: W256 136.5 ->
+// 133.4 us, W1024 244.6 -> 242.1; the forward gains nothing from the same).
+__device__ __forceinline__ int live_keys(const BwdParams& p, const Unit& c, int j) {
+  return j < c.ns ? min(kBlk, p.sinks - j * kBlk) : kBlk;
+}
+__device__ __forceinline__ int in16s(int keys) { return (keys + 15) >> 4; }
 
 // dk and dv of the walks that were cut: the shares of a walk (one at the start
 // of its run's CTA and the next ones'), added in order.  The row warps that have no
@@ -754,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         if (one) {
-          mma_kk(tmem + 128, base + kDO, base + kV + nb * kTile);
+          mma_kk(tmem + 128, base + kDO, base + kV + nb * kTile, in16s(live_keys(p, c, j)));
           umma_commit(dp_ready);
           umma_commit(&v_free[nb]);
         }
@@ -774,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t base = smem_u32(smem);
     bool ok = true;
     int su = blockIdx.x, sj = 0, sn = 0, sc = 0;  // the next S: its unit, step in it, step and unit of the CTA
-    int slen = su < units ? dq_unit(p, su).n : 0;
+    Unit s_unit = su < units ? dq_unit(p, su) : Unit{};
     auto issue_s = [&]() -> bool {
       if (su >= units) return true;
       const int kb = sn % 3;
@@ -784,16 +791,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         return false;
       tc_fence_after();
       if (one) {
-        mma_kk(tmem + (sn & 1) * 256, base + kQ, base + kK + kb * kTile);
+        mma_kk(tmem + (sn & 1) * 256, base + kQ, base + kK + kb * kTile,
+               in16s(live_keys(p, s_unit, sj)));
         umma_commit(&s_ready[sn & 1]);
       }
       __syncwarp();
       ++sn;
-      if (++sj == slen) {
+      if (++sj == s_unit.n) {
         sj = 0;
         ++sc;
         su += gridDim.x;
-        slen = su < units ? dq_unit(p, su).n : 0;
+        if (su < units) s_unit = dq_unit(p, su);
       }
       return true;
     };
@@ -808,7 +816,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         if (one) {
-          mma_tm_pairs(tmem + 384, tmem + (n & 1) * 256, base + kK + kb * kTile, j == 0);
+          mma_tm_pairs(tmem + 384, tmem + (n & 1) * 256, base + kK + kb * kTile, j == 0,
+                       in16s(live_keys(p, c, j)));
           umma_commit(&k_free[kb]);
           if (j + 1 == c.n) umma_commit(dq_ready);
         }
@@ -871,25 +880,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = warp_wait2(&s_ready[par], static_cast<uint32_t>(n >> 1) & 1u, dp_ready, par, err, kErrWaitAccum);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[32], d[32];
-        tmem_ld_32x32b_x32(col + par * 256, s);
-        tmem_ld_32x32b_x32(col + 128, d);
-        tmem_ld_wait();
-        tc_fence_before();
-        mbar_arrive_warp(sp_free);
-        float2 e[16];
+        if (32 * grp >= live_keys(p, c, j)) {  // dQ does not read this group's columns
+          mbar_arrive_warp(sp_free);
+        } else {
+          uint32_t s[32], d[32];
+          tmem_ld_32x32b_x32(col + par * 256, s);
+          tmem_ld_32x32b_x32(col + 128, d);
+          tmem_ld_wait();
+          tc_fence_before();
+          mbar_arrive_warp(sp_free);
+          float2 e[16];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const float2 a = __ffma2_rn(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), sl2, nlse);
-          const float2 t = __fadd2_rn(make_float2(__uint_as_float(d[2 * q]), __uint_as_float(d[2 * q + 1])), ndi);
-          e[q] = __fmul2_rn(make_float2(exp2_approx(a.x), exp2_approx(a.y)), t);
+          for (int q = 0; q < 16; ++q) {
+            const float2 a = __ffma2_rn(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), sl2, nlse);
+            const float2 t = __fadd2_rn(make_float2(__uint_as_float(d[2 * q]), __uint_as_float(d[2 * q + 1])), ndi);
+            e[q] = __fmul2_rn(make_float2(exp2_approx(a.x), exp2_approx(a.y)), t);
+          }
+          keep_live(live, e);
+          uint32_t w[16];
+          pack16(e, w);
+          tmem_st_32x32b_x16(col + par * 256, w);
+          tmem_st_wait();
+          tc_fence_before();
         }
-        keep_live(live, e);
-        uint32_t w[16];
-        pack16(e, w);
-        tmem_st_32x32b_x16(col + par * 256, w);
-        tmem_st_wait();
-        tc_fence_before();
         mbar_arrive_warp(&ds_ready[par]);
         if (j == 0 && uc > 0) ok = finish(last, uc - 1);
         if (!ok) break;
