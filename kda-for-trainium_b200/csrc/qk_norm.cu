@@ -234,14 +234,34 @@ struct BwdParams {
 };
 
 // CTAs [0, blocks[0]) walk the queries, the others the keys; a group of LPR
-// lanes takes up to hp heads of a token, U at a time.  Each thread sums its columns of
-// dg over all its rows in registers; the CTA's sums go to `partial` in a fixed
-// order, so the result does not depend on timing.
-template <typename T, int D, int U>
+// lanes takes up to hp heads of a token, one after the other.  Each thread sums its
+// columns of dg over all its rows in registers; the CTA's sums go to `partial` in a
+// fixed order, so the result does not depend on timing.
+// The registers that dg takes leave two CTAs of 8 warps per SM, too few to cover the
+// memory's latency with loads into registers (B2 S4096 of 40 heads: 51 us, two rows at
+// a time), so the rows come through a ring of 4 per thread in shared memory, 64 KB a
+// CTA: 45 us, 5.6 TB/s (6 rows: 46; three CTAs with rings of 3, which spill: 66).
+constexpr int kRing = 4;
+constexpr size_t kRingBytes = kRing * 4 * kThreads * 16;
+constexpr int kBwdHeads = 4;  // heads per item (8: 46 us)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) norm_rope_bwd_kernel(const BwdParams p, unsigned* err) {
   constexpr int VE = Vec<T>::kN;
   constexpr int LPR = D / (2 * VE);
   constexpr int kGroups = kThreads / LPR;
+  extern __shared__ __align__(16) uint8_t norm_ring[];
   __shared__ __align__(8) float red[kThreads / 32][D];
   pdl_trigger();  // the join may take its place while this runs
   const int lane = threadIdx.x % LPR;
@@ -259,75 +279,103 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_bwd_kernel(const BwdPar
 #pragma unroll
   for (int i = 0; i < N; ++i) a0[i] = a1[i] = both(0.f);
 
-  // every group of a warp makes the same number of rounds (the shuffles need all lanes)
+  // Every group of a warp makes the same number of rounds (the shuffles need all
+  // lanes).  Rows come through a ring in shared memory, kRing - 1 of them on their way
+  // while one is worked on; a thread copies what it reads itself, so nothing is
+  // synchronised but its own copies.
+  struct Item {
+    const T *xs, *ds;
+    T* dst;
+    int nh;
+    int64_t pos;
+  };
   const unsigned step = static_cast<unsigned>(p.blocks[w]) * kGroups;
-  for (unsigned base = static_cast<unsigned>(block) * kGroups; base < items; base += step) {
+  auto locate = [&](unsigned base) -> Item {
     const unsigned item = base + threadIdx.x / LPR;
     const bool live = item < items;
     const unsigned tok = live ? item / nc : 0;
     const int h0 = live ? static_cast<int>(item - tok * nc) * hp : 0;
-    const int nh = live ? min(hp, H - h0) : 0;
     const int b = static_cast<int>(tok / static_cast<unsigned>(p.S));
     const int s = static_cast<int>(tok - static_cast<unsigned>(b) * static_cast<unsigned>(p.S));
-    const T* xs = static_cast<const T*>(xr.p) + b * xr.sb + s * xr.ss + h0 * xr.sh + lane * VE;
-    const T* ds = static_cast<const T*>(dyr.p) + b * dyr.sb + s * dyr.ss + h0 * dyr.sh + lane * VE;
-    T* dst = static_cast<T*>(dxr.p) + b * dxr.sb + s * dxr.ss + h0 * dxr.sh + lane * VE;
-    int64_t pos = s;
-    if (p.positions) pos = __ldg(p.positions + tok);
-    const bool bad = pos < 0 || pos >= p.table_len;
-    if (bad && live && lane == 0) atomicOr(err, static_cast<unsigned>(kErrRange));
+    Item c;
+    c.nh = live ? min(hp, H - h0) : 0;
+    c.xs = static_cast<const T*>(xr.p) + b * xr.sb + s * xr.ss + h0 * xr.sh + lane * VE;
+    c.ds = static_cast<const T*>(dyr.p) + b * dyr.sb + s * dyr.ss + h0 * dyr.sh + lane * VE;
+    c.dst = static_cast<T*>(dxr.p) + b * dxr.sb + s * dxr.ss + h0 * dxr.sh + lane * VE;
+    c.pos = p.positions ? __ldg(p.positions + tok) : s;
+    return c;
+  };
+  const unsigned base0 = static_cast<unsigned>(block) * kGroups;
+  const uint32_t ring = smem_u32(norm_ring) + threadIdx.x * 16;
+  unsigned abase = base0;  // the next row to ask for: its item, row of the item
+  int ah = 0;
+  Item a = locate(base0);
+  auto ask = [&](int stage) {
+    if (abase < items) {
+      const bool there = ah < a.nh;
+      const int64_t row = there ? ah : 0;
+      const uint32_t to = ring + stage * (4 * kThreads * 16);
+      cp_async16(to, a.xs + row * xr.sh, there);
+      cp_async16(to + kThreads * 16, a.xs + row * xr.sh + D / 2, there);
+      cp_async16(to + 2 * kThreads * 16, a.ds + row * dyr.sh, there);
+      cp_async16(to + 3 * kThreads * 16, a.ds + row * dyr.sh + D / 2, there);
+      if (++ah == hp) {
+        ah = 0;
+        abase += step;
+        if (abase < items) a = locate(abase);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) ask(i);
+  int stage = 0;
+  for (unsigned base = base0; base < items; base += step) {
+    const Item c = locate(base);
+    const bool bad = c.pos < 0 || c.pos >= p.table_len;
+    if (bad && c.nh > 0 && lane == 0) atomicOr(err, static_cast<unsigned>(kErrRange));
     float2 cs[N], sn[N];
-    load_angles(p.table + ((bad ? 0 : pos) * (D / 2) + lane * VE) * 2, cs, sn);
+    load_angles(p.table + ((bad ? 0 : c.pos) * (D / 2) + lane * VE) * 2, cs, sn);
     if (bad) {  // the position's rows come out as NaN
 #pragma unroll
       for (int i = 0; i < N; ++i) cs[i] = both(__int_as_float(0x7fffffff));
     }
-    for (int h = 0; h < hp; h += U) {
-      uint4 xl[U], xh[U], dl[U], dh[U];
+    for (int h = 0; h < hp; ++h) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      float2 x0[N], x1[N], y0[N], y1[N];
+      const uint32_t at = ring + stage * (4 * kThreads * 16);
+      Vec<T>::unpack(ld_shared16(at), x0);
+      Vec<T>::unpack(ld_shared16(at + kThreads * 16), x1);
+      Vec<T>::unpack(ld_shared16(at + 2 * kThreads * 16), y0);
+      Vec<T>::unpack(ld_shared16(at + 3 * kThreads * 16), y1);
+      float2 ss = both(0.f), xt = both(0.f);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        xl[u] = xh[u] = dl[u] = dh[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (h + u < nh) {
-          xl[u] = ld_stream(xs + (h + u) * xr.sh);
-          xh[u] = ld_stream(xs + (h + u) * xr.sh + D / 2);
-          dl[u] = ld_stream(ds + (h + u) * dyr.sh);
-          dh[u] = ld_stream(ds + (h + u) * dyr.sh + D / 2);
-        }
+      for (int i = 0; i < N; ++i) {
+        // dn = the rotation's transpose applied to dy
+        const float2 n0 = __ffma2_rn(y0[i], cs[i], __fmul2_rn(y1[i], sn[i]));
+        const float2 n1 = __ffma2_rn(y1[i], cs[i], neg(__fmul2_rn(y0[i], sn[i])));
+        y0[i] = n0;
+        y1[i] = n1;
+        ss = __ffma2_rn(x0[i], x0[i], __ffma2_rn(x1[i], x1[i], ss));
+        xt = __ffma2_rn(x0[i], __fmul2_rn(n0, g0[i]), __ffma2_rn(x1[i], __fmul2_rn(n1, g1[i]), xt));
       }
+      ask(stage == 0 ? kRing - 1 : stage - 1);  // into the row before's place
+      stage = stage + 1 == kRing ? 0 : stage + 1;
+      const float rs = rsqrtf(row_sum<LPR>(ss.x + ss.y) * (1.0f / D) + p.eps);
+      const float2 r = both(rs);
+      // dx = r t - x r^3 mean(x t)
+      const float2 k = both(-row_sum<LPR>(xt.x + xt.y) * (1.0f / D) * rs * rs * rs);
+      if (h >= c.nh) continue;  // after the shuffles; no row, no share of dg
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float2 x0[N], x1[N], y0[N], y1[N];
-        Vec<T>::unpack(xl[u], x0);
-        Vec<T>::unpack(xh[u], x1);
-        Vec<T>::unpack(dl[u], y0);
-        Vec<T>::unpack(dh[u], y1);
-        float2 ss = both(0.f), xt = both(0.f);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          // dn = the rotation's transpose applied to dy
-          const float2 n0 = __ffma2_rn(y0[i], cs[i], __fmul2_rn(y1[i], sn[i]));
-          const float2 n1 = __ffma2_rn(y1[i], cs[i], neg(__fmul2_rn(y0[i], sn[i])));
-          y0[i] = n0;
-          y1[i] = n1;
-          ss = __ffma2_rn(x0[i], x0[i], __ffma2_rn(x1[i], x1[i], ss));
-          xt = __ffma2_rn(x0[i], __fmul2_rn(n0, g0[i]), __ffma2_rn(x1[i], __fmul2_rn(n1, g1[i]), xt));
-        }
-        const float rs = rsqrtf(row_sum<LPR>(ss.x + ss.y) * (1.0f / D) + p.eps);
-        const float2 r = both(rs);
-        // dx = r t - x r^3 mean(x t)
-        const float2 k = both(-row_sum<LPR>(xt.x + xt.y) * (1.0f / D) * rs * rs * rs);
-        if (h + u >= nh) continue;  // after the shuffles; no row, no share of dg
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float2 m0 = __fmul2_rn(r, y0[i]), m1 = __fmul2_rn(r, y1[i]);
-          a0[i] = __ffma2_rn(x0[i], m0, a0[i]);
-          a1[i] = __ffma2_rn(x1[i], m1, a1[i]);
-          x0[i] = __ffma2_rn(m0, g0[i], __fmul2_rn(x0[i], k));
-          x1[i] = __ffma2_rn(m1, g1[i], __fmul2_rn(x1[i], k));
-        }
-        st_stream(dst + (h + u) * dxr.sh, Vec<T>::pack(x0));
-        st_stream(dst + (h + u) * dxr.sh + D / 2, Vec<T>::pack(x1));
+      for (int i = 0; i < N; ++i) {
+        const float2 m0 = __fmul2_rn(r, y0[i]), m1 = __fmul2_rn(r, y1[i]);
+        a0[i] = __ffma2_rn(x0[i], m0, a0[i]);
+        a1[i] = __ffma2_rn(x1[i], m1, a1[i]);
+        x0[i] = __ffma2_rn(m0, g0[i], __fmul2_rn(x0[i], k));
+        x1[i] = __ffma2_rn(m1, g1[i], __fmul2_rn(x1[i], k));
       }
+      st_stream(c.dst + h * dxr.sh, Vec<T>::pack(x0));
+      st_stream(c.dst + h * dxr.sh + D / 2, Vec<T>::pack(x1));
     }
   }
   // the groups of a warp, then the warps of the CTA
@@ -390,15 +438,14 @@ __global__ void __launch_bounds__(256) rope_table_any_kernel(float2* __restrict_
   tab[i] = make_float2(static_cast<float>(cs), static_cast<float>(sn));
 }
 
-constexpr int kFwdRows = 4, kBwdRows = 2;  // rows whose loads a group has in flight
+constexpr int kFwdRows = 4;  // rows whose loads a group has in flight
 
 // Heads per item: two rounds of `rows` where the rows fill the GPU many times
 // over, so that the token's angles and the weights (as many load instructions
 // as four bf16 rows) are paid once for both; one round otherwise.  Measured,
 // forward B8 S4096 of 40 heads, 1 / 2 / 4 / 8 rounds: 120 / 109 / 140 / 127 us
-// (few, short-lived items keep the reads of a CTA close together); backward
-// B2 S4096, 1 / 2 / 3 / 16 rounds: 53 / 51 / 55 / 65 us; fp32 B3 S1001 of 16
-// heads, 1 / 2 rounds: 4.8 / 5.0 us.
+// (few, short-lived items keep the reads of a CTA close together); fp32 B3 S1001 of
+// 16 heads, 1 / 2 rounds: 4.8 / 5.0 us.
 int heads_per_item(int64_t tokens, int64_t heads, int64_t lanes, int rows) {
   return tokens * heads * lanes >= 16 * 512ll * num_sms() ? 2 * rows : rows;
 }
@@ -435,21 +482,21 @@ kda_status launch_fwd(FwdParams& p, int64_t D, cudaStream_t st) {
   }
 }
 
-// The backward's items and CTAs: one CTA per round of work up to four per SM;
+// The backward's items and CTAs: one CTA per round of work up to eight per SM;
 // beyond that the two that are resident on each SM, shared between queries and
-// keys in proportion to their rows (a CTA that walks many rounds leaves fewer
-// shares of dg to join: 51 against 53 us at B2 S4096 of 40 heads; a short call
-// gains from the parallelism: 6.7 against 8.1 us at 777 tokens of 9 heads).
+// keys in proportion to their rows.  A CTA per round / resident CTAs: 777 tokens of
+// 9 heads of 256 6.7 / 8.4 us, 2048 of 24 heads of 128 11.3 / 12.8, 8192 of 10 (five
+// rounds per SM) 19.2 / 20.6, 8192 of 40 (17 per SM: the shares of dg) 60 / 45.
 void bwd_split(int64_t tokens, int64_t QH, int64_t KH, int64_t D, bool f32, int (&hp)[2], int (&blocks)[2]) {
   const int64_t lanes = D / (f32 ? 8 : 16);
   const int64_t groups = kThreads / lanes;
   const int64_t heads[2] = {QH, KH};
   int64_t rounds[2];
   for (int w = 0; w < 2; ++w) {
-    hp[w] = heads_per_item(tokens, QH + KH, lanes, kBwdRows);
+    hp[w] = kBwdHeads;
     rounds[w] = (tokens * ((heads[w] + hp[w] - 1) / hp[w]) + groups - 1) / groups;
   }
-  const bool few = rounds[0] + rounds[1] <= 4ll * num_sms();
+  const bool few = rounds[0] + rounds[1] <= 8ll * num_sms();
   for (int w = 0; w < 2; ++w) {
     const int64_t share = std::max<int64_t>(1, 2ll * num_sms() * heads[w] / (QH + KH));
     blocks[w] = static_cast<int>(few ? rounds[w] : std::min(rounds[w], share));
@@ -461,8 +508,17 @@ kda_status launch_bwd_d(const BwdParams& p, float* dgq, float* dgk, cudaStream_t
   const int64_t most = static_cast<int64_t>(p.B) * p.S *
                        std::max((p.H[0] + p.hp[0] - 1) / p.hp[0], (p.H[1] + p.hp[1] - 1) / p.hp[1]);
   KDA_CHECK_SUPPORTED(most < (1ll << 31), "qk_norm_rope_backward: too many rows (%lld tokens)", (long long)p.B * p.S);
-  norm_rope_bwd_kernel<T, D, kBwdRows>
-      <<<static_cast<unsigned>(p.blocks[0] + p.blocks[1]), kThreads, 0, st>>>(p, kda_err_ptr_qk_norm());
+  static std::atomic<bool> attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(norm_rope_bwd_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kRingBytes)) != cudaSuccess)
+      return launch_status("qk_norm_rope_backward: cudaFuncSetAttribute");
+    attr_set[dev].store(true, std::memory_order_release);
+  }
+  norm_rope_bwd_kernel<T, D>
+      <<<static_cast<unsigned>(p.blocks[0] + p.blocks[1]), kThreads, kRingBytes, st>>>(p, kda_err_ptr_qk_norm());
   const kda_status s = launch_status("qk_norm_rope_backward");
   if (s != KDA_OK) return s;
   cudaLaunchConfig_t cfg{};
