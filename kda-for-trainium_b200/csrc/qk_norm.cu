@@ -131,6 +131,8 @@ template <typename T, int D, int U, bool kAppend>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const FwdParams p, unsigned* err) {
   constexpr int VE = Vec<T>::kN;
   constexpr int LPR = D / (2 * VE);
+  pdl_trigger();  // the next launch may start
+  pdl_wait();     // the one before is done: what it wrote is there, what it read may be written
   const int lane = threadIdx.x % LPR;  // owns values [VE lane, + VE) of both halves
   const unsigned nc = p.cq + p.ck * (kAppend ? 2 : 1);
   const unsigned item = (blockIdx.x * static_cast<unsigned>(kThreads) + threadIdx.x) / LPR;
@@ -459,7 +461,16 @@ kda_status launch_fwd_u(FwdParams& p, int hp, cudaStream_t st) {
   const int64_t items = static_cast<int64_t>(p.B) * p.S * (p.cq + p.ck * (kAppend ? 2 : 1));
   KDA_CHECK_SUPPORTED(items * LPR < (1ll << 32), "qk_norm_rope: too many rows (%lld tokens)", (long long)p.B * p.S);
   const int64_t grid = (items * LPR + kThreads - 1) / kThreads;
-  norm_rope_kernel<T, D, U, kAppend><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p, kda_err_ptr_qk_norm());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, norm_rope_kernel<T, D, U, kAppend>, p, kda_err_ptr_qk_norm());
   return launch_status(kAppend ? "qk_norm_rope_append" : "qk_norm_rope");
 }
 

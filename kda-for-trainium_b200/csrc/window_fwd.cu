@@ -161,6 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();  // the next launch may start
+  pdl_wait();     // the one before is done
   const uint32_t tmem = *tmem_holder;
   const int units = p.B * p.QH * p.npairs;
 
@@ -532,7 +534,16 @@ extern "C" kda_status kda_gqa_window_bf16(const void* q, const void* k, const vo
   if ((s = tmap_head_rows(&to, out, B, S, QH, dense)) != KDA_OK) return s;
   const int64_t units = B * QH * p.npairs;
   const int grid = static_cast<int>(units < num_sms() ? units : num_sms());
-  window_fwd_kernel<<<grid, kThreads, Smem::kBytes, static_cast<cudaStream_t>(stream)>>>(tq, tk, tv, to, p,
-                                                                                         kda_err_ptr_window_fwd());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Smem::kBytes;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, window_fwd_kernel, tq, tk, tv, to, p, kda_err_ptr_window_fwd());
   return launch_status("gqa_window");
 }
