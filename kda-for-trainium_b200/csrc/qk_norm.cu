@@ -16,7 +16,7 @@
 // fp32; bf16 rows are rounded once, when they are stored.
 #include <algorithm>
 
-#include "common.cuh"
+#include "launch.cuh"
 
 KDA_DEFINE_ERROR_WORD(qk_norm)
 
@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_bwd_kernel(const BwdPar
   extern __shared__ __align__(16) uint8_t norm_ring[];
   __shared__ __align__(8) float red[kThreads / 32][D];
   pdl_trigger();  // the join may take its place while this runs
+  pdl_wait();     // the launch before this one is done
   const int lane = threadIdx.x % LPR;
   const int w = static_cast<int>(blockIdx.x) < p.blocks[0] ? 0 : 1;
   const int block = static_cast<int>(blockIdx.x) - (w ? p.blocks[0] : 0);
@@ -461,17 +462,8 @@ kda_status launch_fwd_u(FwdParams& p, int hp, cudaStream_t st) {
   const int64_t items = static_cast<int64_t>(p.B) * p.S * (p.cq + p.ck * (kAppend ? 2 : 1));
   KDA_CHECK_SUPPORTED(items * LPR < (1ll << 32), "qk_norm_rope: too many rows (%lld tokens)", (long long)p.B * p.S);
   const int64_t grid = (items * LPR + kThreads - 1) / kThreads;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, norm_rope_kernel<T, D, U, kAppend>, p, kda_err_ptr_qk_norm());
-  return launch_status(kAppend ? "qk_norm_rope_append" : "qk_norm_rope");
+  return launch_after(kAppend ? "qk_norm_rope_append" : "qk_norm_rope", norm_rope_kernel<T, D, U, kAppend>,
+                      dim3(static_cast<unsigned>(grid)), kThreads, 0, st, p, kda_err_ptr_qk_norm());
 }
 
 template <typename T, int D, bool kAppend>
@@ -528,22 +520,12 @@ kda_status launch_bwd_d(const BwdParams& p, float* dgq, float* dgk, cudaStream_t
       return launch_status("qk_norm_rope_backward: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  norm_rope_bwd_kernel<T, D>
-      <<<static_cast<unsigned>(p.blocks[0] + p.blocks[1]), kThreads, kRingBytes, st>>>(p, kda_err_ptr_qk_norm());
-  const kda_status s = launch_status("qk_norm_rope_backward");
+  const kda_status s = launch_after("qk_norm_rope_backward", norm_rope_bwd_kernel<T, D>,
+                                    dim3(static_cast<unsigned>(p.blocks[0] + p.blocks[1])), kThreads, kRingBytes, st, p,
+                                    kda_err_ptr_qk_norm());
   if (s != KDA_OK) return s;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(D / 32, 2);
-  cfg.blockDim = dim3(1024);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, dg_join_kernel, static_cast<const float*>(p.partial), dgq, dgk, D, p.blocks[0],
-                     p.blocks[1]);
-  return launch_status("qk_norm_rope_backward: dg");
+  return launch_after("qk_norm_rope_backward: dg", dg_join_kernel, dim3(D / 32, 2), 1024, 0, st, p.partial, dgq, dgk, D,
+                      p.blocks[0], p.blocks[1]);
 }
 
 template <typename T>

@@ -37,6 +37,7 @@
 
 #include <algorithm>
 
+#include "launch.cuh"
 #include "window.cuh"
 
 KDA_DEFINE_ERROR_WORD(window_bwd)
@@ -931,6 +932,9 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* _
                                                           const float* __restrict__ lse, float* __restrict__ ndi,
                                                           float* __restrict__ nlse, unsigned* __restrict__ counter,
                                                           int S, int SP, int QH) {
+  // First the launch before this one, then the next: its producers load operands, and it
+  // writes to the workspace, without waiting for this one.
+  pdl_wait();
   pdl_trigger();
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *counter = 0u;
   const int lane = threadIdx.x & 15;
@@ -985,26 +989,6 @@ Plan make_plan(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t window, int
   c.total = c.steps * B * KH;
   c.ctas = std::min<int64_t>(num_sms(), c.total);
   return c;
-}
-
-// `args...` launched so that its CTAs may take their places while the launch
-// before it drains; the kernels wait (griddepcontrol.wait) before they read
-// what that launch wrote.
-template <typename... P, typename... A>
-kda_status launch_after(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
-                        A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-  return launch_status(what);
 }
 
 }  // namespace
@@ -1082,10 +1066,10 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
       return launch_status("gqa_window_backward: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  window_rows_kernel<<<dim3(static_cast<unsigned>((SP / kRowsEach * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
-      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi, nlse, p.counter, p.S,
-      p.sp, p.QH);
-  KDA_WB_TRY(launch_status("gqa_window_backward: rows"));
+  KDA_WB_TRY(launch_after("gqa_window_backward: rows", window_rows_kernel,
+                          dim3(static_cast<unsigned>((SP / kRowsEach * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0,
+                          st, static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi,
+                          nlse, p.counter, p.S, p.sp, p.QH));
   // after a launch, which makes the device's context current in a thread that
   // has not used it yet (autograd's); the encoder is a driver call and needs one
   CUtensorMap tk, tv, tq, tdo;

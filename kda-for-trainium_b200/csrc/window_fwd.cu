@@ -37,6 +37,7 @@
 // All mbarrier waits are bounded (common.cuh); every TMA load targets one CTA.
 #include <math.h>
 
+#include "launch.cuh"
 #include "window.cuh"
 
 KDA_DEFINE_ERROR_WORD(window_fwd)
@@ -534,16 +535,6 @@ extern "C" kda_status kda_gqa_window_bf16(const void* q, const void* k, const vo
   if ((s = tmap_head_rows(&to, out, B, S, QH, dense)) != KDA_OK) return s;
   const int64_t units = B * QH * p.npairs;
   const int grid = static_cast<int>(units < num_sms() ? units : num_sms());
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Smem::kBytes;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, window_fwd_kernel, tq, tk, tv, to, p, kda_err_ptr_window_fwd());
-  return launch_status("gqa_window");
+  return launch_after("gqa_window", window_fwd_kernel, dim3(grid), kThreads, Smem::kBytes,
+                      static_cast<cudaStream_t>(stream), tq, tk, tv, to, p, kda_err_ptr_window_fwd());
 }
