@@ -932,9 +932,6 @@ __global__ void __launch_bounds__(256) window_rows_kernel(const __nv_bfloat16* _
                                                           const float* __restrict__ lse, float* __restrict__ ndi,
                                                           float* __restrict__ nlse, unsigned* __restrict__ counter,
                                                           int S, int SP, int QH) {
-  // First the launch before this one, then the next: its producers load operands, and it
-  // writes to the workspace, without waiting for this one.
-  pdl_wait();
   pdl_trigger();
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *counter = 0u;
   const int lane = threadIdx.x & 15;
@@ -1066,10 +1063,13 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
       return launch_status("gqa_window_backward: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  KDA_WB_TRY(launch_after("gqa_window_backward: rows", window_rows_kernel,
-                          dim3(static_cast<unsigned>((SP / kRowsEach * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0,
-                          st, static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi,
-                          nlse, p.counter, p.S, p.sp, p.QH));
+  // An ordinary launch: the next one's producers load operands, and it writes to the
+  // workspace, without waiting for this one (with this one early too and the next held
+  // until it has waited: S4096 W1024 of 16 heads 122.4 -> 123.8 us).
+  window_rows_kernel<<<dim3(static_cast<unsigned>((SP / kRowsEach * QH + 15) / 16), static_cast<unsigned>(B)), 256, 0, st>>>(
+      static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), lse, ndi, nlse, p.counter, p.S,
+      p.sp, p.QH);
+  KDA_WB_TRY(launch_status("gqa_window_backward: rows"));
   // after a launch, which makes the device's context current in a thread that
   // has not used it yet (autograd's); the encoder is a driver call and needs one
   CUtensorMap tk, tv, tq, tdo;
