@@ -53,7 +53,6 @@ namespace {
 
 constexpr int kRowWarps = 16;
 constexpr int kThreads = 128 + 32 * kRowWarps;
-constexpr int kRowThreads = 32 * kRowWarps;
 
 struct BwdParams {
   int B, S, QH, KH, rep;
