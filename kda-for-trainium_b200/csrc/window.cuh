@@ -166,6 +166,19 @@ __device__ __forceinline__ void mma_tm_pairs(uint32_t d, uint32_t a, uint32_t b,
     if (kk < k16)
       umma_bf16_ts(d, a + 32 * (kk >> 1) + 8 * (kk & 1), db + mnmajor_step(kk), kIdKM, (!first || kk != 0) ? 1u : 0u);
 }
+// The shares of a walk that is cut between CTAs: the first in slot 2 c + 1 of the CTA c
+// that began it, the others in slots 2 (c + 1), 2 (c + 2), ...  The slot after `slot`,
+// or -1 where the walk has all its steps (`steps` so far; advanced) or its records end:
+// a launch whose wait expired leaves some of them empty.
+__host__ __device__ __forceinline__ int next_share(const int4* pieces, int slots, int slot, int walk, int* steps) {
+  if (*steps >= walk) return -1;
+  const int next = (slot | 1) + 1;
+  if (next >= slots) return -1;
+  const int n = pieces[next].z;
+  if (n <= 0) return -1;
+  *steps += n < walk - *steps ? n : walk - *steps;
+  return next;
+}
 // 128 rows x 128 columns as two halves
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int head, int row, int b) {
   tma_load_4d(dst, m, bar, 0, head, row, b);

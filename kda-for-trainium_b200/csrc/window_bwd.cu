@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Piece c = piece_at(p, x, end - x);
     first_s[0] = c.bg, first_s[1] = c.j, first_s[2] = c.it0, first_s[3] = c.n, first_s[4] = c.walk, first_s[5] = c.nq;
     first_s[6] = static_cast<int>(end - x);
-    // no cut walk starts here, unless the row warps say so
-    if (c.it0 > 0 || c.n == c.walk) p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
+    // no share of a cut walk here, until the row warps say so (which they may not reach)
+    p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
   }
   tc_fence_before();
   __syncthreads();
@@ -610,12 +610,17 @@ __device__ __forceinline__ int in16s(int keys) { return (keys + 15) >> 4; }
 // of its run's CTA and the next ones'), added in order.  The row warps that have no
 // unit left take the items -- (CTA, dV or dK, 32 keys, 32 of d) -- one by one from
 // a counter, so the CTAs that had one unit fewer do most of it; which warp takes an
-// item makes no difference to its sum.
-__device__ __forceinline__ void join_cut_walks(const BwdParams& p) {
+// item makes no difference to its sum.  Nothing is joined once a wait has expired, here
+// or in the launch before: shares may be missing.
+__device__ __forceinline__ void join_cut_walks(const BwdParams& p, const unsigned* err) {
   const int lane = threadIdx.x & 31;
+  const bool failed = *reinterpret_cast<const volatile unsigned*>(err) != 0u;
   for (;;) {
     unsigned item = 0;
-    if (lane == 0) item = atomicAdd(p.counter, 1u);
+    if (lane == 0) {
+      item = atomicAdd(p.counter, 1u);
+      if (failed) item = 0xffffffffu;
+    }
     item = __shfl_sync(0xffffffffu, item, 0);
     if (item >= 32u * static_cast<unsigned>(p.ctas)) return;
     const int cta = static_cast<int>(item >> 5), which = (item >> 4) & 1, k0 = ((item >> 2) & 3) * 32, d0 = (item & 3) * 32;
@@ -624,13 +629,11 @@ __device__ __forceinline__ void join_cut_walks(const BwdParams& p) {
     float v[32];  // d0 + e of key k0 + lane
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] = 0.f;
-    int64_t slot = 2 * cta + 1;
-    for (int steps = w.z;; steps += p.pieces[slot].z) {
-      const float* src = p.partial + ((slot * 2 + which) * kD + d0) * kBlk + k0 + lane;
+    int steps = w.z;
+    for (int slot = 2 * cta + 1; slot >= 0; slot = next_share(p.pieces, 2 * p.ctas, slot, w.w, &steps)) {
+      const float* src = p.partial + ((static_cast<int64_t>(slot) * 2 + which) * kD + d0) * kBlk + k0 + lane;
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] += src[e * kBlk];
-      if (steps >= w.w) break;
-      slot = (slot | 1) + 1;
     }
     const float f = which == 0 ? 1.f : p.scale;
     const int b = w.x / p.KH, g = w.x - b * p.KH;
@@ -912,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ok && uc > 0) ok = finish(last, uc - 1);
     pdl_wait();  // the shares are written by the launch before this one
-    if (ok) join_cut_walks(p);
+    if (ok) join_cut_walks(p, err);
   }
 
   tc_fence_before();
