@@ -96,11 +96,12 @@ Tensor out_or_empty(const OptTensor& out, const char* name, at::IntArrayRef shap
   return *out;
 }
 
-// The caller's workspace (on `dev`, at least n bytes) or a fresh one.
+// The caller's workspace (on `dev`, at least n bytes, which lie together) or a fresh one.
 Tensor workspace_or_empty(const OptTensor& ws, size_t n, const at::Device& dev) {
   if (!ws) return empty({static_cast<int64_t>(n > 0 ? n : 1)}, at::kByte, dev);
   if (ws->device() != dev)
     value_error("workspace is on " + ws->device().str() + ", the operands on " + dev.str());
+  if (!ws->is_contiguous()) value_error("workspace must be contiguous");
   const size_t have = static_cast<size_t>(ws->numel()) * ws->element_size();
   if (have < n) value_error("workspace of " + std::to_string(n) + " bytes required, got " + std::to_string(have));
   return *ws;

@@ -1,0 +1,43 @@
+"""The local attention operators as they are called: buffers of the caller's, the
+registered forms, the C entry points, and what is refused."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def kda():
+    import kda as k
+    return k
+
+
+@pytest.fixture(autouse=True)
+def no_device_error(request, kda):
+    yield
+    if "gpu" in request.keywords:
+        torch.cuda.synchronize()
+        assert kda.device_error() == 0
+
+
+def rows(*shape, seed=0, dtype=BF16):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=gen, device="cuda").to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ws", ["expanded", "strided"])
+def test_a_workspace_whose_bytes_do_not_lie_together_is_refused(kda, ws):
+    """Its size counts bytes that it does not have, or that belong to its neighbours."""
+    q, kv = rows(1, 40, 4, 128), rows(1, 40, 2, 128, seed=1)
+    out, lse = kda.gqa_window_lse(q, kv, kv, 9)
+    g, table = torch.ones(128, device="cuda"), kda.rope_table(40, 128)
+    n = 1 << 26
+    ws = (torch.empty(1, dtype=torch.uint8, device="cuda").expand(n) if ws == "expanded"
+          else torch.empty(2 * n, dtype=torch.uint8, device="cuda")[::2])
+    with pytest.raises(ValueError, match="contiguous"):
+        kda.gqa_window_backward(out, q, kv, kv, out, lse, 9, workspace=ws)
+    with pytest.raises(ValueError, match="contiguous"):
+        kda.qk_norm_rope_backward(q, kv, q, kv, g, g, table, workspace=ws)
