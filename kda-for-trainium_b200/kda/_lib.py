@@ -135,16 +135,26 @@ def lib():
     return _lib
 
 
-def binding():
-    """The native binding of the local-attention operators.  It resolves the C
-    ABI in the library that ``lib()`` has loaded (matched by its soname)."""
-    lib()
-    try:
-        from . import _binding
-    except ImportError as e:
-        raise ImportError(f"kda/_binding.so is missing or was built against another torch ({e}); build it with "
-                          f"`python kda-for-trainium_b200/build.py`") from e
-    return _binding
+class _Binding:
+    """The native binding of the local-attention operators, loaded at the first
+    call of one of them: the other operators need only libkda.so.  It resolves
+    the C ABI in the library that ``lib()`` has loaded (matched by its soname)."""
+
+    def __getattr__(self, name):
+        if name.startswith("__"):  # asked for by introspection, not by a call
+            raise AttributeError(name)
+        lib()
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise ImportError(f"kda/_binding.so is missing or was built against another torch ({e}); build it with "
+                              f"`python kda-for-trainium_b200/build.py`") from e
+        fn = getattr(_binding, name)
+        setattr(self, name, fn)  # found there from now on
+        return fn
+
+
+binding = _Binding()
 
 
 _attached = set()

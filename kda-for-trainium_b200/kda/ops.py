@@ -616,7 +616,7 @@ def gqa_full_backward(dout, q, k, v, causal=False, rope_theta=None, *, fwd_out=N
 # ------------------------------------------------------------ local attention
 # One native call each (csrc/binding.cpp): argument checks, outputs, workspace,
 # current stream and the C entry point.
-_native = _lib.binding()
+_native = _lib.binding
 
 
 def rope_table(length, head_dim, theta=10000.0, *, device="cuda"):

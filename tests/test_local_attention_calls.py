@@ -41,3 +41,30 @@ def test_a_workspace_whose_bytes_do_not_lie_together_is_refused(kda, ws):
         kda.gqa_window_backward(out, q, kv, kv, out, lse, 9, workspace=ws)
     with pytest.raises(ValueError, match="contiguous"):
         kda.qk_norm_rope_backward(q, kv, q, kv, g, g, table, workspace=ws)
+
+
+def test_the_other_operators_do_not_need_the_native_binding():
+    """It is compiled against one torch; they are called through libkda.so alone."""
+    import os
+    import subprocess
+    import sys
+
+    from conftest import PKG_ROOT
+    code = """
+import sys
+sys.modules["kda._binding"] = None  # as if the file were missing, or did not load
+import torch
+import kda
+try:
+    kda.matmul(torch.zeros(4, 4), torch.zeros(4, 4))
+except ValueError:
+    print("matmul checked its arguments")
+try:
+    kda.gqa_window(torch.zeros(1, 4, 2, 128), None, None, 2)
+except ImportError as e:
+    print(e)
+"""
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": str(PKG_ROOT)},
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert "matmul checked its arguments" in r.stdout and "_binding.so is missing" in r.stdout
