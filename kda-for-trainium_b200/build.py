@@ -5,9 +5,11 @@
 Each ``csrc/*.cu`` is compiled separately (in parallel, skipped when up to
 date) into ``_build/`` and linked with the static CUDA runtime into
 ``kda/libkda.so``; ``csrc/binding.cpp`` (the local-attention operators' native
-Python binding, against the installed torch) becomes ``kda/_binding.so``.  The library does not link libcuda: the driver entry point
-it needs (``cuTensorMapEncodeTiled``) is resolved at run time, so the library
-loads -- and its symbols can be inspected -- on a machine without a GPU.
+Python binding, against the installed torch) becomes ``kda/_binding.so``.
+Without torch the library alone is built, for callers of the C ABI.  The library
+does not link libcuda: the driver entry point it needs
+(``cuTensorMapEncodeTiled``) is resolved at run time, so the library loads --
+and its symbols can be inspected -- on a machine without a GPU.
 """
 
 from __future__ import annotations
@@ -19,6 +21,7 @@ import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+from typing import Optional
 
 PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
@@ -62,10 +65,16 @@ def _compile(src: Path, force: bool, verbose: bool, extra) -> Path:
     return obj
 
 
-def _build_binding(force: bool, verbose: bool) -> Path:
-    """kda/_binding.so: host code only, resolved against the libkda.so beside it."""
+def _build_binding(force: bool, verbose: bool) -> Optional[Path]:
+    """kda/_binding.so: host code only, resolved against the libkda.so beside it;
+    None where there is no torch to build it against."""
+    import importlib.util
     import sysconfig
 
+    if importlib.util.find_spec("torch") is None:
+        print("torch is not installed: kda/_binding.so (the local-attention operators in Python) is not built",
+              file=sys.stderr)
+        return None
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 

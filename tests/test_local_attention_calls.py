@@ -68,3 +68,25 @@ except ImportError as e:
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
     assert "matmul checked its arguments" in r.stdout and "_binding.so is missing" in r.stdout
+
+
+def test_the_library_builds_without_torch(monkeypatch, tmp_path):
+    """For callers of the C ABI alone; the compiler and the linker are stand-ins here."""
+    import importlib.util
+    import sys
+
+    from conftest import PKG_ROOT
+    spec = importlib.util.spec_from_file_location("kda_build", PKG_ROOT / "build.py")
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    obj = tmp_path / "one.o"
+    obj.touch()
+    monkeypatch.setattr(b, "BUILD", tmp_path)
+    monkeypatch.setattr(b, "LIB", tmp_path / "libkda.so")
+    monkeypatch.setattr(b, "BINDING", tmp_path / "_binding.so")
+    monkeypatch.setattr(b, "_compile", lambda *a: obj)
+    ran = []
+    monkeypatch.setattr(b.subprocess, "run", lambda cmd, **kw: ran.append(cmd) or type("R", (), {"returncode": 0})())
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert b.build() == tmp_path / "libkda.so"
+    assert len(ran) == 1 and "-soname=libkda.so" in ran[0]  # the link, nothing else
