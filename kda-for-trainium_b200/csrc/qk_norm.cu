@@ -538,9 +538,10 @@ kda_status launch_bwd(const BwdParams& p, int64_t D, float* dgq, float* dgk, cud
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-// every row starts on 16 bytes
-bool rows_ok(const void* p, const int64_t* s, int es) {
-  return al16(p) && s[0] * es % 16 == 0 && s[1] * es % 16 == 0 && s[2] * es % 16 == 0;
+// every row of [n0][n1][n2] starts on 16 bytes (an axis of one entry may have any stride)
+bool rows_ok(const void* p, const int64_t* s, int64_t n0, int64_t n1, int64_t n2, int es) {
+  return al16(p) && (n0 == 1 || s[0] * es % 16 == 0) && (n1 == 1 || s[1] * es % 16 == 0) &&
+         (n2 == 1 || s[2] * es % 16 == 0);
 }
 
 kda_status common_check(const char* op, int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, float eps) {
@@ -587,8 +588,8 @@ extern "C" kda_status kda_qk_norm_rope(const void* q, const void* k, const float
   KDA_CHECK_ARG(table_len > 0 && (positions || table_len >= S), "%s: table of %lld positions for %lld tokens", op,
                 (long long)table_len, (long long)S);
   const int es = f32 ? 4 : 2;
-  KDA_CHECK_SUPPORTED(rows_ok(q, q_strides, es) && rows_ok(k, k_strides, es) && al16(gq) && al16(gk) && al16(table) &&
-                          al16(q_out) && al16(k_out),
+  KDA_CHECK_SUPPORTED(rows_ok(q, q_strides, B, S, QH, es) && rows_ok(k, k_strides, B, S, KH, es) && al16(gq) &&
+                          al16(gk) && al16(table) && al16(q_out) && al16(k_out),
                       "%s: pointers and rows must be 16-byte aligned", op);
   FwdParams p{};
   p.q = {q, q_strides[0], q_strides[1], q_strides[2]};
@@ -623,9 +624,10 @@ extern "C" kda_status kda_qk_norm_rope_append_bf16(const void* q, const void* k,
                     v_strides && k_cache_strides && v_cache_strides,
                 "%s: null pointer", op);
   KDA_CHECK_ARG(table_len > 0 && cache_len > 0, "%s: empty table or cache", op);
-  KDA_CHECK_SUPPORTED(rows_ok(q, q_strides, 2) && rows_ok(k, k_strides, 2) && rows_ok(v, v_strides, 2) &&
-                          rows_ok(k_cache, k_cache_strides, 2) && rows_ok(v_cache, v_cache_strides, 2) && al16(gq) &&
-                          al16(gk) && al16(table) && al16(q_out),
+  KDA_CHECK_SUPPORTED(rows_ok(q, q_strides, B, S, QH, 2) && rows_ok(k, k_strides, B, S, KH, 2) &&
+                          rows_ok(v, v_strides, B, S, KH, 2) && rows_ok(k_cache, k_cache_strides, B, cache_len, KH, 2) &&
+                          rows_ok(v_cache, v_cache_strides, B, cache_len, KH, 2) && al16(gq) && al16(gk) && al16(table) &&
+                          al16(q_out),
                       "%s: pointers and rows must be 16-byte aligned", op);
   FwdParams p{};
   p.q = {q, q_strides[0], q_strides[1], q_strides[2]};
@@ -669,8 +671,8 @@ extern "C" kda_status kda_qk_norm_rope_backward(const void* dq_out, const void* 
   KDA_CHECK_ARG(table_len > 0 && (positions || table_len >= S), "%s: table of %lld positions for %lld tokens", op,
                 (long long)table_len, (long long)S);
   const int es = f32 ? 4 : 2;
-  KDA_CHECK_SUPPORTED(rows_ok(q, q_strides, es) && rows_ok(k, k_strides, es) && al16(dq_out) && al16(dk_out) &&
-                          al16(gq) && al16(gk) && al16(table) && al16(dq) && al16(dk),
+  KDA_CHECK_SUPPORTED(rows_ok(q, q_strides, B, S, QH, es) && rows_ok(k, k_strides, B, S, KH, es) && al16(dq_out) &&
+                          al16(dk_out) && al16(gq) && al16(gk) && al16(table) && al16(dq) && al16(dk),
                       "%s: pointers and rows must be 16-byte aligned", op);
   const size_t need = kda_qk_norm_rope_backward_workspace_size(B, S, QH, KH, D, f32);
   KDA_CHECK_ARG(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes required, got %zu", op, need,

@@ -185,13 +185,13 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, ui
   tma_load_4d(dst + kHalf, m, bar, 64, head, row, b);
 }
 
-// The entry points' size checks; whether strided head rows start on 16 bytes; the
-// TMA map of [B][S][H][128] rows with element strides of batch, token and head
-// (128-row boxes of 64 columns; rows past S read as zeros, an axis of one entry
-// may have any stride).
+// The entry points' size checks; whether the strided rows of [n0][n1][n2] start on 16
+// bytes; the TMA map of [B][S][H][128] rows with element strides of batch, token and
+// head (128-row boxes of 64 columns; rows past S read as zeros).  In both an axis of one
+// entry may have any stride.
 kda_status gqa_window_check(const char* op, int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int64_t window,
                             int64_t sinks);
-bool head_rows_ok(const void* p, const int64_t* strides);
+bool head_rows_ok(const void* p, const int64_t* strides, int64_t n0, int64_t n1, int64_t n2);
 kda_status tmap_head_rows(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H, const int64_t* strides);
 
 }  // namespace kda

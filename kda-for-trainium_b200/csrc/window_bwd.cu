@@ -1013,9 +1013,10 @@ extern "C" kda_status kda_gqa_window_backward_bf16(const void* dout, const void*
   KDA_CHECK_ARG(dout && q && k && v && out && lse && dq && dk && dv && q_strides && k_strides && v_strides,
                 "%s: null pointer", op);
   const int64_t dense_q[3] = {S * QH * kD, QH * kD, kD}, dense_k[3] = {S * KH * kD, KH * kD, kD};
-  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
-                          head_rows_ok(dout, dense_q) && head_rows_ok(out, dense_q) && head_rows_ok(dq, dense_q) &&
-                          head_rows_ok(dk, dense_k) && head_rows_ok(dv, dense_k),
+  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides, B, S, QH) && head_rows_ok(k, k_strides, B, S, KH) &&
+                          head_rows_ok(v, v_strides, B, S, KH) && head_rows_ok(dout, dense_q, B, S, QH) &&
+                          head_rows_ok(out, dense_q, B, S, QH) && head_rows_ok(dq, dense_q, B, S, QH) &&
+                          head_rows_ok(dk, dense_k, B, S, KH) && head_rows_ok(dv, dense_k, B, S, KH),
                       "%s: pointers and rows must be 16-byte aligned", op);
   const size_t need = kda_gqa_window_backward_workspace_size(B, S, QH, KH, D, window, sinks);
   KDA_CHECK_ARG(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes required, got %zu", op, need,

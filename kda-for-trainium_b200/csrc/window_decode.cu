@@ -378,8 +378,8 @@ extern "C" kda_status kda_gqa_window_decode_bf16(const void* q, const void* k_ca
   KDA_CHECK_ARG(q && k_cache && v_cache && lengths && out && q_strides && k_strides && v_strides, "%s: null pointer",
                 op);
   const int64_t qs[3] = {q_strides[0], q_strides[1], 0};
-  KDA_CHECK_SUPPORTED(head_rows_ok(q, qs) && head_rows_ok(k_cache, k_strides) && head_rows_ok(v_cache, v_strides) &&
-                          (reinterpret_cast<uintptr_t>(out) & 15u) == 0,
+  KDA_CHECK_SUPPORTED(head_rows_ok(q, qs, B, QH, 1) && head_rows_ok(k_cache, k_strides, B, T, KH) &&
+                          head_rows_ok(v_cache, v_strides, B, T, KH) && (reinterpret_cast<uintptr_t>(out) & 15u) == 0,
                       "%s: pointers and rows must be 16-byte aligned", op);
   DecodeParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q);

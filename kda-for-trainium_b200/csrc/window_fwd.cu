@@ -470,9 +470,11 @@ kda_status gqa_window_check(const char* op, int64_t B, int64_t S, int64_t QH, in
   return KDA_OK;
 }
 
-bool head_rows_ok(const void* p, const int64_t* s) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0 &&
-         s[0] >= 0 && s[1] >= 0 && s[2] >= 0;
+bool head_rows_ok(const void* p, const int64_t* s, int64_t n0, int64_t n1, int64_t n2) {
+  const int64_t n[3] = {n0, n1, n2};
+  bool ok = (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (n[i] == 1 || (s[i] >= 0 && s[i] % 8 == 0));
+  return ok;
 }
 
 kda_status tmap_head_rows(CUtensorMap* m, const void* base, int64_t B, int64_t S, int64_t H, const int64_t* strides) {
@@ -498,8 +500,8 @@ extern "C" kda_status kda_gqa_window_bf16(const void* q, const void* k, const vo
   if ((s = gqa_window_check(op, B, S, QH, KH, D, window, sinks)) != KDA_OK) return s;
   KDA_CHECK_ARG(q && k && v && out && q_strides && k_strides && v_strides, "%s: null pointer", op);
   const int64_t dense[3] = {S * QH * kD, QH * kD, kD};
-  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides) && head_rows_ok(k, k_strides) && head_rows_ok(v, v_strides) &&
-                          head_rows_ok(out, dense),
+  KDA_CHECK_SUPPORTED(head_rows_ok(q, q_strides, B, S, QH) && head_rows_ok(k, k_strides, B, S, KH) &&
+                          head_rows_ok(v, v_strides, B, S, KH) && head_rows_ok(out, dense, B, S, QH),
                       "%s: pointers and rows must be 16-byte aligned", op);
   FwdParams p{};
   p.B = static_cast<int>(B);

@@ -90,3 +90,60 @@ def test_the_library_builds_without_torch(monkeypatch, tmp_path):
     monkeypatch.setitem(sys.modules, "torch", None)
     assert b.build() == tmp_path / "libkda.so"
     assert len(ran) == 1 and "-soname=libkda.so" in ran[0]  # the link, nothing else
+
+
+def strides(*s):
+    import ctypes as C
+    return (C.c_int64 * 3)(*s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("odd", [7, -3])
+def test_c_entries_take_any_stride_of_an_axis_of_one_entry(kda, odd):
+    from kda import _lib
+    B, QH, KH, D, T = 1, 4, 1, 128, 24
+    g, table = torch.ones(D, device="cuda"), kda.rope_table(T, D)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def call(fn, *args):
+        _lib.call(fn, *(a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args), stream)
+
+    for S in (1, 5):
+        tok = odd if S == 1 else QH * D, odd if S == 1 else KH * D
+        qs, ks = strides(odd, tok[0], D), strides(odd, tok[1], odd)
+        q, k, v = rows(B, S, QH, D), rows(B, S, KH, D, seed=1), rows(B, S, KH, D, seed=2)
+        qr, kr = kda.qk_norm_rope(q, k, g, g, table)
+        a, b = torch.empty_like(q), torch.empty_like(k)
+        call("kda_qk_norm_rope", q, k, g, g, table, T, None, 1e-6, a, b, B, S, QH, KH, D, qs, ks, 0)
+        assert torch.equal(a, qr) and torch.equal(b, kr)
+
+        kc, vc, kc2, vc2 = (torch.zeros(B, T, KH, D, dtype=BF16, device="cuda") for _ in range(4))
+        n = torch.tensor([3], dtype=torch.int32, device="cuda")
+        want = kda.qk_norm_rope_append(q, k, v, g, g, table, kc, vc, n)
+        cs = strides(odd, KH * D, odd)
+        call("kda_qk_norm_rope_append_bf16", q, k, v, g, g, table, T, n, 1e-6, a, kc2, vc2, T, B, S, QH, KH, D, qs, ks, ks,
+             cs, cs)
+        assert torch.equal(a, want) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+
+        dq, dk, dgq, dgk = kda.qk_norm_rope_backward(qr, kr, q, k, g, g, table)
+        c, d = torch.empty_like(g), torch.empty_like(g)
+        nb = _lib._attach(_lib.lib(), "kda_qk_norm_rope_backward_workspace_size")(B, S, QH, KH, D, 0)
+        call("kda_qk_norm_rope_backward", qr, kr, q, k, g, g, table, T, None, 1e-6, a, b, c, d, B, S, QH, KH, D, qs, ks, 0,
+             torch.empty(nb, dtype=torch.uint8, device="cuda"), nb)
+        assert torch.equal(a, dq) and torch.equal(b, dk) and torch.equal(c, dgq) and torch.equal(d, dgk)
+
+        out, lse = kda.gqa_window_lse(q, k, v, 3, 1)
+        lse2 = torch.empty_like(lse)
+        call("kda_gqa_window_bf16", q, k, v, a, lse2, B, S, QH, KH, D, 3, 1, qs, ks, ks)
+        assert torch.equal(a, out) and torch.equal(lse, lse2)
+
+        grads = kda.gqa_window_backward(qr, q, k, v, out, lse, 3, 1)
+        e = torch.empty_like(v)
+        nb = _lib._attach(_lib.lib(), "kda_gqa_window_backward_workspace_size")(B, S, QH, KH, D, 3, 1)
+        call("kda_gqa_window_backward_bf16", qr, q, k, v, out, lse, a, b, e, B, S, QH, KH, D, 3, 1, qs, ks, ks,
+             torch.empty(nb, dtype=torch.uint8, device="cuda"), nb)
+        assert all(torch.equal(x, y) for x, y in zip((a, b, e), grads))
+
+        y, row = kda.gqa_window_decode(q[:, 0], kc, vc, n + S, 3, 1), torch.empty(B, QH, D, dtype=BF16, device="cuda")
+        call("kda_gqa_window_decode_bf16", q, kc, vc, n + S, row, B, T, QH, KH, D, 3, 1, strides(odd, D, 0), cs, cs)
+        assert torch.equal(row, y)
