@@ -23,7 +23,8 @@
  *     ABI.  kda_last_error() gives the calling thread's detail message.
  *   - Kernels bound every internal wait; a wait that expires writes a code to
  *     a device error word that kda_device_error() reads after the stream is
- *     synchronised.
+ *     synchronised.  The local-attention kernels report a position or length
+ *     outside its table or cache there too, with the value 8.
  *   - Ops that need scratch memory take (workspace, workspace_bytes); the
  *     required size comes from the matching *_workspace_size() query.
  */
@@ -53,7 +54,9 @@ const char* kda_status_string(kda_status s);
 /* Detail message of the last non-OK status returned on this thread. */
 const char* kda_last_error(void);
 /* Reads (and with clear != 0 resets) the OR of the device error words of the
- * current device.  *word == 0 means no kernel reported an expired wait.
+ * current device.  *word == 0 (KDA_OK): no kernel reported anything.  A word
+ * of 8 (KDA_INVALID_ARG): a position or length lay outside its table or cache.
+ * Any other (KDA_TIMEOUT): a kernel's wait expired.
  * Synchronous with respect to the device (cudaMemcpyFromSymbol). */
 kda_status kda_device_error(unsigned* word, int clear);
 
@@ -461,7 +464,7 @@ kda_status kda_rope_table_f32(float* table, int64_t length, int64_t D, float the
  * (half-split rotation), written contiguous to q_out, k_out in the inputs'
  * type (bf16, or fp32 with f32 != 0); gq, gk (D,) fp32; D 64, 128 or 256.
  * positions: int32 [B][S], or NULL for 0 .. S-1.  A position outside
- * [0, table_len) gives NaN rows and sets bit 8 of the device error word. */
+ * [0, table_len) gives NaN rows and sets 8 in the device error word. */
 kda_status kda_qk_norm_rope(const void* q, const void* k, const float* gq, const float* gk, const float* table,
                             int64_t table_len, const int* positions, float eps, void* q_out, void* k_out, int64_t B,
                             int64_t S, int64_t QH, int64_t KH, int64_t D, const int64_t* q_strides,
@@ -471,7 +474,7 @@ kda_status kda_qk_norm_rope(const void* q, const void* k, const float* gq, const
  * positions lengths[b] + s (int32 [B], tokens already cached): q_out (B,S,QH,D)
  * contiguous, the rotated k and v as it is into the caches (B,cache_len,KH,D,
  * strided) at those positions.  lengths[b] < 0: an idle slot, zeros and no
- * write.  A position outside the cache or the table: NaN, no write, bit 8 of
+ * write.  A position outside the cache or the table: NaN, no write, 8 in
  * the device error word. */
 kda_status kda_qk_norm_rope_append_bf16(const void* q, const void* k, const void* v, const float* gq,
                                         const float* gk, const float* table, int64_t table_len, const int* lengths,
@@ -514,7 +517,7 @@ kda_status kda_gqa_window_backward_bf16(const void* dout, const void* q, const v
  * request, q (B,QH,D) (strides of batch and head), against the caches
  * (B,T,KH,D, strided) of which lengths[b] tokens are valid, the newest among
  * them; out (B,QH,D) contiguous.  lengths[b] <= 0: zeros; a length past T is
- * cut to T and sets bit 8 of the device error word.  No workspace. */
+ * cut to T and sets 8 in the device error word.  No workspace. */
 kda_status kda_gqa_window_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const int* lengths,
                                       void* out, int64_t B, int64_t T, int64_t QH, int64_t KH, int64_t D,
                                       int64_t window, int64_t sinks, const int64_t* q_strides,

@@ -167,9 +167,15 @@ kda_status kda_device_error(unsigned* word, int clear) {
     acc |= w;
   }
   *word = acc;
-  if (acc != 0) {
-    kda::set_error("a kernel reported an expired wait (device error word 0x%x)", acc);
+  const bool range = (acc & kda::kErrRange) != 0;
+  if ((acc & ~static_cast<unsigned>(kda::kErrRange)) != 0) {
+    kda::set_error("a kernel reported an expired wait%s (device error word 0x%x)",
+                   range ? " and a position or length outside its table or cache" : "", acc);
     return KDA_TIMEOUT;
+  }
+  if (range) {
+    kda::set_error("a kernel met a position or length outside its table or cache (device error word 0x%x)", acc);
+    return KDA_INVALID_ARG;
   }
   return KDA_OK;
 }

@@ -147,3 +147,18 @@ def test_c_entries_take_any_stride_of_an_axis_of_one_entry(kda, odd):
         y, row = kda.gqa_window_decode(q[:, 0], kc, vc, n + S, 3, 1), torch.empty(B, QH, D, dtype=BF16, device="cuda")
         call("kda_gqa_window_decode_bf16", q, kc, vc, n + S, row, B, T, QH, KH, D, 3, 1, strides(odd, D, 0), cs, cs)
         assert torch.equal(row, y)
+
+
+@pytest.mark.gpu
+def test_a_position_outside_its_table_is_not_called_an_expired_wait(kda):
+    import ctypes as C
+
+    from kda import _lib
+    t, g = rows(1, 3, 2, 128), torch.ones(128, device="cuda")
+    pos = torch.tensor([[0, 1, 4]], dtype=torch.int32, device="cuda")
+    kda.qk_norm_rope(t, t, g, g, kda.rope_table(4, 128), positions=pos)
+    torch.cuda.synchronize()
+    word, h = C.c_uint(0), _lib.lib()
+    assert h.kda_device_error(C.byref(word), 1) == 1 and word.value == 8  # KDA_INVALID_ARG
+    assert "outside its table" in h.kda_last_error().decode()
+    assert h.kda_device_error(C.byref(word), 1) == 0 and word.value == 0
