@@ -82,6 +82,25 @@ def gqa_full(q, k, v, causal=False, rope_theta=None):
     return _GQA.apply(q, k, v, causal, rope_theta)
 
 
+class _FirstOnly(torch.autograd.Function):
+    """The first n of ``tensors``, a backward's gradients, unchanged; the others are
+    what they were computed from.  Differentiating them again raises."""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("kda.autograd: second derivatives of this operator are not implemented")
+
+
+def _first_only(grads, *computed_from):
+    """With create_graph=True the gradients become part of a graph; the kernels are
+    not, so a term that goes through them would be left out without a word."""
+    return _FirstOnly.apply(len(grads), *grads, *computed_from) if torch.is_grad_enabled() else grads
+
+
 class _QKNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, gq, gk, table, positions, eps):
@@ -94,12 +113,12 @@ class _QKNormRope(torch.autograd.Function):
         q, k, gq, gk, table, positions = ctx.saved_tensors
         grads = ops.qk_norm_rope_backward(dq.to(q.dtype).contiguous(), dk.to(q.dtype).contiguous(), q, k, gq, gk,
                                           table, positions=positions, eps=ctx.eps)
-        return (*grads, None, None, None)
+        return (*_first_only(grads, dq, dk, q, k, gq, gk), None, None, None)
 
 
 def qk_norm_rope(q, k, gq, gk, table, *, positions=None, eps=1e-6):
     """Differentiable ``kda.qk_norm_rope``: gradients for q, k, gq and gk come
-    from ``kda.qk_norm_rope_backward``."""
+    from ``kda.qk_norm_rope_backward``; second derivatives raise."""
     return _QKNormRope.apply(q, k, gq, gk, table, positions, eps)
 
 
@@ -115,10 +134,11 @@ class _GQAWindow(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         grads = ops.gqa_window_backward(dout.to(torch.bfloat16).contiguous(), q, k, v, out, lse, ctx.window, ctx.sinks)
-        return (*grads, None, None)
+        return (*_first_only(grads, dout, q, k, v), None, None)
 
 
 def gqa_window(q, k, v, window, sinks=0):
     """Differentiable ``kda.gqa_window`` (bf16): the forward keeps its row
-    log2-sum-exp, the gradients come from ``kda.gqa_window_backward``."""
+    log2-sum-exp, the gradients come from ``kda.gqa_window_backward``; second
+    derivatives raise."""
     return _GQAWindow.apply(q, k, v, window, sinks)

@@ -162,3 +162,47 @@ def test_a_position_outside_its_table_is_not_called_an_expired_wait(kda):
     assert h.kda_device_error(C.byref(word), 1) == 1 and word.value == 8  # KDA_INVALID_ARG
     assert "outside its table" in h.kda_last_error().decode()
     assert h.kda_device_error(C.byref(word), 1) == 0 and word.value == 0
+
+
+@torch.no_grad()
+def _stand_in_norm(q, k, gq, gk, table, positions=None, eps=1e-6):
+    return q * gq, k * gk
+
+
+@torch.no_grad()
+def _stand_in_norm_backward(dq, dk, q, k, gq, gk, table, positions=None, eps=1e-6):
+    return dq * gq, dk * gk, (dq * q).sum((0, 1, 2)), (dk * k).sum((0, 1, 2))
+
+
+@torch.no_grad()
+def _stand_in_window(q, k, v, window, sinks):
+    return q * k * v, q[..., 0].float()
+
+
+@torch.no_grad()
+def _stand_in_window_backward(dout, q, k, v, out, lse, window, sinks):
+    return dout * k * v, dout * q * v, dout * q * k
+
+
+@pytest.mark.parametrize("op", ["norm", "window"])
+@pytest.mark.parametrize("loss", ["sum", "square"])
+def test_second_derivatives_raise(kda, monkeypatch, op, loss):
+    """The kernels give first derivatives.  What depends on a gradient must not lose that
+    gradient's own part silently (stand-ins for the kernels: no GPU)."""
+    import kda.autograd as ka
+    for name, fn in (("qk_norm_rope", _stand_in_norm), ("qk_norm_rope_backward", _stand_in_norm_backward),
+                     ("gqa_window_lse", _stand_in_window), ("gqa_window_backward", _stand_in_window_backward)):
+        monkeypatch.setattr(ka.ops, name, fn)
+    gen = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(1, 3, 2, 4, generator=gen).to(BF16).requires_grad_() for _ in range(3))
+    gq, gk = torch.ones(4, dtype=BF16, requires_grad=True), torch.ones(4, dtype=BF16)
+
+    def value():
+        y = ka.qk_norm_rope(q, k, gq, gk, None)[0] if op == "norm" else ka.gqa_window(q, k, v, 2)
+        return y.sum() if loss == "sum" else y.square().sum()
+
+    want = torch.autograd.grad(value(), q)[0]
+    first, = torch.autograd.grad(value(), q, create_graph=True)
+    assert torch.equal(first, want)  # first derivatives as ever
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        (first.square().sum() + q.square().sum()).backward()
