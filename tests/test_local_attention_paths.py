@@ -1,0 +1,88 @@
+"""The local attention kernels where they run as in large calls -- many items, units and
+pieces for each CTA -- against their formulas in 64 bits, row by row or value by value,
+and their order among streams, graphs and launches.
+
+Bounds.  u = 2^-8 is the most that rounding to bf16 moves a value by, relative to it.
+Norms, each row's error: u of the row for bf16, and 1e-5 of |r t| (|y| in the forward), the
+scale of the terms that fp32 subtracts, for 30 roundings of 2^-24 or so along a row's sums,
+rsqrt and the products.  dg, whole: 1e-5, the fp32 gate.
+Attention, each value: a product of 128 terms is off by at most 2^-16 of the sum of its
+terms' sizes (fp32, truncated additions), which enters the softmax weights as a relative
+error eps; weights and dS round to bf16 (u) where they meet the tensor core, sums over up
+to 2^11 steps of 16 keys or queries are off by 2^-12 of the sum of their terms' sizes, and
+the result rounds (u).  The gradients are checked as functions of the saved out and lse.
+"""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+BF16, F32 = torch.bfloat16, torch.float32
+U = 2.0 ** -8
+
+
+@pytest.fixture(scope="module")
+def kda():
+    import kda as k
+    return k
+
+
+@pytest.fixture(autouse=True)
+def no_device_error(request, kda):
+    yield
+    torch.cuda.synchronize()
+    assert kda.device_error() == 0
+
+
+def normal(gen, *shape, dtype=BF16):
+    return torch.randn(shape, generator=gen, device="cuda").to(dtype)
+
+
+def packed(gen, B, S, heads, D, dtype=BF16):
+    """Head rows as slices of one projection."""
+    x = normal(gen, B, S, sum(heads) * D, dtype=dtype)
+    return [t.unflatten(-1, (-1, D)) for t in x.split([h * D for h in heads], dim=-1)]
+
+
+# ------------------------------------------------------------------ the norms
+def norm64(x, g, cs, dy, eps=1e-6):
+    """y, dx, dg and the rows' |r t| in 64 bits; cs: cos, sin of each token."""
+    x, g, dy = x.double(), g.double(), dy.double()
+    c, s = cs.double()[:, :, None, :, 0], cs.double()[:, :, None, :, 1]
+    h = x.shape[-1] // 2
+    r = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+    n = x * r * g
+    y = torch.cat([n[..., :h] * c - n[..., h:] * s, n[..., :h] * s + n[..., h:] * c], -1)
+    dn = torch.cat([dy[..., :h] * c + dy[..., h:] * s, dy[..., h:] * c - dy[..., :h] * s], -1)
+    t = g * dn
+    dx = r * t - x * r ** 3 * (x * t).mean(-1, keepdim=True)
+    return y, dx, (x * r * dn).sum((0, 1, 2)), (r * t).norm(dim=-1)
+
+
+# Enough rows that the forward takes its items in two rounds and the backward's CTAs loop
+# over items, queries and keys sharing the CTAs; tokens and heads that leave remainders.
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,QH,KH,D,dtype,docs", [(2, 4099, 33, 5, 128, BF16, False), (1, 5003, 12, 3, 256, F32, True),
+                                                    (3, 3001, 18, 2, 64, F32, False), (4, 4099, 25, 4, 64, BF16, True),
+                                                    (1, 4501, 17, 3, 256, BF16, False), (1, 9001, 1, 17, 128, F32, True)])
+def test_norms_of_many_rows(kda, B, S, QH, KH, D, dtype, docs):
+    gen = torch.Generator(device="cuda").manual_seed(S)
+    q, k = packed(gen, B, S, (QH, KH), D, dtype)
+    gq, gk = (normal(gen, D, dtype=F32) for _ in range(2))
+    dq, dk = normal(gen, B, S, QH, D, dtype=dtype), normal(gen, B, S, KH, D, dtype=dtype)
+    table = kda.rope_table(S + 3, D)
+    pos = torch.randint(0, S + 3, (B, S), generator=gen, device="cuda", dtype=torch.int32) if docs else None
+    cs = table[pos.long()] if docs else table[None, :S]
+    y = kda.qk_norm_rope(q, k, gq, gk, table, positions=pos)
+    grads = kda.qk_norm_rope_backward(dq, dk, q, k, gq, gk, table, positions=pos)
+    u = U if dtype == BF16 else 0.0
+    for i, (x, g, dy) in enumerate(((q, gq, dq), (k, gk, dk))):
+        wy, wdx, wdg, rt = norm64(x, g, cs, dy)
+        err = (y[i].double() - wy).norm(dim=-1)
+        assert (err <= (u + 1e-5) * wy.norm(dim=-1)).all()
+        err = (grads[i].double() - wdx).norm(dim=-1)
+        assert (err <= u * wdx.norm(dim=-1) + 1e-5 * rt).all()
+        assert (grads[2 + i].double() - wdg).norm() <= 1e-5 * wdg.norm()
+    for a, b in zip(grads, kda.qk_norm_rope_backward(dq, dk, q, k, gq, gk, table, positions=pos)):
+        assert torch.equal(a, b)
