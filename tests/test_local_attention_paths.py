@@ -86,3 +86,64 @@ def test_norms_of_many_rows(kda, B, S, QH, KH, D, dtype, docs):
         assert (grads[2 + i].double() - wdg).norm() <= 1e-5 * wdg.norm()
     for a, b in zip(grads, kda.qk_norm_rope_backward(dq, dk, q, k, gq, gk, table, positions=pos)):
         assert torch.equal(a, b)
+
+
+# -------------------------------------------------------------- the attention
+def check_window(q, k, v, dout, out, lse, grads, window, sinks):
+    """One batch entry, every value of the output and the gradients against its bound."""
+    S, QH, D = q.shape
+    KH, scale = k.shape[1], 128 ** -0.5
+    i = torch.arange(S, device="cuda")
+    seen = (i[None] <= i[:, None]) & ((i[:, None] - i[None] < window) | (i[None] < sinks))
+    want = {n: 0.0 for n in ("dk", "dv")}
+    bound = {n: 0.0 for n in ("dk", "dv")}
+
+    def within(name, got, want, err):
+        worst = ((got.double() - want).abs() / (1.01 * (err + U * want.abs()))).max().item()
+        assert worst <= 1.0, (name, worst)
+
+    for h in range(QH):
+        g = h // (QH // KH)
+        qh, kh, vh, dh, oh = (t.double() for t in (q[:, h], k[:, g], v[:, g], dout[:, h], out[:, h]))
+        s = scale * (qh @ kh.T)
+        eps = 2.0 ** -16 * scale * (qh.abs() @ kh.abs().T) + 2.0 ** -20
+        p = torch.softmax(s.masked_fill(~seen, -torch.inf), dim=-1)
+        within("out", out[:, h], p @ vh, (p * (U + 2.0 ** -12 + 2 * eps)) @ vh.abs())
+        # gradients, given out and lse
+        p = torch.exp2(s / np.log(2.0) - lse[h].double()[:, None]).masked_fill(~seen, 0.0)
+        dp, di = dh @ vh.T, (dh * oh).sum(-1, keepdim=True)
+        ds = p * (dp - di)
+        eta = 2.0 ** -16 * (dh.abs() @ vh.abs().T + (dh * oh).abs().sum(-1, keepdim=True))
+        ds_err = (U + 2.0 ** -12 + eps) * ds.abs() + p * eta
+        within("dq", grads[0][:, h], scale * (ds @ kh), scale * (ds_err @ kh.abs()))
+        want["dk"] = want["dk"] + scale * (ds.T @ qh)
+        bound["dk"] = bound["dk"] + scale * (ds_err.T @ qh.abs())
+        want["dv"] = want["dv"] + p.T @ dh
+        bound["dv"] = bound["dv"] + (p * (U + 2.0 ** -12 + eps)).T @ dh.abs()
+        if (h + 1) % (QH // KH) == 0:
+            within("dk", grads[1][:, g], want["dk"], bound["dk"])
+            within("dv", grads[2][:, g], want["dv"], bound["dv"])
+            for d in (want, bound):
+                d.update(dk=0.0, dv=0.0)
+
+
+# Five units of the forward and more for each CTA: short ones, and long ones of uneven walks.
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,QH,KH,window,sinks", [(4, 2100, 32, 8, 62, 0), (2, 1500, 64, 16, 1, 3),
+                                                    (3, 4700, 16, 2, 500, 0), (1, 9000, 24, 8, 1000, 130),
+                                                    (2, 2100, 48, 3, 2100, 4)])
+def test_window_of_many_units(kda, B, S, QH, KH, window, sinks):
+    gen = torch.Generator(device="cuda").manual_seed(S)
+    q, dout = normal(gen, B, S, QH, 128), normal(gen, B, S, QH, 128)
+    k, v = normal(gen, B, S, KH, 128), normal(gen, B, S, KH, 128)
+
+    def step():
+        out, lse = kda.gqa_window_lse(q, k, v, window, sinks)
+        return out, lse, *kda.gqa_window_backward(dout, q, k, v, out, lse, window, sinks)
+
+    first = step()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    out, lse, *grads = first
+    for b in range(B):
+        check_window(q[b], k[b], v[b], dout[b], out[b], lse[b], [t[b] for t in grads], window, sinks)
