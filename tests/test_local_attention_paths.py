@@ -147,3 +147,22 @@ def test_window_of_many_units(kda, B, S, QH, KH, window, sinks):
     out, lse, *grads = first
     for b in range(B):
         check_window(q[b], k[b], v[b], dout[b], out[b], lse[b], [t[b] for t in grads], window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["packed", "heads first"])
+def test_window_of_views_gives_the_bits_of_their_copies(kda, layout):
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    B, S, QH, KH = 2, 700, 6, 2
+    if layout == "packed":
+        q, k, v = packed(gen, B, S, (QH, KH, KH), 128)
+    else:
+        q, k, v = (normal(gen, B, h, S, 128).transpose(1, 2) for h in (QH, KH, KH))
+    dout = normal(gen, B, S, QH, 128)
+    copies = [t.contiguous() for t in (q, k, v)]
+    got, want = [], []
+    for args, to in (((q, k, v), got), (copies, want)):
+        out, lse = kda.gqa_window_lse(*args, 90, 140)
+        to += [out, lse, *kda.gqa_window_backward(dout, *args, out, lse, 90, 140)]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
