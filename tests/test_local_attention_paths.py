@@ -166,3 +166,43 @@ def test_window_of_views_gives_the_bits_of_their_copies(kda, layout):
         to += [out, lse, *kda.gqa_window_backward(dout, *args, out, lse, 90, 140)]
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def layer(kda, q, k, v, dout, g, table, n):
+    """Every kernel of the forward, the backward and the decode, one behind the other."""
+    a, b = kda.qk_norm_rope(q, k, g, g, table)
+    out, lse = kda.gqa_window_lse(a, b, v, 150, 2)
+    da, db, dv = kda.gqa_window_backward(dout, a, b, v, out, lse, 150, 2)
+    return out, lse, da, db, dv, *kda.qk_norm_rope_backward(da, db, q, k, g, g, table), \
+        kda.gqa_window_decode(a[:, -1], b, v, n, 150, 2)
+
+
+@pytest.mark.gpu
+def test_streams_and_graph_replays_give_the_bits_of_plain_calls(kda):
+    """The kernels start while the ones before them drain.  A graph replayed with other inputs
+    each time must not find what an earlier replay left."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    B, S, QH, KH = 2, 900, 8, 4
+    x, dout = normal(gen, B, S, (QH + 2 * KH) * 128), normal(gen, B, S, QH, 128)
+    q, k, v = (t.unflatten(-1, (-1, 128)) for t in x.split([QH * 128, KH * 128, KH * 128], dim=-1))
+    args = (kda, q, k, v, dout, torch.ones(128, device="cuda"), kda.rope_table(S, 128),
+            torch.full((B,), S, dtype=torch.int32, device="cuda"))
+    layer(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = layer(*args)
+    side = torch.cuda.Stream()
+    for _ in range(8):
+        x.normal_(generator=gen)
+        dout.normal_(generator=gen)
+        graph.replay()
+        got = [t.clone() for t in replayed]
+        torch.cuda.synchronize()
+        want = layer(*args)
+        torch.cuda.synchronize()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            aside = layer(*args)
+        torch.cuda.current_stream().wait_stream(side)
+        for a, b, c in zip(got, want, aside):
+            assert torch.equal(a, b) and torch.equal(c, b)
