@@ -206,3 +206,23 @@ def test_streams_and_graph_replays_give_the_bits_of_plain_calls(kda):
         torch.cuda.current_stream().wait_stream(side)
         for a, b, c in zip(got, want, aside):
             assert torch.equal(a, b) and torch.equal(c, b)
+
+
+@pytest.mark.gpu
+def test_backward_positions_outside_the_table_give_nan_and_are_reported(kda):
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    q, k = normal(gen, 2, 3, 5, 128), normal(gen, 2, 3, 2, 128)
+    dq, dk = normal(gen, 2, 3, 5, 128), normal(gen, 2, 3, 2, 128)
+    g, table = torch.ones(128, device="cuda"), kda.rope_table(4, 128)
+    good = torch.tensor([[0, 3, 1], [2, 0, 3]], dtype=torch.int32, device="cuda")
+    bad = good.clone()
+    bad[0, 1], bad[1, 2] = 4, -1
+    want = kda.qk_norm_rope_backward(dq, dk, q, k, g, g, table, positions=good)
+    got = kda.qk_norm_rope_backward(dq, dk, q, k, g, g, table, positions=bad)
+    torch.cuda.synchronize()
+    assert kda.device_error() == 8
+    off = good != bad
+    for a, b in zip(got[:2], want[:2]):
+        assert torch.isnan(a[off]).all() and torch.equal(a[~off], b[~off])
+    for a in got[2:]:  # sums over those rows too
+        assert torch.isnan(a).all()
