@@ -206,3 +206,25 @@ def test_second_derivatives_raise(kda, monkeypatch, op, loss):
     assert torch.equal(first, want)  # first derivatives as ever
     with pytest.raises(RuntimeError, match="second derivatives"):
         (first.square().sum() + q.square().sum()).backward()
+
+
+@pytest.mark.gpu
+def test_registered_forms_are_the_functions(kda):
+    """torch.ops.kda.<op>; the append's caches are written in place."""
+    q, k, v = rows(2, 20, 4, 128), rows(2, 20, 2, 128, seed=1), rows(2, 20, 2, 128, seed=2)
+    g, table = torch.full((128,), 0.5, device="cuda"), kda.rope_table(64, 128)
+    pos = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+    for got, want in ((torch.ops.kda.qk_norm_rope(q, k, g, g, table), kda.qk_norm_rope(q, k, g, g, table)),
+                      (torch.ops.kda.qk_norm_rope(q, k, g, g, table, pos, 1e-3),
+                       kda.qk_norm_rope(q, k, g, g, table, positions=pos, eps=1e-3)),
+                      ((torch.ops.kda.gqa_window(q, k, v, 7, 3),), (kda.gqa_window(q, k, v, 7, 3),))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    caches = [[rows(2, 64, 2, 128, seed=s) for s in (3, 4)] for _ in range(2)]
+    n = torch.tensor([0, 31], dtype=torch.int32, device="cuda")
+    got = torch.ops.kda.qk_norm_rope_append(q, k, v, g, g, table, *caches[0], n)
+    want = kda.qk_norm_rope_append(q, k, v, g, g, table, *caches[1], n)
+    assert torch.equal(got, want)
+    for a, b, s in zip(*caches, (3, 4)):
+        assert torch.equal(a, b) and not torch.equal(a, rows(2, 64, 2, 128, seed=s))
+    got = torch.ops.kda.gqa_window_decode(q[:, 0], *caches[0], n + 20, 9, 2)
+    assert torch.equal(got, kda.gqa_window_decode(q[:, 0], *caches[1], n + 20, 9, 2))
