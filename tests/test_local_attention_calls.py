@@ -228,3 +228,48 @@ def test_registered_forms_are_the_functions(kda):
         assert torch.equal(a, b) and not torch.equal(a, rows(2, 64, 2, 128, seed=s))
     got = torch.ops.kda.gqa_window_decode(q[:, 0], *caches[0], n + 20, 9, 2)
     assert torch.equal(got, kda.gqa_window_decode(q[:, 0], *caches[1], n + 20, 9, 2))
+
+
+@pytest.mark.gpu
+def test_the_callers_buffers_are_used(kda):
+    """out, q_out, k_out and workspace: written there, the same bits, whatever was in them."""
+    q, k, v = rows(2, 300, 4, 128), rows(2, 300, 2, 128, seed=1), rows(2, 300, 2, 128, seed=2)
+    dout = rows(2, 300, 4, 128, seed=3)
+    g, table = torch.full((128,), 0.5, device="cuda"), kda.rope_table(300, 128)
+
+    def nan(t):
+        return torch.full_like(t, float("nan"), memory_format=torch.contiguous_format)
+
+    def same(got, buffers, want):
+        for a, b, c in zip(got, buffers, want):
+            assert a.data_ptr() == b.data_ptr() and torch.equal(a, c) and torch.equal(b, c)
+
+    a, b = nan(q), nan(k)
+    same(kda.qk_norm_rope(q, k, g, g, table, q_out=a, k_out=b), (a, b), kda.qk_norm_rope(q, k, g, g, table))
+    a = nan(q)
+    same((kda.gqa_window(q, k, v, 70, 3, out=a),), (a,), (kda.gqa_window(q, k, v, 70, 3),))
+    n = torch.tensor([200, 300], dtype=torch.int32, device="cuda")
+    a = nan(q[:, 0])
+    same((kda.gqa_window_decode(q[:, 0], k, v, n, 70, 3, out=a),), (a,), (kda.gqa_window_decode(q[:, 0], k, v, n, 70, 3),))
+    kc, vc = rows(2, 304, 2, 128), rows(2, 304, 2, 128)
+    a, n = nan(q[:, :4]), torch.tensor([3, 300], dtype=torch.int32, device="cuda")
+    args = (q[:, :4], k[:, :4], v[:, :4], g, g, kda.rope_table(304, 128), kc, vc, n)
+    same((kda.qk_norm_rope_append(*args, q_out=a),), (a,), (kda.qk_norm_rope_append(*args),))
+
+    out, lse = kda.gqa_window_lse(q, k, v, 70, 3)
+    calls = ((kda.gqa_window_backward, (dout, q, k, v, out, lse, 70, 3)),
+             (kda.qk_norm_rope_backward, (dout, v, q, k, g, g, table)))
+    for fn, args in calls:
+        want = fn(*args)
+        for fill in (0x00, 0x7f, 0xff):
+            ws = torch.full((1 << 26,), fill, dtype=torch.uint8, device="cuda")
+            for _ in range(2):  # the second time with what the first has left
+                assert all(torch.equal(x, y) for x, y in zip(fn(*args, workspace=ws), want))
+        with pytest.raises(ValueError, match="bytes required"):
+            fn(*args, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    for bad in (lambda: kda.gqa_window(q, k, v, 70, 3, out=nan(k)),
+                lambda: kda.gqa_window(q, k, v, 70, 3, out=torch.empty(2, 4, 300, 128, dtype=BF16, device="cuda").transpose(1, 2)),
+                lambda: kda.qk_norm_rope(q, k, g, g, table, q_out=nan(q).float()),
+                lambda: kda.gqa_window_decode(q[:, 0], k, v, n, 70, 3, out=nan(q[:, 0]).cpu())):
+        with pytest.raises(ValueError):
+            bad()
