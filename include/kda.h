@@ -456,8 +456,8 @@ kda_status kda_gqa_full_backward_saved_bf16(const void* dout, const void* q, con
  * every row must start on 16 bytes.  An axis of one entry may have any stride. */
 
 /* rope_table: table [length][D/2][2] = cos, sin of position * theta^(-2 i / D)
- * (angles in double precision). */
-kda_status kda_rope_table_f32(float* table, int64_t length, int64_t D, float theta, void* stream);
+ * (theta and the angles in double precision). */
+kda_status kda_rope_table_f32(float* table, int64_t length, int64_t D, double theta, void* stream);
 
 /* qk_norm_rope: for each head row x of q (B,S,QH,D) and k (B,S,KH,D),
  *   y = rotate(x / sqrt(mean x^2 + eps) * g, table[position])

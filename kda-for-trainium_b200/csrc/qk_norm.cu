@@ -567,13 +567,13 @@ using namespace kda;
     if (s_ != KDA_OK) return s_; \
   } while (0)
 
-extern "C" kda_status kda_rope_table_f32(float* table, int64_t length, int64_t D, float theta, void* stream) {
-  KDA_CHECK_ARG(table && length > 0 && D > 0 && D % 2 == 0 && theta > 0.f,
+extern "C" kda_status kda_rope_table_f32(float* table, int64_t length, int64_t D, double theta, void* stream) {
+  KDA_CHECK_ARG(table && length > 0 && D > 0 && D % 2 == 0 && theta > 0.0,
                 "rope_table: bad arguments length=%lld D=%lld theta=%g", (long long)length, (long long)D, theta);
   KDA_CHECK_SUPPORTED(length <= (1ll << 38) / D, "rope_table: too many positions (%lld)", (long long)length);
   const int64_t n = length * (D / 2);
   rope_table_any_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      reinterpret_cast<float2*>(table), n, static_cast<int>(D / 2), log2(static_cast<double>(theta)));
+      reinterpret_cast<float2*>(table), n, static_cast<int>(D / 2), log2(theta));
   return launch_status("rope_table");
 }
 

@@ -94,7 +94,7 @@ PROTOTYPES = {
     "kda_zero1_adamw_f32": (INT, [P, P, INT, INT, I64, I64, P, P, D, D, D, D, D, I64, P]),
     "kda_gqa_full_f32_workspace_size": (SZ, [I64, I64, I64, I64, I64]),
     "kda_gqa_full_f32": (INT, [P, P, P, P, I64, I64, I64, I64, I64, INT, F, INT, P, SZ, P]),
-    "kda_rope_table_f32": (INT, [P, I64, I64, F, P]),
+    "kda_rope_table_f32": (INT, [P, I64, I64, D, P]),
     "kda_qk_norm_rope": (INT, [P, P, P, P, P, I64, P, F, P, P, I64, I64, I64, I64, I64, P, P, INT, P]),
     "kda_qk_norm_rope_append_bf16": (INT, [P, P, P, P, P, P, I64, P, F, P, P, P, I64, I64, I64, I64, I64, I64, P, P,
                                            P, P, P, P]),

@@ -60,6 +60,16 @@ def norm64(x, g, cs, dy, eps=1e-6):
     return y, dx, (x * r * dn).sum((0, 1, 2)), (r * t).norm(dim=-1)
 
 
+@pytest.mark.gpu
+def test_rope_table_of_a_theta_that_no_float_holds(kda):
+    """Angles in double precision: theta too.  (sincos and exp2 are good to a few 2^-53 of angles
+    of up to 2^17; the entries round to fp32.)"""
+    from oracle import ops as ref
+    theta = 10000.0 * 8.0 ** (128 / 126)
+    got = kda.rope_table(1 << 17, 128, theta)[-64:].double().cpu().numpy()
+    assert np.abs(got - ref.rope_table(1 << 17, 128, theta)[-64:]).max() <= 2.0 ** -23
+
+
 # Enough rows that the forward takes its items in two rounds and the backward's CTAs loop
 # over items, queries and keys sharing the CTAs; tokens and heads that leave remainders.
 @pytest.mark.gpu
