@@ -484,7 +484,9 @@ kda_status kda_qk_norm_rope_append_bf16(const void* q, const void* k, const void
                                         const int64_t* k_cache_strides, const int64_t* v_cache_strides, void* stream);
 
 /* Gradients of qk_norm_rope given those of its outputs (contiguous): dq, dk
- * contiguous in the inputs' type, dgq, dgk fp32 (D,), summed in a fixed order. */
+ * contiguous in the inputs' type, dgq, dgk fp32 (D,), summed in a fixed order.
+ * A position outside the table: NaN (its rows, dgq, dgk) and 8 in the device
+ * error word. */
 size_t kda_qk_norm_rope_backward_workspace_size(int64_t B, int64_t S, int64_t QH, int64_t KH, int64_t D, int f32);
 kda_status kda_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q, const void* k,
                                      const float* gq, const float* gk, const float* table, int64_t table_len,

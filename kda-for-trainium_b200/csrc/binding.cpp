@@ -2,8 +2,8 @@
 // and workspace allocation (torch's caching allocator), current stream, and
 // the C ABI call in one native function per operator.  A decode step makes two
 // of these calls per layer on kernels of a few microseconds; the same checks
-// in Python and ctypes cost 23 to 29 us a call, here 5 to 10 (the attention
-// backward, with three launches: 18).
+// in Python and ctypes cost 23 to 29 us a call, here 5 to 7 (the backward
+// passes, with two and three launches: 10 to 13).
 // The semantics are those of the functions in kda/ops.py that call it.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>

@@ -14,7 +14,7 @@
 // (7 products a block pair instead of 5): with one kernel that adds dQ into an
 // fp32 buffer the L2 took the additions at 2.3 TB/s (64 KB a block pair,
 // red.global and bulk reductions alike), which bound it at 172 us for S4096 W1024
-// of 16 heads, where the whole call now takes 125.
+// of 16 heads, where the whole call now takes 123.
 //
 // P^T, dS^T and dS are written to TMEM as bf16, each thread's into the columns of S
 // that it has read, and are the A operand of their products there: through shared
@@ -576,9 +576,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 // dQ's operand there.  dP(n + 1) is issued as soon as the rows have copied step n,
 // S(n + 2) (two regions) when dQ(n) has read dS(n); units follow one another
 // without a gap.
-// A step takes about 1,950 cycles, the row warps' chain again (1,024 of them the
-// exponentials' pipe); the tensor core works 1,536.  60 us at S4096 W1024 of 16
-// heads, cut walks joined: 512 units in 3.5 waves.
+// A step inside a unit takes about 1,950 cycles, the row warps' chain again (1,024 of
+// them the exponentials' pipe); the tensor core works 1,536.  Over a launch it works less
+// of the time: 61 us at S4096 W1024 of 16 heads, cut walks joined, are 93,400 cycles of an
+// SM, of which 43,200 of tensor work (27 whole steps and 2.5 narrow ones on average).  The
+// 512 units leave the CTAs with 23 to 32 whole steps; first loads, the units' ends and
+// the join are the rest.
 // TMEM columns: S [0,128) and [256,384), dP [128,256), dQ [384,512).
 struct Unit {
   int b, h, i;         // batch, query head, query block

@@ -6,7 +6,7 @@
 //   out = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  s_j = q . k_j log2e / sqrt(128)
 //
 // HBM-bound: every visible key and value row is read once, 256 bytes each, for
-// all query heads of its group.  The visible keys are numbered through
+// up to 16 query heads of its group (once more for each 16 beyond).  The visible keys are numbered through
 // (x < ns: the sinks before the window, then the window) and cut into tiles of
 // 16; a cluster of CTAs shares the tiles of one (request, kv head), and every
 // warp streams its own tiles through a private cp.async ring, so the loop has

@@ -27,8 +27,8 @@
 // V is read as stored (MN-major B).
 // TMEM columns: S [0,128), P_0 [128,192), P_1 [192,256), O_0 [256,384), O_1 [384,512).
 // Shared memory: Q_0 | Q_1 | outgoing O_0 | O_1 | ring (3 x 32 KB) | row exchange.
-// 1.17 ms at S32768 W2048 of 32 heads (1.07 TFLOP on visible pairs: 910 TFLOP/s, 0.53
-// of the measured bf16 rate): a step of two tiles takes about 3,250 cycles, of
+// 1.16 ms at S32768 W2048 of 32 heads (1.07 TFLOP on visible pairs: 923 TFLOP/s, 0.54
+// of the measured bf16 rate; 1.14 to 1.19 from box to box): a step of two tiles takes about 3,250 cycles, of
 // which the tensor core works 2,048 and the exponentials' pipe 2,048; the rest is the
 // latency of a tile's chain (wait, TMEM load, maximum, exponentials, store).  With P
 // through shared memory, S_t of each tile its own: 1.43 ms.  One of eight pairs by

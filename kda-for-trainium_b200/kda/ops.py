@@ -638,7 +638,7 @@ def qk_norm_rope(q, k, gq, gk, table, *, positions=None, eps=1e-6, q_out=None, k
     """Per-head RMS norm of queries and keys and the half-split rotation, in one
     pass: y = rotate(x / sqrt(mean_d x^2 + eps) * g), q (B,S,QH,D), k (B,S,KH,D)
     bf16 or fp32 (views of a packed projection are fine), gq, gk fp32 (D,), D 64,
-    128 or 256.  ``table`` is ``rope_table``'s; ``positions`` int32 (B,S) picks
+    128 or 256 (the attention below: 128).  ``table`` is ``rope_table``'s; ``positions`` int32 (B,S) picks
     its rows (default 0 .. S-1).  A position outside the table gives NaN and
     sets ``device_error``.  Returns (q', k'), contiguous, in q's dtype."""
     return _native.qk_norm_rope(q, k, gq, gk, table, positions, eps, q_out, k_out)
@@ -648,7 +648,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, gq, gk, table, *, positions=None
     """Gradients of ``qk_norm_rope(q, k, gq, gk, table)`` given those of its two
     outputs (contiguous, q's dtype): returns (dq, dk) shaped like q and k,
     contiguous, and (dgq, dgk) fp32, summed over tokens and heads in a fixed
-    order."""
+    order.  A position outside the table gives NaN (its rows, dgq and dgk) and
+    sets ``device_error``."""
     return _native.qk_norm_rope_backward(dq_out, dk_out, q, k, gq, gk, table, positions, eps, workspace)
 
 
@@ -667,7 +668,8 @@ def gqa_window(q, k, v, window, sinks=0, *, out=None):
     """Causal grouped-query attention inside a sliding window with sinks: query i
     sees key j <= i where i - j < window or j < sinks.  q (B,S,QH,128), k, v
     (B,S,KH,128) bf16, views are fine; returns (B,S,QH,128).  No rotation (see
-    ``qk_norm_rope``); scores scaled by 1 / sqrt(128)."""
+    ``qk_norm_rope``) and no document boundaries: a batch row is one sequence.
+    Scores scaled by 1 / sqrt(128)."""
     return _native.gqa_window(q, k, v, window, sinks, out, False)[0]
 
 
