@@ -525,6 +525,81 @@ kda_status kda_gqa_window_decode_bf16(const void* q, const void* k_cache, const 
                                       int64_t window, int64_t sinks, const int64_t* q_strides,
                                       const int64_t* k_strides, const int64_t* v_strides, void* stream);
 
+/* ------------------------------------- packed sequences, 4-bit caches --
+ * Attention over whole contexts: sequences of different lengths one behind
+ * the other in one buffer of tokens, and a key/value cache held in 4 bits.  No
+ * reference counterpart (the neighbours of gqa_full).  Rows and strides as
+ * above; here *_strides have two entries, token and head, unless stated. */
+
+/* packed_plan: the tables that gqa_packed and its backward work by, for
+ * sequences s = rows [offsets[s], offsets[s+1]) of a buffer of `tokens` rows;
+ * offsets: int32 [sequences+1] on the device, not falling, within [0, tokens]
+ * (else: a plan of no sequences and 8 in the device error word).  One plan serves
+ * every call on buffers of these offsets.  plan: 16-byte aligned, exactly the
+ * size that the query returns. */
+size_t kda_packed_plan_size(int64_t tokens, int64_t sequences);
+kda_status kda_packed_plan(const int* offsets, int64_t sequences, int64_t tokens, void* plan, size_t plan_bytes,
+                           void* stream);
+
+/* gqa_packed (bf16, D 128): causal attention within each sequence, scores
+ * scaled by 1/sqrt(D).  q (tokens,QH,D), k, v (tokens,KH,D); out
+ * (tokens,QH,D) contiguous; lse, if not NULL, [QH][tokens] fp32: each row's
+ * log2-sum-exp of the scaled scores, for the backward.  Rows of no sequence are
+ * never read into a result; in out and lse they become zeros (zero_rest != 0)
+ * or stay as they are.  A plan for another number of tokens: nothing is done
+ * and 8 is set in the device error word.  No workspace. */
+kda_status kda_gqa_packed_bf16(const void* q, const void* k, const void* v, const void* plan, size_t plan_bytes,
+                               void* out, float* lse, int zero_rest, int64_t tokens, int64_t QH, int64_t KH,
+                               int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                               const int64_t* v_strides, void* stream);
+
+/* Gradients of gqa_packed given dout and the forward's out (tokens,QH,D,
+ * contiguous) and lse: dq, dk, dv bf16, contiguous; rows of no sequence as in
+ * the forward. */
+size_t kda_gqa_packed_backward_workspace_size(int64_t tokens, size_t plan_bytes, int64_t QH, int64_t KH, int64_t D);
+kda_status kda_gqa_packed_backward_bf16(const void* dout, const void* q, const void* k, const void* v,
+                                        const void* out, const float* lse, const void* plan, size_t plan_bytes,
+                                        void* dq, void* dk, void* dv, int zero_rest, int64_t tokens, int64_t QH,
+                                        int64_t KH, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                                        const int64_t* v_strides, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+
+/* The 4-bit cache: (B, KH, blocks, bytes of a block) uint8, for keys and for
+ * values each, strided over request and head (byte strides, multiples of 16).
+ * A block holds 16 tokens of one head: 16 rows of 64 bytes of codes, then
+ * [16][128/group] pairs (step, low) of bf16; channel 32 g + 8 c + i of token t
+ * is nibble i of the 32-bit word at byte 64 t + 16 (c ^ (t/2 & 3)) + 4 g, and
+ * its value code * step + low with its group's pair.  group: 32, 64 or 128
+ * channels.  All zeros is a valid cache.  q4_block_bytes: 1024 + 8192/group. */
+size_t kda_q4_block_bytes(int64_t group);
+
+/* kv_append_q4: new rows of k and v (bf16) into the caches, per group low =
+ * min, step = bf16((max - low)/15), code = round((x - low)/step) (single fp32
+ * operations; a group that holds an infinity or a NaN reads back as NaN).
+ * offsets NULL: tokens/B rows of each request, k and v (B,S,KH,D) with strides
+ * of request, token and head; else int32 [B+1]: rows [offsets[b], offsets[b+1])
+ * of k, v (tokens,KH,D) are request b's (strides[0] is not used), rows of none
+ * are skipped.  Row i of request b goes to position lengths[b] + i (int32 [B]);
+ * lengths[b] < 0: an idle slot, no write.  A position past the cache: no write
+ * and 8 in the device error word. */
+kda_status kda_kv_append_q4(const void* k, const void* v, const int* offsets, const int* lengths, void* k_cache,
+                            void* v_cache, int64_t tokens, int64_t B, int64_t blocks, int64_t KH, int64_t D,
+                            int64_t group, const int64_t* k_strides, const int64_t* v_strides,
+                            const int64_t* k_cache_strides, const int64_t* v_cache_strides, void* stream);
+
+/* kv_read_q4: every value of a cache, out (B, 16 blocks, KH, D) bf16. */
+kda_status kda_kv_read_q4(const void* cache, void* out, int64_t B, int64_t blocks, int64_t KH, int64_t D,
+                          int64_t group, const int64_t* cache_strides, void* stream);
+
+/* gqa_decode_q4 (q, out bf16, D 128): gqa_window_decode against 4-bit caches.
+ * A window of the cache's length or more sees all of it. */
+size_t kda_gqa_decode_q4_workspace_size(int64_t QH, int64_t KH);
+kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, const void* v_cache, const int* lengths, void* out,
+                             int64_t B, int64_t blocks, int64_t QH, int64_t KH, int64_t D, int64_t group,
+                             int64_t window, int64_t sinks, const int64_t* q_strides,
+                             const int64_t* k_cache_strides, const int64_t* v_cache_strides, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,4 +1,4 @@
-// Python binding of the local-attention entry points: argument checks, output
+// Python binding of the attention entry points (local, packed, 4-bit cache): argument checks, output
 // and workspace allocation (torch's caching allocator), current stream, and
 // the C ABI call in one native function per operator.  A decode step makes two
 // of these calls per layer on kernels of a few microseconds; the same checks
@@ -277,14 +277,177 @@ Tensor gqa_window_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v
   return y;
 }
 
+// ------------------------------------------------ packed sequences, 4-bit caches
+Tensor packed_plan(const Tensor& offsets, int64_t tokens, const OptTensor& out) {
+  check_kind(offsets, "offsets", at::kInt, false, nullptr);
+  check_shape(offsets, "offsets", {-1});
+  if (!offsets.is_contiguous()) value_error("offsets must be contiguous");
+  const at::Device dev = offsets.device();
+  const int64_t n = offsets.size(0) - 1;
+  if (n < 1) value_error("offsets must have two entries or more, got " + std::to_string(n + 1));
+  if (tokens < 1) value_error("tokens must be positive, got " + std::to_string(tokens));
+  const size_t nb = kda_packed_plan_size(tokens, n);
+  if (nb == 0) value_error("too many tokens or sequences: " + std::to_string(tokens) + " and " + std::to_string(n));
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor plan = out_or_empty(out, "out", {static_cast<int64_t>(nb / 4)}, at::kInt, dev);
+  done("kda_packed_plan", kda_packed_plan(ptr<int>(offsets), n, tokens, plan.data_ptr(), nb, stream(dev)));
+  return plan;
+}
+
+struct PackedArgs {
+  Strides q, k, v;
+  int64_t T, QH, KH, D;
+  at::Device dev;
+  size_t plan;  // bytes
+};
+
+PackedArgs packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan) {
+  const Strides qs = check_rows(q, "q", kBf16, false, {-1, -1, 128});
+  const int64_t T = q.size(0);
+  const at::Device dev = q.device();
+  const Strides ks = check_rows(k, "k", kBf16, false, {T, -1, 128}, &dev);
+  const Strides vs = check_rows(v, "v", kBf16, false, {T, k.size(1), 128}, &dev);
+  check_groups(q.size(1), k.size(1));
+  check_dense(plan, "plan", at::kInt, {-1}, dev);
+  return {qs, ks, vs, T, q.size(1), k.size(1), 128, dev, static_cast<size_t>(plan.numel()) * 4};
+}
+
+std::tuple<Tensor, OptTensor> gqa_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan,
+                                         const OptTensor& out, bool with_lse) {
+  const PackedArgs a = packed_args(q, k, v, plan);
+  const c10::cuda::CUDAGuard guard(a.dev);
+  Tensor y = out_or_empty(out, "out", {a.T, a.QH, a.D}, kBf16, a.dev);
+  OptTensor lse;
+  if (with_lse) lse = empty({a.QH, a.T}, kF32, a.dev);
+  done("kda_gqa_packed_bf16",
+       kda_gqa_packed_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), plan.data_ptr(), a.plan, y.data_ptr(),
+                           ptr<float>(lse), !out, a.T, a.QH, a.KH, a.D, a.q.s, a.k.s, a.v.s, stream(a.dev)));
+  return {y, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gqa_packed_backward(const Tensor& dout, const Tensor& q, const Tensor& k,
+                                                       const Tensor& v, const Tensor& out, const Tensor& lse,
+                                                       const Tensor& plan, const OptTensor& workspace) {
+  const PackedArgs a = packed_args(q, k, v, plan);
+  check_dense(dout, "dout", kBf16, {a.T, a.QH, a.D}, a.dev);
+  check_dense(out, "out", kBf16, {a.T, a.QH, a.D}, a.dev);
+  check_dense(lse, "lse", kF32, {a.QH, a.T}, a.dev);
+  const c10::cuda::CUDAGuard guard(a.dev);
+  Tensor dq = empty({a.T, a.QH, a.D}, kBf16, a.dev);
+  Tensor dk = empty({a.T, a.KH, a.D}, kBf16, a.dev), dv = empty({a.T, a.KH, a.D}, kBf16, a.dev);
+  const size_t nb = kda_gqa_packed_backward_workspace_size(a.T, a.plan, a.QH, a.KH, a.D);
+  Tensor ws = workspace_or_empty(workspace, nb, a.dev);
+  done("kda_gqa_packed_backward_bf16",
+       kda_gqa_packed_backward_bf16(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                    ptr<float>(lse), plan.data_ptr(), a.plan, dq.data_ptr(), dk.data_ptr(),
+                                    dv.data_ptr(), 1, a.T, a.QH, a.KH, a.D, a.q.s, a.k.s, a.v.s, ws.data_ptr(), nb,
+                                    stream(a.dev)));
+  return {dq, dk, dv};
+}
+
+// A 4-bit cache (B, KH, blocks, bytes): its last two axes lie together, blocks start on 16
+// bytes, no expanded axis.  Returns the group its block size stands for.
+int64_t check_q4(const Tensor& t, const char* name, at::IntArrayRef want, const at::Device* dev, int64_t (&strides)[2]) {
+  check_kind(t, name, at::kByte, false, dev);
+  check_shape(t, name, want);
+  if (t.numel() == 0) value_error(std::string(name) + " must not be empty, got shape " + shape_str(t.sizes()));
+  int64_t group = 0;
+  for (const int64_t g : {32, 64, 128})
+    if (static_cast<int64_t>(kda_q4_block_bytes(g)) == t.size(3)) group = g;
+  if (group == 0)
+    value_error(std::string(name) + " must have blocks of 1280, 1152 or 1088 bytes (groups of 32, 64 or 128), got " +
+                std::to_string(t.size(3)));
+  bool ok = t.stride(3) == 1 && (t.size(2) == 1 || t.stride(2) == t.size(3)) &&
+            reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 2; ++i) {
+    strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    ok = ok && (t.size(i) == 1 || (strides[i] > 0 && strides[i] % 16 == 0));
+  }
+  if (!ok)
+    value_error(std::string(name) +
+                " must have contiguous blocks on 16-byte boundaries and no expanded axis, got strides " +
+                shape_str(t.strides()));
+  return group;
+}
+
+void kv_append_q4(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache,
+                  const Tensor& lengths, const OptTensor& offsets) {
+  Strides ks, vs;
+  int64_t B, KH, tokens;
+  if (offsets) {
+    ks = check_rows(k, "k", kBf16, false, {-1, -1, 128});
+    tokens = k.size(0), KH = k.size(1);
+  } else {
+    ks = check_rows(k, "k", kBf16, false, {-1, -1, -1, 128});
+    tokens = k.size(0) * k.size(1), KH = k.size(2);
+  }
+  const at::Device dev = k.device();
+  vs = check_rows(v, "v", kBf16, false, k.sizes(), &dev);
+  if (offsets) {  // strides of token and head
+    ks = {{0, ks.s[0], ks.s[1]}};
+    vs = {{0, vs.s[0], vs.s[1]}};
+  }
+  int64_t kc[2], vc[2];
+  const int64_t group = check_q4(k_cache, "k_cache", {offsets ? -1 : k.size(0), KH, -1, -1}, &dev, kc);
+  B = k_cache.size(0);
+  check_q4(v_cache, "v_cache", k_cache.sizes(), &dev, vc);
+  check_dense(lengths, "lengths", at::kInt, {B}, dev);
+  if (offsets) check_dense(*offsets, "offsets", at::kInt, {B + 1}, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  done("kda_kv_append_q4",
+       kda_kv_append_q4(k.data_ptr(), v.data_ptr(), ptr<int>(offsets), ptr<int>(lengths), k_cache.data_ptr(),
+                        v_cache.data_ptr(), tokens, B, k_cache.size(2), KH, 128, group, ks.s, vs.s, kc, vc,
+                        stream(dev)));
+}
+
+Tensor kv_read_q4(const Tensor& cache, const OptTensor& out) {
+  int64_t cs[2];
+  const int64_t group = check_q4(cache, "cache", {-1, -1, -1, -1}, nullptr, cs);
+  const at::Device dev = cache.device();
+  const int64_t B = cache.size(0), KH = cache.size(1), n = cache.size(2);
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor y = out_or_empty(out, "out", {B, 16 * n, KH, 128}, kBf16, dev);
+  done("kda_kv_read_q4", kda_kv_read_q4(cache.data_ptr(), y.data_ptr(), B, n, KH, 128, group, cs, stream(dev)));
+  return y;
+}
+
+Tensor gqa_decode_q4(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& lengths,
+                     const c10::optional<int64_t>& window, int64_t sinks, const OptTensor& out,
+                     const OptTensor& workspace) {
+  const Strides qs = check_rows(q, "q", kBf16, false, {-1, -1, 128});
+  const int64_t B = q.size(0), QH = q.size(1), D = 128;
+  const at::Device dev = q.device();
+  int64_t kc[2], vc[2];
+  const int64_t group = check_q4(k_cache, "k_cache", {B, -1, -1, -1}, &dev, kc);
+  check_q4(v_cache, "v_cache", k_cache.sizes(), &dev, vc);
+  const int64_t KH = k_cache.size(1), n = k_cache.size(2);
+  check_groups(QH, KH);
+  check_dense(lengths, "lengths", at::kInt, {B}, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor y = out_or_empty(out, "out", {B, QH, D}, kBf16, dev);
+  const size_t nb = kda_gqa_decode_q4_workspace_size(QH, KH);
+  Tensor ws = workspace_or_empty(workspace, nb, dev);
+  done("kda_gqa_decode_q4",
+       kda_gqa_decode_q4(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ptr<int>(lengths), y.data_ptr(), B, n,
+                         QH, KH, D, group, window ? *window : 16 * n, sinks, qs.s, kc, vc, ws.data_ptr(), nb,
+                         stream(dev)));
+  return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_binding, m) {
-  m.doc() = "Native calls of the local-attention operators (see kda.ops).";
+  m.doc() = "Native calls of the attention operators: local, packed, 4-bit cache (see kda.ops).";
   m.def("qk_norm_rope", &qk_norm_rope);
   m.def("qk_norm_rope_backward", &qk_norm_rope_backward);
   m.def("qk_norm_rope_append", &qk_norm_rope_append);
   m.def("gqa_window", &gqa_window);
   m.def("gqa_window_backward", &gqa_window_backward);
   m.def("gqa_window_decode", &gqa_window_decode);
+  m.def("packed_plan", &packed_plan);
+  m.def("gqa_packed", &gqa_packed);
+  m.def("gqa_packed_backward", &gqa_packed_backward);
+  m.def("kv_append_q4", &kv_append_q4);
+  m.def("kv_read_q4", &kv_read_q4);
+  m.def("gqa_decode_q4", &gqa_decode_q4);
 }

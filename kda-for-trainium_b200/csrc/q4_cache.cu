@@ -1,0 +1,250 @@
+// Writing and reading back the 4-bit key/value cache (layout: q4.cuh).
+//
+// Append, per (token, head) row of k and of v and per group of channels:
+//   low = min x,  step = bf16((max x - low) / 15),  code = round((x - low) / step)
+// low is one of the bf16 inputs, so it is exact.  The operations are single fp32 ones in
+// this order: x - low, times the fp32 reciprocal of step, rounded to nearest even, at most
+// 15; (max - low) times the fp32 1/15.  A step below 2^-126 becomes zero (every value reads
+// back as low).  A group with an infinity or a NaN, or wider than fp32 holds, reads back as NaN.
+//
+// Bandwidth-bound: 16 lanes take a row, 8 channels each (one 16-byte load, one 4-byte store
+// of codes), a group's minimum and maximum by exchanges of bf16 pairs.
+#include "launch.cuh"
+#include "q4.cuh"
+
+KDA_DEFINE_ERROR_WORD(q4_cache)
+
+namespace kda {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendParams {
+  const __nv_bfloat16 *k, *v;
+  uint8_t *k_cache, *v_cache;
+  const int* offsets;  // [B + 1] rows of each request, or null: `per` rows each
+  const int* lengths;  // [B] tokens cached already; below zero: an idle slot
+  int64_t rows;        // tokens in k and v
+  int64_t per;
+  int64_t k_b, k_t, k_h, v_b, v_t, v_h;  // element strides
+  int64_t kc_b, kc_h, vc_b, vc_h;        // byte strides
+  int64_t cache_len;
+  int B, KH;
+};
+
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// One row's 8 channels of this lane: codes (the word's nibbles) and the group's (step, low).
+template <int GROUP>
+__device__ __forceinline__ void quantise(const uint4 x, unsigned mask, uint32_t* word, uint32_t* pair) {
+  uint32_t lo = min2(min2(x.x, x.y), min2(x.z, x.w)), hi = max2(max2(x.x, x.y), max2(x.z, x.w));
+#pragma unroll
+  for (int d = 1; d < GROUP / 8; d <<= 1) {
+    lo = min2(lo, __shfl_xor_sync(mask, lo, d));
+    hi = max2(hi, __shfl_xor_sync(mask, hi, d));
+  }
+  lo = min2(lo, lo >> 16 | lo << 16);
+  hi = max2(hi, hi >> 16 | hi << 16);
+  const float low = __uint_as_float(lo << 16), high = __uint_as_float(hi << 16);
+  float step = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f)));
+  if (step < 1.1754943508222875e-38f) step = 0.f;
+  if (step > 3.3895313892515355e38f) step = __uint_as_float(0x7fc00000u);  // an infinity, or past bf16's largest
+  const float inv = step > 0.f ? __frcp_rn(step) : 0.f;  // NaN: zero codes beside a NaN pair
+  float f[8];
+  unpack_bf16x8(x, f);
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // adding 2^23 rounds to a whole number (ties to even), left in the low mantissa bits
+    const float t = fminf(__fmul_rn(__fsub_rn(f[i], low), inv), 15.f);
+    w |= (__float_as_uint(__fadd_rn(t, 8388608.f)) & 15u) << (4 * i);
+  }
+  *word = w;
+  *pair = (__float_as_uint(step) >> 16) | (lo << 16);
+}
+
+// Grid-stride over (token, head), 16 lanes each, k and v together.
+template <int GROUP>
+__global__ void __launch_bounds__(kThreads) q4_append_kernel(const AppendParams p, unsigned* err) {
+  pdl_trigger();
+  pdl_wait();
+  const int l = threadIdx.x & 15;
+  const unsigned mask = 0xffffu << (threadIdx.x & 16);
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
+  if (i >= p.rows * p.KH) return;  // 16 lanes alike
+  const int64_t row = i / p.KH;
+  const int h = static_cast<int>(i - row * p.KH);
+  // the row's request b and place in it
+  int b;
+  int64_t at;
+  if (p.offsets) {
+    // the last one whose first row is not after `row`, 16 at a time
+    int lo = 0, n = p.B;  // among [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + 15) >> 4;
+      const int j = lo + l * step;
+      const bool in = l == 0 || (l * step < n && __ldg(p.offsets + j) <= row);
+      const int last = 31 - __clz(static_cast<int>((__ballot_sync(mask, in) & mask) >> (threadIdx.x & 16)));
+      n = min(step, n - last * step);
+      lo += last * step;
+    }
+    b = lo;
+    const int first = __ldg(p.offsets + b);
+    if (row < first || row >= __ldg(p.offsets + b + 1)) return;  // of no request
+    at = row - first;
+  } else {
+    b = static_cast<int>(row / p.per);
+    at = row - b * p.per;
+  }
+  const int64_t cached = __ldg(p.lengths + b);
+  if (cached < 0) return;  // an idle slot
+  const int64_t pos = cached + at;
+  if (pos >= p.cache_len) {
+    if (l == 0) atomicOr(err, static_cast<unsigned>(kErrRange));
+    return;
+  }
+  const int64_t in_b = p.offsets ? 0 : b, in_t = p.offsets ? row : at;
+  const uint4 xk = *reinterpret_cast<const uint4*>(p.k + in_b * p.k_b + in_t * p.k_t + h * p.k_h + 8 * l);
+  const uint4 xv = *reinterpret_cast<const uint4*>(p.v + in_b * p.v_b + in_t * p.v_t + h * p.v_h + 8 * l);
+  const int t = static_cast<int>(pos % kQ4Tokens);
+  const int64_t block = pos / kQ4Tokens * q4_block_bytes(GROUP);
+  const uint32_t code_at = q4_word(t, l & 3, l >> 2);
+  const uint32_t pair_at = kQ4Codes + (t * (128 / GROUP) + l / (GROUP / 8)) * 4;
+  uint32_t word, pair;
+  uint8_t* dst = p.k_cache + b * p.kc_b + h * p.kc_h + block;
+  quantise<GROUP>(xk, mask, &word, &pair);
+  *reinterpret_cast<uint32_t*>(dst + code_at) = word;
+  if (l % (GROUP / 8) == 0) *reinterpret_cast<uint32_t*>(dst + pair_at) = pair;
+  dst = p.v_cache + b * p.vc_b + h * p.vc_h + block;
+  quantise<GROUP>(xv, mask, &word, &pair);
+  *reinterpret_cast<uint32_t*>(dst + code_at) = word;
+  if (l % (GROUP / 8) == 0) *reinterpret_cast<uint32_t*>(dst + pair_at) = pair;
+}
+
+// A warp reads a block; 16 lanes write a token's row of values, 16 bytes each.
+template <int GROUP>
+__global__ void __launch_bounds__(kThreads) q4_read_kernel(const uint8_t* __restrict__ cache, int64_t c_b,
+                                                           int64_t c_h, __nv_bfloat16* __restrict__ out,
+                                                           int64_t all, int64_t blocks, int KH) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (i >= all) return;
+  const int64_t bh = i / blocks, block = i - bh * blocks;
+  const int64_t b = bh / KH;
+  const int h = static_cast<int>(bh - b * KH);
+  const int l = threadIdx.x & 15, half = (threadIdx.x >> 4) & 1;
+  const uint8_t* src = cache + b * c_b + h * c_h + block * q4_block_bytes(GROUP);
+  uint32_t w[8], pair[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int t = 2 * k + half;
+    w[k] = __ldg(reinterpret_cast<const uint32_t*>(src + q4_word(t, l & 3, l >> 2)));
+    pair[k] = __ldg(reinterpret_cast<const uint32_t*>(src + kQ4Codes + (t * (128 / GROUP) + l / (GROUP / 8)) * 4));
+  }
+  __nv_bfloat16* dst = out + ((b * blocks + block) * kQ4Tokens * KH + h) * 128 + 8 * l;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float step = __uint_as_float(pair[k] << 16), low = __uint_as_float(pair[k] & 0xffff0000u);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      f[j] = fmaf(static_cast<float>((w[k] >> (4 * j)) & 15u), step, low);  // code * step is exact in fp32
+    *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(2 * k + half) * KH * 128) =
+        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+}
+
+}  // namespace
+}  // namespace kda
+
+using namespace kda;
+
+extern "C" size_t kda_q4_block_bytes(int64_t group) {
+  return group == 32 || group == 64 || group == 128 ? q4_block_bytes(static_cast<int>(group)) : 0;
+}
+
+extern "C" kda_status kda_kv_append_q4(const void* k, const void* v, const int* offsets, const int* lengths,
+                                       void* k_cache, void* v_cache, int64_t tokens, int64_t B, int64_t blocks,
+                                       int64_t KH, int64_t D, int64_t group, const int64_t* k_strides,
+                                       const int64_t* v_strides, const int64_t* k_cache_strides,
+                                       const int64_t* v_cache_strides, void* stream) {
+  const char* op = "kv_append_q4";
+  KDA_CHECK_ARG(tokens > 0 && B > 0 && blocks > 0 && KH > 0 && (offsets || tokens % B == 0),
+                "%s: bad sizes tokens=%lld B=%lld blocks=%lld KH=%lld", op, (long long)tokens, (long long)B,
+                (long long)blocks, (long long)KH);
+  KDA_CHECK_SUPPORTED(D == 128, "%s: head_dim must be 128, got %lld", op, (long long)D);
+  KDA_CHECK_ARG(group == 32 || group == 64 || group == 128, "%s: group must be 32, 64 or 128, got %lld", op,
+                (long long)group);
+  KDA_CHECK_SUPPORTED(B < (1ll << 24) && KH <= 65535 && blocks < (1ll << 26) && tokens < (1ll << 31) &&
+                          tokens * KH < (1ll << 34),
+                      "%s: too large (tokens=%lld B=%lld blocks=%lld KH=%lld)", op, (long long)tokens, (long long)B,
+                      (long long)blocks, (long long)KH);
+  KDA_CHECK_ARG(k && v && lengths && k_cache && v_cache && k_strides && v_strides && k_cache_strides &&
+                    v_cache_strides,
+                "%s: null pointer", op);
+  const int64_t n0 = offsets ? 1 : B, n1 = offsets ? tokens : tokens / B;
+  auto rows_ok = [&](const void* p, const int64_t* s) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (n0 == 1 || (s[0] > 0 && s[0] % 8 == 0)) &&
+           (n1 == 1 || (s[1] > 0 && s[1] % 8 == 0)) && (KH == 1 || (s[2] > 0 && s[2] % 8 == 0));
+  };
+  KDA_CHECK_SUPPORTED(rows_ok(k, k_strides) && rows_ok(v, v_strides) &&
+                          q4_cache_ok(k_cache, k_cache_strides, B, KH) && q4_cache_ok(v_cache, v_cache_strides, B, KH),
+                      "%s: pointers and rows must be 16-byte aligned", op);
+  AppendParams p{};
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.k_cache = static_cast<uint8_t*>(k_cache);
+  p.v_cache = static_cast<uint8_t*>(v_cache);
+  p.offsets = offsets;
+  p.lengths = lengths;
+  p.rows = tokens;
+  p.per = n1;
+  p.k_b = n0 > 1 ? k_strides[0] : 0, p.k_t = n1 > 1 ? k_strides[1] : 0, p.k_h = KH > 1 ? k_strides[2] : 0;
+  p.v_b = n0 > 1 ? v_strides[0] : 0, p.v_t = n1 > 1 ? v_strides[1] : 0, p.v_h = KH > 1 ? v_strides[2] : 0;
+  p.kc_b = B > 1 ? k_cache_strides[0] : 0, p.kc_h = KH > 1 ? k_cache_strides[1] : 0;
+  p.vc_b = B > 1 ? v_cache_strides[0] : 0, p.vc_h = KH > 1 ? v_cache_strides[1] : 0;
+  p.cache_len = blocks * kQ4Tokens;
+  p.B = static_cast<int>(B);
+  p.KH = static_cast<int>(KH);
+  const dim3 grid(static_cast<unsigned>((tokens * KH + kThreads / 16 - 1) / (kThreads / 16)));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned* err = kda_err_ptr_q4_cache();
+  if (group == 32) return launch_after(op, q4_append_kernel<32>, grid, kThreads, 0, st, p, err);
+  if (group == 64) return launch_after(op, q4_append_kernel<64>, grid, kThreads, 0, st, p, err);
+  return launch_after(op, q4_append_kernel<128>, grid, kThreads, 0, st, p, err);
+}
+
+extern "C" kda_status kda_kv_read_q4(const void* cache, void* out, int64_t B, int64_t blocks, int64_t KH, int64_t D,
+                                     int64_t group, const int64_t* cache_strides, void* stream) {
+  const char* op = "kv_read_q4";
+  KDA_CHECK_ARG(B > 0 && blocks > 0 && KH > 0, "%s: bad sizes B=%lld blocks=%lld KH=%lld", op, (long long)B,
+                (long long)blocks, (long long)KH);
+  KDA_CHECK_SUPPORTED(D == 128, "%s: head_dim must be 128, got %lld", op, (long long)D);
+  KDA_CHECK_ARG(group == 32 || group == 64 || group == 128, "%s: group must be 32, 64 or 128, got %lld", op,
+                (long long)group);
+  KDA_CHECK_SUPPORTED(B < (1ll << 24) && KH <= 65535 && blocks < (1ll << 26) && B * KH < (1ll << 33) / blocks,
+                      "%s: too large (B=%lld blocks=%lld KH=%lld)", op, (long long)B, (long long)blocks, (long long)KH);
+  KDA_CHECK_ARG(cache && out && cache_strides, "%s: null pointer", op);
+  KDA_CHECK_SUPPORTED(q4_cache_ok(cache, cache_strides, B, KH) && (reinterpret_cast<uintptr_t>(out) & 15u) == 0,
+                      "%s: pointers and blocks must be 16-byte aligned", op);
+  const int64_t all = B * KH * blocks;
+  const dim3 grid(static_cast<unsigned>((all + kThreads / 32 - 1) / (kThreads / 32)));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const uint8_t* c = static_cast<const uint8_t*>(cache);
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
+  const int64_t cb = B > 1 ? cache_strides[0] : 0, ch = KH > 1 ? cache_strides[1] : 0;
+  const int kh = static_cast<int>(KH);
+  if (group == 32) return launch_after(op, q4_read_kernel<32>, grid, kThreads, 0, st, c, cb, ch, o, all, blocks, kh);
+  if (group == 64) return launch_after(op, q4_read_kernel<64>, grid, kThreads, 0, st, c, cb, ch, o, all, blocks, kh);
+  return launch_after(op, q4_read_kernel<128>, grid, kThreads, 0, st, c, cb, ch, o, all, blocks, kh);
+}

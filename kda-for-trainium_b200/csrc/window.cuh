@@ -185,6 +185,49 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, ui
   tma_load_4d(dst + kHalf, m, bar, 64, head, row, b);
 }
 
+__device__ __forceinline__ void pack16(const float2 (&e)[16], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(e[i].x, e[i].y);
+}
+
+// A warp's 32 rows x 32 columns of bf16 results, a row per lane (w: its 64 bytes),
+// to rows of global memory: first the four lanes of a quad exchange 16-byte pieces
+// (lane i gets piece i of the quad's four rows), so that a quad's stores fill whole
+// sectors of a row.  dst: row 0, `stride` elements between rows; rows from `rows`
+// on are not written.
+__device__ __forceinline__ void store_rows(uint32_t (&w)[16], __nv_bfloat16* dst, int64_t stride, int rows) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d <= 2; d *= 2) {
+    const bool up = (lane & d) != 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((i / 4) & d) continue;  // pieces i / 4 and i / 4 + d
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[i] : w[i + 4 * d], d);
+      w[i] = up ? got : w[i];
+      w[i + 4 * d] = up ? w[i + 4 * d] : got;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = (lane & ~3) + r;
+    if (row < rows)
+      reinterpret_cast<uint4*>(dst + row * stride)[lane & 3] = make_uint4(w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]);
+  }
+}
+
+// Values of hidden pairs become exactly zero: pair i of e is live where bits
+// 2i and 2i + 1 of `live` are set.
+__device__ __forceinline__ void keep_live(uint32_t live, float2 (&e)[16]) {
+  if (live != 0xffffffffu) {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      e[q].x = (live >> (2 * q)) & 1u ? e[q].x : 0.f;
+      e[q].y = (live >> (2 * q + 1)) & 1u ? e[q].y : 0.f;
+    }
+  }
+}
+
 // The entry points' size checks; whether the strided rows of [n0][n1][n2] start on 16
 // bytes; the TMA map of [B][S][H][128] rows with element strides of batch, token and
 // head (128-row boxes of 64 columns; rows past S read as zeros).  In both an axis of one

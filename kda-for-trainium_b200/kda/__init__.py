@@ -14,7 +14,8 @@ provides the numpy-in / numpy-out shim ``kda.compat.<op>``.
 from ._lib import KdaError, lib as _load_lib
 from .ops import (  # noqa: F401
     adamw, adamw_multi, add_rmsnorm_matmul, bmm, bmm_softmax, device_error, gqa_full, gqa_full_backward,
-    gqa_full_lse, gqa_window, gqa_window_backward, gqa_window_decode, gqa_window_lse, lora,
+    gqa_decode_q4, gqa_full_lse, gqa_packed, gqa_packed_backward, gqa_packed_lse, gqa_window, gqa_window_backward,
+    gqa_window_decode, gqa_window_lse, kv_append_q4, kv_cache_q4, kv_read_q4, lora, packed_plan,
     mamba, matmul, matmul_add_rmsnorm, qk_norm_rope, qk_norm_rope_append, qk_norm_rope_backward, rmsnorm_matmul,
     rmsnorm_matmul_backward, rope_single_freq_apply, rope_table, silu, swiglu, swiglu_backward, swiglu_gu,
     transpose_matmul,
@@ -31,4 +32,5 @@ from . import compat, library  # noqa: E402,F401  (torch.ops.kda.<op> and the nu
 __all__ = list(OPS) + ["adamw_multi", "rmsnorm_matmul_backward", "swiglu_backward", "gqa_full_backward",
                        "gqa_full_lse", "swiglu_gu", "rope_table", "qk_norm_rope", "qk_norm_rope_backward",
                        "qk_norm_rope_append", "gqa_window", "gqa_window_lse", "gqa_window_backward",
-                       "gqa_window_decode", "KdaError", "device_error"]
+                       "gqa_window_decode", "packed_plan", "gqa_packed", "gqa_packed_lse", "gqa_packed_backward",
+                       "kv_cache_q4", "kv_append_q4", "kv_read_q4", "gqa_decode_q4", "KdaError", "device_error"]

@@ -106,6 +106,17 @@ PROTOTYPES = {
     "kda_gqa_window_backward_bf16": (INT, [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P,
                                            SZ, P]),
     "kda_gqa_window_decode_bf16": (INT, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P, P, P]),
+    "kda_packed_plan_size": (SZ, [I64, I64]),
+    "kda_packed_plan": (INT, [P, I64, I64, P, SZ, P]),
+    "kda_gqa_packed_bf16": (INT, [P, P, P, P, SZ, P, P, INT, I64, I64, I64, I64, P, P, P, P]),
+    "kda_gqa_packed_backward_workspace_size": (SZ, [I64, SZ, I64, I64, I64]),
+    "kda_gqa_packed_backward_bf16": (INT, [P, P, P, P, P, P, P, SZ, P, P, P, INT, I64, I64, I64, I64, P, P, P, P, SZ,
+                                           P]),
+    "kda_q4_block_bytes": (SZ, [I64]),
+    "kda_kv_append_q4": (INT, [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, P, P, P, P, P]),
+    "kda_kv_read_q4": (INT, [P, P, I64, I64, I64, I64, I64, P, P]),
+    "kda_gqa_decode_q4_workspace_size": (SZ, [I64, I64]),
+    "kda_gqa_decode_q4": (INT, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, P, P, P, P, SZ, P]),
 }
 
 
@@ -136,7 +147,7 @@ def lib():
 
 
 class _Binding:
-    """The native binding of the local-attention operators, loaded at the first
+    """The native binding of the local-attention, packed and 4-bit-cache operators, loaded at the first
     call of one of them: the other operators need only libkda.so.  It resolves
     the C ABI in the library that ``lib()`` has loaded (matched by its soname)."""
 

@@ -7,6 +7,7 @@ differentiable op for training code.
     o = kda.autograd.gqa_full(q, k, v, causal=True, rope_theta=1e4)  # bf16; dq, dk, dv from the kernels
     q, k = kda.autograd.qk_norm_rope(q, k, gq, gk, table)            # dq, dk, dgq, dgk from the kernels
     o = kda.autograd.gqa_window(q, k, v, 1024, sinks=4)              # bf16; dq, dk, dv from the kernels
+    o = kda.autograd.gqa_packed(q, k, v, plan)                       # bf16; dq, dk, dv from the kernels
 """
 
 from __future__ import annotations
@@ -142,3 +143,24 @@ def gqa_window(q, k, v, window, sinks=0):
     log2-sum-exp, the gradients come from ``kda.gqa_window_backward``; second
     derivatives raise."""
     return _GQAWindow.apply(q, k, v, window, sinks)
+
+
+class _GQAPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, plan):
+        out, lse = ops.gqa_packed_lse(q, k, v, plan)
+        ctx.save_for_backward(q, k, v, out, lse, plan)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, plan = ctx.saved_tensors
+        grads = ops.gqa_packed_backward(dout.to(torch.bfloat16).contiguous(), q, k, v, out, lse, plan)
+        return (*_first_only(grads, dout, q, k, v), None)
+
+
+def gqa_packed(q, k, v, plan):
+    """Differentiable ``kda.gqa_packed`` (bf16): the forward keeps its row
+    log2-sum-exp, the gradients come from ``kda.gqa_packed_backward``; second
+    derivatives raise."""
+    return _GQAPacked.apply(q, k, v, plan)

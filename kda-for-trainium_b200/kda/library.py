@@ -227,6 +227,62 @@ def _(q, k_cache, v_cache, lengths, window, sinks=0):
     return q.new_empty(q.shape)
 
 
+# --------------------------------------------- packed sequences, 4-bit caches
+@torch.library.custom_op("kda::packed_plan", mutates_args=())
+def packed_plan(offsets: torch.Tensor, tokens: int) -> torch.Tensor:
+    return ops.packed_plan(offsets, tokens)
+
+
+@packed_plan.register_fake
+def _(offsets, tokens):
+    n = offsets.shape[0] - 1
+    # its size in int32, as kda_packed_plan_size gives it in bytes
+    return offsets.new_empty((8 + 14 * (tokens // 128 + n) + 2 * n + n + n % 2,))
+
+
+@torch.library.custom_op("kda::gqa_packed", mutates_args=())
+def gqa_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: torch.Tensor) -> torch.Tensor:
+    return ops.gqa_packed(q, k, v, plan)
+
+
+@gqa_packed.register_fake
+def _(q, k, v, plan):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("kda::kv_append_q4", mutates_args=("k_cache", "v_cache"))
+def kv_append_q4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 lengths: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> None:
+    ops.kv_append_q4(k, v, k_cache, v_cache, lengths, offsets)
+
+
+@kv_append_q4.register_fake
+def _(k, v, k_cache, v_cache, lengths, offsets=None):
+    return None
+
+
+@torch.library.custom_op("kda::kv_read_q4", mutates_args=())
+def kv_read_q4(cache: torch.Tensor) -> torch.Tensor:
+    return ops.kv_read_q4(cache)
+
+
+@kv_read_q4.register_fake
+def _(cache):
+    B, KH, blocks, _ = cache.shape
+    return cache.new_empty((B, 16 * blocks, KH, 128), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("kda::gqa_decode_q4", mutates_args=())
+def gqa_decode_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                  window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
+    return ops.gqa_decode_q4(q, k_cache, v_cache, lengths, window, sinks)
+
+
+@gqa_decode_q4.register_fake
+def _(q, k_cache, v_cache, lengths, window=None, sinks=0):
+    return q.new_empty(q.shape)
+
+
 OPS = ("silu", "rmsnorm_matmul", "add_rmsnorm_matmul", "matmul_add_rmsnorm", "swiglu", "matmul",
        "transpose_matmul", "bmm", "bmm_softmax", "gqa_full", "rope_single_freq_apply", "lora", "adamw",
        "mamba")

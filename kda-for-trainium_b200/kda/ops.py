@@ -696,6 +696,84 @@ def gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks=0, *, out=None
     return _native.gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks, out)
 
 
+# ------------------------------------------- packed sequences, 4-bit caches
+def packed_plan(offsets, tokens, *, out=None):
+    """The tables that ``gqa_packed`` and its backward work by, for sequences s =
+    rows offsets[s] .. offsets[s + 1] - 1 of a buffer of ``tokens`` rows (offsets
+    int32 (N + 1,), not falling, within 0 .. tokens; sequences may be empty, rows
+    before the first and behind the last belong to none).  Built on the device,
+    once for all the calls on buffers of these offsets: every layer's forward and
+    backward.  Returns an int32 tensor.  Offsets that fall or leave the buffer
+    give a plan of no sequences and set ``device_error``."""
+    return _native.packed_plan(offsets, tokens, out)
+
+
+def gqa_packed(q, k, v, plan, *, out=None):
+    """Causal grouped-query attention of sequences packed one behind another: query
+    i sees key j <= i of its own sequence.  q (T,QH,128), k, v (T,KH,128) bf16, views
+    are fine; ``plan`` is ``packed_plan(offsets, T)``'s; returns (T,QH,128).  Rows of
+    no sequence are zeros (in a given ``out``: left as they were), and what they or
+    another sequence hold, NaN included, changes nothing.  No rotation (see
+    ``qk_norm_rope``'s ``positions``).  Scores scaled by 1 / sqrt(128).  A plan for
+    another T does nothing and sets ``device_error``."""
+    return _native.gqa_packed(q, k, v, plan, out, False)[0]
+
+
+def gqa_packed_lse(q, k, v, plan):
+    """``gqa_packed`` that also returns each query row's log2-sum-exp of the scaled
+    scores, (QH, T) fp32: the forward of a training step."""
+    return _native.gqa_packed(q, k, v, plan, None, True)
+
+
+def gqa_packed_backward(dout, q, k, v, out, lse, plan, *, workspace=None):
+    """Gradients of ``gqa_packed(q, k, v, plan)`` given dout (T,QH,128) bf16 and
+    ``gqa_packed_lse``'s two outputs: returns (dq, dk, dv) bf16, shaped like q, k, v,
+    contiguous; rows of no sequence are zeros."""
+    return _native.gqa_packed_backward(dout, q, k, v, out, lse, plan, workspace)
+
+
+def kv_cache_q4(batch, length, kv_heads, group=64, *, device="cuda"):
+    """An empty 4-bit cache of keys or of values for ``batch`` requests of up to
+    ``length`` tokens (in blocks of 16) and head_dim 128: uint8 (B, KH, blocks,
+    bytes of a block), values code * step + low with a bf16 pair (step, low) for
+    each ``group`` (32, 64 or 128) channels of a token: 5, 4.5 or 4.25 bits a
+    value.  ``include/kda.h`` gives the layout."""
+    batch, length, kv_heads = int(batch), int(length), int(kv_heads)
+    if batch < 1 or length < 1 or kv_heads < 1:
+        raise ValueError(f"batch, length and kv_heads must be positive, got {batch}, {length} and {kv_heads}")
+    if group not in (32, 64, 128):
+        raise ValueError(f"group must be 32, 64 or 128, got {group}")
+    return torch.zeros((batch, kv_heads, (length + 15) // 16, 1024 + 8192 // group), dtype=torch.uint8, device=device)
+
+
+def kv_append_q4(k, v, k_cache, v_cache, lengths, offsets=None):
+    """Holds new rows of k and v (bf16, views are fine) in 4 bits in k_cache, v_cache
+    (``kv_cache_q4``), row i of request b at position lengths[b] + i (int32 (B,),
+    tokens already cached).  k, v (B,S,KH,128): S rows of each request; with
+    ``offsets`` (int32 (B + 1,)) (T,KH,128): rows offsets[b] .. offsets[b + 1] - 1
+    are request b's, rows of none are skipped.  Per group low is the minimum, step
+    bf16((max - low) / 15), code round((x - low) / step): a value is at most about
+    half a step off.  A group with an infinity or a NaN reads back as NaN.  A
+    negative length marks an idle slot: nothing is written.  A position past the
+    cache is not written and sets ``device_error``.  ``lengths`` is left as it is."""
+    _native.kv_append_q4(k, v, k_cache, v_cache, lengths, offsets)
+
+
+def kv_read_q4(cache, *, out=None):
+    """The values that a 4-bit cache stands for, rounded to bf16: (B, 16 blocks, KH,
+    128), positions that were never written among them."""
+    return _native.kv_read_q4(cache, out)
+
+
+def gqa_decode_q4(q, k_cache, v_cache, lengths, window=None, sinks=0, *, out=None, workspace=None):
+    """``gqa_window_decode`` against 4-bit caches (``kv_cache_q4``): q (B,QH,128) bf16,
+    lengths[b] valid tokens of request b (int32, the newest among them), of which the
+    last ``window`` are seen (None: all) and the first ``sinks``.  A request without
+    tokens (length 0 or less) gives zeros; a length past the cache is cut to it and
+    sets ``device_error``.  Returns (B,QH,128)."""
+    return _native.gqa_decode_q4(q, k_cache, v_cache, lengths, window, sinks, out, workspace)
+
+
 def device_error(clear: bool = True) -> int:
     """Device error word of the current device (0 = no kernel wait expired, no
     position or length outside its table or cache)."""

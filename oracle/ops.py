@@ -14,6 +14,8 @@ from __future__ import annotations
 
 import numpy as np
 
+from .bf16 import to_bf16_rne
+
 f32 = np.float32
 
 
@@ -483,4 +485,74 @@ def gqa_window_decode(q, k_cache, v_cache, lengths, window, sinks=0):
             s = k[b, j, h // rep] @ q[b, h] / np.sqrt(D)
             p = np.exp(s - s.max())
             out[b, h] = (p / p.sum()) @ v[b, j, h // rep]
+    return out
+
+
+def _sequences(offsets):
+    return [(int(a), int(b)) for a, b in zip(offsets[:-1], offsets[1:])]
+
+
+def gqa_packed(q, k, v, offsets):
+    """(out (T,QH,D), lse (QH,T) in log2) of causal attention within each sequence
+    [offsets[s], offsets[s + 1]); zeros in the rows of none."""
+    out, lse = np.zeros(np.shape(q)), np.zeros((np.shape(q)[1], np.shape(q)[0]))
+    for a, b in _sequences(offsets):
+        if b > a:
+            o, z = gqa_window(q[None, a:b], k[None, a:b], v[None, a:b], b - a)
+            out[a:b], lse[:, a:b] = o[0], z[0]
+    return out, lse
+
+
+def gqa_packed_backward(dout, q, k, v, offsets):
+    """(dq, dk, dv) of ``gqa_packed``."""
+    grads = np.zeros(np.shape(q)), np.zeros(np.shape(k)), np.zeros(np.shape(v))
+    for a, b in _sequences(offsets):
+        if b > a:
+            got = gqa_window_backward(dout[None, a:b], q[None, a:b], k[None, a:b], v[None, a:b], b - a)
+            for g, w in zip(grads, got):
+                g[a:b] = w[0]
+    return grads
+
+
+def q4_quantise(x, group):
+    """Codes, steps and lows of rows (..., 128) of bf16 values: per group of channels low =
+    min, step = bf16((max - low) / 15), code = round((x - low) / step), each a single
+    fp32 operation (the quotients by fp32 reciprocals).  A step below 2^-126 is zero; NaN where the group is not finite."""
+    f32 = np.float32
+    x = np.asarray(x, f32)
+    rows = x.reshape(*x.shape[:-1], -1, group)
+    with np.errstate(all="ignore"):
+        low, high = rows.min(-1), rows.max(-1)
+        step = to_bf16_rne((high - low) * f32(1.0 / 15.0))
+        step = np.where(step < f32(2.0 ** -126), f32(0), step).astype(f32)
+        step = np.where(np.isinf(step), f32(np.nan), step)
+        inv = np.where(step > 0, f32(1) / step, f32(0)).astype(f32)
+        codes = np.minimum(np.rint((rows - low[..., None]) * inv[..., None]), f32(15))
+    bad = ~np.isfinite(step)
+    codes = np.where(bad[..., None], 0, codes).astype(np.int64)
+    return codes.reshape(x.shape), step, low
+
+
+def q4_values(codes, step, low):
+    """code * step + low in 64 bits."""
+    c = codes.reshape(*step.shape, -1).astype(np.float64)
+    with np.errstate(all="ignore"):
+        return (c * step[..., None].astype(np.float64) + low[..., None].astype(np.float64)).reshape(codes.shape)
+
+
+def q4_pack(codes, step, low):
+    """The bytes of a 4-bit cache (B,KH,blocks,bytes) of rows (B,KH,T,128), T a multiple of 16."""
+    B, KH, T, _ = codes.shape
+    out = np.zeros((B, KH, T // 16, 1024 + 64 * step.shape[-1]), np.uint8)
+    side = np.stack([step, low], -1).astype(np.float32).view(np.uint32) >> 16
+    for t in range(T):
+        rows = out[:, :, t // 16]
+        u = t % 16
+        for ch in range(128):
+            g, c, i = ch // 32, ch % 32 // 8, ch % 8
+            at = 64 * u + 16 * (c ^ ((u >> 1) & 3)) + 4 * g + i // 2
+            rows[..., at] |= (codes[:, :, t, ch] << (4 * (i % 2))).astype(np.uint8)
+        pairs = side[:, :, t].reshape(B, KH, -1).astype("<u2")
+        n = pairs.shape[-1] * 2
+        rows[..., 1024 + u * n:1024 + (u + 1) * n] = np.ascontiguousarray(pairs).view(np.uint8)
     return out
