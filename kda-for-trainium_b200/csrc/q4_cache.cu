@@ -24,8 +24,9 @@ struct AppendParams {
   uint8_t *k_cache, *v_cache;
   const int* offsets;  // [B + 1] rows of each request, or null: `per` rows each
   const int* lengths;  // [B] tokens cached already; below zero: an idle slot
-  int64_t rows;        // tokens in k and v
-  int64_t per;
+  unsigned rows;       // tokens in k and v
+  unsigned per;
+  unsigned kh_mul, kh_shift;  // i / KH = (i kh_mul) >> (31 + kh_shift) for i < 2^31
   int64_t k_b, k_t, k_h, v_b, v_t, v_h;  // element strides
   int64_t kc_b, kc_h, vc_b, vc_h;        // byte strides
   int64_t cache_len;
@@ -59,75 +60,103 @@ __device__ __forceinline__ void quantise(const uint4 x, unsigned mask, uint32_t*
   if (step < 1.1754943508222875e-38f) step = 0.f;
   if (step > 3.3895313892515355e38f) step = __uint_as_float(0x7fc00000u);  // an infinity, or past bf16's largest
   const float inv = step > 0.f ? __frcp_rn(step) : 0.f;  // NaN: zero codes beside a NaN pair
+  // Adding 2^23 rounds to a whole number (ties to even), left in the low mantissa bits; the
+  // shifted sum of the eight bit patterns is the word, and eight times 2^23's pattern shifted.
+  // No code is past 15: step is off by 2^-9 of itself at most, and (max - low) / step then
+  // below 15.03.
   float f[8];
   unpack_bf16x8(x, f);
-  uint32_t w = 0;
+  uint32_t w = 0u - 0x4b000000u * 0x11111111u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // adding 2^23 rounds to a whole number (ties to even), left in the low mantissa bits
-    const float t = fminf(__fmul_rn(__fsub_rn(f[i], low), inv), 15.f);
-    w |= (__float_as_uint(__fadd_rn(t, 8388608.f)) & 15u) << (4 * i);
+  for (int i = 0; i < 4; ++i) {
+    float2 t = __fadd2_rn(make_float2(f[2 * i], f[2 * i + 1]), make_float2(-low, -low));
+    // __fmul_rn, not __fmul2_rn, which the compiler may fuse with the addition: a product that
+    // rounds to a tie would then be rounded as what it was before
+    t = __fadd2_rn(make_float2(__fmul_rn(t.x, inv), __fmul_rn(t.y, inv)), make_float2(8388608.f, 8388608.f));
+    w += __float_as_uint(t.x) * (1u << (8 * i)) + __float_as_uint(t.y) * (16u << (8 * i));
   }
   *word = w;
   *pair = (__float_as_uint(step) >> 16) | (lo << 16);
 }
 
-// Grid-stride over (token, head), 16 lanes each, k and v together.
+// The request that row `row` belongs to: the last one whose first row is not after it, 16 at
+// a time by the 16 lanes of `mask` (l: which of them).
+__device__ __forceinline__ int request_of(const int* offsets, int B, int row, int l, unsigned mask) {
+  int lo = 0, n = B;  // among [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 15) >> 4;
+    const bool in = l == 0 || (l * step < n && __ldg(offsets + lo + l * step) <= row);
+    const int last = 31 - __clz(static_cast<int>((__ballot_sync(mask, in) & mask) >> (threadIdx.x & 16)));
+    n = min(step, n - last * step);
+    lo += last * step;
+  }
+  return lo;
+}
+
+// A CTA takes 16 (token, head) pairs, 16 lanes each, k and v together: the loads are issued
+// first, and while they are under way the tokens' requests are looked up, once for each token
+// (each pair for itself, before its loads: 41 us for 19,000 tokens of 8 heads against 27; two or
+// four pairs for 16 lanes: 25 and 26, but 2.9 and 4.0 against 2.5 for a decode step's 64 tokens).
+constexpr int kItems = kThreads / 16;
 template <int GROUP>
 __global__ void __launch_bounds__(kThreads) q4_append_kernel(const AppendParams p, unsigned* err) {
+  __shared__ int request[kItems], place[kItems];    // of the CTA's tokens; place -1: not written
   pdl_trigger();
   pdl_wait();
-  const int l = threadIdx.x & 15;
+  const int l = threadIdx.x & 15, hw = threadIdx.x >> 4;
   const unsigned mask = 0xffffu << (threadIdx.x & 16);
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
-  if (i >= p.rows * p.KH) return;  // 16 lanes alike
-  const int64_t row = i / p.KH;
+  const unsigned all = p.rows * p.KH, i0 = blockIdx.x * kItems;  // < 2^31
+  auto token = [&](unsigned i) {
+    return static_cast<unsigned>((static_cast<uint64_t>(i) * p.kh_mul) >> (31 + p.kh_shift));
+  };
+  const unsigned row0 = token(i0);
+  const unsigned i = min(i0 + hw, all - 1), row = token(i);
   const int h = static_cast<int>(i - row * p.KH);
-  // the row's request b and place in it
-  int b;
-  int64_t at;
-  if (p.offsets) {
-    // the last one whose first row is not after `row`, 16 at a time
-    int lo = 0, n = p.B;  // among [lo, lo + n)
-    while (n > 1) {
-      const int step = (n + 15) >> 4;
-      const int j = lo + l * step;
-      const bool in = l == 0 || (l * step < n && __ldg(p.offsets + j) <= row);
-      const int last = 31 - __clz(static_cast<int>((__ballot_sync(mask, in) & mask) >> (threadIdx.x & 16)));
-      n = min(step, n - last * step);
-      lo += last * step;
+  const unsigned of = p.offsets ? 0u : row / p.per, in = p.offsets ? row : row - of * p.per;
+  const uint4 xk = *reinterpret_cast<const uint4*>(p.k + of * p.k_b + in * p.k_t + h * p.k_h + 8 * l);
+  const uint4 xv = *reinterpret_cast<const uint4*>(p.v + of * p.v_b + in * p.v_t + h * p.v_h + 8 * l);
+  const int tokens = static_cast<int>(token(min(i0 + kItems, all) - 1) - row0) + 1;
+  if (hw < tokens) {
+    const int row = static_cast<int>(row0) + hw;
+    int b, at;
+    bool any = true;
+    if (p.offsets) {
+      b = request_of(p.offsets, p.B, row, l, mask);
+      const int first = __ldg(p.offsets + b);
+      any = row >= first && row < __ldg(p.offsets + b + 1);  // of some request
+      at = any ? row - first : 0;
+    } else {
+      b = static_cast<int>(static_cast<unsigned>(row) / p.per);
+      at = row - b * static_cast<int>(p.per);
     }
-    b = lo;
-    const int first = __ldg(p.offsets + b);
-    if (row < first || row >= __ldg(p.offsets + b + 1)) return;  // of no request
-    at = row - first;
-  } else {
-    b = static_cast<int>(row / p.per);
-    at = row - b * p.per;
+    const int cached = __ldg(p.lengths + b);
+    any = any && cached >= 0;  // not an idle slot
+    const int64_t pos = static_cast<int64_t>(cached) + at;
+    if (l == 0) {
+      if (any && pos >= p.cache_len) atomicOr(err, static_cast<unsigned>(kErrRange));
+      request[hw] = b;
+      place[hw] = any && pos < p.cache_len ? static_cast<int>(pos) : -1;
+    }
   }
-  const int64_t cached = __ldg(p.lengths + b);
-  if (cached < 0) return;  // an idle slot
-  const int64_t pos = cached + at;
-  if (pos >= p.cache_len) {
-    if (l == 0) atomicOr(err, static_cast<unsigned>(kErrRange));
-    return;
-  }
-  const int64_t in_b = p.offsets ? 0 : b, in_t = p.offsets ? row : at;
-  const uint4 xk = *reinterpret_cast<const uint4*>(p.k + in_b * p.k_b + in_t * p.k_t + h * p.k_h + 8 * l);
-  const uint4 xv = *reinterpret_cast<const uint4*>(p.v + in_b * p.v_b + in_t * p.v_t + h * p.v_h + 8 * l);
-  const int t = static_cast<int>(pos % kQ4Tokens);
-  const int64_t block = pos / kQ4Tokens * q4_block_bytes(GROUP);
+  __syncthreads();
+  uint32_t kw, kp, vw, vp;
+  quantise<GROUP>(xk, mask, &kw, &kp);
+  quantise<GROUP>(xv, mask, &vw, &vp);
+  const int pos = place[row - row0];
+  if (pos < 0 || i0 + hw >= all) return;
+  const int64_t b = request[row - row0];
+  const int t = pos & (kQ4Tokens - 1);
+  const int64_t block = static_cast<int64_t>(pos >> 4) * q4_block_bytes(GROUP);
   const uint32_t code_at = q4_word(t, l & 3, l >> 2);
   const uint32_t pair_at = kQ4Codes + (t * (128 / GROUP) + l / (GROUP / 8)) * 4;
-  uint32_t word, pair;
-  uint8_t* dst = p.k_cache + b * p.kc_b + h * p.kc_h + block;
-  quantise<GROUP>(xk, mask, &word, &pair);
-  *reinterpret_cast<uint32_t*>(dst + code_at) = word;
-  if (l % (GROUP / 8) == 0) *reinterpret_cast<uint32_t*>(dst + pair_at) = pair;
-  dst = p.v_cache + b * p.vc_b + h * p.vc_h + block;
-  quantise<GROUP>(xv, mask, &word, &pair);
-  *reinterpret_cast<uint32_t*>(dst + code_at) = word;
-  if (l % (GROUP / 8) == 0) *reinterpret_cast<uint32_t*>(dst + pair_at) = pair;
+  uint8_t* kd = p.k_cache + b * p.kc_b + h * p.kc_h + block;
+  uint8_t* vd = p.v_cache + b * p.vc_b + h * p.vc_h + block;
+  *reinterpret_cast<uint32_t*>(kd + code_at) = kw;
+  *reinterpret_cast<uint32_t*>(vd + code_at) = vw;
+  if (l % (GROUP / 8) == 0) {
+    *reinterpret_cast<uint32_t*>(kd + pair_at) = kp;
+    *reinterpret_cast<uint32_t*>(vd + pair_at) = vp;
+  }
 }
 
 // A warp reads a block; 16 lanes write a token's row of values, 16 bytes each.
@@ -164,6 +193,13 @@ __global__ void __launch_bounds__(kThreads) q4_read_kernel(const uint8_t* __rest
   }
 }
 
+template <int GROUP>
+kda_status launch_append(const AppendParams& p, cudaStream_t st) {
+  const unsigned all = p.rows * p.KH;
+  return launch_after("kv_append_q4", q4_append_kernel<GROUP>, dim3((all + kItems - 1) / kItems), kThreads, 0, st, p,
+                      kda_err_ptr_q4_cache());
+}
+
 }  // namespace
 }  // namespace kda
 
@@ -186,7 +222,7 @@ extern "C" kda_status kda_kv_append_q4(const void* k, const void* v, const int* 
   KDA_CHECK_ARG(group == 32 || group == 64 || group == 128, "%s: group must be 32, 64 or 128, got %lld", op,
                 (long long)group);
   KDA_CHECK_SUPPORTED(B < (1ll << 24) && KH <= 65535 && blocks < (1ll << 26) && tokens < (1ll << 31) &&
-                          tokens * KH < (1ll << 34),
+                          tokens * KH < (1ll << 31),
                       "%s: too large (tokens=%lld B=%lld blocks=%lld KH=%lld)", op, (long long)tokens, (long long)B,
                       (long long)blocks, (long long)KH);
   KDA_CHECK_ARG(k && v && lengths && k_cache && v_cache && k_strides && v_strides && k_cache_strides &&
@@ -207,8 +243,11 @@ extern "C" kda_status kda_kv_append_q4(const void* k, const void* v, const int* 
   p.v_cache = static_cast<uint8_t*>(v_cache);
   p.offsets = offsets;
   p.lengths = lengths;
-  p.rows = tokens;
-  p.per = n1;
+  p.rows = static_cast<unsigned>(tokens);
+  p.per = static_cast<unsigned>(n1);
+  while ((1ll << p.kh_shift) < KH) ++p.kh_shift;
+  // 2^(31 + s) / KH rounded up, of 32 bits: more by less than KH / 2^(31 + s) <= 2^-31 of itself
+  p.kh_mul = static_cast<unsigned>(((1ull << (31 + p.kh_shift)) + KH - 1) / KH);
   p.k_b = n0 > 1 ? k_strides[0] : 0, p.k_t = n1 > 1 ? k_strides[1] : 0, p.k_h = KH > 1 ? k_strides[2] : 0;
   p.v_b = n0 > 1 ? v_strides[0] : 0, p.v_t = n1 > 1 ? v_strides[1] : 0, p.v_h = KH > 1 ? v_strides[2] : 0;
   p.kc_b = B > 1 ? k_cache_strides[0] : 0, p.kc_h = KH > 1 ? k_cache_strides[1] : 0;
@@ -216,12 +255,8 @@ extern "C" kda_status kda_kv_append_q4(const void* k, const void* v, const int* 
   p.cache_len = blocks * kQ4Tokens;
   p.B = static_cast<int>(B);
   p.KH = static_cast<int>(KH);
-  const dim3 grid(static_cast<unsigned>((tokens * KH + kThreads / 16 - 1) / (kThreads / 16)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  unsigned* err = kda_err_ptr_q4_cache();
-  if (group == 32) return launch_after(op, q4_append_kernel<32>, grid, kThreads, 0, st, p, err);
-  if (group == 64) return launch_after(op, q4_append_kernel<64>, grid, kThreads, 0, st, p, err);
-  return launch_after(op, q4_append_kernel<128>, grid, kThreads, 0, st, p, err);
+  return group == 32 ? launch_append<32>(p, st) : group == 64 ? launch_append<64>(p, st) : launch_append<128>(p, st);
 }
 
 extern "C" kda_status kda_kv_read_q4(const void* cache, void* out, int64_t B, int64_t blocks, int64_t KH, int64_t D,

@@ -7,17 +7,21 @@
 //
 // HBM-bound: every block of 16 tokens with a visible one is read once (1,152 bytes for K and
 // as many for V at groups of 64) for up to 16 query heads of its group.  At 4 bits the codes
-// are also the most arithmetic: some 14 warp instructions for each token of a head, of 25
-// that an SM has while it reads one.  So codes become operands without arithmetic on values:
-// (word & 0x00780078) | 0x41804180 is a pair of bf16 16 + code, exactly, and steps, lows and
-// the 16 are applied to sums.  With x = step c + low, over a group G of channels
-//   sum_G q x       = step sum_G q (16 + c) + (low - 16 step) sum_G q
-//   sum_t p_t x_td  = sum_t (p_t step_t)(16 + c_td) - 16 sum_t (p_t step_t) + sum_t p_t low_t
-// where p_t step_t, rounded to bf16 as the operand that meets V's codes, is summed by the
-// tensor core as well (a row of ones), so that the 16s cancel to the last bits of fp32.  (The
-// nibble at the top of the mantissa, not its end, where the number would be 128 + code: the
-// tensor core's sums are cut off, not rounded, and an output that averages 130,000 tokens
-// was 0.0045 off in relative L2, with 16 0.0020.)
+// are also the most arithmetic, so they become operands with little of it, and steps and lows
+// are applied to sums.  With x = step c + low, over a group G of channels
+//   sum_G q x       = step sum_G q c + low sum_G q
+//   sum_t p_t x_td  = sum_t (p_t step_t) c_td + sum_t p_t low_t
+// The bits of a number below 2^-13 are linear in fp16: a byte in each half of a word is
+// (c + 16 c') 2^-24 of two neighbouring codes as it stands, its low nibble c 2^-24.  So these
+// two are operands, q' / 16 and q - q' / 16 what meets them in K, and in V the difference of
+// the two sums is 16 times the second channel's: 4.5 integer operations for 8 codes.
+// (As bf16 16 + code, the 16s subtracted from the sums: 241 us for 64 requests; as fp16
+// code - 8 by one more multiply-add a pair: 194; a nibble each, a block at a time: 151;
+// two blocks at a time: 143.)
+// The other operands are fp16 then, with ranges of their own: q times a power of two per head
+// that brings its largest value to 1 .. 2, and p step times one per head that keeps it below
+// 2^15 and was last chosen where the largest so far became 1 .. 2 (in the manner of the running
+// maximum: what is too small for fp16 beside it is too small to matter).
 //
 // The products are transposed so that the few query heads are the narrow side of the
 // m16n8k16 matrix instruction:
@@ -31,6 +35,7 @@
 // ends of walks.  Where a walk ends, or the run does, the warps join through shared memory:
 // a whole walk's output leaves, a cut one's share goes to the workspace, and a second launch
 // joins the shares in the order of the walk: one fixed order of summation.
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include "launch.cuh"
@@ -46,7 +51,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRow = kD + 4;       // floats of a head's share: the output row, maximum, sum
-constexpr int kLeast = 2 * kWarps;  // blocks of a CTA's run, where there are as many
+constexpr int kLeast = kWarps;      // chunks of a CTA's run, where there are as many
 constexpr unsigned kFull = 0xffffffffu;
 
 struct DecodeParams {
@@ -56,41 +61,41 @@ struct DecodeParams {
   const int* lengths;
   int64_t q_b, q_h;          // element strides
   int64_t k_b, k_h, v_b, v_h;  // byte strides
-  int64_t cache_len;
-  int64_t window, sinks;
+  int cache_len, window, sinks;
   int B, QH, KH, rep, parts;  // parts: groups of 8 NT query heads per kv head
   float scale_log2;
   float* shares;             // [2 x CTAs][8 NT][kRow]
-  int4* pieces;              // [2 x CTAs]: walk, 0, blocks of the share, of the walk
+  int4* pieces;              // [2 x CTAs]: walk, 0, chunks of the share, of the walk
   unsigned* length_err;
 };
 
-// The blocks of a request's walk: [0, ns) (sinks), then [ns + skip, n + skip).
+// A request's visible tokens as chunks of two blocks: `ns` over blocks [0, sb) (sinks), then
+// those over [first, end).
 struct Walk {
-  int n, ns, skip;
-  int64_t len, start;
+  int n, ns, sb, first, end;
+  int len, start;
 };
 __device__ __forceinline__ Walk walk_of(const DecodeParams& p, int b) {
   Walk w;
-  int64_t n = __ldg(p.lengths + b);
-  if (n > p.cache_len) n = p.cache_len;  // the cache's end is the end (reported where outputs of no token are)
-  if (n < 0) n = 0;
-  w.len = n;
-  w.start = n > p.window ? n - p.window : 0;
-  const int64_t sinks = p.sinks < w.start ? p.sinks : w.start;
-  const int first = static_cast<int>(w.start / kQ4Tokens), end = static_cast<int>((n + kQ4Tokens - 1) / kQ4Tokens);
-  w.ns = min(static_cast<int>((sinks + kQ4Tokens - 1) / kQ4Tokens), first);
-  w.skip = first - w.ns;
-  w.n = w.ns + end - first;
+  w.len = max(0, min(__ldg(p.lengths + b), p.cache_len));  // the cache's end is the end (reported elsewhere)
+  w.start = max(0, w.len - p.window);
+  w.first = w.start / kQ4Tokens;
+  w.end = (w.len + kQ4Tokens - 1) / kQ4Tokens;
+  w.sb = min((min(p.sinks, w.start) + kQ4Tokens - 1) / kQ4Tokens, w.first);
+  w.ns = (w.sb + 1) >> 1;
+  w.n = w.ns + ((w.end - w.first + 1) >> 1);
   return w;
 }
+// Chunk x's first block, and whether it has a second one.
+__device__ __forceinline__ int block_of(const Walk& w, int x) { return x < w.ns ? 2 * x : w.first + 2 * (x - w.ns); }
+__device__ __forceinline__ bool second_of(const Walk& w, int x, int block) { return block + 1 < (x < w.ns ? w.sb : w.end); }
 
-// Where a run stands: block x of walk (b, hp), hp = kv head * parts + part.
+// Where a run stands: chunk x of walk (b, hp), hp = kv head * parts + part.
 struct Cursor {
   int b, hp, x;
   Walk w;
 };
-// `by` blocks on, over the ends of walks (those of requests without tokens are empty).
+// `by` chunks on, over the ends of walks (those of requests without tokens are empty).
 __device__ __forceinline__ void move(const DecodeParams& p, Cursor* c, int by) {
   c->x += by;
   while (c->x >= c->w.n) {
@@ -104,16 +109,15 @@ __device__ __forceinline__ void move(const DecodeParams& p, Cursor* c, int by) {
     }
   }
 }
-__device__ __forceinline__ int64_t block_of(const Cursor& c) { return c.x < c.w.ns ? c.x : c.x + c.w.skip; }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -127,10 +131,32 @@ __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
-// Nibbles I and I + 4 of a word as bf16 16 + code.
-template <int I>
-__device__ __forceinline__ uint32_t codes2(uint32_t w) {
-  return ((I == 0 ? w << 3 : w >> (4 * I - 3)) & 0x00780078u) | 0x41804180u;
+constexpr uint32_t kEven = 0x000f000fu;
+constexpr float kUnit = 16777216.f;  // 2^24
+// Bytes 0 and 2 (second: 1 and 3) of a word, in its halves.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t w, int second) {
+  return second ? __byte_perm(w, 0u, 0x4341) : w & 0x00ff00ffu;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// The exponent field of a float that is not negative, within [lo, hi]; and 2^(e - 127).
+__device__ __forceinline__ int exponent(float x, int lo, int hi) {
+  return min(max(static_cast<int>(__float_as_uint(x) >> 23), lo), hi);
+}
+__device__ __forceinline__ float power(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }
+template <int N>
+__device__ __forceinline__ void ld_shared_n(uint32_t addr, uint32_t (&r)[N]) {
+  if constexpr (N == 1) {
+    r[0] = ld_shared(addr);
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+  } else {
+    const uint4 v = ld_shared_v4(addr);
+    r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+  }
 }
 __device__ __forceinline__ float step_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
@@ -139,7 +165,7 @@ __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(
 // nothing finite has sums of zeros, which may be added as they are, or of NaN, which must be.
 __device__ __forceinline__ float share_weight(float m, float mm) { return m == -INFINITY ? 1.f : exp2_approx(m - mm); }
 
-// A run's start in blocks, of `total` over `ctas`.
+// A run's start in chunks, of `total` over `ctas`.
 __device__ __forceinline__ int64_t run_at(int64_t total, int c, int ctas) { return total * c / ctas; }
 
 // NT: groups of 8 query heads a CTA works on.
@@ -148,7 +174,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   constexpr int H = 8 * NT;
   constexpr int NG = 128 / GROUP;                       // pairs of a token
   constexpr int RUNS = 4 / NG;                          // 32-channel runs of a group
-  constexpr uint32_t kBlock = q4_block_bytes(GROUP);    // of K; V's lies behind it in a stage
+  constexpr uint32_t kBlock = q4_block_bytes(GROUP);
+  constexpr uint32_t kStage = 4 * kBlock;               // a chunk's blocks of K, then of V
+  constexpr int kTop = 100;                             // P' is scaled by 2^kTop at most
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][STAGES];
   __shared__ int64_t sums[kWarps];
@@ -166,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   pdl_wait();
   if (threadIdx.x == 0) p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
 
-  // The run: blocks [r0, r1) of all walks.  Each thread counts the requests [b0, b1).
+  // The run: chunks [r0, r1) of all walks.  Each thread counts the requests [b0, b1).
   const int heads = p.KH * p.parts;
   const int each = (p.B + kThreads - 1) / kThreads;
   const int b0 = min(static_cast<int>(threadIdx.x) * each, p.B), b1 = min(b0 + each, p.B);
@@ -218,64 +246,94 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   at.hp = static_cast<int>(first_x / at.w.n);
   at.x = static_cast<int>(first_x - static_cast<int64_t>(at.hp) * at.w.n);
 
-  // this warp's blocks: warp, warp + kWarps, ... of the run
-  const uint32_t ring = smem_u32(smem) + warp * (STAGES * 2 * kBlock);
+  // this warp's chunks: warp, warp + kWarps, ... of the run
+  uint8_t* ring = smem + warp * (STAGES * kStage);
   Cursor ahead = at;  // of the next load
   if (warp > 0) move(p, &ahead, warp);
   int loads = 0;
+  // Loads one behind the other in a walk are kWarps chunks apart: `left` of them, of so many bytes.
+  int left = 0;
+  uint32_t bytes = 0;
+  const uint8_t *kp = nullptr, *vp = nullptr;
   auto load = [&]() {
     if (warp + loads * kWarps >= run) return;
+    if (left == 0) {
+      if (loads > 0) move(p, &ahead, 0);
+      const int g = ahead.hp / p.parts, block = block_of(ahead.w, ahead.x);
+      const int whole = ahead.x < ahead.w.ns ? ahead.w.sb >> 1 : ahead.w.ns + ((ahead.w.end - ahead.w.first) >> 1);
+      left = max(1, (whole - ahead.x + kWarps - 1) / kWarps);
+      bytes = ahead.x < whole ? 2 * kBlock : kBlock;
+      const int64_t off = static_cast<int64_t>(block) * kBlock;
+      kp = p.k + ahead.b * p.k_b + g * p.k_h + off;
+      vp = p.v + ahead.b * p.v_b + g * p.v_h + off;
+    }
     const int s = loads % STAGES;
     if (lane == 0) {
-      const int g = ahead.hp / p.parts;
-      const int64_t off = block_of(ahead) * kBlock;
-      mbar_arrive_expect_tx(&full[warp][s], 2 * kBlock);
-      uint8_t* dst = smem + warp * (STAGES * 2 * kBlock) + s * 2 * kBlock;
-      bulk_load_1d(dst, p.k + ahead.b * p.k_b + g * p.k_h + off, kBlock, &full[warp][s]);
-      bulk_load_1d(dst + kBlock, p.v + ahead.b * p.v_b + g * p.v_h + off, kBlock, &full[warp][s]);
+      mbar_arrive_expect_tx(&full[warp][s], 2 * bytes);
+      bulk_load_1d(ring + s * kStage, kp, bytes, &full[warp][s]);
+      bulk_load_1d(ring + s * kStage + 2 * kBlock, vp, bytes, &full[warp][s]);
     }
     ++loads;
-    if (warp + loads * kWarps < run) move(p, &ahead, kWarps);
+    --left;
+    kp += 2 * kWarps * kBlock;
+    vp += 2 * kWarps * kBlock;
+    ahead.x += kWarps;
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load();
 
-  float* parts = reinterpret_cast<float*>(smem + kWarps * STAGES * 2 * kBlock);  // [kWarps][min(rep, H)][kRow]
+  float* parts = reinterpret_cast<float*>(smem + kWarps * STAGES * kStage);  // [kWarps][min(rep, H)][kRow]
   const int held = min(p.rep, H);
   bool ok = true;
-  int done = 0;       // this warp's blocks
-  int piece_at = 0;   // the piece's first block in the run
+  int done = 0;       // this warp's chunks
+  int piece_at = 0;   // the piece's first chunk in the run
   while (piece_at < run) {
     const int left = run - piece_at;
-    const int n = min(left, at.w.n - at.x);  // blocks of the piece
+    const int n = min(left, at.w.n - at.x);  // chunks of the piece
     const int g = at.hp / p.parts, part = at.hp - g * p.parts;
     const int h0 = g * p.rep + part * H;  // first query head
     const int nh = min(H, p.rep - part * H);
 
     // q^T operands: for run g and step s of its two, head lane / 4, channels of this lane's
-    // word: (2 s, 2 s + 4) and (2 s + 1, 2 s + 5); and the sums over groups of the heads of
-    // this lane's accumulators, 2 (lane % 4) + {0, 1}
+    // word: (2 s, 2 s + 4) less a sixteenth of (2 s + 1, 2 s + 5), and the latter, times a
+    // power of two; and for the heads of
+    // this lane's accumulators, 2 (lane % 4) + {0, 1}, the sums over groups and the factor
+    // that makes scores of the products
     uint32_t qf[NT][4][2][2];
-    float qsum[NT][NG][2];
+    float qsum[NT][NG][2], sl2[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int h = t * 8 + r;
-      float sum[NG];
-#pragma unroll
-      for (int j = 0; j < NG; ++j) sum[j] = 0.f;
+      float f[4][8], top = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint4 w = h < nh ? __ldg(reinterpret_cast<const uint4*>(p.q + at.b * p.q_b +
                                                                       static_cast<int64_t>(h0 + h) * p.q_h + 32 * k) + c4)
                                : make_uint4(0u, 0u, 0u, 0u);
-        qf[t][k][0][0] = __byte_perm(w.x, w.z, 0x5410);
-        qf[t][k][0][1] = __byte_perm(w.x, w.z, 0x7632);
-        qf[t][k][1][0] = __byte_perm(w.y, w.w, 0x5410);
-        qf[t][k][1][1] = __byte_perm(w.y, w.w, 0x7632);
-        float f[8];
-        unpack_bf16x8(w, f);
-        sum[k / RUNS] += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+        unpack_bf16x8(w, f[k]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[k][i]));
       }
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+      const int ex = exponent(top, 1, 253);
+      const float f0 = power(254 - ex);
+      float sum[NG];
+#pragma unroll
+      for (int j = 0; j < NG; ++j) sum[j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f1 = f0 * 0.0625f;
+          qf[t][k][i >> 1][i & 1] = (i & 1) ? pack_f16x2(f[k][i] * f1, f[k][i + 4] * f1)
+                                            : pack_f16x2(fmaf(f[k][i + 1], -f1, f[k][i] * f0),
+                                                         fmaf(f[k][i + 5], -f1, f[k][i + 4] * f0));
+          sum[k / RUNS] += (f[k][i] + f[k][i + 4]) * (f0 / kUnit);  // in the products' unit
+        }
+      const float back = power(ex) * (p.scale_log2 * kUnit);
+      sl2[t][0] = __shfl_sync(kFull, back, 8 * c4);
+      sl2[t][1] = __shfl_sync(kFull, back, 8 * c4 + 4);
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         sum[j] += __shfl_xor_sync(kFull, sum[j], 1);
@@ -284,27 +342,29 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
         qsum[t][j][1] = __shfl_sync(kFull, sum[j], 8 * c4 + 4);
       }
     }
+    float nm[NT][2];                // -m, or zero where that is infinite
     float m[NT][2], l[NT][2];       // heads 8 t + 2 (lane % 4) + {0, 1}; l: this lane's keys only
+    int vs[NT][2];                  // P' = 2^(vs - 127) p step
     float lows[NT][NG][2];          // sums of p low, this lane's keys only
-    float ones[NT][NG][4];          // sums of p step (the same in every row)
-    float o[NT][4][2][4];           // run, step: channels 32 run + 4 (lane / 4) + 2 step (+ 1)
+    float o[NT][4][2][4];           // run, step: channels 32 run + 4 (lane / 4) + 2 step, of P' c 2^-24, and + 1, of P' (c + 16 c') 2^-24
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t][0] = m[t][1] = -INFINITY;
+      nm[t][0] = nm[t][1] = 0.f;
       l[t][0] = l[t][1] = 0.f;
+      vs[t][0] = vs[t][1] = 127 + kTop;
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        lows[t][j][0] = lows[t][j][1] = 0.f;
-        ones[t][j][0] = ones[t][j][1] = ones[t][j][2] = ones[t][j][3] = 0.f;
-      }
+      for (int j = 0; j < NG; ++j) lows[t][j][0] = lows[t][j][1] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int s = 0; s < 2; ++s) o[t][k][s][0] = o[t][k][s][1] = o[t][k][s][2] = o[t][k][s][3] = 0.f;
     }
 
-    for (; ok && warp + done * kWarps < piece_at + n; ++done) {
-      const int x = at.x + warp + done * kWarps - piece_at;
+    // chunks [xa, xb) are visible whole
+    const int xa = at.w.ns + (at.w.start % kQ4Tokens != 0), xb = at.w.ns + (at.w.len - at.w.first * kQ4Tokens) / (2 * kQ4Tokens);
+    const int x_end = at.x + n;
+    for (int x = at.x + warp + done * kWarps - piece_at; ok && x < x_end; ++done, x += kWarps) {
       __syncwarp();  // every lane is done with the stage refilled here
       load();
       const int s = done % STAGES;
@@ -312,24 +372,34 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
         ok = false;
         break;
       }
-      const uint32_t ks = ring + s * 2 * kBlock, vs = ks + kBlock;
-      const int64_t tok = (x < at.w.ns ? x : x + at.w.skip) * static_cast<int64_t>(kQ4Tokens);
-      // tokens of this lane's accumulators: r and r + 8
-      bool see0 = true, see1 = true;
-      const bool whole = tok + kQ4Tokens <= at.w.len && (tok >= at.w.start || tok + kQ4Tokens <= p.sinks);
+      const bool whole = x >= xa && x < xb;
+      const uint32_t ks = smem_u32(ring) + s * kStage, vb = ks + 2 * kBlock;
+      // block i of the two: the tokens of this lane's accumulators are its r and r + 8
+      bool see[2][2] = {{true, true}, {true, true}};
       if (!whole) {
-        const int64_t t0 = tok + r, t1 = t0 + 8;
-        see0 = t0 < at.w.len && (t0 >= at.w.start || t0 < p.sinks);
-        see1 = t1 < at.w.len && (t1 >= at.w.start || t1 < p.sinks);
+        const int block = block_of(at.w, x);
+        const bool two = second_of(at.w, x, block);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int tok = (block + i) * kQ4Tokens + r + 8 * c;
+            see[i][c] = (i == 0 || two) && tok < at.w.len && (tok >= at.w.start || tok < p.sinks);
+          }
       }
 
-      float sc[NT][4];
+      float sc[2][NT][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-      {
-        const uint32_t row = ks + r * 64 + ((c4 ^ ((r >> 1) & 3)) << 4);  // chunk lane % 4 of tokens r and r + 8
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t kb = ks + i * kBlock;
+        const uint32_t row = kb + r * 64 + ((c4 ^ ((r >> 1) & 3)) << 4);  // chunk lane % 4 of tokens r and r + 8
         const uint4 k0 = ld_shared_v4(row), k1 = ld_shared_v4(row + 512);
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+        uint32_t p0[NG], p1[NG];
+        ld_shared_n<NG>(kb + kQ4Codes + r * NG * 4, p0);
+        ld_shared_n<NG>(kb + kQ4Codes + (r + 8) * NG * 4, p1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[i][t][0] = sc[i][t][1] = sc[i][t][2] = sc[i][t][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
           float acc[NT][4];
@@ -339,54 +409,134 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
           for (int k = j * RUNS; k < (j + 1) * RUNS; ++k)
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-              const uint32_t a[4] = {st ? codes2<2>(w0[k]) : codes2<0>(w0[k]), st ? codes2<2>(w1[k]) : codes2<0>(w1[k]),
-                                     st ? codes2<3>(w0[k]) : codes2<1>(w0[k]), st ? codes2<3>(w1[k]) : codes2<1>(w1[k])};
+              const uint32_t b0 = bytes_of(w0[k], st), b1 = bytes_of(w1[k], st);
+              const uint32_t a[4] = {b0 & kEven, b1 & kEven, b0, b1};
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma_bf16(acc[t], a, qf[t][k][st][0], qf[t][k][st][1]);
+              for (int t = 0; t < NT; ++t) mma_f16(acc[t], a, qf[t][k][st][0], qf[t][k][st][1]);
             }
-          const uint32_t p0 = ld_shared(ks + kQ4Codes + (r * NG + j) * 4);
-          const uint32_t p1 = ld_shared(ks + kQ4Codes + ((r + 8) * NG + j) * 4);
-          const float s0 = step_of(p0), s1 = step_of(p1);
-          const float z0 = fmaf(-16.f, s0, low_of(p0)), z1 = fmaf(-16.f, s1, low_of(p1));
+          const float s0 = step_of(p0[j]), s1 = step_of(p1[j]);
+          const float z0 = low_of(p0[j]), z1 = low_of(p1[j]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            sc[t][0] = fmaf(s0, acc[t][0], fmaf(z0, qsum[t][j][0], sc[t][0]));
-            sc[t][1] = fmaf(s0, acc[t][1], fmaf(z0, qsum[t][j][1], sc[t][1]));
-            sc[t][2] = fmaf(s1, acc[t][2], fmaf(z1, qsum[t][j][0], sc[t][2]));
-            sc[t][3] = fmaf(s1, acc[t][3], fmaf(z1, qsum[t][j][1], sc[t][3]));
+            sc[i][t][0] = fmaf(s0, acc[t][0], fmaf(z0, qsum[t][j][0], sc[i][t][0]));
+            sc[i][t][1] = fmaf(s0, acc[t][1], fmaf(z0, qsum[t][j][1], sc[i][t][1]));
+            sc[i][t][2] = fmaf(s1, acc[t][2], fmaf(z1, qsum[t][j][0], sc[i][t][2]));
+            sc[i][t][3] = fmaf(s1, acc[t][3], fmaf(z1, qsum[t][j][1], sc[i][t][3]));
           }
         }
       }
       if (!whole) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (!see0) sc[t][0] = sc[t][1] = -INFINITY;
-          if (!see1) sc[t][2] = sc[t][3] = -INFINITY;
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (!see[i][0]) sc[i][t][0] = sc[i][t][1] = -INFINITY;
+            if (!see[i][1]) sc[i][t][2] = sc[i][t][3] = -INFINITY;
+          }
       }
       bool grow = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) grow |= fmaxf(sc[t][c], sc[t][c + 2]) * p.scale_log2 > m[t][c] + 8.f;
+        for (int c = 0; c < 2; ++c)
+          grow |= fmaxf(fmax3(sc[0][t][c], sc[0][t][c + 2], sc[1][t][c]), sc[1][t][c + 2]) * sl2[t][c] > m[t][c] + 8.f;
       if (__any_sync(kFull, grow)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(sc[t][c], sc[t][c + 2]) * p.scale_log2;
+            float mx = fmaxf(fmax3(sc[0][t][c], sc[0][t][c + 2], sc[1][t][c]), sc[1][t][c + 2]) * sl2[t][c];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, d));
             mx = fmaxf(mx, m[t][c]);
             // nothing finite yet: keep the (empty) sums as they are
             const float f = mx == -INFINITY ? 1.f : exp2_approx(m[t][c] - mx);
+            // what the old sums lose, P' may gain
+            const int up = min(127 + kTop - vs[t][c], static_cast<int>(fminf(mx - m[t][c], 1000.f)));
+            const float fo = mx == -INFINITY ? 1.f : exp2_approx(m[t][c] - mx + static_cast<float>(up));
+            vs[t][c] += mx == -INFINITY ? 0 : up;
             m[t][c] = mx;
+            nm[t][c] = mx == -INFINITY ? 0.f : -mx;
             l[t][c] *= f;
 #pragma unroll
-            for (int j = 0; j < NG; ++j) {
-              lows[t][j][c] *= f;
-              ones[t][j][c] *= f;
-            }
+            for (int j = 0; j < NG; ++j) lows[t][j][c] *= f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int st = 0; st < 2; ++st) {
+                o[t][k][st][c] *= fo;
+                o[t][k][st][c + 2] *= fo;
+              }
+          }
+      }
+      float e[2][NT][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) e[i][t][c] = exp2_approx(fmaf(sc[i][t][c], sl2[t][c & 1], nm[t][c & 1]));
+          l[t][0] += e[i][t][0] + e[i][t][2];
+          l[t][1] += e[i][t][1] + e[i][t][3];
+        }
+      // P' = p step 2^vs, which meets the codes as fp16, the tensor core's operand type
+      uint32_t pp[2][NT][NG][2];
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t p0[NG], p1[NG];
+        ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + r * NG * 4, p0);
+        ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + (r + 8) * NG * 4, p1);
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {  // whatever is there must not meet its weight of zero
+            if (!see[i][0]) p0[j] = 0u;
+            if (!see[i][1]) p1[j] = 0u;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float v0 = power(vs[t][0]), v1 = power(vs[t][1]);
+          const float ev[4] = {e[i][t][0] * v0, e[i][t][1] * v1, e[i][t][2] * v0, e[i][t][3] * v1};
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const float s0 = step_of(p0[j]), s1 = step_of(p1[j]), z0 = low_of(p0[j]), z1 = low_of(p1[j]);
+            lows[t][j][0] = fmaf(e[i][t][0], z0, fmaf(e[i][t][2], z1, lows[t][j][0]));
+            lows[t][j][1] = fmaf(e[i][t][1], z0, fmaf(e[i][t][3], z1, lows[t][j][1]));
+            const float pv[4] = {ev[0] * s0, ev[1] * s0, ev[2] * s1, ev[3] * s1};
+            top = fmax3(fmax3(top, pv[0], pv[1]), pv[2], pv[3]);
+            pp[i][t][j][0] = pack_f16x2(pv[0], pv[1]);
+            pp[i][t][j][1] = pack_f16x2(pv[2], pv[3]);
+          }
+        }
+      }
+      if (__any_sync(kFull, top > 32768.f)) {
+        uint32_t p0[2][NG], p1[2][NG];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + r * NG * 4, p0[i]);
+          ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + (r + 8) * NG * 4, p1[i]);
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            if (!see[i][0]) p0[i][j] = 0u;
+            if (!see[i][1]) p1[i][j] = 0u;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < NG; ++j)
+                most = fmax3(most, e[i][t][c] * step_of(p0[i][j]), e[i][t][c + 2] * step_of(p1[i][j]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, d));
+            const int to = min(vs[t][c], 254 - exponent(most, 127 - kTop, 253));
+            const float f = exp2_approx(static_cast<float>(to - vs[t][c]));
+            vs[t][c] = to;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -395,54 +545,45 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
                 o[t][k][st][c + 2] *= f;
               }
           }
-      }
-      float e[NT][4];
+          const float v0 = power(vs[t][0]), v1 = power(vs[t][1]);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float mm = m[t][c & 1] == -INFINITY ? 0.f : m[t][c & 1];
-          e[t][c] = exp2_approx(fmaf(sc[t][c], p.scale_log2, -mm));
+            for (int j = 0; j < NG; ++j) {
+              const float s0 = step_of(p0[i][j]), s1 = step_of(p1[i][j]);
+              pp[i][t][j][0] = pack_f16x2(e[i][t][0] * v0 * s0, e[i][t][1] * v1 * s0);
+              pp[i][t][j][1] = pack_f16x2(e[i][t][2] * v0 * s1, e[i][t][3] * v1 * s1);
+            }
         }
-        l[t][0] += e[t][0] + e[t][2];
-        l[t][1] += e[t][1] + e[t][3];
       }
-      // tokens 2 (lane % 4) + {0, 1} and 8 on: their chunk r / 2, of which this lane takes half
-      // of each word: channels 32 run + 4 r + {0 .. 3}
-      const uint32_t col = vs + c4 * 128 + (((r >> 1) ^ c4) << 4);
-      const uint4 va = ld_shared_v4(col), vb = ld_shared_v4(col + 64), vc = ld_shared_v4(col + 512),
-                  vd = ld_shared_v4(col + 576);
-      const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w},
-                     wc[4] = {vc.x, vc.y, vc.z, vc.w}, wd[4] = {vd.x, vd.y, vd.z, vd.w};
-      const uint32_t pick = (r & 1) ? 0x7632u : 0x5410u;
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        uint32_t p0 = ld_shared(vs + kQ4Codes + (r * NG + j) * 4);
-        uint32_t p1 = ld_shared(vs + kQ4Codes + ((r + 8) * NG + j) * 4);
-        if (!see0) p0 = 0u;  // whatever is there must not meet its weight of zero
-        if (!see1) p1 = 0u;
-        const float s0 = step_of(p0), s1 = step_of(p1), z0 = low_of(p0), z1 = low_of(p1);
-        uint32_t pb[NT][2];
+      for (int i = 0; i < 2; ++i) {
+        // tokens 2 (lane % 4) + {0, 1} and 8 on: their chunk r / 2, of which this lane takes half
+        // of each word: channels 32 run + 4 r + {0 .. 3}
+        const uint32_t col = vb + i * kBlock + c4 * 128 + (((r >> 1) ^ c4) << 4);
+        const uint4 va = ld_shared_v4(col), vc = ld_shared_v4(col + 64), vd = ld_shared_v4(col + 512),
+                    ve = ld_shared_v4(col + 576);
+        const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vc.x, vc.y, vc.z, vc.w},
+                       wc[4] = {vd.x, vd.y, vd.z, vd.w}, wd[4] = {ve.x, ve.y, ve.z, ve.w};
+        const uint32_t pick = (r & 1) ? 0x7632u : 0x5410u;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          lows[t][j][0] = fmaf(e[t][0], z0, fmaf(e[t][2], z1, lows[t][j][0]));
-          lows[t][j][1] = fmaf(e[t][1], z0, fmaf(e[t][3], z1, lows[t][j][1]));
-          // weight times step meets the codes as bf16, the tensor core's operand type
-          pb[t][0] = transpose8x8(pack_bf16x2(e[t][0] * s0, e[t][1] * s0));
-          pb[t][1] = transpose8x8(pack_bf16x2(e[t][2] * s1, e[t][3] * s1));
-        }
-        const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        for (int j = 0; j < NG; ++j) {
+          uint32_t pb[NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma_bf16(ones[t][j], one, pb[t][0], pb[t][1]);
+          for (int t = 0; t < NT; ++t) {
+            pb[t][0] = transpose8x8(pp[i][t][j][0]);
+            pb[t][1] = transpose8x8(pp[i][t][j][1]);
+          }
 #pragma unroll
-        for (int k = j * RUNS; k < (j + 1) * RUNS; ++k) {
-          const uint32_t lo = __byte_perm(wa[k], wb[k], pick), hi = __byte_perm(wc[k], wd[k], pick);
+          for (int k = j * RUNS; k < (j + 1) * RUNS; ++k) {
+            const uint32_t lo = __byte_perm(wa[k], wb[k], pick), hi = __byte_perm(wc[k], wd[k], pick);
 #pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            const uint32_t a[4] = {st ? codes2<2>(lo) : codes2<0>(lo), st ? codes2<3>(lo) : codes2<1>(lo),
-                                   st ? codes2<2>(hi) : codes2<0>(hi), st ? codes2<3>(hi) : codes2<1>(hi)};
+            for (int st = 0; st < 2; ++st) {
+              const uint32_t b0 = bytes_of(lo, st), b1 = bytes_of(hi, st);
+              const uint32_t a[4] = {b0 & kEven, b0, b1 & kEven, b1};
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_bf16(o[t][k][st], a, pb[t][0], pb[t][1]);
+              for (int t = 0; t < NT; ++t) mma_f16(o[t][k][st], a, pb[t][0], pb[t][1]);
+            }
           }
         }
       }
@@ -463,10 +604,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
           add[j] = lows[t][j][c];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) add[j] += __shfl_xor_sync(kFull, add[j], d);
-          add[j] = fmaf(-16.f, ones[t][j][c], add[j]);
         }
         if (h < nh) {
           float* dst = parts + (warp * held + h) * kRow;
+          const float f0 = power(254 - vs[t][c]) * kUnit, f1 = f0 * 0.0625f;
           if (r == 0) {
             dst[kD] = m[t][c];
             dst[kD + 1] = sum;
@@ -476,7 +617,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
 #pragma unroll
             for (int st = 0; st < 2; ++st)
               *reinterpret_cast<float2*>(dst + 32 * k + 4 * r + 2 * st) =
-                  make_float2(o[t][k][st][c] + add[k / RUNS], o[t][k][st][c + 2] + add[k / RUNS]);
+                  make_float2(fmaf(o[t][k][st][c], f0, add[k / RUNS]),
+                              fmaf(o[t][k][st][c + 2] - o[t][k][st][c], f1, add[k / RUNS]));
         }
       }
     __syncthreads();
@@ -529,18 +671,24 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
   const int b = w.x / heads, hp = w.x - b * heads, g = hp / p.parts, part = hp - g * p.parts;
   const int h = blockIdx.y;
   if (h >= min(H, p.rep - part * H)) return;
-  int steps = w.z, count = 1;  // shares: slots 2 x + 1, 2 (x + 1), 2 (x + 2), ...
-  for (int slot = 2 * blockIdx.x + 1;; ++count) {
-    slot = next_share(p.pieces, 2 * ctas, slot, w.w, &steps);
-    if (slot < 0) break;
-  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // shares: slots 2 x + 1, 2 (x + 1), 2 (x + 2), ..., the latter while they are of this walk
+  int count = 1;
+  for (bool more = true; more;) {
+    const int c = blockIdx.x + count + lane;
+    const int4 s = c < ctas ? p.pieces[2 * c] : make_int4(0, 0, 0, 0);
+    const unsigned others = ~__ballot_sync(kFull, s.z > 0 && s.x == w.x);
+    count += others ? __ffs(static_cast<int>(others)) - 1 : 32;
+    more = others == 0u;
+  }
   auto share = [&](int i) {
     const int slot = i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i);
     return p.shares + (static_cast<int64_t>(slot) * H + h) * kRow;
   };
   float mm = -INFINITY;
-  for (int i = warp; i < count; i += kWarps) mm = fmaxf(mm, share(i)[kD]);
+  for (int i = lane; i < count; i += 32) mm = fmaxf(mm, share(i)[kD]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(kFull, mm, d));
   float ll = 0.f;
   float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -552,21 +700,15 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
     oo.x += f * v.x, oo.y += f * v.y, oo.z += f * v.z, oo.w += f * v.w;
   }
   reinterpret_cast<float4*>(parts[warp])[lane] = oo;
-  if (lane == 0) {
-    parts[warp][kD] = mm;
-    parts[warp][kD + 1] = ll;
-  }
+  if (lane == 0) parts[warp][kD + 1] = ll;
   __syncthreads();
   if (threadIdx.x < kD) {
     const int d = threadIdx.x;
-    float m2 = -INFINITY, l2 = 0.f, o2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) m2 = fmaxf(m2, parts[i][kD]);
+    float l2 = 0.f, o2 = 0.f;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-      const float f = share_weight(parts[i][kD], m2);
-      l2 += f * parts[i][kD + 1];
-      o2 += f * parts[i][d];
+      l2 += parts[i][kD + 1];
+      o2 += parts[i][d];
     }
     p.out[(static_cast<int64_t>(b) * p.QH + g * p.rep + part * H + h) * kD + d] = __float2bfloat16_rn(o2 / l2);
   }
@@ -575,10 +717,10 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
 template <int NT, int GROUP>
 kda_status launch_decode(const DecodeParams& p, int ctas, cudaStream_t st) {
   // rings of the depth that leaves two CTAs an SM (one where a group has more than 8 heads)
-  constexpr int kStages = NT == 1 ? (GROUP == 32 ? 3 : 4) : 6;
+  constexpr int kStages = NT == 1 ? 2 : 4;
   constexpr int H = 8 * NT;
-  constexpr size_t kMost = kWarps * (kStages * 2 * q4_block_bytes(GROUP) + H * kRow * 4);
-  static_assert(kMost <= (NT == 1 ? 112 : 226) * 1024, "shared memory budget");
+  constexpr size_t kMost = kWarps * (kStages * 4 * q4_block_bytes(GROUP) + H * kRow * 4);
+  static_assert(kMost <= (NT == 1 ? 113 : 226) * 1024, "shared memory budget");
   auto* kernel = q4_decode_kernel<NT, GROUP, kStages>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
@@ -589,7 +731,7 @@ kda_status launch_decode(const DecodeParams& p, int ctas, cudaStream_t st) {
       return launch_status("gqa_decode_q4: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  const size_t smem = kWarps * (kStages * 2 * q4_block_bytes(GROUP) + (p.rep < H ? p.rep : H) * kRow * 4);
+  const size_t smem = kWarps * (kStages * 4 * q4_block_bytes(GROUP) + (p.rep < H ? p.rep : H) * kRow * 4);
   const kda_status s = launch_after("gqa_decode_q4", kernel, dim3(static_cast<unsigned>(ctas)), kThreads, smem, st, p,
                                     kda_err_ptr_q4_decode());
   if (s != KDA_OK) return s;
@@ -648,9 +790,10 @@ extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, cons
   p.q_h = QH > 1 ? q_strides[1] : 0;
   p.k_b = B > 1 ? k_cache_strides[0] : 0, p.k_h = KH > 1 ? k_cache_strides[1] : 0;
   p.v_b = B > 1 ? v_cache_strides[0] : 0, p.v_h = KH > 1 ? v_cache_strides[1] : 0;
-  p.cache_len = blocks * kQ4Tokens;
-  p.window = window < p.cache_len ? window : p.cache_len;
-  p.sinks = sinks < p.cache_len ? sinks : p.cache_len;
+  const int64_t T = blocks * kQ4Tokens;
+  p.cache_len = static_cast<int>(T);
+  p.window = static_cast<int>(window < T ? window : T);
+  p.sinks = static_cast<int>(sinks < T ? sinks : T);
   p.B = static_cast<int>(B);
   p.QH = static_cast<int>(QH);
   p.KH = static_cast<int>(KH);
