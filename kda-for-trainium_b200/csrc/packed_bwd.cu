@@ -119,6 +119,26 @@ __device__ __forceinline__ Piece piece_at(const BwdParams& p, int64_t x, int64_t
   c.n = static_cast<int>(min(most, static_cast<int64_t>(c.walk - c.it0)));
   return c;
 }
+// The step at which a run starts that has x of the walks' cost before it, where a walk
+// costs its steps and kWalkCost before the first of them (loads without a step beside them,
+// results on their way out: by steps alone the CTA with the short walks at a sequence's end
+// worked 270,000 cycles at S4096 of 16 heads, the others 200,000; with 1 to 3: 212,000).
+constexpr int kWalkCost = 2;
+__device__ __forceinline__ int64_t step_at_cost(const BwdParams& p, int64_t x) {
+  auto cost_before = [&](int e) { return p.plan.before[e] * p.QH + static_cast<int64_t>(e) * p.KH * kWalkCost; };
+  int lo = 0, hi = p.plan.head->blocks;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cost_before(mid) <= x) lo = mid;
+    else hi = mid;
+  }
+  Piece c;
+  c.e = lo;
+  set_block(p, &c);
+  const int64_t y = x - cost_before(lo);
+  const int64_t g = y / (c.walk + kWalkCost), in = y - g * (c.walk + kWalkCost);
+  return p.plan.before[lo] * p.QH + g * c.walk + (in > kWalkCost ? in - kWalkCost : 0);
+}
 // The piece after c, of at most `most` steps: the next walk from its start.
 __device__ __forceinline__ Piece piece_after(const BwdParams& p, const Piece& c, int most) {
   Piece d = c;
@@ -202,10 +222,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   int* first_s = reinterpret_cast<int*>(smem + Smem::kFirst);
   if (warp == 3 && lane == 0) {
-    const int64_t total = plan_matches(p.plan, p.tokens) ? p.plan.head->steps * p.QH : 0;
-    // fewer steps than CTAs: the first ones take one each, so that a walk's shares follow one another
-    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total), cta = blockIdx.x;
-    const int64_t x = cta < ctas ? total * cta / ctas : 0, end = cta < ctas ? total * (cta + 1) / ctas : 0;
+    const PlanHead& head = *p.plan.head;
+    const bool fits = plan_matches(p.plan, p.tokens);
+    const int64_t total = fits ? head.steps * p.QH : 0;
+    const int64_t cost = fits ? total + static_cast<int64_t>(head.blocks) * p.KH * kWalkCost : 0;
+    // Fewer than CTAs: the first ones take one each, so that a walk's shares follow one
+    // another.  (A run between two walks may still be empty.)
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), cost), cta = blockIdx.x;
+    const int64_t x = cta < ctas ? step_at_cost(p, cost * cta / ctas) : 0;
+    const int64_t end = cta + 1 < ctas ? step_at_cost(p, cost * (cta + 1) / ctas) : cta < ctas ? total : 0;
     Piece c{};
     if (end > x) c = piece_at(p, x, end - x);
     first_s[0] = c.e, first_s[1] = c.g, first_s[2] = c.it0, first_s[3] = c.n, first_s[4] = c.walk, first_s[5] = c.nq;

@@ -16,33 +16,32 @@ namespace kda {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kBins = 4096;  // places from here on share the first bin: they are sorted no further
+constexpr int kBins = kThreads;  // places from here on share the first bin: they are sorted no further
 constexpr unsigned kFull = 0xffffffffu;
 
 // The sums over the threads before this one, and over all.
-template <typename T>
-__device__ __forceinline__ T scan_block(T v, T* warp_sums, T* total) {
+__device__ __forceinline__ int64_t scan_block(int64_t v, int64_t* warp_sums, int64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T sum = v;
+  int64_t sum = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const T o = __shfl_up_sync(kFull, sum, d);
+    const int64_t o = __shfl_up_sync(kFull, sum, d);
     if (lane >= d) sum += o;
   }
   if (lane == 31) warp_sums[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    T w = warp_sums[lane];
+    int64_t w = warp_sums[lane];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const T o = __shfl_up_sync(kFull, w, d);
+      const int64_t o = __shfl_up_sync(kFull, w, d);
       if (lane >= d) w += o;
     }
     warp_sums[lane] = w;
   }
   __syncthreads();
   *total = warp_sums[31];
-  const T before = (warp > 0 ? warp_sums[warp - 1] : T(0)) + sum - v;
+  const int64_t before = (warp > 0 ? warp_sums[warp - 1] : 0) + sum - v;
   __syncthreads();  // warp_sums may be used again
   return before;
 }
@@ -53,9 +52,8 @@ __device__ __forceinline__ int bin_of(int z) { return kBins - 1 - min(z, kBins -
 __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const int* __restrict__ offsets, int sequences,
                                                                int tokens, uint8_t* plan, int64_t most,
                                                                unsigned* err) {
-  __shared__ int bins[2][kBins];
-  __shared__ int64_t sums64[32];
-  __shared__ int sums[32];
+  __shared__ int bins[2][kBins];  // all blocks, those at even places
+  __shared__ int64_t sums[32];
   pdl_trigger();
   pdl_wait();
   PlanHead* head = reinterpret_cast<PlanHead*>(plan);
@@ -66,7 +64,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const int* __rest
   int64_t* seq_steps = before + most;
   int* seq_block = reinterpret_cast<int*>(seq_steps + sequences);
 
-  for (int i = threadIdx.x; i < kBins; i += kThreads) bins[0][i] = bins[1][i] = 0;
+  bins[0][threadIdx.x] = bins[1][threadIdx.x] = 0;
   bool bad = false;
   int blocks = 0;
   int64_t steps = 0;
@@ -79,16 +77,15 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const int* __rest
       else n = (b - a + 127) >> 7;
     }
     if (__syncthreads_or(bad)) break;  // no table is read or written past its end
-    int all;
-    int64_t all64;
-    const int at = blocks + scan_block(n, sums, &all);
-    const int64_t at64 = steps + scan_block(static_cast<int64_t>(n) * (n + 1) / 2, sums64, &all64);
+    // both sums in one scan: blocks (below 2^24 together) beneath steps (below 2^35)
+    int64_t all;
+    const int64_t at = scan_block((static_cast<int64_t>(n) * (n + 1) / 2) << 24 | n, sums, &all);
     if (s < sequences) {
-      seq_block[s] = at;
-      seq_steps[s] = at64;
+      seq_block[s] = blocks + static_cast<int>(at & 0xffffff);
+      seq_steps[s] = steps + (at >> 24);
     }
-    blocks += all;
-    steps += all64;
+    blocks += static_cast<int>(all & 0xffffff);
+    steps += all >> 24;
   }
   if (__syncthreads_or(bad)) {
     if (threadIdx.x == 0) {
@@ -113,20 +110,11 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const int* __rest
     if ((z & 1) == 0) atomicAdd(&bins[1][bin_of(static_cast<int>(z))], 1);
   }
   __syncthreads();
-  int num_pairs = 0;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {  // the bins' first places
-    int v[kBins / kThreads], sum = 0, all;
-#pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      v[i] = sum;
-      sum += bins[k][threadIdx.x * (kBins / kThreads) + i];
-    }
-    const int at = scan_block(sum, sums, &all);
-#pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) bins[k][threadIdx.x * (kBins / kThreads) + i] = at + v[i];
-    num_pairs = all;
-  }
+  // the bins' first places, of both in one scan
+  int64_t all;
+  const int64_t at = scan_block(static_cast<int64_t>(bins[1][threadIdx.x]) << 32 | bins[0][threadIdx.x], sums, &all);
+  bins[0][threadIdx.x] = static_cast<int>(at & 0xffffffff);
+  bins[1][threadIdx.x] = static_cast<int>(at >> 32);
   __syncthreads();
   for (int e = threadIdx.x; e < blocks; e += kThreads) {
     const Block b = natural[e];
@@ -134,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) packed_plan_kernel(const int* __rest
     if ((b.z & 1) == 0) pairs[atomicAdd(&bins[1][bin_of(b.z)], 1)] = b;
   }
   if (threadIdx.x == 0)
-    *head = PlanHead{kPlanMagic, blocks, num_pairs, offsets[0], offsets[sequences], tokens, steps};
+    *head = PlanHead{kPlanMagic, blocks, static_cast<int>(all >> 32), offsets[0], offsets[sequences], tokens, steps};
 }
 
 }  // namespace

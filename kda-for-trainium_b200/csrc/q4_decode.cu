@@ -665,28 +665,30 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
   __shared__ __align__(16) float parts[kWarps][kRow];
   pdl_trigger();
   pdl_wait();
-  const int4 w = p.pieces[2 * blockIdx.x + 1];
-  if (w.z == 0) return;
-  const int heads = p.KH * p.parts;
-  const int b = w.x / heads, hp = w.x - b * heads, g = hp / p.parts, part = hp - g * p.parts;
-  const int h = blockIdx.y;
-  if (h >= min(H, p.rep - part * H)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // shares: slots 2 x + 1, 2 (x + 1), 2 (x + 2), ..., the latter while they are of this walk
-  int count = 1;
-  for (bool more = true; more;) {
-    const int c = blockIdx.x + count + lane;
-    const int4 s = c < ctas ? p.pieces[2 * c] : make_int4(0, 0, 0, 0);
-    const unsigned others = ~__ballot_sync(kFull, s.z > 0 && s.x == w.x);
-    count += others ? __ffs(static_cast<int>(others)) - 1 : 32;
-    more = others == 0u;
-  }
+  // What may be this walk's is asked for at once, whether or not it is: the piece, the next
+  // ones, and the shares' maxima (a share's memory is there in any case).
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y;
+  const int x = static_cast<int>(blockIdx.x);
+  // share i: slot 2 x + 1, then 2 (x + 1), 2 (x + 2), ..., while they are of this walk
   auto share = [&](int i) {
-    const int slot = i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i);
+    const int slot = i == 0 ? 2 * x + 1 : 2 * min(x + i, ctas - 1);
     return p.shares + (static_cast<int64_t>(slot) * H + h) * kRow;
   };
-  float mm = -INFINITY;
-  for (int i = lane; i < count; i += 32) mm = fmaxf(mm, share(i)[kD]);
+  const int4 w = p.pieces[2 * x + 1];
+  int4 next = p.pieces[2 * min(x + 1 + lane, ctas - 1)];
+  float mm = share(lane)[kD];
+  const int heads = p.KH * p.parts;
+  const int b = w.x / heads, hp = w.x - b * heads, g = hp / p.parts, part = hp - g * p.parts;
+  if (w.z == 0 || h >= min(H, p.rep - part * H)) return;
+  int count = 1;
+  for (;;) {
+    const unsigned others = ~__ballot_sync(kFull, x + count + lane < ctas && next.z > 0 && next.x == w.x);
+    count += others ? __ffs(static_cast<int>(others)) - 1 : 32;
+    if (others) break;
+    next = p.pieces[2 * min(x + count + lane, ctas - 1)];
+  }
+  if (lane >= count) mm = -INFINITY;
+  for (int i = lane + 32; i < count; i += 32) mm = fmaxf(mm, share(i)[kD]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(kFull, mm, d));
   float ll = 0.f;

@@ -182,7 +182,7 @@ def test_plan_tables(kda, lens, T):
     for rows, keep in ((plan[at + 4 * most:][:4 * E], slice(None)),
                        (plan[at + 8 * most:][:4 * plan[2]], want[:, 2] % 2 == 0)):
         rows = rows.reshape(-1, 4)
-        assert (np.diff(np.minimum(rows[:, 2], 4095)) <= 0).all()
+        assert (np.diff(np.minimum(rows[:, 2], 1023)) <= 0).all()
         assert np.array_equal(rows[np.lexsort(rows.T)], want[keep][np.lexsort(want[keep].T)])
     assert np.array_equal(plan[at + 12 * most:][:2 * E].view(np.int64), before)
 
