@@ -118,20 +118,21 @@ __global__ void __launch_bounds__(kThreads) q4_append_kernel(const AppendParams 
   const int tokens = static_cast<int>(token(min(i0 + kItems, all) - 1) - row0) + 1;
   if (hw < tokens) {
     const int row = static_cast<int>(row0) + hw;
-    int b, at;
+    int b;
+    int64_t at;
     bool any = true;
     if (p.offsets) {
       b = request_of(p.offsets, p.B, row, l, mask);
       const int first = __ldg(p.offsets + b);
       any = row >= first && row < __ldg(p.offsets + b + 1);  // of some request
-      at = any ? row - first : 0;
+      at = static_cast<int64_t>(row) - first;
     } else {
       b = static_cast<int>(static_cast<unsigned>(row) / p.per);
       at = row - b * static_cast<int>(p.per);
     }
     const int cached = __ldg(p.lengths + b);
     any = any && cached >= 0;  // not an idle slot
-    const int64_t pos = static_cast<int64_t>(cached) + at;
+    const int64_t pos = cached + at;
     if (l == 0) {
       if (any && pos >= p.cache_len) atomicOr(err, static_cast<unsigned>(kErrRange));
       request[hw] = b;

@@ -17,7 +17,7 @@
 // the two sums is 16 times the second channel's: 4.5 integer operations for 8 codes.
 // (As bf16 16 + code, the 16s subtracted from the sums: 241 us for 64 requests; as fp16
 // code - 8 by one more multiply-add a pair: 194; a nibble each, a block at a time: 151;
-// two blocks at a time: 143.)
+// two blocks at a time: 139, and 124 for two kv heads together.)
 // The other operands are fp16 then, with ranges of their own: q times a power of two per head
 // that brings its largest value to 1 .. 2, and p step times one per head that keeps it below
 // 2^15 and was last chosen where the largest so far became 1 .. 2 (in the manner of the running
@@ -62,19 +62,32 @@ struct DecodeParams {
   int64_t q_b, q_h;          // element strides
   int64_t k_b, k_h, v_b, v_h;  // byte strides
   int cache_len, window, sinks;
-  int B, QH, KH, rep, parts;  // parts: groups of 8 NT query heads per kv head
+  int B, QH, KH, rep;
+  int parts;                 // groups of 8 NT query heads per kv head; 0: two kv heads together
+  int walks;                 // of a request
   float scale_log2;
   float* shares;             // [2 x CTAs][8 NT][kRow]
   int4* pieces;              // [2 x CTAs]: walk, 0, chunks of the share, of the walk
   unsigned* length_err;
 };
 
-// A request's visible tokens as chunks of two blocks: `ns` over blocks [0, sb) (sinks), then
+// Walk hp of a request: its (first) kv head and its query heads, which follow one another.
+struct Heads {
+  int kv, first, n;
+};
+__device__ __forceinline__ Heads heads_of(const DecodeParams& p, int most, int hp) {
+  if (p.parts == 0) return {2 * hp, 2 * hp * p.rep, 2 * p.rep};
+  const int g = hp / p.parts, part = hp - g * p.parts;
+  return {g, g * p.rep + part * most, min(most, p.rep - part * most)};
+}
+
+// A request's visible tokens as chunks of PER blocks of each of the walk's kv heads: `ns` over blocks [0, sb) (sinks), then
 // those over [first, end).
 struct Walk {
   int n, ns, sb, first, end;
   int len, start;
 };
+template <int PER>
 __device__ __forceinline__ Walk walk_of(const DecodeParams& p, int b) {
   Walk w;
   w.len = max(0, min(__ldg(p.lengths + b), p.cache_len));  // the cache's end is the end (reported elsewhere)
@@ -82,29 +95,33 @@ __device__ __forceinline__ Walk walk_of(const DecodeParams& p, int b) {
   w.first = w.start >> 4;
   w.end = (w.len + kQ4Tokens - 1) >> 4;
   w.sb = min((min(p.sinks, w.start) + kQ4Tokens - 1) >> 4, w.first);
-  w.ns = (w.sb + 1) >> 1;
-  w.n = w.ns + ((w.end - w.first + 1) >> 1);
+  w.ns = (w.sb + PER - 1) / PER;
+  w.n = w.ns + (w.end - w.first + PER - 1) / PER;
   return w;
 }
 // Chunk x's first block, and whether it has a second one.
-__device__ __forceinline__ int block_of(const Walk& w, int x) { return x < w.ns ? 2 * x : w.first + 2 * (x - w.ns); }
+template <int PER>
+__device__ __forceinline__ int block_of(const Walk& w, int x) {
+  return x < w.ns ? PER * x : w.first + PER * (x - w.ns);
+}
 __device__ __forceinline__ bool second_of(const Walk& w, int x, int block) { return block + 1 < (x < w.ns ? w.sb : w.end); }
 
-// Where a run stands: chunk x of walk (b, hp), hp = kv head * parts + part.
+// Where a run stands: chunk x of walk (b, hp).
 struct Cursor {
   int b, hp, x;
   Walk w;
 };
 // `by` chunks on, over the ends of walks (those of requests without tokens are empty).
+template <int PER>
 __device__ __forceinline__ void move(const DecodeParams& p, Cursor* c, int by) {
   c->x += by;
   while (c->x >= c->w.n) {
     c->x -= c->w.n;
-    if (++c->hp == p.KH * p.parts) {
+    if (++c->hp == p.walks) {
       c->hp = 0;
       do {
         if (++c->b >= p.B) return;  // past the last walk: not read
-        c->w = walk_of(p, c->b);
+        c->w = walk_of<PER>(p, c->b);
       } while (c->w.n == 0);
     }
   }
@@ -170,14 +187,21 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : a / b;
 }
 
-// NT: groups of 8 query heads a CTA works on.
-template <int NT, int GROUP, int STAGES>
+// NT: groups of 8 query heads a CTA works on.  PAIR: two kv heads of at most 4 query heads each;
+// a tile of 16 rows of the matrix instruction is then 8 tokens of either, and of S^T the two
+// quarters count in which rows and columns are of one kv head: a lane's two values instead of
+// four for the same codes, half of the work between the products (64 requests, 4 query heads for
+// each of 8 kv heads: 139 us without, 124 with).
+template <int NT, int GROUP, int STAGES, bool PAIR>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(const DecodeParams p, unsigned* err) {
   constexpr int H = 8 * NT;
   constexpr int NG = 128 / GROUP;                       // pairs of a token
   constexpr int RUNS = 4 / NG;                          // 32-channel runs of a group
   constexpr uint32_t kBlock = q4_block_bytes(GROUP);
   constexpr uint32_t kStage = 4 * kBlock;               // a chunk's blocks of K, then of V
+  constexpr int PER = PAIR ? 1 : 2;                     // blocks of a chunk, of each kv head
+  constexpr int ROWS = PAIR ? 1 : 2;                    // tokens of a lane in a tile of S^T
+  static_assert(!PAIR || NT == 1, "8 columns");
   constexpr int kTop = 100;                             // P' is scaled by 2^kTop at most
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][STAGES];
@@ -197,11 +221,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   if (threadIdx.x == 0) p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
 
   // The run: chunks [r0, r1) of all walks.  Each thread counts the requests [b0, b1).
-  const int heads = p.KH * p.parts;
+  const int heads = p.walks;
   const int each = (p.B + kThreads - 1) / kThreads;
   const int b0 = min(static_cast<int>(threadIdx.x) * each, p.B), b1 = min(b0 + each, p.B);
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += walk_of(p, b).n;
+  for (int b = b0; b < b1; ++b) mine += walk_of<PER>(p, b).n;
   int64_t upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -227,10 +251,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   const int run = cta < ctas ? static_cast<int>(r1 - r0) : 0;
   if (run > 0 && before * heads <= r0 && r0 < (before + mine) * heads) {
     int64_t x = before;
-    int b = b0, n = walk_of(p, b).n;
+    int b = b0, n = walk_of<PER>(p, b).n;
     while (n == 0 || (x + n) * heads <= r0) {
       x += n;
-      n = walk_of(p, ++b).n;
+      n = walk_of<PER>(p, ++b).n;
     }
     first_b = b;
     first_x = r0 - x * heads;
@@ -248,14 +272,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
 
   Cursor at;  // of the piece in work
   at.b = first_b;
-  at.w = walk_of(p, at.b);
+  at.w = walk_of<PER>(p, at.b);
   at.hp = static_cast<int>(divide(first_x, at.w.n));
   at.x = static_cast<int>(first_x - static_cast<int64_t>(at.hp) * at.w.n);
 
   // this warp's chunks: warp, warp + kWarps, ... of the run
   uint8_t* ring = smem + warp * (STAGES * kStage);
   Cursor ahead = at;  // of the next load
-  if (warp > 0) move(p, &ahead, warp);
+  if (warp > 0) move<PER>(p, &ahead, warp);
   int loads = 0;
   // Loads one behind the other in a walk are kWarps chunks apart: `left` of them, of so many bytes.
   int left = 0;
@@ -264,41 +288,47 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   auto load = [&]() {
     if (warp + loads * kWarps >= run) return;
     if (left == 0) {
-      if (loads > 0) move(p, &ahead, 0);
-      const int g = ahead.hp / p.parts, block = block_of(ahead.w, ahead.x);
-      const int whole = ahead.x < ahead.w.ns ? ahead.w.sb >> 1 : ahead.w.ns + ((ahead.w.end - ahead.w.first) >> 1);
+      if (loads > 0) move<PER>(p, &ahead, 0);
+      const int g = heads_of(p, H, ahead.hp).kv, block = block_of<PER>(ahead.w, ahead.x);
+      const int whole = ahead.x < ahead.w.ns ? ahead.w.sb / PER : ahead.w.ns + (ahead.w.end - ahead.w.first) / PER;
       left = max(1, (whole - ahead.x + kWarps - 1) / kWarps);
-      bytes = ahead.x < whole ? 2 * kBlock : kBlock;
+      bytes = ahead.x < whole ? PER * kBlock : kBlock;
       const int64_t off = static_cast<int64_t>(block) * kBlock;
       kp = p.k + ahead.b * p.k_b + g * p.k_h + off;
       vp = p.v + ahead.b * p.v_b + g * p.v_h + off;
     }
     const int s = loads % STAGES;
     if (lane == 0) {
-      mbar_arrive_expect_tx(&full[warp][s], 2 * bytes);
-      bulk_load_1d(ring + s * kStage, kp, bytes, &full[warp][s]);
-      bulk_load_1d(ring + s * kStage + 2 * kBlock, vp, bytes, &full[warp][s]);
+      uint8_t* dst = ring + s * kStage;
+      mbar_arrive_expect_tx(&full[warp][s], PAIR ? 4 * kBlock : 2 * bytes);
+      bulk_load_1d(dst, kp, bytes, &full[warp][s]);
+      bulk_load_1d(dst + 2 * kBlock, vp, bytes, &full[warp][s]);
+      if (PAIR) {  // the second kv head's
+        bulk_load_1d(dst + kBlock, kp + p.k_h, kBlock, &full[warp][s]);
+        bulk_load_1d(dst + 3 * kBlock, vp + p.v_h, kBlock, &full[warp][s]);
+      }
     }
     ++loads;
     --left;
-    kp += 2 * kWarps * kBlock;
-    vp += 2 * kWarps * kBlock;
+    kp += PER * kWarps * kBlock;
+    vp += PER * kWarps * kBlock;
     ahead.x += kWarps;
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load();
 
-  float* parts = reinterpret_cast<float*>(smem + kWarps * STAGES * kStage);  // [kWarps][min(rep, H)][kRow]
-  const int held = min(p.rep, H);
+  float* parts = reinterpret_cast<float*>(smem + kWarps * STAGES * kStage);  // [kWarps][held][kRow]
+  const int held = PAIR ? 2 * p.rep : min(p.rep, H);
   bool ok = true;
   int done = 0;       // this warp's chunks
   int piece_at = 0;   // the piece's first chunk in the run
   while (piece_at < run) {
     const int left = run - piece_at;
     const int n = min(left, at.w.n - at.x);  // chunks of the piece
-    const int g = at.hp / p.parts, part = at.hp - g * p.parts;
-    const int h0 = g * p.rep + part * H;  // first query head
-    const int nh = min(H, p.rep - part * H);
+    const Heads hs = heads_of(p, H, at.hp);
+    const int h0 = hs.first, nh = hs.n;
+    // the place among them of column h of a tile, or nh: of none
+    auto head_at = [&](int h) { return PAIR ? ((h & 3) < p.rep ? (h >> 2) * p.rep + (h & 3) : nh) : h; };
 
     // q^T operands: for run g and step s of its two, head lane / 4, channels of this lane's
     // word: (2 s, 2 s + 4) less a sixteenth of (2 s + 1, 2 s + 5), and the latter, times a
@@ -309,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     float qsum[NT][NG][2], sl2[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int h = t * 8 + r;
+      const int h = head_at(t * 8 + r);
       float f[4][8], top = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -368,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     }
 
     // chunks [xa, xb) are visible whole
-    const int xa = at.w.ns + ((at.w.start & (kQ4Tokens - 1)) != 0), xb = at.w.ns + ((at.w.len - at.w.first * kQ4Tokens) >> 5);
+    const int xa = at.w.ns + ((at.w.start & (kQ4Tokens - 1)) != 0), xb = at.w.ns + (at.w.len - at.w.first * kQ4Tokens) / (PER * kQ4Tokens);
     const int x_end = at.x + n;
     for (int x = at.x + warp + done * kWarps - piece_at; ok && x < x_end; ++done, x += kWarps) {
       __syncwarp();  // every lane is done with the stage refilled here
@@ -380,32 +410,45 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
       }
       const bool whole = x >= xa && x < xb;
       const uint32_t ks = smem_u32(ring) + s * kStage, vb = ks + 2 * kBlock;
-      // block i of the two: the tokens of this lane's accumulators are its r and r + 8
-      bool see[2][2] = {{true, true}, {true, true}};
+      // Tile i of the two: block i, the tokens of this lane's accumulators its r and r + 8; or
+      // (PAIR) tokens 8 i on of one block of two kv heads, this lane's r of the head of its columns.
+      bool see[2][ROWS];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < ROWS; ++c) see[i][c] = true;
       if (!whole) {
-        const int block = block_of(at.w, x);
-        const bool two = second_of(at.w, x, block);
+        const int block = block_of<PER>(at.w, x);
+        const bool two = PAIR || second_of(at.w, x, block);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int tok = (block + i) * kQ4Tokens + r + 8 * c;
+          for (int c = 0; c < ROWS; ++c) {
+            const int tok = PAIR ? block * kQ4Tokens + 8 * i + r : (block + i) * kQ4Tokens + r + 8 * c;
             see[i][c] = (i == 0 || two) && tok < at.w.len && (tok >= at.w.start || tok < p.sinks);
           }
       }
+      // rows r and r + 8 of tile i, and the pairs of this lane's tokens, in a block of K or of V
+      auto row_at = [&](uint32_t base, int i, int c) {
+        return base + (PAIR ? c * kBlock + (8 * i + r) * 64 : i * kBlock + (r + 8 * c) * 64);
+      };
+      auto pairs_at = [&](uint32_t base, int i, int c) {
+        return base + kQ4Codes + (PAIR ? (c4 >> 1) * kBlock + (8 * i + r) * NG * 4 : i * kBlock + (r + 8 * c) * NG * 4);
+      };
 
-      float sc[2][NT][4];
+      float sc[2][NT][2 * ROWS];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t kb = ks + i * kBlock;
-        const uint32_t row = kb + r * 64 + ((c4 ^ ((r >> 1) & 3)) << 4);  // chunk lane % 4 of tokens r and r + 8
-        const uint4 k0 = ld_shared_v4(row), k1 = ld_shared_v4(row + 512);
+        const uint32_t chunk = (c4 ^ ((r >> 1) & 3)) << 4;  // chunk lane % 4 of tokens r (+ 8)
+        const uint4 k0 = ld_shared_v4(row_at(ks, i, 0) + chunk), k1 = ld_shared_v4(row_at(ks, i, 1) + chunk);
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-        uint32_t p0[NG], p1[NG];
-        ld_shared_n<NG>(kb + kQ4Codes + r * NG * 4, p0);
-        ld_shared_n<NG>(kb + kQ4Codes + (r + 8) * NG * 4, p1);
+        uint32_t pr[ROWS][NG];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sc[i][t][0] = sc[i][t][1] = sc[i][t][2] = sc[i][t][3] = 0.f;
+        for (int c = 0; c < ROWS; ++c) ld_shared_n<NG>(pairs_at(ks, i, c), pr[c]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int c = 0; c < 2 * ROWS; ++c) sc[i][t][c] = 0.f;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
           float acc[NT][4];
@@ -420,38 +463,41 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
 #pragma unroll
               for (int t = 0; t < NT; ++t) mma_f16(acc[t], a, qf[t][k][st][0], qf[t][k][st][1]);
             }
-          const float s0 = step_of(p0[j]), s1 = step_of(p1[j]);
-          const float z0 = low_of(p0[j]), z1 = low_of(p1[j]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            sc[i][t][0] = fmaf(s0, acc[t][0], fmaf(z0, qsum[t][j][0], sc[i][t][0]));
-            sc[i][t][1] = fmaf(s0, acc[t][1], fmaf(z0, qsum[t][j][1], sc[i][t][1]));
-            sc[i][t][2] = fmaf(s1, acc[t][2], fmaf(z1, qsum[t][j][0], sc[i][t][2]));
-            sc[i][t][3] = fmaf(s1, acc[t][3], fmaf(z1, qsum[t][j][1], sc[i][t][3]));
-          }
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < 2 * ROWS; ++c) {
+              const float dot = PAIR ? (c4 < 2 ? acc[t][c] : acc[t][c + 2]) : acc[t][c];
+              sc[i][t][c] = fmaf(step_of(pr[c >> 1][j]), dot, fmaf(low_of(pr[c >> 1][j]), qsum[t][j][c & 1], sc[i][t][c]));
+            }
         }
       }
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (!see[i][0]) sc[i][t][0] = sc[i][t][1] = -INFINITY;
-            if (!see[i][1]) sc[i][t][2] = sc[i][t][3] = -INFINITY;
-          }
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < 2 * ROWS; ++c)
+              if (!see[i][c >> 1]) sc[i][t][c] = -INFINITY;
       }
+      // the highest of this lane's scores of head c
+      auto most = [&](int t, int c) {
+        return PAIR ? fmaxf(sc[0][t][c], sc[1][t][c])
+                    : fmaxf(fmax3(sc[0][t][c], sc[0][t][(c + 2) % (2 * ROWS)], sc[1][t][c]), sc[1][t][(c + 2) % (2 * ROWS)]);
+      };
       bool grow = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          grow |= fmaxf(fmax3(sc[0][t][c], sc[0][t][c + 2], sc[1][t][c]), sc[1][t][c + 2]) * sl2[t][c] > m[t][c] + 8.f;
+          grow |= most(t, c) * sl2[t][c] > m[t][c] + 8.f;
       if (__any_sync(kFull, grow)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(fmax3(sc[0][t][c], sc[0][t][c + 2], sc[1][t][c]), sc[1][t][c + 2]) * sl2[t][c];
+            float mx = most(t, c) * sl2[t][c];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, d));
             mx = fmaxf(mx, m[t][c]);
@@ -475,74 +521,72 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
               }
           }
       }
-      float e[2][NT][4];
+      float e[2][NT][2 * ROWS];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) e[i][t][c] = exp2_approx(fmaf(sc[i][t][c], sl2[t][c & 1], nm[t][c & 1]));
-          l[t][0] += e[i][t][0] + e[i][t][2];
-          l[t][1] += e[i][t][1] + e[i][t][3];
-        }
+          for (int c = 0; c < 2 * ROWS; ++c) {
+            e[i][t][c] = exp2_approx(fmaf(sc[i][t][c], sl2[t][c & 1], nm[t][c & 1]));
+            l[t][c & 1] += e[i][t][c];
+          }
       // P' = p step 2^vs, which meets the codes as fp16, the tensor core's operand type
-      uint32_t pp[2][NT][NG][2];
+      uint32_t pp[2][NT][NG][ROWS];
       float top = 0.f;
+      auto load_pairs = [&](int i, uint32_t (&pr)[ROWS][NG]) {
+#pragma unroll
+        for (int c = 0; c < ROWS; ++c) {
+          ld_shared_n<NG>(pairs_at(vb, i, c), pr[c]);
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < NG; ++j)  // whatever is there must not meet its weight of zero
+              if (!see[i][c]) pr[c][j] = 0u;
+          }
+        }
+      };
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t p0[NG], p1[NG];
-        ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + r * NG * 4, p0);
-        ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + (r + 8) * NG * 4, p1);
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {  // whatever is there must not meet its weight of zero
-            if (!see[i][0]) p0[j] = 0u;
-            if (!see[i][1]) p1[j] = 0u;
-          }
-        }
+        uint32_t pr[ROWS][NG];
+        load_pairs(i, pr);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float v0 = power(vs[t][0]), v1 = power(vs[t][1]);
-          const float ev[4] = {e[i][t][0] * v0, e[i][t][1] * v1, e[i][t][2] * v0, e[i][t][3] * v1};
+          const float v[2] = {power(vs[t][0]), power(vs[t][1])};
 #pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            const float s0 = step_of(p0[j]), s1 = step_of(p1[j]), z0 = low_of(p0[j]), z1 = low_of(p1[j]);
-            lows[t][j][0] = fmaf(e[i][t][0], z0, fmaf(e[i][t][2], z1, lows[t][j][0]));
-            lows[t][j][1] = fmaf(e[i][t][1], z0, fmaf(e[i][t][3], z1, lows[t][j][1]));
-            const float pv[4] = {ev[0] * s0, ev[1] * s0, ev[2] * s1, ev[3] * s1};
-            top = fmax3(fmax3(top, pv[0], pv[1]), pv[2], pv[3]);
-            pp[i][t][j][0] = pack_f16x2(pv[0], pv[1]);
-            pp[i][t][j][1] = pack_f16x2(pv[2], pv[3]);
-          }
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int c = 0; c < ROWS; ++c) {
+              const float step = step_of(pr[c][j]), low = low_of(pr[c][j]);
+              const float p0 = e[i][t][2 * c] * v[0] * step, p1 = e[i][t][2 * c + 1] * v[1] * step;
+              lows[t][j][0] = fmaf(e[i][t][2 * c], low, lows[t][j][0]);
+              lows[t][j][1] = fmaf(e[i][t][2 * c + 1], low, lows[t][j][1]);
+              top = fmax3(top, p0, p1);
+              pp[i][t][j][c] = pack_f16x2(p0, p1);
+            }
         }
       }
       if (__any_sync(kFull, top > 32768.f)) {
-        uint32_t p0[2][NG], p1[2][NG];
+        uint32_t pr[2][ROWS][NG];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + r * NG * 4, p0[i]);
-          ld_shared_n<NG>(vb + i * kBlock + kQ4Codes + (r + 8) * NG * 4, p1[i]);
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            if (!see[i][0]) p0[i][j] = 0u;
-            if (!see[i][1]) p1[i][j] = 0u;
-          }
-        }
+        for (int i = 0; i < 2; ++i) load_pairs(i, pr[i]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+          float v[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float most = 0.f;
+            float high = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int j = 0; j < NG; ++j)
-                most = fmax3(most, e[i][t][c] * step_of(p0[i][j]), e[i][t][c + 2] * step_of(p1[i][j]));
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, d));
-            const int to = min(vs[t][c], 254 - exponent(most, 127 - kTop, 253));
+                for (int d = 0; d < ROWS; ++d) high = fmaxf(high, e[i][t][2 * d + c] * step_of(pr[i][d][j]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) high = fmaxf(high, __shfl_xor_sync(kFull, high, d));
+            const int to = min(vs[t][c], 254 - exponent(high, 127 - kTop, 253));
             const float f = exp2_approx(static_cast<float>(to - vs[t][c]));
             vs[t][c] = to;
+            v[c] = power(to);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -551,24 +595,25 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
                 o[t][k][st][c + 2] *= f;
               }
           }
-          const float v0 = power(vs[t][0]), v1 = power(vs[t][1]);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < NG; ++j) {
-              const float s0 = step_of(p0[i][j]), s1 = step_of(p1[i][j]);
-              pp[i][t][j][0] = pack_f16x2(e[i][t][0] * v0 * s0, e[i][t][1] * v1 * s0);
-              pp[i][t][j][1] = pack_f16x2(e[i][t][2] * v0 * s1, e[i][t][3] * v1 * s1);
-            }
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+              for (int c = 0; c < ROWS; ++c) {
+                const float step = step_of(pr[i][c][j]);
+                pp[i][t][j][c] = pack_f16x2(e[i][t][2 * c] * v[0] * step, e[i][t][2 * c + 1] * v[1] * step);
+              }
         }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        // tokens 2 (lane % 4) + {0, 1} and 8 on: their chunk r / 2, of which this lane takes half
-        // of each word: channels 32 run + 4 r + {0 .. 3}
-        const uint32_t col = vb + i * kBlock + c4 * 128 + (((r >> 1) ^ c4) << 4);
-        const uint4 va = ld_shared_v4(col), vc = ld_shared_v4(col + 64), vd = ld_shared_v4(col + 512),
-                    ve = ld_shared_v4(col + 576);
+        // tokens 2 (lane % 4) + {0, 1} of a tile's first 8 rows and of the others: their chunk
+        // r / 2, of which this lane takes half of each word: channels 32 run + 4 r + {0 .. 3}
+        const uint32_t in = c4 * 128 + (((r >> 1) ^ c4) << 4);
+        const uint32_t col = vb + in + (PAIR ? i * 512 : i * kBlock), other = col + (PAIR ? kBlock : 512);
+        const uint4 va = ld_shared_v4(col), vc = ld_shared_v4(col + 64), vd = ld_shared_v4(other),
+                    ve = ld_shared_v4(other + 64);
         const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vc.x, vc.y, vc.z, vc.w},
                        wc[4] = {vd.x, vd.y, vd.z, vd.w}, wd[4] = {ve.x, ve.y, ve.z, ve.w};
         const uint32_t pick = (r & 1) ? 0x7632u : 0x5410u;
@@ -577,8 +622,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
           uint32_t pb[NT][2];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            pb[t][0] = transpose8x8(pp[i][t][j][0]);
-            pb[t][1] = transpose8x8(pp[i][t][j][1]);
+            // (PAIR: the rows of the other kv head weigh nothing)
+            pb[t][0] = transpose8x8(PAIR && c4 >= 2 ? 0u : pp[i][t][j][0]);
+            pb[t][1] = transpose8x8(PAIR && c4 < 2 ? 0u : pp[i][t][j][ROWS - 1]);
           }
 #pragma unroll
           for (int k = j * RUNS; k < (j + 1) * RUNS; ++k) {
@@ -600,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int h = t * 8 + 2 * c4 + c;
+        const int h = head_at(t * 8 + 2 * c4 + c);
         float sum = l[t][c];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(kFull, sum, d);
@@ -662,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     if (cut && threadIdx.x == 0) p.pieces[slot] = make_int4(at.b * heads + at.hp, 0, n, at.w.n);
     __syncthreads();  // parts are free
     piece_at += n;
-    if (piece_at < run) move(p, &at, n);
+    if (piece_at < run) move<PER>(p, &at, n);
   }
   if (!ok && lane == 0) {  // no copy may still be writing shared memory when the CTA exits
     for (int i = max(0, loads - STAGES); i < loads; ++i)
@@ -689,9 +735,9 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
   const int4 w = p.pieces[2 * x + 1];
   int4 next = p.pieces[2 * min(x + 1 + lane, ctas - 1)];
   float mm = share(lane)[kD];
-  const int heads = p.KH * p.parts;
-  const int b = w.x / heads, hp = w.x - b * heads, g = hp / p.parts, part = hp - g * p.parts;
-  if (w.z == 0 || h >= min(H, p.rep - part * H)) return;
+  const int b = w.x / p.walks;
+  const Heads hs = heads_of(p, H, w.x - b * p.walks);
+  if (w.z == 0 || h >= hs.n) return;
   int count = 1;
   for (;;) {
     const unsigned others = ~__ballot_sync(kFull, x + count + lane < ctas && next.z > 0 && next.x == w.x);
@@ -724,18 +770,18 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
       l2 += parts[i][kD + 1];
       o2 += parts[i][d];
     }
-    p.out[(static_cast<int64_t>(b) * p.QH + g * p.rep + part * H + h) * kD + d] = __float2bfloat16_rn(o2 / l2);
+    p.out[(static_cast<int64_t>(b) * p.QH + hs.first + h) * kD + d] = __float2bfloat16_rn(o2 / l2);
   }
 }
 
-template <int NT, int GROUP>
+template <int NT, int GROUP, bool PAIR>
 kda_status launch_decode(const DecodeParams& p, int ctas, cudaStream_t st) {
   // rings of the depth that leaves two CTAs an SM (one where a group has more than 8 heads)
   constexpr int kStages = NT == 1 ? 2 : 4;
   constexpr int H = 8 * NT;
   constexpr size_t kMost = kWarps * (kStages * 4 * q4_block_bytes(GROUP) + H * kRow * 4);
   static_assert(kMost <= (NT == 1 ? 113 : 226) * 1024, "shared memory budget");
-  auto* kernel = q4_decode_kernel<NT, GROUP, kStages>;
+  auto* kernel = q4_decode_kernel<NT, GROUP, kStages, PAIR>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -745,13 +791,18 @@ kda_status launch_decode(const DecodeParams& p, int ctas, cudaStream_t st) {
       return launch_status("gqa_decode_q4: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  const size_t smem = kWarps * (kStages * 4 * q4_block_bytes(GROUP) + (p.rep < H ? p.rep : H) * kRow * 4);
+  const int held = PAIR ? 2 * p.rep : p.rep < H ? p.rep : H;  // query heads of a walk
+  const size_t smem = kWarps * (kStages * 4 * q4_block_bytes(GROUP) + held * kRow * 4);
   const kda_status s = launch_after("gqa_decode_q4", kernel, dim3(static_cast<unsigned>(ctas)), kThreads, smem, st, p,
                                     kda_err_ptr_q4_decode());
   if (s != KDA_OK) return s;
-  return launch_after("gqa_decode_q4: join", q4_join_kernel<H>,
-                      dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(p.rep < H ? p.rep : H)), kThreads, 0, st, p,
-                      ctas);
+  return launch_after("gqa_decode_q4: join", q4_join_kernel<H>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(held)),
+                      kThreads, 0, st, p, ctas);
+}
+template <int GROUP>
+kda_status launch_group(const DecodeParams& p, int ctas, cudaStream_t st) {
+  if (p.rep > 8) return launch_decode<2, GROUP, false>(p, ctas, st);
+  return p.parts == 0 ? launch_decode<1, GROUP, true>(p, ctas, st) : launch_decode<1, GROUP, false>(p, ctas, st);
 }
 
 int decode_ctas(int64_t rep) { return num_sms() * (rep > 8 ? 1 : 2); }
@@ -812,21 +863,22 @@ extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, cons
   p.QH = static_cast<int>(QH);
   p.KH = static_cast<int>(KH);
   p.rep = static_cast<int>(QH / KH);
-  p.parts = p.rep > 8 ? (p.rep + 15) / 16 : 1;
+  // Two kv heads together take less work for each token, and more of it at the end of each walk
+  // and share of one (4 query heads of 8 kv heads, us without and with: 1 request of 8,192 tokens
+  // 10.7, 15.0; 16 40.6, 41.1; 32 69.2, 67.1; 64 126, 119; of 1,024 tokens 32 20.7, 21.1; 64
+  // 31.0, 28.3; 2 of 32,768 24.5, 25.3; 8 66.4, 65.9; 32 229, 219).  Lengths are not known
+  // here, the room for them is.
+  const bool pair = p.rep <= 4 && KH % 2 == 0 && (B * KH >= 512 || B * KH * T >= (1ll << 21));
+  p.parts = p.rep > 8 ? (p.rep + 15) / 16 : pair ? 0 : 1;
+  p.walks = static_cast<int>(p.parts == 0 ? KH / 2 : KH * p.parts);
   p.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(kD)));
   const int ctas = decode_ctas(p.rep);
   p.pieces = static_cast<int4*>(workspace);
   p.shares = reinterpret_cast<float*>(p.pieces + 2 * ctas);
   p.length_err = kda_err_ptr_q4_decode_length();
   // the longest run, and the number of walks
-  KDA_CHECK_SUPPORTED(B * KH * p.parts < (1ll << 31) && B * KH * p.parts < (1ll << 31) * ctas / blocks,
+  KDA_CHECK_SUPPORTED(B * p.walks < (1ll << 31) && B * p.walks < (1ll << 30) * ctas / blocks,
                       "%s: too large (B=%lld KH=%lld blocks=%lld)", op, (long long)B, (long long)KH, (long long)blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p.rep > 8)
-    return group == 32   ? launch_decode<2, 32>(p, ctas, st)
-           : group == 64 ? launch_decode<2, 64>(p, ctas, st)
-                         : launch_decode<2, 128>(p, ctas, st);
-  return group == 32   ? launch_decode<1, 32>(p, ctas, st)
-         : group == 64 ? launch_decode<1, 64>(p, ctas, st)
-                       : launch_decode<1, 128>(p, ctas, st);
+  return group == 32 ? launch_group<32>(p, ctas, st) : group == 64 ? launch_group<64>(p, ctas, st) : launch_group<128>(p, ctas, st);
 }

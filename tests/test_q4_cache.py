@@ -280,6 +280,9 @@ DECODE_CASES = [
     (1, 320, 32, 8, None, 0, [5111]), (2, 200, 20, 4, 1, 0, [3200, 1600]), (1, 600, 8, 1, None, 0, [9600]),
     (70, 4, 4, 2, None, 0, [0] * 33 + [64, 1, 33] + [0] * 33 + [5]), (1, 300, 9, 1, None, 0, [4800]),
     (300, 1, 2, 1, None, 0, [b % 17 for b in range(300)]), (1, 40, 5, 1, 17, 15, [640]),
+    # enough requests for two kv heads to be taken together, with 1 to 4 query heads for each
+    (256, 2, 8, 2, None, 0, [b % 33 for b in range(256)]), (130, 3, 12, 4, 9, 3, [(7 * b) % 49 for b in range(130)]),
+    (64, 5, 8, 8, None, 0, [80 - b for b in range(64)]), (86, 9, 12, 6, 100, 20, [144 - b for b in range(86)]),
 ]
 
 
