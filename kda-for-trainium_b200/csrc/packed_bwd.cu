@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       bool ok = true;
       int qs = 0, dos = 0, vs = 0, ks = 0;  // loads issued
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      for (int r = 0, u = blockIdx.x; u < units && ok; u = unit_of_round(++r)) {
         const Unit c = dq_unit(p, u);
         const int g = c.h / p.rep;
         for (int j = 0; j < c.n && ok; ++j, ++n) {
@@ -730,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool one = elect_one();
     const uint32_t base = smem_u32(smem);
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
+    for (int u = blockIdx.x; u < units && ok; u = unit_of_round(++uc)) {
       const Unit c = dq_unit(p, u);
       for (int j = 0; j < c.n; ++j, ++n) {
         const uint32_t nb = static_cast<uint32_t>(n) & 1u;
@@ -777,14 +777,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++sn;
       if (++sj == s_unit.n) {
         sj = 0;
-        ++sc;
-        su += gridDim.x;
+        su = unit_of_round(++sc);
         if (su < units) s_unit = dq_unit(p, su);
       }
       return true;
     };
     ok = issue_s() && issue_s();
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
+    for (int u = blockIdx.x; u < units && ok; u = unit_of_round(++uc)) {
       const Unit c = dq_unit(p, u);
       for (int j = 0; j < c.n && ok; ++j, ++n) {
         // dQ += dS(n) K (the first of a unit once the last unit's dQ is read)
@@ -844,12 +843,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       nd = __ldcg(p.ndi + at);
     }
     Unit last = {};  // the unit before this one
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++uc) {
+    for (int u = blockIdx.x; u < units && ok; u = unit_of_round(++uc)) {
       const Unit c = dq_unit(p, u);
       const int qpos = c.b.z * kBlk + r;
       const float2 nlse = make_float2(nl, nl), ndi = make_float2(nd, nd);
-      if (u + static_cast<int>(gridDim.x) < units) {
-        at = row_at(dq_unit(p, u + gridDim.x));
+      const int next = unit_of_round(uc + 1);
+      if (next < units) {
+        at = row_at(dq_unit(p, next));
         nl = __ldcg(p.nlse + at);
         nd = __ldcg(p.ndi + at);
       }

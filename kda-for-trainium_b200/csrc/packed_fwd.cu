@@ -9,7 +9,7 @@
 // heads of a group where its heads are even in number, else two consecutive blocks of a
 // head.  (Heads first because both tiles then have rows at every block: a short sequence
 // has one block only.)  Units come from the plan's tables, those with the most keys
-// first; one persistent CTA per SM takes every gridDim-th.  A unit's K and V blocks pass
+// first; the persistent CTAs, one per SM, take them in turn.  A unit's K and V blocks pass
 // through rings of 3 and 2 tiles and serve both tiles.
 //
 // A tile of a sequence's last block also holds rows of whatever lies behind it.  Such
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int ks = 0, slot = 0, lap = 0;  // loads of K issued; slot of the next, and its use of that slot
       int qs[2] = {0, 0};
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      for (int k = 0, u = blockIdx.x; u < units && ok; u = unit_of_round(++k)) {
         const Unit c = unit_at(p, u);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     int vs = 0, cleared = 0;       // loads; of those, to v_landed
     int direct0 = -1, direct1 = -1;  // a slot's last load if it was not: its phase of v_full
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int k = 0, u = blockIdx.x; u < units && ok; u = unit_of_round(++k)) {
       const Unit c = unit_at(p, u);
       const int g = c.head[0] / p.rep;
       for (int j = 0; j < c.nb && ok; ++j, ++vs) {
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t np[2] = {0u, 0u};   // a tile's P V so far
     uint32_t un[2] = {0u, 0u};   // and its units
     bool ok = true, any = false;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int k = 0, u = blockIdx.x; u < units && ok; u = unit_of_round(++k)) {
       const Unit c = unit_at(p, u);
       for (int j = 0; j < c.nb && ok; ++j) {
         const uint32_t tile = base + (is_s ? Smem::kK : Smem::kV) + slot * kTile;
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     uint32_t n = 0;   // blocks seen so far
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int k = 0, u = blockIdx.x; u < units && ok; u = unit_of_round(++k)) {
       const Unit c = unit_at(p, u);
       const int to = t == 0 ? c.to[0] : c.to[1], block = t == 0 ? c.block[0] : c.block[1];
       const int head = t == 0 ? c.head[0] : c.head[1];
