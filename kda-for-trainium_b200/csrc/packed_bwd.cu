@@ -151,13 +151,13 @@ __device__ __forceinline__ Piece piece_after(const BwdParams& p, const Piece& c,
   d.n = min(most, d.walk);
   return d;
 }
-// Rows from `rows` on of a tile become zeros, by the 512 threads of the row warps.
+// Rows from `rows` on of a tile become zeros, by the 512 threads of the row warps, which
+// fence them to the tensor core's reads afterwards.
 __device__ __forceinline__ void clear_rows(uint32_t tile, int rows, int thread) {
   for (int i = rows * 8 + thread; i < kBlk * 8; i += 32 * kRowWarps) {
     st_shared_v4(tile + i * 16, 0u, 0u, 0u, 0u);
     st_shared_v4(tile + kHalf + i * 16, 0u, 0u, 0u, 0u);
   }
-  fence_proxy_async_smem();
 }
 
 // ---------------------------------------------------------------- dK and dV
@@ -173,9 +173,14 @@ __device__ __forceinline__ void clear_rows(uint32_t tile, int rows, int thread) 
 // S^T(n) column by column.  S^T(n+1) is issued as soon as the row warps have copied
 // dP^T(n), dV(n) and dK(n) as soon as they have written P^T(n) and dS^T(n), and
 // dP^T(n+1) once both are done with the region it overwrites.
-// A step takes about 2,900 cycles, the row warps' chain: wait, TMEM load, 16,384
+// A step takes about 3,050 cycles, the row warps' chain: wait, TMEM load, 16,384
 // exponentials (1,024 cycles of their pipe), store, wait, load, store.  The tensor
-// core works 2,048 of them.
+// core works 2,048 of them.  A walk costs some 8,000 cycles more: 3,000 to 4,000 until its
+// results have left (stores and the exchanges before them), the first loads of K, V and dO
+// behind the last products.  133 us at S4096 of 16 heads, 103 at 12 sequences of 8,192 tokens.
+// With dS^T through shared memory, which lets dP^T run a step ahead, a call is 6 % slower
+// (a product with both operands there needs all of its bandwidth); with the next walk's K
+// loaded a walk ahead, or results out before the first dS, it is no faster.
 // TMEM columns: regions [0,128), [128,256), dV [256,384), dK [384,512).
 __global__ void __launch_bounds__(kThreads, 1)
     packed_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -508,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           clear_rows(smem_u32(smem) + kQ + par * kTile, own, threadIdx.x - 128);
           clear_rows(smem_u32(smem) + kDO + par * kTile, own, threadIdx.x - 128);
+          fence_proxy_async_smem();
         }
         tmem_st_wait();
         tc_fence_before();
@@ -564,8 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // dQ's operand there.  dP(n + 1) is issued as soon as the rows have copied step n,
 // S(n + 2) (two regions) when dQ(n) has read dS(n); units follow one another
 // without a gap.
-// A step inside a unit takes about 1,950 cycles, the row warps' chain again (1,024 of
-// them the exponentials' pipe); the tensor core works 1,536.
+// A step takes about 2,500 cycles over a launch, the row warps' chain again (1,024 of
+// them the exponentials' pipe); the tensor core works 1,536.  96 us at S4096 of 16 heads.
 // TMEM columns: S [0,128) and [256,384), dP [128,256), dQ [384,512).
 struct Unit {
   Block b;
@@ -880,7 +886,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           pack16(e, w);
           tmem_st_32x32b_x16(col + par * 256, w);
           // S(n) has read K
-          if ((j + 1) * kBlk > c.b.y) clear_rows(smem_u32(smem) + kK + (n % 3) * kTile, c.b.y - j * kBlk, threadIdx.x - 128);
+          if ((j + 1) * kBlk > c.b.y) {
+            clear_rows(smem_u32(smem) + kK + (n % 3) * kTile, c.b.y - j * kBlk, threadIdx.x - 128);
+            fence_proxy_async_smem();
+          }
           tmem_st_wait();
           tc_fence_before();
         }

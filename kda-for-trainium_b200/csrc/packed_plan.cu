@@ -3,7 +3,7 @@
 // and backward).
 //
 // One CTA.  Bound by latency: a scan over the sequences, a binary search for each block's
-// sequence and a counting sort by the block's place, 4.5 us for 24 sequences of 16,384
+// sequence and a counting sort by the block's place, 3.7 us for 24 sequences of 16,384
 // tokens.  The tables hold the same values every time; only the order of blocks at the
 // same place in `sorted` and `pairs` may differ, which moves work between CTAs and changes
 // no result.
