@@ -29,12 +29,15 @@
 // The running maximum moves only when a score exceeds it by 2^8, which fp32 sums and bf16
 // weights hold exactly as well; so a block usually needs no exchange between lanes.
 //
-// The blocks of all (request, kv head) walks, one behind the other, are cut into equal runs,
-// one for each CTA (lengths are ragged and known on the device only); a run's blocks go to the
-// CTA's warps in turn, each through a ring of bulk copies of its own that runs on across the
-// ends of walks.  Where a walk ends, or the run does, the warps join through shared memory:
-// a whole walk's output leaves, a cut one's share goes to the workspace, and a second launch
-// joins the shares in the order of the walk: one fixed order of summation.
+// A walk is a request's blocks of a kv head.  Short ones: a cluster of 1 to 8 CTAs for each; the
+// blocks go to their warps in turn, each through a ring of bulk copies of its own, and the
+// warps join through shared memory, the CTAs through the cluster's: one launch.
+// Long ones: the walks, one behind the other, are cut into equal runs, one for each CTA
+// (lengths are ragged and known on the device only); a run's blocks go to the CTA's warps in
+// turn, the rings run on across the ends of walks.  Where a walk ends, or the run does, the
+// warps join: a whole walk's output leaves, a cut one's share goes to the workspace, and a
+// second launch joins the shares in the order of the walk.  The order of summation is fixed
+// in both.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -81,8 +84,8 @@ __device__ __forceinline__ Heads heads_of(const DecodeParams& p, int most, int h
   return {g, g * p.rep + part * most, min(most, p.rep - part * most)};
 }
 
-// A request's visible tokens as chunks of PER blocks of each of the walk's kv heads: `ns` over blocks [0, sb) (sinks), then
-// those over [first, end).
+// A request's visible tokens as chunks of PER blocks of each of the walk's kv heads: `ns` over
+// blocks [0, sb) (sinks), then those over [first, end).
 struct Walk {
   int n, ns, sb, first, end;
   int len, start;
@@ -143,6 +146,19 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
@@ -192,7 +208,8 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
 // quarters count in which rows and columns are of one kv head: a lane's two values instead of
 // four for the same codes, half of the work between the products (64 requests, 4 query heads for
 // each of 8 kv heads: 139 us without, 124 with).
-template <int NT, int GROUP, int STAGES, bool PAIR>
+// CLUSTER: no runs; the CTAs of a cluster share one walk; grid (cluster size, walks, B).
+template <int NT, int GROUP, int STAGES, bool PAIR, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(const DecodeParams p, unsigned* err) {
   constexpr int H = 8 * NT;
   constexpr int NG = 128 / GROUP;                       // pairs of a token
@@ -201,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   constexpr uint32_t kStage = 4 * kBlock;               // a chunk's blocks of K, then of V
   constexpr int PER = PAIR ? 1 : 2;                     // blocks of a chunk, of each kv head
   constexpr int ROWS = PAIR ? 1 : 2;                    // tokens of a lane in a tile of S^T
-  static_assert(!PAIR || NT == 1, "8 columns");
+  static_assert(!PAIR || (NT == 1 && !CLUSTER), "8 columns, runs");
   constexpr int kTop = 100;                             // P' is scaled by 2^kTop at most
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][STAGES];
@@ -218,80 +235,101 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   }
   pdl_trigger();
   pdl_wait();
-  if (threadIdx.x == 0) p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
-
-  // The run: chunks [r0, r1) of all walks.  Each thread counts the requests [b0, b1).
-  const int heads = p.walks;
-  const int each = (p.B + kThreads - 1) / kThreads;
-  const int b0 = min(static_cast<int>(threadIdx.x) * each, p.B), b1 = min(b0 + each, p.B);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += walk_of<PER>(p, b).n;
-  int64_t upto = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t o = __shfl_up_sync(kFull, upto, d);
-    if (lane >= d) upto += o;
-  }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  int64_t before = upto - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += sums[w];
-    total += sums[w];
-  }
-  total *= heads;
-  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total / kLeast > 0 ? total / kLeast : 1));
-  const int cta = static_cast<int>(blockIdx.x);
-  // equal runs: [total c / ctas, total (c + 1) / ctas)
-  const int64_t each_run = divide(total, ctas);
-  const unsigned longer = static_cast<unsigned>(total - each_run * ctas), n_ctas = static_cast<unsigned>(ctas);
-  const int64_t r0 = cta * each_run + longer * static_cast<unsigned>(cta) / n_ctas;
-  const int64_t r1 = (cta + 1) * each_run + longer * static_cast<unsigned>(cta + 1) / n_ctas;
-  const int run = cta < ctas ? static_cast<int>(r1 - r0) : 0;
-  if (run > 0 && before * heads <= r0 && r0 < (before + mine) * heads) {
-    int64_t x = before;
-    int b = b0, n = walk_of<PER>(p, b).n;
-    while (n == 0 || (x + n) * heads <= r0) {
-      x += n;
-      n = walk_of<PER>(p, ++b).n;
-    }
-    first_b = b;
-    first_x = r0 - x * heads;
-  }
-  __syncthreads();
-  // outputs of requests without tokens, and lengths past the cache
-  for (int b = cta; b < p.B; b += gridDim.x) {
-    const int n = __ldg(p.lengths + b);
-    if (threadIdx.x == 0 && n > p.cache_len) atomicOr(p.length_err, static_cast<unsigned>(kErrRange));
-    if (n <= 0)
-      for (int i = threadIdx.x; i < p.QH * (kD / 8); i += kThreads)
-        reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(b) * p.QH * kD)[i] = make_uint4(0u, 0u, 0u, 0u);
-  }
-  if (run == 0) return;
 
   Cursor at;  // of the piece in work
-  at.b = first_b;
-  at.w = walk_of<PER>(p, at.b);
-  at.hp = static_cast<int>(divide(first_x, at.w.n));
-  at.x = static_cast<int>(first_x - static_cast<int64_t>(at.hp) * at.w.n);
+  int run, cta = 0, rank = 0, size = 1;
+  if constexpr (CLUSTER) {
+    rank = static_cast<int>(cluster_ctarank());
+    size = static_cast<int>(gridDim.x);
+    at.b = blockIdx.z;
+    at.hp = blockIdx.y;
+    at.x = 0;
+    at.w = walk_of<PER>(p, at.b);
+    run = at.w.n;
+    if (threadIdx.x == 0 && rank == 0 && at.hp == 0 && __ldg(p.lengths + at.b) > p.cache_len)
+      atomicOr(p.length_err, static_cast<unsigned>(kErrRange));
+    if (run == 0) {  // no tokens
+      const Heads hs = heads_of(p, H, at.hp);
+      uint4* out = reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(at.b) * p.QH + hs.first) * kD);
+      if (rank == 0)
+        for (int i = threadIdx.x; i < hs.n * (kD / 8); i += kThreads) out[i] = make_uint4(0u, 0u, 0u, 0u);
+      return;
+    }
+  } else {
+    if (threadIdx.x == 0) p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
+    // The run: chunks [r0, r1) of all walks.  Each thread counts the requests [b0, b1).
+    const int heads = p.walks;
+    const int each = (p.B + kThreads - 1) / kThreads;
+    const int b0 = min(static_cast<int>(threadIdx.x) * each, p.B), b1 = min(b0 + each, p.B);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += walk_of<PER>(p, b).n;
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(kFull, upto, d);
+      if (lane >= d) upto += o;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int64_t before = upto - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sums[w];
+      total += sums[w];
+    }
+    total *= heads;
+    const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total / kLeast > 0 ? total / kLeast : 1));
+    cta = static_cast<int>(blockIdx.x);
+    // equal runs: [total c / ctas, total (c + 1) / ctas)
+    const int64_t each_run = divide(total, ctas);
+    const unsigned longer = static_cast<unsigned>(total - each_run * ctas), n_ctas = static_cast<unsigned>(ctas);
+    const int64_t r0 = cta * each_run + longer * static_cast<unsigned>(cta) / n_ctas;
+    const int64_t r1 = (cta + 1) * each_run + longer * static_cast<unsigned>(cta + 1) / n_ctas;
+    run = cta < ctas ? static_cast<int>(r1 - r0) : 0;
+    if (run > 0 && before * heads <= r0 && r0 < (before + mine) * heads) {
+      int64_t x = before;
+      int b = b0, n = walk_of<PER>(p, b).n;
+      while (n == 0 || (x + n) * heads <= r0) {
+        x += n;
+        n = walk_of<PER>(p, ++b).n;
+      }
+      first_b = b;
+      first_x = r0 - x * heads;
+    }
+    __syncthreads();
+    // outputs of requests without tokens, and lengths past the cache
+    for (int b = cta; b < p.B; b += gridDim.x) {
+      const int n = __ldg(p.lengths + b);
+      if (threadIdx.x == 0 && n > p.cache_len) atomicOr(p.length_err, static_cast<unsigned>(kErrRange));
+      if (n <= 0)
+        for (int i = threadIdx.x; i < p.QH * (kD / 8); i += kThreads)
+          reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(b) * p.QH * kD)[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (run == 0) return;
+    at.b = first_b;
+    at.w = walk_of<PER>(p, at.b);
+    at.hp = static_cast<int>(divide(first_x, at.w.n));
+    at.x = static_cast<int>(first_x - static_cast<int64_t>(at.hp) * at.w.n);
+  }
 
-  // this warp's chunks: warp, warp + kWarps, ... of the run
+  // this warp's chunks: first, first + stride, ... of the run
+  const int first = rank * kWarps + warp, stride = CLUSTER ? size * kWarps : kWarps;
   uint8_t* ring = smem + warp * (STAGES * kStage);
   Cursor ahead = at;  // of the next load
-  if (warp > 0) move<PER>(p, &ahead, warp);
+  if (CLUSTER) ahead.x = first;
+  else if (warp > 0) move<PER>(p, &ahead, warp);
   int loads = 0;
-  // Loads one behind the other in a walk are kWarps chunks apart: `left` of them, of so many bytes.
+  // Loads one behind the other in a walk are `stride` chunks apart: `left` of them, of so many bytes.
   int left = 0;
   uint32_t bytes = 0;
   const uint8_t *kp = nullptr, *vp = nullptr;
   auto load = [&]() {
-    if (warp + loads * kWarps >= run) return;
+    if (first + loads * stride >= run) return;
     if (left == 0) {
-      if (loads > 0) move<PER>(p, &ahead, 0);
+      if (!CLUSTER && loads > 0) move<PER>(p, &ahead, 0);
       const int g = heads_of(p, H, ahead.hp).kv, block = block_of<PER>(ahead.w, ahead.x);
       const int whole = ahead.x < ahead.w.ns ? ahead.w.sb / PER : ahead.w.ns + (ahead.w.end - ahead.w.first) / PER;
-      left = max(1, (whole - ahead.x + kWarps - 1) / kWarps);
+      left = max(1, (whole - ahead.x + stride - 1) / stride);
       bytes = ahead.x < whole ? PER * kBlock : kBlock;
       const int64_t off = static_cast<int64_t>(block) * kBlock;
       kp = p.k + ahead.b * p.k_b + g * p.k_h + off;
@@ -310,9 +348,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     }
     ++loads;
     --left;
-    kp += PER * kWarps * kBlock;
-    vp += PER * kWarps * kBlock;
-    ahead.x += kWarps;
+    kp += PER * stride * kBlock;
+    vp += PER * stride * kBlock;
+    ahead.x += stride;
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load();
@@ -400,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     // chunks [xa, xb) are visible whole
     const int xa = at.w.ns + ((at.w.start & (kQ4Tokens - 1)) != 0), xb = at.w.ns + (at.w.len - at.w.first * kQ4Tokens) / (PER * kQ4Tokens);
     const int x_end = at.x + n;
-    for (int x = at.x + warp + done * kWarps - piece_at; ok && x < x_end; ++done, x += kWarps) {
+    for (int x = at.x + first + done * stride - piece_at; ok && x < x_end; ++done, x += stride) {
       __syncwarp();  // every lane is done with the stage refilled here
       load();
       const int s = done % STAGES;
@@ -674,7 +712,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
         }
       }
     __syncthreads();
-    const bool cut = n < at.w.n;
+    const bool cut = n < at.w.n;  // (never in a cluster)
+    float* joined = parts + kWarps * held * kRow;
     const int slot = 2 * cta + (at.x == 0 ? 1 : 0);
     for (int i = threadIdx.x; i < nh * (kD / 4); i += kThreads) {  // four columns of a head
       const int h = i / (kD / 4), d = i % (kD / 4) * 4;
@@ -693,8 +732,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
         ll += f * src[kD + 1];
         oo.x += f * v.x, oo.y += f * v.y, oo.z += f * v.z, oo.w += f * v.w;
       }
-      if (cut) {
-        float* dst = p.shares + (static_cast<int64_t>(slot) * H + h) * kRow;
+      if (cut || size > 1) {
+        float* dst = size > 1 ? joined + h * kRow : p.shares + (static_cast<int64_t>(slot) * H + h) * kRow;
         *reinterpret_cast<float4*>(dst + d) = oo;
         if (d == 0) {
           dst[kD] = mm;
@@ -705,10 +744,31 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
             make_uint2(pack_bf16x2(oo.x / ll, oo.y / ll), pack_bf16x2(oo.z / ll, oo.w / ll));
       }
     }
-    if (cut && threadIdx.x == 0) p.pieces[slot] = make_int4(at.b * heads + at.hp, 0, n, at.w.n);
+    if (cut && threadIdx.x == 0) p.pieces[slot] = make_int4(at.b * p.walks + at.hp, 0, n, at.w.n);
+    if (CLUSTER && size > 1) {
+      cluster_sync_all();
+      const uint32_t base = smem_u32(joined);
+      for (int i = rank * kThreads + threadIdx.x; i < nh * (kD / 4); i += size * kThreads) {
+        const int h = i / (kD / 4), d = i % (kD / 4) * 4;
+        float mm = -INFINITY, ll = 0.f;
+        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < size; ++c) mm = fmaxf(mm, ld_cluster_f32(mapa_shared(base + (h * kRow + kD) * 4, c)));
+#pragma unroll 4
+        for (int c = 0; c < size; ++c) {
+          const uint32_t src = mapa_shared(base + h * kRow * 4, c);
+          const float f = share_weight(ld_cluster_f32(src + kD * 4), mm);
+          const float4 v = ld_cluster_f32x4(src + d * 4);
+          ll += f * ld_cluster_f32(src + kD * 4 + 4);
+          oo.x += f * v.x, oo.y += f * v.y, oo.z += f * v.z, oo.w += f * v.w;
+        }
+        *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(at.b) * p.QH + h0 + h) * kD + d) =
+            make_uint2(pack_bf16x2(oo.x / ll, oo.y / ll), pack_bf16x2(oo.z / ll, oo.w / ll));
+      }
+      cluster_sync_all();  // a CTA's sums are read until here
+    }
     __syncthreads();  // parts are free
     piece_at += n;
-    if (piece_at < run) move<PER>(p, &at, n);
+    if (!CLUSTER && piece_at < run) move<PER>(p, &at, n);
   }
   if (!ok && lane == 0) {  // no copy may still be writing shared memory when the CTA exits
     for (int i = max(0, loads - STAGES); i < loads; ++i)
@@ -774,38 +834,83 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
   }
 }
 
-template <int NT, int GROUP, bool PAIR>
-kda_status launch_decode(const DecodeParams& p, int ctas, cudaStream_t st) {
+// cluster: CTAs that share a walk, or 0: runs over `ctas` CTAs and a second launch.
+template <int NT, int GROUP, bool PAIR, bool CLUSTER>
+kda_status launch_decode(const DecodeParams& p, int ctas, int cluster, cudaStream_t st) {
   // rings of the depth that leaves two CTAs an SM (one where a group has more than 8 heads)
-  constexpr int kStages = NT == 1 ? 2 : 4;
+  constexpr int kStages = NT == 1 ? 2 : CLUSTER ? 3 : 4;
   constexpr int H = 8 * NT;
-  constexpr size_t kMost = kWarps * (kStages * 4 * q4_block_bytes(GROUP) + H * kRow * 4);
-  static_assert(kMost <= (NT == 1 ? 113 : 226) * 1024, "shared memory budget");
-  auto* kernel = q4_decode_kernel<NT, GROUP, kStages, PAIR>;
+  auto bytes = [](int held) {
+    return kWarps * (kStages * 4 * q4_block_bytes(GROUP) + held * kRow * 4) + (CLUSTER ? held * kRow * 4 : 0);
+  };
+  static_assert(kWarps * (kStages * 4 * q4_block_bytes(GROUP) + H * kRow * 4) <= (NT == 1 ? 113 : CLUSTER ? 218 : 226) * 1024,
+                "shared memory budget");
+  auto* kernel = q4_decode_kernel<NT, GROUP, kStages, PAIR, CLUSTER>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMost)) !=
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes(H))) !=
         cudaSuccess)
       return launch_status("gqa_decode_q4: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
   const int held = PAIR ? 2 * p.rep : p.rep < H ? p.rep : H;  // query heads of a walk
-  const size_t smem = kWarps * (kStages * 4 * q4_block_bytes(GROUP) + held * kRow * 4);
-  const kda_status s = launch_after("gqa_decode_q4", kernel, dim3(static_cast<unsigned>(ctas)), kThreads, smem, st, p,
-                                    kda_err_ptr_q4_decode());
+  if (CLUSTER) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(cluster), static_cast<unsigned>(p.walks), static_cast<unsigned>(p.B));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = bytes(held);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kernel, p, kda_err_ptr_q4_decode());
+    return launch_status("gqa_decode_q4");
+  }
+  const kda_status s = launch_after("gqa_decode_q4", kernel, dim3(static_cast<unsigned>(ctas)), kThreads, bytes(held), st,
+                                    p, kda_err_ptr_q4_decode());
   if (s != KDA_OK) return s;
   return launch_after("gqa_decode_q4: join", q4_join_kernel<H>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(held)),
                       kThreads, 0, st, p, ctas);
 }
 template <int GROUP>
-kda_status launch_group(const DecodeParams& p, int ctas, cudaStream_t st) {
-  if (p.rep > 8) return launch_decode<2, GROUP, false>(p, ctas, st);
-  return p.parts == 0 ? launch_decode<1, GROUP, true>(p, ctas, st) : launch_decode<1, GROUP, false>(p, ctas, st);
+kda_status launch_group(const DecodeParams& p, int ctas, int cluster, cudaStream_t st) {
+  if (cluster > 0)
+    return p.rep > 8 ? launch_decode<2, GROUP, false, true>(p, ctas, cluster, st)
+                     : launch_decode<1, GROUP, false, true>(p, ctas, cluster, st);
+  if (p.rep > 8) return launch_decode<2, GROUP, false, false>(p, ctas, 0, st);
+  return p.parts == 0 ? launch_decode<1, GROUP, true, false>(p, ctas, 0, st)
+                      : launch_decode<1, GROUP, false, false>(p, ctas, 0, st);
 }
 
 int decode_ctas(int64_t rep) { return num_sms() * (rep > 8 ? 1 : 2); }
+
+// How many CTAs share each of `walks` walks of up to `chunks` chunks, or 0: runs.  As many as have
+// room at once and find a chunk for each warp (of 8 with an SM to each CTA, 16 clusters do not fit:
+// 8 requests of 2,048 tokens, 16 query heads for each of 2 kv heads, 16.5 us with them, 9.8
+// with 4).  Clusters save the second launch and the ends of walks within a run, where several
+// short ones meet; but they take their time by the longest walk, so that runs are for long
+// ones, sooner where clusters leave SMs idle.  32 query and 8 kv heads, us with runs and so:
+//   1 request of 1,024 tokens 10.3, 6.2; 8,192 11.8, 10.5; 16,384 (8 chunks a warp) 14.5, 15.4
+//   3 of 2,048 10.7, 8.2; 16,384 21.6, 21.0; 32,768 (16) 32.5, 36.7
+//   16 of 2,048 19.2, 13.5; 8,192 (16) 40.3, 36.9; 64 of 128 12.3, 9.7; 4,096 (16) 68.2, 67.7;
+//   16 of 1 to 8,192 48.1, 34.8; 64 of 1 to 4,096 64.8, 51.2; 32 of 1 to 8,192 (32) 52.7, 62.9
+// Thousands of walks of equal, short lengths are the exception: 1,024 of 512 tokens 166, 199
+// (of 1 to 512 186, 163).
+int cluster_of(int64_t walks, int64_t chunks, int64_t rep) {
+  const int64_t ctas = decode_ctas(rep);
+  int64_t c = 1;
+  while (c < 8 && 2 * c * walks <= (rep > 8 && c == 4 ? ctas * 3 / 4 : ctas) && c * kWarps < chunks) c *= 2;
+  const int64_t most = 2 * c * walks < ctas ? 4 : 4 * c * walks < 3 * ctas ? 8 : 16;  // chunks of a warp
+  return chunks <= most * c * kWarps ? static_cast<int>(c) : 0;
+}
 
 }  // namespace
 }  // namespace kda
@@ -863,13 +968,14 @@ extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, cons
   p.QH = static_cast<int>(QH);
   p.KH = static_cast<int>(KH);
   p.rep = static_cast<int>(QH / KH);
-  // Two kv heads together take less work for each token, and more of it at the end of each walk
-  // and share of one (4 query heads of 8 kv heads, us without and with: 1 request of 8,192 tokens
-  // 10.7, 15.0; 16 40.6, 41.1; 32 69.2, 67.1; 64 126, 119; of 1,024 tokens 32 20.7, 21.1; 64
-  // 31.0, 28.3; 2 of 32,768 24.5, 25.3; 8 66.4, 65.9; 32 229, 219).  Lengths are not known
-  // here, the room for them is.
-  const bool pair = p.rep <= 4 && KH % 2 == 0 && (B * KH >= 512 || B * KH * T >= (1ll << 21));
-  p.parts = p.rep > 8 ? (p.rep + 15) / 16 : pair ? 0 : 1;
+  p.parts = p.rep > 8 ? (p.rep + 15) / 16 : 1;
+  const int64_t tokens = p.window + static_cast<int64_t>(p.sinks) < T ? p.window + static_cast<int64_t>(p.sinks) : T;
+  const int cluster = cluster_of(B * KH * p.parts, (tokens + 31) / 32 + (tokens < T ? 2 : 0), p.rep);
+  // Runs: two kv heads together take less work for each token, and more of it at the end of each
+  // walk and share of one (4 query heads of 8 kv heads, us without and with: 8 requests of 8,192
+  // tokens 25.1, 26.7; 16 40.6, 41.1; 32 69.2, 67.1; 64 126, 119; 2 of 32,768 24.5, 25.3; 8
+  // 66.4, 65.9; 32 229, 219).  Lengths are not known here, the room for them is.
+  if (cluster == 0 && p.rep <= 4 && KH % 2 == 0 && (B * KH >= 512 || B * KH * T >= (1ll << 21))) p.parts = 0;
   p.walks = static_cast<int>(p.parts == 0 ? KH / 2 : KH * p.parts);
   p.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(kD)));
   const int ctas = decode_ctas(p.rep);
@@ -880,5 +986,7 @@ extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, cons
   KDA_CHECK_SUPPORTED(B * p.walks < (1ll << 31) && B * p.walks < (1ll << 30) * ctas / blocks,
                       "%s: too large (B=%lld KH=%lld blocks=%lld)", op, (long long)B, (long long)KH, (long long)blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return group == 32 ? launch_group<32>(p, ctas, st) : group == 64 ? launch_group<64>(p, ctas, st) : launch_group<128>(p, ctas, st);
+  return group == 32   ? launch_group<32>(p, ctas, cluster, st)
+         : group == 64 ? launch_group<64>(p, ctas, cluster, st)
+                       : launch_group<128>(p, ctas, cluster, st);
 }

@@ -280,7 +280,7 @@ DECODE_CASES = [
     (1, 320, 32, 8, None, 0, [5111]), (2, 200, 20, 4, 1, 0, [3200, 1600]), (1, 600, 8, 1, None, 0, [9600]),
     (70, 4, 4, 2, None, 0, [0] * 33 + [64, 1, 33] + [0] * 33 + [5]), (1, 300, 9, 1, None, 0, [4800]),
     (300, 1, 2, 1, None, 0, [b % 17 for b in range(300)]), (1, 40, 5, 1, 17, 15, [640]),
-    # enough requests for two kv heads to be taken together, with 1 to 4 query heads for each
+    # many requests
     (256, 2, 8, 2, None, 0, [b % 33 for b in range(256)]), (130, 3, 12, 4, 9, 3, [(7 * b) % 49 for b in range(130)]),
     (64, 5, 8, 8, None, 0, [80 - b for b in range(64)]), (86, 9, 12, 6, 100, 20, [144 - b for b in range(86)]),
 ]
@@ -317,6 +317,62 @@ def test_decode(kda, group, B, blocks, QH, KH, window, sinks, lengths):
         else:
             assert rel_l2(host(out[b]), want[b]) <= 2 * U
     assert torch.equal(out, kda.gqa_decode_q4(*args))
+
+
+def values64(raw):
+    """Every value of a cache (B,KH,blocks,bytes) on the GPU: (B,KH,T,128) in 64 bits."""
+    t, ch = torch.arange(16, device="cuda")[:, None], torch.arange(128, device="cuda")
+    at = 64 * t + 16 * ((ch % 32 // 8) ^ (t // 2 % 4)) + 4 * (ch // 32) + ch % 8 // 2
+    codes = (raw[..., at.flatten()].unflatten(-1, (16, 128)) >> (4 * (ch % 2)).to(torch.uint8)) & 15
+    side = raw[..., 1024:].contiguous().view(BF16).double().unflatten(-1, (16, -1, 2))
+    v = codes.double().unflatten(-1, (side.shape[-2], -1)) * side[..., :1] + side[..., 1:]
+    return v.flatten(-2).flatten(2, 3)
+
+
+# Walks too long for a cluster: runs over all CTAs, cut walks joined by a second launch.  The second,
+# third and seventh take two kv heads together; the last ones are clusters of 1 and 4.
+LONG_CASES = [
+    # B, blocks, QH, KH, group, window, sinks
+    (1, 1400, 6, 1, 64, None, 0), (64, 260, 16, 8, 32, None, 0), (4, 4200, 16, 8, 128, 50000, 33),
+    (3, 700, 5, 5, 32, None, 0), (2, 1300, 34, 2, 64, 20000, 1), (1, 2600, 16, 1, 32, None, 0),
+    (130, 259, 8, 4, 128, None, 0), (300, 66, 8, 4, 128, None, 0), (9, 400, 48, 6, 64, None, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,blocks,QH,KH,group,window,sinks", LONG_CASES)
+def test_decode_of_long_walks(kda, B, blocks, QH, KH, group, window, sinks):
+    gen = torch.Generator(device="cuda").manual_seed(blocks)
+    rng = np.random.default_rng(blocks)
+    T, seen = 16 * blocks, 10 ** 9 if window is None else window
+    lens = rng.integers(0, T + 1, size=B)
+    lens[0] = T
+    if B > 2:
+        lens[1], lens[2] = 0, -5
+    caches = []
+    for _ in range(2):
+        c = torch.randint(0, 256, (B, KH, blocks, 1024 + 8192 // group), generator=gen, device="cuda", dtype=torch.uint8)
+        step = 0.3 + 0.1 * torch.rand(B, KH, blocks, 16 * (128 // group), generator=gen, device="cuda")
+        c[..., 1024:] = torch.stack([step, -7.5 * step], -1).to(BF16).flatten(-2).view(torch.uint8)
+        caches.append(c)
+    q = torch.randn(B, QH, 128, generator=gen, device="cuda").to(BF16)
+    args = (q, *caches, ints(lens.tolist()), window, sinks)
+    out = kda.gqa_decode_q4(*args)
+    for b in range(B):
+        n = int(lens[b])
+        if n <= 0:
+            assert not out[b].any()
+            continue
+        if b > 3 and b % 17:
+            continue
+        k, v = (values64(c[b:b + 1])[0, :, :n] for c in caches)
+        j = torch.arange(n, device="cuda")
+        s = q[b].double().unflatten(0, (KH, -1)) @ k.transpose(-1, -2) / np.sqrt(128.0)
+        s = s.masked_fill((j < n - seen) & (j >= sinks), -torch.inf)
+        want = (torch.softmax(s, -1) @ v).flatten(0, 1)
+        assert (out[b].double() - want).norm() <= 2 * U * want.norm()
+    for _ in range(3):
+        assert torch.equal(out, kda.gqa_decode_q4(*args))
 
 
 @pytest.mark.gpu
