@@ -8,9 +8,8 @@
 // back as low).  A group with an infinity or a NaN, or wider than fp32 holds, reads back as NaN.
 //
 // 16 lanes take a row, 8 channels each (one 16-byte load, one 4-byte store of codes), a
-// group's minimum and maximum by exchanges of bf16 pairs.  Bandwidth-bound in its bytes (656
-// a row of k and v), in fact by its 145 instructions for them: 27 us for 19,000 tokens of 8
-// heads, floor 15.  Reading back: 12.5 us for 32,768 tokens of 8 heads, floor 13.1 at the copy
+// group's minimum and maximum by exchanges of bf16 pairs.  Bandwidth-bound: 656 bytes a
+// row of k and v; 20.4 us for 18,700 tokens of 8 heads, floor 15.0; 92 for 100,000, floor 80.  Reading back: 12.5 us for 32,768 tokens of 8 heads, floor 13.1 at the copy
 // rate (13.7 with codes converted one by one: the integer pipe was full).
 #include <cuda_fp16.h>
 
@@ -31,11 +30,11 @@ struct AppendParams {
   const int* lengths;  // [B] tokens cached already; below zero: an idle slot
   unsigned rows;       // tokens in k and v
   unsigned per;
-  unsigned kh_mul, kh_shift;  // i / KH = (i kh_mul) >> (31 + kh_shift) for i < 2^31
   int64_t k_b, k_t, k_h, v_b, v_t, v_h;  // element strides
   int64_t kc_b, kc_h, vc_b, vc_h;        // byte strides
   int64_t cache_len;
   int B, KH;
+  int heads;           // of a CTA
 };
 
 __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
@@ -53,15 +52,12 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 template <int GROUP>
 __device__ __forceinline__ void quantise(const uint4 x, unsigned mask, uint32_t* word, uint32_t* pair) {
   uint32_t lo = min2(min2(x.x, x.y), min2(x.z, x.w)), hi = max2(max2(x.x, x.y), max2(x.z, x.w));
+  lo ^= 0x80008000u;  // the least is the negative of the largest -x, so one word holds both
+  uint32_t most = max2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
 #pragma unroll
-  for (int d = 1; d < GROUP / 8; d <<= 1) {
-    lo = min2(lo, __shfl_xor_sync(mask, lo, d));
-    hi = max2(hi, __shfl_xor_sync(mask, hi, d));
-  }
-  lo = min2(lo, lo >> 16 | lo << 16);
-  hi = max2(hi, hi >> 16 | hi << 16);
-  const float low = __uint_as_float(lo << 16), high = __uint_as_float(hi << 16);
-  float step = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f)));
+  for (int d = 1; d < GROUP / 8; d <<= 1) most = max2(most, __shfl_xor_sync(mask, most, d));
+  const float nlow = __uint_as_float(most << 16), high = __uint_as_float(most & 0xffff0000u);
+  float step = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fadd_rn(high, nlow), 1.0f / 15.0f)));
   if (step < 1.1754943508222875e-38f) step = 0.f;
   if (step > 3.3895313892515355e38f) step = __uint_as_float(0x7fc00000u);  // an infinity, or past bf16's largest
   const float inv = step > 0.f ? __frcp_rn(step) : 0.f;  // NaN: zero codes beside a NaN pair
@@ -74,14 +70,14 @@ __device__ __forceinline__ void quantise(const uint4 x, unsigned mask, uint32_t*
   uint32_t w = 0u - 0x4b000000u * 0x11111111u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 t = __fadd2_rn(make_float2(f[2 * i], f[2 * i + 1]), make_float2(-low, -low));
+    float2 t = __fadd2_rn(make_float2(f[2 * i], f[2 * i + 1]), make_float2(nlow, nlow));
     // __fmul_rn, not __fmul2_rn, which the compiler may fuse with the addition: a product that
     // rounds to a tie would then be rounded as what it was before
     t = __fadd2_rn(make_float2(__fmul_rn(t.x, inv), __fmul_rn(t.y, inv)), make_float2(8388608.f, 8388608.f));
     w += __float_as_uint(t.x) * (1u << (8 * i)) + __float_as_uint(t.y) * (16u << (8 * i));
   }
   *word = w;
-  *pair = (__float_as_uint(step) >> 16) | (lo << 16);
+  *pair = __byte_perm(__float_as_uint(step), most ^ 0x8000u, 0x5432);
 }
 
 // The request that row `row` belongs to: the last one whose first row is not after it, 16 at
@@ -98,70 +94,66 @@ __device__ __forceinline__ int request_of(const int* offsets, int B, int row, in
   return lo;
 }
 
-// A CTA takes 16 (token, head) pairs, 16 lanes each, k and v together: the loads are issued
-// first, and while they are under way the tokens' requests are looked up, once for each token
-// (each pair for itself, before its loads: 41 us for 19,000 tokens of 8 heads against 27; two or
-// four pairs for 16 lanes: 25 and 26, but 2.9 and 4.0 against 2.5 for a decode step's 64 tokens).
+// A CTA takes 16 tokens, 16 lanes each, and p.heads of their heads one after the other, k and v
+// together: the first head's loads are issued first, and while they are under way each token's
+// request is looked up, once for all heads; the next head's loads are issued before a head is
+// quantised.  (A CTA of 16 (token, head) pairs, nothing under way while they are quantised: 27.2 us
+// for 18,700 tokens of 8 heads against 20.4, 134 for 100,000 against 92, 2.1 for 64 against 1.8.)
 constexpr int kItems = kThreads / 16;
 template <int GROUP>
 __global__ void __launch_bounds__(kThreads) q4_append_kernel(const AppendParams p, unsigned* err) {
-  __shared__ int request[kItems], place[kItems];    // of the CTA's tokens; place -1: not written
   pdl_trigger();
   pdl_wait();
-  const int l = threadIdx.x & 15, hw = threadIdx.x >> 4;
+  const int l = threadIdx.x & 15;
   const unsigned mask = 0xffffu << (threadIdx.x & 16);
-  const unsigned all = p.rows * p.KH, i0 = blockIdx.x * kItems;  // < 2^31
-  auto token = [&](unsigned i) {
-    return static_cast<unsigned>((static_cast<uint64_t>(i) * p.kh_mul) >> (31 + p.kh_shift));
-  };
-  const unsigned row0 = token(i0);
-  const unsigned i = min(i0 + hw, all - 1), row = token(i);
-  const int h = static_cast<int>(i - row * p.KH);
-  const unsigned of = p.offsets ? 0u : row / p.per, in = p.offsets ? row : row - of * p.per;
-  const uint4 xk = *reinterpret_cast<const uint4*>(p.k + of * p.k_b + in * p.k_t + h * p.k_h + 8 * l);
-  const uint4 xv = *reinterpret_cast<const uint4*>(p.v + of * p.v_b + in * p.v_t + h * p.v_h + 8 * l);
-  const int tokens = static_cast<int>(token(min(i0 + kItems, all) - 1) - row0) + 1;
-  if (hw < tokens) {
-    const int row = static_cast<int>(row0) + hw;
-    int b;
-    int64_t at;
-    bool any = true;
-    if (p.offsets) {
-      b = request_of(p.offsets, p.B, row, l, mask);
-      const int first = __ldg(p.offsets + b);
-      any = row >= first && row < __ldg(p.offsets + b + 1);  // of some request
-      at = static_cast<int64_t>(row) - first;
-    } else {
-      b = static_cast<int>(static_cast<unsigned>(row) / p.per);
-      at = row - b * static_cast<int>(p.per);
-    }
-    const int cached = __ldg(p.lengths + b);
-    any = any && cached >= 0;  // not an idle slot
-    const int64_t pos = cached + at;
-    if (l == 0) {
-      if (any && pos >= p.cache_len) atomicOr(err, static_cast<unsigned>(kErrRange));
-      request[hw] = b;
-      place[hw] = any && pos < p.cache_len ? static_cast<int>(pos) : -1;
-    }
+  const unsigned i = blockIdx.x * kItems + (threadIdx.x >> 4);  // < 2^31
+  const unsigned row = min(i, p.rows - 1);
+  const int h0 = blockIdx.y * p.heads;
+  int left = min(p.heads, p.KH - h0);
+  const unsigned of = p.offsets ? 0u : row / p.per, in = row - of * p.per;
+  const __nv_bfloat16* k = p.k + of * p.k_b + in * p.k_t + h0 * p.k_h + 8 * l;
+  const __nv_bfloat16* v = p.v + of * p.v_b + in * p.v_t + h0 * p.v_h + 8 * l;
+  uint4 xk = *reinterpret_cast<const uint4*>(k), xv = *reinterpret_cast<const uint4*>(v);
+  int b = static_cast<int>(of);
+  int64_t at = in;
+  bool write = i < p.rows;
+  if (p.offsets) {
+    b = request_of(p.offsets, p.B, static_cast<int>(row), l, mask);
+    const int first = __ldg(p.offsets + b);
+    write = write && static_cast<int>(row) >= first && static_cast<int>(row) < __ldg(p.offsets + b + 1);  // of some request
+    at = static_cast<int64_t>(row) - first;
   }
-  __syncthreads();
-  uint32_t kw, kp, vw, vp;
-  quantise<GROUP>(xk, mask, &kw, &kp);
-  quantise<GROUP>(xv, mask, &vw, &vp);
-  const int pos = place[row - row0];
-  if (pos < 0 || i0 + hw >= all) return;
-  const int64_t b = request[row - row0];
-  const int t = pos & (kQ4Tokens - 1);
-  const int64_t block = static_cast<int64_t>(pos >> 4) * q4_block_bytes(GROUP);
+  const int cached = __ldg(p.lengths + b);
+  write = write && cached >= 0;  // not an idle slot
+  const int64_t pos = cached + at;
+  if (write && pos >= p.cache_len) {
+    if (l == 0) atomicOr(err, static_cast<unsigned>(kErrRange));
+    write = false;
+  }
+  if (!write) return;  // (all 16 lanes of the row)
+  const int t = static_cast<int>(pos) & (kQ4Tokens - 1);
+  const int64_t block = (pos >> 4) * q4_block_bytes(GROUP);
   const uint32_t code_at = q4_word(t, l & 3, l >> 2);
   const uint32_t pair_at = kQ4Codes + (t * (128 / GROUP) + l / (GROUP / 8)) * 4;
-  uint8_t* kd = p.k_cache + b * p.kc_b + h * p.kc_h + block;
-  uint8_t* vd = p.v_cache + b * p.vc_b + h * p.vc_h + block;
-  *reinterpret_cast<uint32_t*>(kd + code_at) = kw;
-  *reinterpret_cast<uint32_t*>(vd + code_at) = vw;
-  if (l % (GROUP / 8) == 0) {
-    *reinterpret_cast<uint32_t*>(kd + pair_at) = kp;
-    *reinterpret_cast<uint32_t*>(vd + pair_at) = vp;
+  uint8_t* kd = p.k_cache + b * p.kc_b + h0 * p.kc_h + block;
+  uint8_t* vd = p.v_cache + b * p.vc_b + h0 * p.vc_h + block;
+  for (;;) {
+    const uint4 yk = xk, yv = xv;
+    if (--left > 0) {
+      k += p.k_h, v += p.v_h;
+      xk = *reinterpret_cast<const uint4*>(k), xv = *reinterpret_cast<const uint4*>(v);
+    }
+    uint32_t kw, kp, vw, vp;
+    quantise<GROUP>(yk, mask, &kw, &kp);
+    quantise<GROUP>(yv, mask, &vw, &vp);
+    *reinterpret_cast<uint32_t*>(kd + code_at) = kw;
+    *reinterpret_cast<uint32_t*>(vd + code_at) = vw;
+    if (l % (GROUP / 8) == 0) {
+      *reinterpret_cast<uint32_t*>(kd + pair_at) = kp;
+      *reinterpret_cast<uint32_t*>(vd + pair_at) = vp;
+    }
+    if (left <= 0) break;
+    kd += p.kc_h, vd += p.vc_h;
   }
 }
 
@@ -207,10 +199,15 @@ __global__ void __launch_bounds__(kThreads) q4_read_kernel(const uint8_t* __rest
 }
 
 template <int GROUP>
-kda_status launch_append(const AppendParams& p, cudaStream_t st) {
-  const unsigned all = p.rows * p.KH;
-  return launch_after("kv_append_q4", q4_append_kernel<GROUP>, dim3((all + kItems - 1) / kItems), kThreads, 0, st, p,
-                      kda_err_ptr_q4_cache());
+kda_status launch_append(AppendParams p, cudaStream_t st) {
+  const unsigned groups = (p.rows + kItems - 1) / kItems;
+  // heads are split over as many CTAs as the GPU has room for (8 an SM): 4,096 tokens of 8 heads 6.6 us,
+  // 7.9 with a head to each CTA; 18,700 20.4 and 30.7
+  const int64_t splits = static_cast<int64_t>(num_sms()) * 8 / groups;
+  const int n = static_cast<int>(splits < 1 ? 1 : splits < p.KH ? splits : p.KH);
+  p.heads = (p.KH + n - 1) / n;
+  return launch_after("kv_append_q4", q4_append_kernel<GROUP>, dim3(groups, (p.KH + p.heads - 1) / p.heads), kThreads,
+                      0, st, p, kda_err_ptr_q4_cache());
 }
 
 }  // namespace
@@ -258,9 +255,6 @@ extern "C" kda_status kda_kv_append_q4(const void* k, const void* v, const int* 
   p.lengths = lengths;
   p.rows = static_cast<unsigned>(tokens);
   p.per = static_cast<unsigned>(n1);
-  while ((1ll << p.kh_shift) < KH) ++p.kh_shift;
-  // 2^(31 + s) / KH rounded up, of 32 bits: more by less than KH / 2^(31 + s) <= 2^-31 of itself
-  p.kh_mul = static_cast<unsigned>(((1ull << (31 + p.kh_shift)) + KH - 1) / KH);
   p.k_b = n0 > 1 ? k_strides[0] : 0, p.k_t = n1 > 1 ? k_strides[1] : 0, p.k_h = KH > 1 ? k_strides[2] : 0;
   p.v_b = n0 > 1 ? v_strides[0] : 0, p.v_t = n1 > 1 ? v_strides[1] : 0, p.v_h = KH > 1 ? v_strides[2] : 0;
   p.kc_b = B > 1 ? k_cache_strides[0] : 0, p.kc_h = KH > 1 ? k_cache_strides[1] : 0;

@@ -376,6 +376,47 @@ def test_decode_of_long_walks(kda, B, blocks, QH, KH, group, window, sinks):
 
 
 @pytest.mark.gpu
+def test_decode_of_long_walks_strides_ends_and_graphs(kda):
+    """Runs: strided caches, a length past the cache, a NaN in one kv head, a workspace that two
+    graphs share with a call of short walks."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    B, QH, KH, blocks = 2, 4, 2, 1400
+    both = torch.randint(0, 256, (B, blocks, 2 * KH, 1152), generator=gen, device="cuda", dtype=torch.uint8)
+    both[..., 1024:] = ints([0x3e80, 0xbf80]).to(torch.int16).repeat(32).view(torch.uint8)  # c / 4 - 1
+    kc, vc = (both.permute(0, 2, 1, 3)[:, i::2].contiguous() for i in range(2))
+    wide = torch.empty(B, KH + 1, blocks + 3, 1152, dtype=torch.uint8, device="cuda")
+    wide[:, 1:, :blocks] = kc
+    q = torch.randn(B, QH, 128, generator=gen, device="cuda").to(BF16)
+    n, T = ints([16 * blocks, 9001]), 16 * blocks
+    want = kda.gqa_decode_q4(q, kc, vc, n)
+    assert torch.equal(want, kda.gqa_decode_q4(q, wide[:, 1:].narrow(2, 0, blocks), vc, n))
+    assert torch.equal(want, kda.gqa_decode_q4(q, kc, vc, ints([T + 9, 9001])))
+    torch.cuda.synchronize()
+    assert kda.device_error() == 8
+    bad = vc.clone()
+    bad[0, 1, 700, 1030:1032] = 0xff
+    got = kda.gqa_decode_q4(q, kc, bad, n)
+    assert torch.equal(got[0, :2], want[0, :2]) and torch.equal(got[1], want[1])
+    nan = torch.isnan(got[0, 2:]).any(0)
+    assert nan.sum() == 64 and (nan[:64].all() or nan[64:].all())
+    ws = torch.full((4 << 20,), 0xff, dtype=torch.uint8, device="cuda")
+    short = [c[:, :, :9].contiguous() for c in (kc, vc)]
+    few = ints([130, 77])
+    small = kda.gqa_decode_q4(q, *short, few)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, kda.gqa_decode_q4(q, kc, vc, n, workspace=ws),
+                           kda.gqa_decode_q4(q, *short, few, workspace=ws),
+                           kda.gqa_decode_q4(q, kc, vc, n, workspace=ws)))
+    for _ in range(3):
+        for graph, *_ in graphs:
+            graph.replay()
+        assert all(torch.equal(a, b) for _, *got in graphs for a, b in zip(got, (want, small, want)))
+
+
+@pytest.mark.gpu
 def test_decode_extreme_scores_and_nan(kda):
     """Scores of some hundreds; a NaN among the visible rows reaches its own head alone."""
     rng = np.random.default_rng(8)
