@@ -291,6 +291,8 @@ Tensor packed_plan(const Tensor& offsets, int64_t tokens, const OptTensor& out) 
   const c10::cuda::CUDAGuard guard(dev);
   Tensor plan = out_or_empty(out, "out", {static_cast<int64_t>(nb / 4)}, at::kInt, dev);
   done("kda_packed_plan", kda_packed_plan(ptr<int>(offsets), n, tokens, plan.data_ptr(), nb, stream(dev)));
+  // a backward that still holds the plan from before raises, as after any change in place
+  if (out && !plan.is_inference()) plan.unsafeGetTensorImpl()->bump_version();
   return plan;
 }
 

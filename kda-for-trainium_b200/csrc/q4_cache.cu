@@ -9,8 +9,9 @@
 //
 // 16 lanes take a row, 8 channels each (one 16-byte load, one 4-byte store of codes), a
 // group's minimum and maximum by exchanges of bf16 pairs.  Bandwidth-bound: 656 bytes a
-// row of k and v; 20.4 us for 18,700 tokens of 8 heads, floor 15.0; 92 for 100,000, floor 80.  Reading back: 12.5 us for 32,768 tokens of 8 heads, floor 13.1 at the copy
-// rate (13.7 with codes converted one by one: the integer pipe was full).
+// row of k and v; 20.4 us for 18,700 tokens of 8 heads, floor 15.0; 92 for 100,000, floor 80.
+// Reading back: 12.5 us for 32,768 tokens of 8 heads, floor 13.1 at the copy rate (13.7 with
+// codes converted one by one: the integer pipe was full).
 #include <cuda_fp16.h>
 
 #include "launch.cuh"

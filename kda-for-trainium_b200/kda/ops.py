@@ -703,7 +703,8 @@ def packed_plan(offsets, tokens, *, out=None):
     int32 (N + 1,), not falling, within 0 .. tokens; sequences may be empty, rows
     before the first and behind the last belong to none).  Built on the device,
     once for all the calls on buffers of these offsets: every layer's forward and
-    backward.  Returns an int32 tensor.  Offsets that fall or leave the buffer
+    backward.  Returns an int32 tensor (``out``, where given: a backward pass that
+    still needs the plan which was there raises).  Offsets that fall or leave the buffer
     give a plan of no sequences and set ``device_error``."""
     return _native.packed_plan(offsets, tokens, out)
 

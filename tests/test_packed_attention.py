@@ -330,6 +330,12 @@ def test_autograd(kda):
     with pytest.raises(ValueError, match="expanded"):
         kda.gqa_packed(leaf[0], leaf[1].expand(-1, 2, -1), leaf[2], plan)
     leaf = [dev(x).requires_grad_() for x in (q, k, v)]
+    out = ka.gqa_packed(*leaf, plan)
+    kda.packed_plan(dev(off, torch.int32), len(q), out=plan)  # perhaps of other sequences: the backward cannot know
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        out.float().sum().backward()
+    with torch.inference_mode():
+        kda.packed_plan(dev(off, torch.int32), len(q), out=torch.empty_like(plan))
     g = torch.autograd.grad(ka.gqa_packed(*leaf, plan).float().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivatives"):
         g[0].float().sum().backward()
