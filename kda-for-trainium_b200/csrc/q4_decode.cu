@@ -29,7 +29,7 @@
 // The running maximum moves only when a score exceeds it by 2^8, which fp32 sums and bf16
 // weights hold exactly as well; so a block usually needs no exchange between lanes.
 //
-// A walk is a request's blocks of a kv head.  Short ones: a cluster of 1 to 8 CTAs for each; the
+// A walk is a request's blocks of a kv head.  Short ones: a cluster of 1 to 16 CTAs for each; the
 // blocks go to their warps in turn, each through a ring of bulk copies of its own, and the
 // warps join through shared memory, the CTAs through the cluster's: one launch.
 // Long ones: the walks, one behind the other, are cut into equal runs, one for each CTA
@@ -851,7 +851,8 @@ kda_status launch_decode(const DecodeParams& p, int ctas, int cluster, cudaStrea
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes(H))) !=
-        cudaSuccess)
+            cudaSuccess ||
+        (CLUSTER && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
       return launch_status("gqa_decode_q4: cudaFuncSetAttribute");
     attr_set[dev].store(true, std::memory_order_release);
   }
@@ -895,7 +896,8 @@ int decode_ctas(int64_t rep) { return num_sms() * (rep > 8 ? 1 : 2); }
 // How many CTAs share each of `walks` walks of up to `chunks` chunks, or 0: runs.  As many as have
 // room at once and find a chunk for each warp (of 8 with an SM to each CTA, 16 clusters do not fit:
 // 8 requests of 2,048 tokens, 16 query heads for each of 2 kv heads, 16.5 us with them, 9.8
-// with 4).  Clusters save the second launch and the ends of walks within a run, where several
+// with 4; of 16, two to an SM, one request of 8,192 tokens and 4 query heads for each of 2 kv heads
+// 8.1 us, of 8 9.8; 8 kv heads 10.7 and 10.4: up to a quarter of the GPU then).  Clusters save the second launch and the ends of walks within a run, where several
 // short ones meet; but they take their time by the longest walk, so that runs are for long
 // ones, sooner where clusters leave SMs idle.  32 query and 8 kv heads, us with runs and so:
 //   1 request of 1,024 tokens 10.3, 6.2; 8,192 11.8, 10.5; 16,384 (8 chunks a warp) 14.5, 15.4
@@ -907,7 +909,9 @@ int decode_ctas(int64_t rep) { return num_sms() * (rep > 8 ? 1 : 2); }
 int cluster_of(int64_t walks, int64_t chunks, int64_t rep) {
   const int64_t ctas = decode_ctas(rep);
   int64_t c = 1;
-  while (c < 8 && 2 * c * walks <= (rep > 8 && c == 4 ? ctas * 3 / 4 : ctas) && c * kWarps < chunks) c *= 2;
+  while (c < 16 && c * kWarps < chunks &&
+         2 * c * walks <= (c == 8 ? ctas / 4 : rep > 8 && c == 4 ? ctas * 3 / 4 : ctas))
+    c *= 2;
   const int64_t most = 2 * c * walks < ctas ? 4 : 4 * c * walks < 3 * ctas ? 8 : 16;  // chunks of a warp
   return chunks <= most * c * kWarps ? static_cast<int>(c) : 0;
 }
