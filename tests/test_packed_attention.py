@@ -274,6 +274,34 @@ def test_a_sequence_does_not_depend_on_its_neighbours(kda, QH, KH):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("QH,KH", [(16, 8), (14, 14), (18, 2)])
+def test_a_sequence_among_many_is_the_sequence_alone(kda, QH, KH):
+    """More blocks than SMs, where a unit has two tiles: the bits of the sequence by itself, whatever
+    the others hold, from strided operands, rows of no sequence untouched."""
+    lens = [200, 77, 300, 1, 60, 128, 257, 513, 90, 129, 31, 640]
+    q, k, v, off, rng = inputs(lens, QH, KH, 5, 9)
+    T = len(q)
+    qkv = dev(np.concatenate([q, k, v], 1))
+    args = qkv.split((QH, KH, KH), dim=1)
+    plan = kda.packed_plan(dev(off, torch.int32), T)
+    out, lse = kda.gqa_packed_lse(*args, plan)
+    for s, n in enumerate(lens):
+        keep = slice(off[s], off[s + 1])
+        one = kda.packed_plan(torch.tensor([0, n], dtype=torch.int32, device="cuda"), n)
+        want, wlse = kda.gqa_packed_lse(*(x[keep].contiguous() for x in args), one)
+        assert torch.equal(out[keep], want) and torch.equal(lse[:, keep], wlse)
+        dirty = torch.full_like(qkv, (float("nan"), float("inf"), 1e30)[s % 3])
+        dirty[keep] = qkv[keep]
+        given = torch.full_like(out, 3.0)
+        kda.gqa_packed(*dirty.split((QH, KH, KH), dim=1), plan, out=given)
+        assert torch.equal(given[keep], want)
+        assert (given[:5] == 3).all() and (given[-9:] == 3).all()
+    wout, wl = ref.gqa_packed(q, k, v, off)
+    assert rel_l2(host(out)[5:-9], wout[5:-9]) <= rounds(2)
+    np.testing.assert_allclose(host(lse)[:, 5:-9], wl[:, 5:-9], rtol=2.0 ** -21, atol=1e-5)
+
+
+@pytest.mark.gpu
 def test_a_sequence_alone_is_full_attention(kda):
     rng = np.random.default_rng(1)
     q, k, v = draw(rng, 520, 4, 128), draw(rng, 520, 2, 128), draw(rng, 520, 2, 128)
