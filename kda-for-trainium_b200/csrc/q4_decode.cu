@@ -209,9 +209,10 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
 // four for the same codes, half of the work between the products (64 requests, 4 query heads for
 // each of 8 kv heads: 139 us without, 124 with).
 // CLUSTER: no runs; the CTAs of a cluster share one walk; grid (cluster size, walks, B).
-template <int NT, int GROUP, int STAGES, bool PAIR, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(const DecodeParams p, unsigned* err) {
-  constexpr int H = 8 * NT;
+template <int NT, int GROUP, int STAGES, bool PAIR, bool CLUSTER, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
+    q4_decode_kernel(const DecodeParams p, unsigned* err) {
+  constexpr int H = 8 * NT, THREADS = 32 * WARPS;
   constexpr int NG = 128 / GROUP;                       // pairs of a token
   constexpr int RUNS = 4 / NG;                          // 32-channel runs of a group
   constexpr uint32_t kBlock = q4_block_bytes(GROUP);
@@ -221,8 +222,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   static_assert(!PAIR || (NT == 1 && !CLUSTER), "8 columns, runs");
   constexpr int kTop = 100;                             // P' is scaled by 2^kTop at most
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kWarps][STAGES];
-  __shared__ int64_t sums[kWarps];
+  __shared__ uint64_t full[WARPS][STAGES];
+  __shared__ int64_t sums[WARPS];
   __shared__ int first_b;
   __shared__ int64_t first_x;
   const int warp = threadIdx.x >> 5;
@@ -252,14 +253,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
       const Heads hs = heads_of(p, H, at.hp);
       uint4* out = reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(at.b) * p.QH + hs.first) * kD);
       if (rank == 0)
-        for (int i = threadIdx.x; i < hs.n * (kD / 8); i += kThreads) out[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = threadIdx.x; i < hs.n * (kD / 8); i += THREADS) out[i] = make_uint4(0u, 0u, 0u, 0u);
       return;
     }
   } else {
     if (threadIdx.x == 0) p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
     // The run: chunks [r0, r1) of all walks.  Each thread counts the requests [b0, b1).
     const int heads = p.walks;
-    const int each = (p.B + kThreads - 1) / kThreads;
+    const int each = (p.B + THREADS - 1) / THREADS;
     const int b0 = min(static_cast<int>(threadIdx.x) * each, p.B), b1 = min(b0 + each, p.B);
     int64_t mine = 0;
     for (int b = b0; b < b1; ++b) mine += walk_of<PER>(p, b).n;
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     __syncthreads();
     int64_t before = upto - mine, total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) before += sums[w];
       total += sums[w];
     }
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
       const int n = __ldg(p.lengths + b);
       if (threadIdx.x == 0 && n > p.cache_len) atomicOr(p.length_err, static_cast<unsigned>(kErrRange));
       if (n <= 0)
-        for (int i = threadIdx.x; i < p.QH * (kD / 8); i += kThreads)
+        for (int i = threadIdx.x; i < p.QH * (kD / 8); i += THREADS)
           reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(b) * p.QH * kD)[i] = make_uint4(0u, 0u, 0u, 0u);
     }
     if (run == 0) return;
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
   }
 
   // this warp's chunks: first, first + stride, ... of the run
-  const int first = rank * kWarps + warp, stride = CLUSTER ? size * kWarps : kWarps;
+  const int first = rank * WARPS + warp, stride = CLUSTER ? size * WARPS : WARPS;
   uint8_t* ring = smem + warp * (STAGES * kStage);
   Cursor ahead = at;  // of the next load
   if (CLUSTER) ahead.x = first;
@@ -355,7 +356,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load();
 
-  float* parts = reinterpret_cast<float*>(smem + kWarps * STAGES * kStage);  // [kWarps][held][kRow]
+  // [WARPS][held][kRow]; where the rings leave no room for it, in their place at the end
+  float* parts = reinterpret_cast<float*>(smem + (WARPS == 16 ? 0 : WARPS * STAGES * kStage));
   const int held = PAIR ? 2 * p.rep : min(p.rep, H);
   bool ok = true;
   int done = 0;       // this warp's chunks
@@ -680,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     }
 
     // the piece's end: this warp's share, then all of them
+    if (WARPS == 16) __syncthreads();  // the rings are read
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -713,19 +716,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
       }
     __syncthreads();
     const bool cut = n < at.w.n;  // (never in a cluster)
-    float* joined = parts + kWarps * held * kRow;
+    float* joined = WARPS == 16 ? parts + WARPS * held * kRow : reinterpret_cast<float*>(smem);  // rings are read
     const int slot = 2 * cta + (at.x == 0 ? 1 : 0);
-    for (int i = threadIdx.x; i < nh * (kD / 4); i += kThreads) {  // four columns of a head
+    for (int i = threadIdx.x; i < nh * (kD / 4); i += THREADS) {  // four columns of a head
       const int h = i / (kD / 4), d = i % (kD / 4) * 4;
-      float mw[kWarps], mm = -INFINITY, ll = 0.f;
+      float mw[WARPS], mm = -INFINITY, ll = 0.f;
       float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < WARPS; ++w) {
         mw[w] = parts[(w * held + h) * kRow + kD];
         mm = fmaxf(mm, mw[w]);
       }
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < WARPS; ++w) {
         const float* src = parts + (w * held + h) * kRow;
         const float f = share_weight(mw[w], mm);
         const float4 v = *reinterpret_cast<const float4*>(src + d);
@@ -748,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) q4_decode_kernel(co
     if (CLUSTER && size > 1) {
       cluster_sync_all();
       const uint32_t base = smem_u32(joined);
-      for (int i = rank * kThreads + threadIdx.x; i < nh * (kD / 4); i += size * kThreads) {
+      for (int i = rank * THREADS + threadIdx.x; i < nh * (kD / 4); i += size * THREADS) {
         const int h = i / (kD / 4), d = i % (kD / 4) * 4;
         float mm = -INFINITY, ll = 0.f;
         float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -835,17 +838,16 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
 }
 
 // cluster: CTAs that share a walk, or 0: runs over `ctas` CTAs and a second launch.
-template <int NT, int GROUP, bool PAIR, bool CLUSTER>
+template <int NT, int GROUP, bool PAIR, bool CLUSTER, int WARPS = kWarps>
 kda_status launch_decode(const DecodeParams& p, int ctas, int cluster, cudaStream_t st) {
   // rings of the depth that leaves two CTAs an SM (one where a group has more than 8 heads)
   constexpr int kStages = NT == 1 ? 2 : CLUSTER ? 3 : 4;
   constexpr int H = 8 * NT;
-  auto bytes = [](int held) {
-    return kWarps * (kStages * 4 * q4_block_bytes(GROUP) + held * kRow * 4) + (CLUSTER ? held * kRow * 4 : 0);
-  };
-  static_assert(kWarps * (kStages * 4 * q4_block_bytes(GROUP) + H * kRow * 4) <= (NT == 1 ? 113 : CLUSTER ? 218 : 226) * 1024,
-                "shared memory budget");
-  auto* kernel = q4_decode_kernel<NT, GROUP, kStages, PAIR, CLUSTER>;
+  constexpr int kRing = WARPS * kStages * 4 * q4_block_bytes(GROUP), kRows = WARPS * kRow * 4;
+  static_assert((WARPS + 1) * H * kRow * 4 <= kRing, "shares in the rings' place");
+  auto bytes = [](int held) { return static_cast<size_t>(kRing + (WARPS == 16 ? 0 : held * kRows)); };
+  static_assert(kRing + (WARPS == 16 ? 0 : H * kRows) <= (NT == 1 && WARPS == 8 ? 113 : 226) * 1024, "shared memory budget");
+  auto* kernel = q4_decode_kernel<NT, GROUP, kStages, PAIR, CLUSTER, WARPS>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -860,7 +862,7 @@ kda_status launch_decode(const DecodeParams& p, int ctas, int cluster, cudaStrea
   if (CLUSTER) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(cluster), static_cast<unsigned>(p.walks), static_cast<unsigned>(p.B));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.dynamicSmemBytes = bytes(held);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -881,11 +883,17 @@ kda_status launch_decode(const DecodeParams& p, int ctas, int cluster, cudaStrea
   return launch_after("gqa_decode_q4: join", q4_join_kernel<H>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(held)),
                       kThreads, 0, st, p, ctas);
 }
+// CTAs that share a walk, of so many warps; 0: runs.
+struct Cluster {
+  int64_t ctas, warps;
+};
 template <int GROUP>
-kda_status launch_group(const DecodeParams& p, int ctas, int cluster, cudaStream_t st) {
+kda_status launch_group(const DecodeParams& p, int ctas, const Cluster& c, cudaStream_t st) {
+  const int cluster = static_cast<int>(c.ctas);
   if (cluster > 0)
-    return p.rep > 8 ? launch_decode<2, GROUP, false, true>(p, ctas, cluster, st)
-                     : launch_decode<1, GROUP, false, true>(p, ctas, cluster, st);
+    return c.warps == 16 ? launch_decode<1, GROUP, false, true, 16>(p, ctas, cluster, st)
+           : p.rep > 8   ? launch_decode<2, GROUP, false, true>(p, ctas, cluster, st)
+                         : launch_decode<1, GROUP, false, true>(p, ctas, cluster, st);
   if (p.rep > 8) return launch_decode<2, GROUP, false, false>(p, ctas, 0, st);
   return p.parts == 0 ? launch_decode<1, GROUP, true, false>(p, ctas, 0, st)
                       : launch_decode<1, GROUP, false, false>(p, ctas, 0, st);
@@ -893,27 +901,38 @@ kda_status launch_group(const DecodeParams& p, int ctas, int cluster, cudaStream
 
 int decode_ctas(int64_t rep) { return num_sms() * (rep > 8 ? 1 : 2); }
 
-// How many CTAs share each of `walks` walks of up to `chunks` chunks, or 0: runs.  As many as have
-// room at once and find a chunk for each warp (of 8 with an SM to each CTA, 16 clusters do not fit:
-// 8 requests of 2,048 tokens, 16 query heads for each of 2 kv heads, 16.5 us with them, 9.8
-// with 4; of 16, two to an SM, one request of 8,192 tokens and 4 query heads for each of 2 kv heads
-// 8.1 us, of 8 9.8; 8 kv heads 10.7 and 10.4: up to a quarter of the GPU then).  Clusters save the second launch and the ends of walks within a run, where several
+// As many CTAs as have room at once (`room`) and find a chunk for each warp, up to 8 (of 8 with
+// an SM to each CTA, 16 clusters do not fit: 8 requests of 2,048 tokens, 16 query heads for each of
+// 2 kv heads, 16.5 us with them, 9.8 with 4); 16, two to an SM, up to a quarter of the GPU (one
+// request of 8,192 tokens and 4 query heads for each of 2 kv heads 8.1 us, of 8 9.8; 8 kv heads 10.7
+// and 10.4).  Clusters save the second launch and the ends of walks within a run, where several
 // short ones meet; but they take their time by the longest walk, so that runs are for long
 // ones, sooner where clusters leave SMs idle.  32 query and 8 kv heads, us with runs and so:
-//   1 request of 1,024 tokens 10.3, 6.2; 8,192 11.8, 10.5; 16,384 (8 chunks a warp) 14.5, 15.4
+//   1 request of 1,024 tokens 10.3, 6.2; 8,192 11.8, 10.5; 32,768 (8 chunks a warp) 17.7, 20.2
 //   3 of 2,048 10.7, 8.2; 16,384 21.6, 21.0; 32,768 (16) 32.5, 36.7
 //   16 of 2,048 19.2, 13.5; 8,192 (16) 40.3, 36.9; 64 of 128 12.3, 9.7; 4,096 (16) 68.2, 67.7;
 //   16 of 1 to 8,192 48.1, 34.8; 64 of 1 to 4,096 64.8, 51.2; 32 of 1 to 8,192 (32) 52.7, 62.9
 // Thousands of walks of equal, short lengths are the exception: 1,024 of 512 tokens 166, 199
 // (of 1 to 512 186, 163).
-int cluster_of(int64_t walks, int64_t chunks, int64_t rep) {
-  const int64_t ctas = decode_ctas(rep);
+Cluster cluster_of(int64_t walks, int64_t chunks, int64_t room, bool two_an_sm, int64_t warps) {
   int64_t c = 1;
-  while (c < 16 && c * kWarps < chunks &&
-         2 * c * walks <= (c == 8 ? ctas / 4 : rep > 8 && c == 4 ? ctas * 3 / 4 : ctas))
+  while (c < (two_an_sm ? 16 : 8) && c * warps < chunks &&
+         2 * c * walks <= (c == 8 ? room / 4 : c == 4 && !two_an_sm ? room * 3 / 4 : room))
     c *= 2;
-  const int64_t most = 2 * c * walks < ctas ? 4 : 4 * c * walks < 3 * ctas ? 8 : 16;  // chunks of a warp
-  return chunks <= most * c * kWarps ? static_cast<int>(c) : 0;
+  const int64_t most = 2 * c * walks < room ? 4 : 4 * c * walks < 3 * room ? 8 : 16;  // chunks of a warp
+  return {chunks <= most * c * warps ? c : 0, warps};
+}
+// CTAs of 16 warps take an SM each: where 8 warps would share SMs two by two all the same, or more
+// warps work at once, or a cluster is spared.  1 request of 8,192 tokens 10.6 us, 9.6 so; 16,384 (runs
+// otherwise) 14.5, 13.1; 3 of 2,048 8.2, 7.7; 16 of 512 7.7, 6.6; of 4,096 20.9, 19.3; but 1 of 2,048
+// 6.7, 7.4.  (More than 8 query heads need the registers of 8 warps.)
+Cluster cluster_for(int64_t walks, int64_t chunks, int64_t rep) {
+  const Cluster c8 = cluster_of(walks, chunks, decode_ctas(rep), rep <= 8, 8);
+  if (rep > 8 || c8.ctas == 16 || chunks <= 8) return c8;
+  const Cluster c16 = cluster_of(walks, chunks, num_sms(), false, 16);
+  if (walks > num_sms() || c16.ctas == 0) return c8;
+  const bool more = c8.ctas == 0 || (chunks - 1) / (16 * c16.ctas) < (chunks - 1) / (8 * c8.ctas);
+  return more || c16.ctas == 1 || c8.ctas * walks > num_sms() ? c16 : c8;
 }
 
 }  // namespace
@@ -974,12 +993,12 @@ extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, cons
   p.rep = static_cast<int>(QH / KH);
   p.parts = p.rep > 8 ? (p.rep + 15) / 16 : 1;
   const int64_t tokens = p.window + static_cast<int64_t>(p.sinks) < T ? p.window + static_cast<int64_t>(p.sinks) : T;
-  const int cluster = cluster_of(B * KH * p.parts, (tokens + 31) / 32 + (tokens < T ? 2 : 0), p.rep);
+  const Cluster cluster = cluster_for(B * KH * p.parts, (tokens + 31) / 32 + (tokens < T ? 2 : 0), p.rep);
   // Runs: two kv heads together take less work for each token, and more of it at the end of each
   // walk and share of one (4 query heads of 8 kv heads, us without and with: 8 requests of 8,192
   // tokens 25.1, 26.7; 16 40.6, 41.1; 32 69.2, 67.1; 64 126, 119; 2 of 32,768 24.5, 25.3; 8
   // 66.4, 65.9; 32 229, 219).  Lengths are not known here, the room for them is.
-  if (cluster == 0 && p.rep <= 4 && KH % 2 == 0 && (B * KH >= 512 || B * KH * T >= (1ll << 21))) p.parts = 0;
+  if (cluster.ctas == 0 && p.rep <= 4 && KH % 2 == 0 && (B * KH >= 512 || B * KH * T >= (1ll << 21))) p.parts = 0;
   p.walks = static_cast<int>(p.parts == 0 ? KH / 2 : KH * p.parts);
   p.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(kD)));
   const int ctas = decode_ctas(p.rep);
