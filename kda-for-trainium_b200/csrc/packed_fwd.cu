@@ -8,9 +8,10 @@
 // Work unit = two tiles of 128 query rows that see the same keys: the same block of two
 // heads of a group where its heads are even in number, else two consecutive blocks of a
 // head.  (Heads first because both tiles then have rows at every block: a short sequence
-// has one block only.)  One tile where there are fewer units than SMs all the same.  Units come from the plan's tables, those with the most keys
-// first; the persistent CTAs, one per SM, take them in turn.  A unit's K and V blocks pass
-// through rings of 3 and 2 tiles and serve both tiles.
+// has one block only.)  One tile where there are no more such units than SMs.  Units come
+// from the plan's tables, those with the most keys first; the persistent CTAs, one per SM,
+// take them in turn.  A unit's K and V blocks pass through rings of 3 and 2 tiles and serve
+// both tiles.
 //
 // A tile of a sequence's last block also holds rows of whatever lies behind it.  Such
 // query rows are computed and not stored, and never move a row's reference, so a

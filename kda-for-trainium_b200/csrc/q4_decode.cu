@@ -422,7 +422,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
     float m[NT][2], l[NT][2];       // heads 8 t + 2 (lane % 4) + {0, 1}; l: this lane's keys only
     int vs[NT][2];                  // P' = 2^(vs - 127) p step
     float lows[NT][NG][2];          // sums of p low, this lane's keys only
-    float o[NT][4][2][4];           // run, step: channels 32 run + 4 (lane / 4) + 2 step, of P' c 2^-24, and + 1, of P' (c + 16 c') 2^-24
+    // run, step: channels 32 run + 4 (lane / 4) + 2 step, of P' c 2^-24, and + 1, of P' (c + 16 c') 2^-24
+    float o[NT][4][2][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t][0] = m[t][1] = -INFINITY;
@@ -438,7 +439,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
     }
 
     // chunks [xa, xb) are visible whole
-    const int xa = at.w.ns + ((at.w.start & (kQ4Tokens - 1)) != 0), xb = at.w.ns + (at.w.len - at.w.first * kQ4Tokens) / (PER * kQ4Tokens);
+    const int xa = at.w.ns + ((at.w.start & (kQ4Tokens - 1)) != 0);
+    const int xb = at.w.ns + (at.w.len - at.w.first * kQ4Tokens) / (PER * kQ4Tokens);
     const int x_end = at.x + n;
     for (int x = at.x + first + done * stride - piece_at; ok && x < x_end; ++done, x += stride) {
       __syncwarp();  // every lane is done with the stage refilled here

@@ -216,6 +216,35 @@ def test_append_rows_of_each_request_and_views(kda, S):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,KH,group", [(3000, 9, 32), (20000, 9, 64), (40000, 5, 128)])
+def test_append_of_many_rows_is_each_head_alone(kda, T, KH, group):
+    """Several heads to a CTA: the bytes of appends of one head, requests of any length, rows of
+    none, an idle slot and rows past the cache among them."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    kv = torch.randn(T, 2 * KH + 1, 128, generator=gen, device="cuda").to(BF16)
+    k, v = kv[:, :KH], kv[:, KH + 1:]
+    B, length = 11, T // 4
+    cuts = np.sort(np.random.default_rng(T).integers(5, T - 9, size=B + 1))
+    cuts[4] = cuts[3]
+    off, lens = ints(cuts.tolist()), ints([0, 3, 16, 7, -1, 0, 40, 1, 250, 0, length - 2])
+    got = [kda.kv_cache_q4(B, length, KH, group) for _ in range(2)]
+    want = [kda.kv_cache_q4(B, length, KH, group) for _ in range(2)]
+    kda.kv_append_q4(k, v, *got, lens, off)
+    for h in range(KH):
+        kda.kv_append_q4(k[:, h:h + 1], v[:, h:h + 1], *(c[:, h:h + 1] for c in want), lens, off)
+    torch.cuda.synchronize()
+    assert kda.device_error() == 8
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0].any()
+    step = T // B  # the same rows for each request
+    k2, v2 = (x[:step * B].unflatten(0, (B, step)) for x in (k, v))
+    lens = ints([17, -3] + [5] * (B - 2))
+    kda.kv_append_q4(k2, v2, *got, lens)
+    for h in range(KH):
+        kda.kv_append_q4(k2[:, :, h:h + 1], v2[:, :, h:h + 1], *(c[:, h:h + 1] for c in want), lens)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_append_past_the_cache_is_reported_and_writes_nothing_there(kda):
     rng = np.random.default_rng(3)
     buf = noise(rng, 3, 1, 1, 1152)  # one request's cache between two others
