@@ -359,18 +359,20 @@ def values64(raw):
 
 
 # Walks too long for a cluster: runs over all CTAs, cut walks joined by a second launch.  The second,
-# third and seventh take two kv heads together; the last ones are clusters of 1 and 4.
+# third, seventh and ninth take two kv heads together, the eighth and ninth have some walks to a
+# run; the last two are clusters.
 LONG_CASES = [
-    # B, blocks, QH, KH, group, window, sinks
-    (1, 1400, 6, 1, 64, None, 0), (64, 260, 16, 8, 32, None, 0), (4, 4200, 16, 8, 128, 50000, 33),
-    (3, 700, 5, 5, 32, None, 0), (2, 1300, 34, 2, 64, 20000, 1), (1, 2600, 16, 1, 32, None, 0),
-    (130, 259, 8, 4, 128, None, 0), (300, 66, 8, 4, 128, None, 0), (9, 400, 48, 6, 64, None, 0),
+    # B, blocks, QH, KH, window, sinks
+    (1, 1400, 6, 1, None, 0), (64, 260, 16, 8, None, 0), (4, 4200, 16, 8, 50000, 33), (3, 700, 5, 5, None, 0),
+    (2, 1300, 34, 2, 20000, 1), (1, 2600, 16, 1, None, 0), (130, 259, 8, 4, None, 0), (700, 260, 4, 1, None, 0),
+    (520, 260, 4, 2, None, 0), (300, 66, 8, 4, None, 0), (9, 400, 48, 6, None, 0),
 ]
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,blocks,QH,KH,group,window,sinks", LONG_CASES)
-def test_decode_of_long_walks(kda, B, blocks, QH, KH, group, window, sinks):
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("B,blocks,QH,KH,window,sinks", LONG_CASES)
+def test_decode_of_long_walks(kda, group, B, blocks, QH, KH, window, sinks):
     gen = torch.Generator(device="cuda").manual_seed(blocks)
     rng = np.random.default_rng(blocks)
     T, seen = 16 * blocks, 10 ** 9 if window is None else window
