@@ -13,7 +13,6 @@ query heads that share KH key/value heads):
 rounded once) and the calls a user makes of the ``kda`` package.
 """
 
-import functools
 import math
 import random
 import sys
@@ -348,7 +347,6 @@ def _plain_decode(st):
 
 
 # ------------------------------------------------------------------- calls
-@functools.cache
 def _kda():
     path = str(Path(__file__).resolve().parent.parent / "kda-for-trainium_b200")
     if path not in sys.path:
