@@ -56,6 +56,10 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kRow = kD + 4;       // floats of a head's share: the output row, maximum, sum
 constexpr int kLeast = kWarps;      // chunks of a CTA's run, where there are as many
 constexpr unsigned kFull = 0xffffffffu;
+// Weights are held as 2^(s - m - kUnder): a weight is 2^8 at most, so that sums of up to 2^24 values of any
+// size stay finite in fp32, as the output is.  (Values below 2^-94 of the largest weight lose bits.)
+constexpr int kUnder = 32;
+constexpr int kTop = 126;           // P' is scaled by 2^kTop at most
 
 struct DecodeParams {
   const __nv_bfloat16* q;
@@ -220,7 +224,6 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
   constexpr int PER = PAIR ? 1 : 2;                     // blocks of a chunk, of each kv head
   constexpr int ROWS = PAIR ? 1 : 2;                    // tokens of a lane in a tile of S^T
   static_assert(!PAIR || (NT == 1 && !CLUSTER), "8 columns, runs");
-  constexpr int kTop = 100;                             // P' is scaled by 2^kTop at most
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[WARPS][STAGES];
   __shared__ int64_t sums[WARPS];
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
         qsum[t][j][1] = __shfl_sync(kFull, sum[j], 8 * c4 + 4);
       }
     }
-    float nm[NT][2];                // -m, or zero where that is infinite
+    float nm[NT][2];                // -m - kUnder, or zero where that is infinite
     float m[NT][2], l[NT][2];       // heads 8 t + 2 (lane % 4) + {0, 1}; l: this lane's keys only
     int vs[NT][2];                  // P' = 2^(vs - 127) p step
     float lows[NT][NG][2];          // sums of p low, this lane's keys only
@@ -542,7 +545,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
             float mx = most(t, c) * sl2[t][c];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, d));
-            mx = fmaxf(mx, m[t][c]);
+            const float ref = fmaxf(mx, m[t][c]) + kUnder;
+            mx = ref - kUnder;  // what the weights go by, after ref's rounding
             // nothing finite yet: keep the (empty) sums as they are
             const float f = mx == -INFINITY ? 1.f : exp2_approx(m[t][c] - mx);
             // what the old sums lose, P' may gain
@@ -550,7 +554,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
             const float fo = mx == -INFINITY ? 1.f : exp2_approx(m[t][c] - mx + static_cast<float>(up));
             vs[t][c] += mx == -INFINITY ? 0 : up;
             m[t][c] = mx;
-            nm[t][c] = mx == -INFINITY ? 0.f : -mx;
+            nm[t][c] = mx == -INFINITY ? 0.f : -ref;
             l[t][c] *= f;
 #pragma unroll
             for (int j = 0; j < NG; ++j) lows[t][j][c] *= f;
@@ -625,7 +629,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
                 for (int d = 0; d < ROWS; ++d) high = fmaxf(high, e[i][t][2 * d + c] * step_of(pr[i][d][j]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) high = fmaxf(high, __shfl_xor_sync(kFull, high, d));
-            const int to = min(vs[t][c], 254 - exponent(high, 127 - kTop, 253));
+            const int to = min(vs[t][c], 254 - exponent(high, 127 - kTop, 230));
             const float f = exp2_approx(static_cast<float>(to - vs[t][c]));
             vs[t][c] = to;
             v[c] = power(to);
@@ -702,7 +706,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
         }
         if (h < nh) {
           float* dst = parts + (warp * held + h) * kRow;
-          const float f0 = power(254 - vs[t][c]) * kUnit, f1 = f0 * 0.0625f;
+          const float f0 = power(254 - vs[t][c]) * kUnit, f1 = f0 * 0.0625f;  // vs >= 24: 2^127 at most
           if (r == 0) {
             dst[kD] = m[t][c];
             dst[kD + 1] = sum;

@@ -1,0 +1,151 @@
+"""The 4-bit decode over the range of numbers that a cache may hold: steps from 2^-60 to 2^120.
+
+The bound of a channel, from the kernel's chain.  With weights p (softmax over the visible tokens,
+in 64 bits), A = sum p code step, L = sum p |low| and n tokens:
+  * the result is rounded to bf16: 2^-8 |want|;
+  * weight times step is rounded to fp16: 2^-11 A, and 2^-25 where it falls below the normal numbers,
+    in a unit in which the largest weight times step of the head, M, is 1/2 or more: 15 n 2^-24 M;
+  * fp32 sums of n terms, and the tensor core's, which are cut off: n 2^-23 (A + A' + L), A' the
+    neighbouring channel's (two codes share an operand);
+  * scores: a dozen fp32 operations on numbers of S = sum over groups of |step (q . code)| + |low sum q| in
+    units of log2: weights are off by 12 x 2^-24 (S + 64) log 2 of themselves, their sum as much.
+The queries are small whole numbers times a power of two, exact in the fp16 operands.
+"""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+BF16 = torch.bfloat16
+LOG2E = 1.4426950408889634
+GROUPS = [32, 64, 128]
+
+
+@pytest.fixture(scope="module")
+def kda():
+    import kda as k
+    return k
+
+
+@pytest.fixture(autouse=True)
+def no_device_error(request, kda):
+    yield
+    if "gpu" in request.keywords:
+        torch.cuda.synchronize()
+        assert kda.device_error() == 0
+
+
+def pack(codes, step, low):
+    """The bytes of codes (B,KH,T,128) and of steps and lows (B,KH,T,groups), as kda.h lays them out."""
+    B, KH, T, _ = codes.shape
+    c = codes.reshape(B, KH, T // 16, 16, 128).to(torch.uint8)
+    t, ch = torch.arange(16)[:, None], torch.arange(0, 128, 2)
+    at = (64 * t + 16 * ((ch % 32 // 8) ^ (t // 2 % 4)) + 4 * (ch // 32) + ch % 8 // 2).flatten()
+    rows = torch.empty(B, KH, T // 16, 1024, dtype=torch.uint8, device=codes.device)
+    rows[..., at.to(codes.device)] = (c[..., ::2] | c[..., 1::2] << 4).flatten(-2)
+    side = torch.stack([step, low], -1).to(BF16).reshape(B, KH, T // 16, -1).view(torch.uint8)
+    return torch.cat([rows, side], -1)
+
+
+class Cache:
+    """Random codes with given steps (B,KH,T,groups; powers of two or bf16 numbers) and lows."""
+
+    def __init__(self, gen, step, low, codes=None):
+        B, KH, T, n = step.shape
+        self.step, self.low = step.to(BF16).double(), low.to(BF16).double()
+        if codes is None:
+            codes = torch.randint(0, 16, (B, KH, T, 128), generator=gen, device=step.device)
+        self.codes, self.group = codes, 128 // n
+        self.raw = pack(codes, step, low)
+
+    def head(self, b, g):
+        """Code times step and low of every value of a kv head, (T,128) each."""
+        wide = [x[b, g].repeat_interleave(self.group, -1) for x in (self.step, self.low)]
+        return self.codes[b, g].double() * wide[0], wide[1]
+
+
+def whole(gen, *shape):
+    return torch.randint(-3, 4, shape, generator=gen, device="cuda").double()
+
+
+def compare(out, q, k, v, lengths, requests=None):
+    """Every channel of out (B,QH,128) against the 64-bit value, within the bound above."""
+    rep = q.shape[1] // k.raw.shape[1]
+    for b in requests if requests is not None else range(q.shape[0]):
+        n = int(lengths[b])
+        for g in range(k.raw.shape[1]):
+            kc, kl = (x[:n] for x in k.head(b, g))
+            vc, vl = (x[:n] for x in v.head(b, g))
+            for h in range(g * rep, (g + 1) * rep):
+                qh = q[b, h].double()
+                unit = LOG2E / np.sqrt(128.0)
+                s = (kc + kl) @ qh * unit
+                groups = [((kc @ (qh * m)).abs() + (kl @ (qh * m)).abs()) * unit
+                          for m in torch.eye(128 // k.group, device=q.device, dtype=torch.float64)
+                          .repeat_interleave(k.group, 1)]
+                size = float(sum(groups).max())
+                p = torch.softmax(s / LOG2E, 0)
+                want, A, L = p @ (vc + vl), p @ vc, p @ vl.abs()
+                M = float((p[:, None] * v.step[b, g, :n]).max())
+                A2 = A.unflatten(0, (-1, 2)).flip(1).flatten()
+                bound = (2.0 ** -8 * want.abs() + 2.0 ** -11 * A + 15 * n * 2.0 ** -24 * M
+                         + n * 2.0 ** -23 * (A + A2 + L)
+                         + 2 * 12 * 2.0 ** -24 * (size + 64) * np.log(2.0) * (A + L))
+                got = out[b, h].double()
+                assert torch.isfinite(got).all(), (b, h)
+                off = (got - want).abs() / bound
+                assert float(off.max()) <= 1, (b, h, int(off.argmax()), float(off.max()))
+
+
+def lengths_of(B, T):
+    return [max(1, T - 37 * b - (b > 0) * (T // 3)) for b in range(B)]
+
+
+def spread(B, KH, T, groups, exponents):
+    """Steps 2^e, the exponents by group and token as the function gives them."""
+    t, g = torch.arange(T, device="cuda")[:, None], torch.arange(groups, device="cuda")
+    e = exponents(t, g).double().expand(T, groups)
+    return torch.exp2(e).expand(B, KH, T, groups).contiguous()
+
+
+def test_pack_is_the_layout_of_the_oracle():
+    from oracle import ops as ref
+    rng = np.random.default_rng(0)
+    codes = rng.integers(0, 16, size=(2, 3, 32, 128))
+    step = np.exp2(rng.integers(-4, 5, size=(2, 3, 32, 2))).astype(np.float32)
+    low = -7 * step
+    got = pack(torch.from_numpy(codes), torch.from_numpy(step), torch.from_numpy(low))
+    assert np.array_equal(got.numpy(), ref.q4_pack(codes, step, low))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("e", [-60, 0, 60, 103, 104, 120])
+def test_decode_at_every_size_of_values(kda, group, e):
+    """Steps of 2^e: values of -7 to 8 of them, up to 2^123, finite in fp32 and in bf16."""
+    gen = torch.Generator(device="cuda").manual_seed(e + 100)
+    for B, blocks, QH, KH in ((2, 40, 8, 2), (1, 94, 16, 1), (1, 1400, 6, 1)):
+        T = 16 * blocks
+        k = Cache(gen, *(spread(B, KH, T, 128 // group, lambda t, g: 0 * t + 0 * g - 3) * f for f in (1, -7)))
+        v = Cache(gen, *(spread(B, KH, T, 128 // group, lambda t, g: 0 * t + 0 * g + e) * f for f in (1, -7)))
+        q, lengths = whole(gen, B, QH, 128).to(BF16), lengths_of(B, T)
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+def test_decode_of_constant_groups(kda, group):
+    """Steps of zero beside lows of 2^100, of zero and of -2^120; a lone step among them."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    B, KH, T, groups = 2, 2, 640, 128 // group
+    k = Cache(gen, *(spread(B, KH, T, groups, lambda t, g: 0 * t + 0 * g - 3) * f for f in (1, -7)))
+    q = whole(gen, B, 8, 128).to(BF16)
+    n = torch.tensor([640, 333], dtype=torch.int32, device="cuda")
+    for value in (2.0 ** 100, 0.0, -2.0 ** 120):
+        step = torch.zeros(B, KH, T, groups, device="cuda", dtype=torch.float64)
+        low = torch.full_like(step, value)
+        step[:, :, 301], low[:, :, 301] = 1.0, -7.0
+        v = Cache(gen, step, low)
+        compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, [640, 333])
