@@ -594,7 +594,8 @@ kda_status kda_kv_read_q4(const void* cache, void* out, int64_t B, int64_t block
 /* gqa_decode_q4 (q, out bf16, D 128): gqa_window_decode against 4-bit caches.
  * A window of the cache's length or more sees all of it.  Finite values of any
  * size give the rounded sum, for up to 2^24 visible tokens; a product of weight
- * (relative to the largest) and value that is below 2^-94 loses bits. */
+ * (relative to the largest) and value that is below 2^-94 loses bits.
+ * |q| below 2^120. */
 size_t kda_gqa_decode_q4_workspace_size(int64_t QH, int64_t KH);
 kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, const void* v_cache, const int* lengths, void* out,
                              int64_t B, int64_t blocks, int64_t QH, int64_t KH, int64_t D, int64_t group,

@@ -19,7 +19,7 @@
 // code - 8 by one more multiply-add a pair: 194; a nibble each, a block at a time: 151;
 // two blocks at a time: 139, and 124 for two kv heads together.)
 // The other operands are fp16 then, with ranges of their own: q times a power of two per head
-// that brings its largest value to 1 .. 2, and p step times one per head that keeps it below
+// that brings its largest value to 2^14 .. 2^15, and p step times one per head that keeps it below
 // 2^15 and was last chosen where the largest so far became 1 .. 2 (in the manner of the running
 // maximum: what is too small for fp16 beside it is too small to matter).
 //
@@ -170,6 +170,7 @@ __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
 }
 constexpr uint32_t kEven = 0x000f000fu;
 constexpr float kUnit = 16777216.f;  // 2^24
+constexpr int kQTop = 14;            // q's operands: a head's largest |q| becomes 2^14 to 2^15
 // Bytes 0 and 2 (second: 1 and 3) of a word, in its halves.
 __device__ __forceinline__ uint32_t bytes_of(uint32_t w, int second) {
   return second ? __byte_perm(w, 0u, 0x4341) : w & 0x00ff00ffu;
@@ -395,8 +396,9 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
       }
       top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
       top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-      const int ex = exponent(top, 1, 253);
-      const float f0 = power(254 - ex);
+      // 2^14 and not 1: what f0 brings up, `back` does not have to, which then is finite below |q| = 2^121
+      const int ex = exponent(top, 1 + kQTop, 253);
+      const float f0 = power(254 + kQTop - ex);
       float sum[NG];
 #pragma unroll
       for (int j = 0; j < NG; ++j) sum[j] = 0.f;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
                                                          fmaf(f[k][i + 5], -f1, f[k][i + 4] * f0));
           sum[k / RUNS] += (f[k][i] + f[k][i + 4]) * (f0 / kUnit);  // in the products' unit
         }
-      const float back = power(ex) * (p.scale_log2 * kUnit);
+      const float back = power(ex) * (p.scale_log2 * (kUnit / (1 << kQTop)));
       sl2[t][0] = __shfl_sync(kFull, back, 8 * c4);
       sl2[t][1] = __shfl_sync(kFull, back, 8 * c4 + 4);
 #pragma unroll

@@ -1,4 +1,5 @@
-"""The 4-bit decode over the range of numbers that a cache may hold: steps from 2^-60 to 2^120.
+"""The 4-bit decode over the range of numbers that a cache and a query may hold: steps
+from 2^-60 to 2^120, queries from 2^-100 to 2^119.
 
 The bound of a channel, from the kernel's chain.  With weights p (softmax over the visible tokens,
 in 64 bits), A = sum p code step, L = sum p |low| and n tokens:
@@ -149,3 +150,20 @@ def test_decode_of_constant_groups(kda, group):
         step[:, :, 301], low[:, :, 301] = 1.0, -7.0
         v = Cache(gen, step, low)
         compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, [640, 333])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("e", [-100, -60, 60, 107, 118])
+def test_decode_of_large_and_small_queries(kda, group, e):
+    """|q| up to 3 x 2^e against keys as much smaller: ordinary scores.  (Keys' steps are bf16
+    numbers from 2^-121 on.)"""
+    gen = torch.Generator(device="cuda").manual_seed(e + 100)
+    for B, blocks, QH, KH in ((2, 40, 8, 2), (1, 94, 16, 1)):
+        T = 16 * blocks
+        k = Cache(gen, *(spread(B, KH, T, 128 // group, lambda t, g: 0 * t + 0 * g - e - 3) * f for f in (1, -7)))
+        v = Cache(gen, *(spread(B, KH, T, 128 // group, lambda t, g: 0 * t + 0 * g) * f for f in (1, -7)))
+        q = (whole(gen, B, QH, 128) * 2.0 ** e).to(BF16)
+        lengths = lengths_of(B, T)
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, lengths)
