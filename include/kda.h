@@ -595,7 +595,8 @@ kda_status kda_kv_read_q4(const void* cache, void* out, int64_t B, int64_t block
  * A window of the cache's length or more sees all of it.  Finite values of any
  * size give the rounded sum, for up to 2^24 visible tokens; a product of weight
  * (relative to the largest) and value that is below 2^-94 loses bits.
- * |q| below 2^120. */
+ * |q| below 2^120.  Steps of the groups of a head (among the visible tokens) may
+ * differ by 2^18 before the smaller ones' channels are off by more than bf16's rounding. */
 size_t kda_gqa_decode_q4_workspace_size(int64_t QH, int64_t KH);
 kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, const void* v_cache, const int* lengths, void* out,
                              int64_t B, int64_t blocks, int64_t QH, int64_t KH, int64_t D, int64_t group,

@@ -19,9 +19,12 @@
 // code - 8 by one more multiply-add a pair: 194; a nibble each, a block at a time: 151;
 // two blocks at a time: 139, and 124 for two kv heads together.)
 // The other operands are fp16 then, with ranges of their own: q times a power of two per head
-// that brings its largest value to 2^14 .. 2^15, and p step times one per head that keeps it below
-// 2^15 and was last chosen where the largest so far became 1 .. 2 (in the manner of the running
-// maximum: what is too small for fp16 beside it is too small to matter).
+// that brings its largest value to 2^14 .. 2^15, and P' = p step times one per head that keeps it below
+// 2^15 and was last chosen where the largest so far became 2^6 .. 2^7, in the manner of the running
+// maximum.  fp16's last bit is 2^-24, so a weight times step is held to 2^-11 of itself or, where it is
+// small, 2^-30 of the head's largest: between the groups of a head, whose channels are different
+// outputs, steps may differ by 2^18 before the smaller's are off by more than bf16's rounding.  (The
+// largest at 1 .. 2: 1.4 to 2.5 % off at 2^16, where rounding the result is 0.17 %.)
 //
 // The products are transposed so that the few query heads are the narrow side of the
 // m16n8k16 matrix instruction:
@@ -60,6 +63,8 @@ constexpr unsigned kFull = 0xffffffffu;
 // size stay finite in fp32, as the output is.  (Values below 2^-94 of the largest weight lose bits.)
 constexpr int kUnder = 32;
 constexpr int kTop = 126;           // P' is scaled by 2^kTop at most
+constexpr int kWTop = 6;            // where the scale is chosen, a head's largest P' becomes 2^kWTop or twice that:
+                                    // a weight may then grow by 2^8, as the reference lets it, within fp16
 
 struct DecodeParams {
   const __nv_bfloat16* q;
@@ -551,8 +556,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
             mx = ref - kUnder;  // what the weights go by, after ref's rounding
             // nothing finite yet: keep the (empty) sums as they are
             const float f = mx == -INFINITY ? 1.f : exp2_approx(m[t][c] - mx);
-            // what the old sums lose, P' may gain
-            const int up = min(127 + kTop - vs[t][c], static_cast<int>(fminf(mx - m[t][c], 1000.f)));
+            // what the old sums lose, P' gains, rounded up: however often m moves, the scale does not fall behind
+            const int up = min(127 + kTop - vs[t][c], __float2int_ru(fminf(mx - m[t][c], 1000.f)));
             const float fo = mx == -INFINITY ? 1.f : exp2_approx(m[t][c] - mx + static_cast<float>(up));
             vs[t][c] += mx == -INFINITY ? 0 : up;
             m[t][c] = mx;
@@ -631,7 +636,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
                 for (int d = 0; d < ROWS; ++d) high = fmaxf(high, e[i][t][2 * d + c] * step_of(pr[i][d][j]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) high = fmaxf(high, __shfl_xor_sync(kFull, high, d));
-            const int to = min(vs[t][c], 254 - exponent(high, 127 - kTop, 230));
+            const int to = min(vs[t][c], 254 + kWTop - exponent(high, 127 - kTop + kWTop, 230));
             const float f = exp2_approx(static_cast<float>(to - vs[t][c]));
             vs[t][c] = to;
             v[c] = power(to);
@@ -708,7 +713,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
         }
         if (h < nh) {
           float* dst = parts + (warp * held + h) * kRow;
-          const float f0 = power(254 - vs[t][c]) * kUnit, f1 = f0 * 0.0625f;  // vs >= 24: 2^127 at most
+          const float f0 = power(254 - vs[t][c]) * kUnit, f1 = f0 * 0.0625f;  // vs >= 32: 2^119 at most
           if (r == 0) {
             dst[kD] = m[t][c];
             dst[kD + 1] = sum;

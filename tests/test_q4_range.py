@@ -1,11 +1,12 @@
 """The 4-bit decode over the range of numbers that a cache and a query may hold: steps
-from 2^-60 to 2^120, queries from 2^-100 to 2^119.
+from 2^-60 to 2^120 and such as differ between a head's groups and between tokens, queries from
+2^-100 to 2^119.
 
 The bound of a channel, from the kernel's chain.  With weights p (softmax over the visible tokens,
 in 64 bits), A = sum p code step, L = sum p |low| and n tokens:
   * the result is rounded to bf16: 2^-8 |want|;
   * weight times step is rounded to fp16: 2^-11 A, and 2^-25 where it falls below the normal numbers,
-    in a unit in which the largest weight times step of the head, M, is 1/2 or more: 15 n 2^-24 M;
+    in a unit in which the largest weight times step of the head, M, is 2^5 or more: 15 n 2^-30 M;
   * fp32 sums of n terms, and the tensor core's, which are cut off: n 2^-23 (A + A' + L), A' the
     neighbouring channel's (two codes share an operand);
   * scores: a dozen fp32 operations on numbers of S = sum over groups of |step (q . code)| + |low sum q| in
@@ -21,6 +22,9 @@ torch = pytest.importorskip("torch")
 BF16 = torch.bfloat16
 LOG2E = 1.4426950408889634
 GROUPS = [32, 64, 128]
+# B, blocks, QH, KH: a cluster's walks of 8 warps and of 16, with more than 8 heads, runs, runs of two kv
+# heads together, runs with more than 8 heads
+WALKS = [(2, 40, 8, 2), (1, 512, 16, 8), (1, 94, 16, 1), (1, 1400, 6, 1), (64, 260, 16, 8), (1, 2600, 16, 1)]
 
 
 @pytest.fixture(scope="module")
@@ -90,7 +94,7 @@ def compare(out, q, k, v, lengths, requests=None):
                 want, A, L = p @ (vc + vl), p @ vc, p @ vl.abs()
                 M = float((p[:, None] * v.step[b, g, :n]).max())
                 A2 = A.unflatten(0, (-1, 2)).flip(1).flatten()
-                bound = (2.0 ** -8 * want.abs() + 2.0 ** -11 * A + 15 * n * 2.0 ** -24 * M
+                bound = (2.0 ** -8 * want.abs() + 2.0 ** -11 * A + 15 * n * 2.0 ** -30 * M
                          + n * 2.0 ** -23 * (A + A2 + L)
                          + 2 * 12 * 2.0 ** -24 * (size + 64) * np.log(2.0) * (A + L))
                 got = out[b, h].double()
@@ -167,3 +171,41 @@ def test_decode_of_large_and_small_queries(kda, group, e):
         lengths = lengths_of(B, T)
         n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
         compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("e", [8, 12, 20])
+def test_decode_where_groups_of_a_head_differ(kda, group, e):
+    """Steps 2^e apart between a head's groups: each group is its own outputs, within its own bound."""
+    gen = torch.Generator(device="cuda").manual_seed(e)
+    for B, blocks, QH, KH in ((2, 40, 8, 2), (1, 94, 16, 1), (1, 1400, 6, 1), (64, 260, 16, 8)):
+        T, groups = 16 * blocks, 128 // group
+        k = Cache(gen, *(spread(B, KH, T, groups, lambda t, g: 0 * t + 0 * g - 3) * f for f in (1, -7)))
+        v = Cache(gen, *(spread(B, KH, T, groups, lambda t, g: 0 * t - e * (g % 2)) * f for f in (1, -7)))
+        q, lengths = whole(gen, B, QH, 128).to(BF16), lengths_of(B, T)
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, lengths, range(0, B, 31))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("B,blocks,QH,KH", WALKS)
+def test_decode_where_scores_rise_past_large_steps(kda, group, B, blocks, QH, KH):
+    """The first blocks have steps 2^18 larger; scores then rise all the way, so that those blocks' weights
+    vanish and what stays is small beside them: the scale of a head's weights has to follow."""
+    gen = torch.Generator(device="cuda").manual_seed(blocks)
+    T, groups = 16 * blocks, 128 // group
+    step = spread(B, KH, T, groups, lambda t, g: 18.0 * (t < T // 4) + 0 * g)
+    v = Cache(gen, step, -7 * step)
+    # keys: lows that rise, by 1/16 a token or so that they do not pass 188; codes are noise
+    rise = min(3000.0 / T, 1.0)
+    t = torch.arange(T, device="cuda").double()[:, None]
+    low = (t * rise / 16).to(BF16).double().expand(B, KH, T, groups).contiguous()
+    k = Cache(gen, spread(B, KH, T, groups, lambda t, g: 0 * t + 0 * g - 6), low)
+    q = whole(gen, B, QH, 128)
+    q[..., 0] += 14 - q.sum(-1)  # the sum is 14: a rise of 14 log2e / sqrt(128) = 1.8 for each unit of low
+    q = q.to(BF16)
+    lengths = [T - 16 * (b % 5) for b in range(B)]
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, lengths, range(0, B, 31))
