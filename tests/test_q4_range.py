@@ -1,6 +1,6 @@
 """The 4-bit decode over the range of numbers that a cache and a query may hold: steps
 from 2^-60 to 2^120 and such as differ between a head's groups and between tokens, queries from
-2^-100 to 2^119.
+2^-100 to 2^119; and a long context.
 
 The bound of a channel, from the kernel's chain.  With weights p (softmax over the visible tokens,
 in 64 bits), A = sum p code step, L = sum p |low| and n tokens:
@@ -209,3 +209,57 @@ def test_decode_where_scores_rise_past_large_steps(kda, group, B, blocks, QH, KH
     lengths = [T - 16 * (b % 5) for b in range(B)]
     n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
     compare(kda.gqa_decode_q4(q, k.raw, v.raw, n), q, k, v, lengths, range(0, B, 31))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("e", [8, 12, 16])
+@pytest.mark.parametrize("B,blocks,QH,KH", WALKS)
+def test_decode_where_tokens_differ(kda, group, e, B, blocks, QH, KH):
+    """Small steps, then some blocks with steps 2^e larger, in one group or in all, then small ones: a
+    warp's sums are rescaled with sums there already.  In every other pair of channels the large
+    tokens hold zeros (code 0, low 0), so the small tokens' sums alone are the output there."""
+    gen = torch.Generator(device="cuda").manual_seed(e * blocks)
+    T, groups = 16 * blocks, 128 // group
+    lengths = [T - 16 * (b % 5) for b in range(B)]
+    for which in (0, groups):  # the last group alone, or every one
+
+        def large(t, g):
+            return ((t // 16 % 19 >= 14) & (t // 16 % 19 < 16) | (t == 2 * T // 3)) & (g >= groups - 1 - which)
+
+        big = spread(B, KH, T, groups, large) > 1.5
+        step = torch.where(big, 2.0 ** e, 1.0)
+        codes = torch.randint(0, 16, (B, KH, T, 128), generator=gen, device="cuda")
+        off = torch.arange(128, device="cuda") // 2 % 2 == 1
+        codes[big.repeat_interleave(group, -1) & off] = 0
+        v = Cache(gen, step, 0 * step, codes)
+        k = Cache(gen, *(spread(B, KH, T, groups, lambda t, g: 0 * t + 0 * g - 4) * f for f in (1, -7)))
+        q = whole(gen, B, QH, 128).to(BF16)
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        out = kda.gqa_decode_q4(q, k.raw, v.raw, n)
+        compare(out, q, k, v, lengths, range(0, B, 31))
+        assert torch.equal(out, kda.gqa_decode_q4(q, k.raw, v.raw, n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+def test_decode_of_131072_tokens(kda, group):
+    """Random queries and values, relative L2 over 32 heads.  Rounding the result: at most 2^-8 / sqrt(3) of the
+    values' (every error uniform in half a step, every value at the bottom of its binade), 5 % more for 4,096
+    samples; the weights' and queries' rounding to fp16, 2^-11 each."""
+    gen = torch.Generator(device="cuda").manual_seed(group)
+    T, KH, QH, n = 131072, 8, 32, 131001
+    caches = []
+    for _ in range(2):
+        step = 0.3 + 0.1 * torch.rand(1, KH, T, 128 // group, generator=gen, device="cuda")
+        caches.append(Cache(gen, step, -7.5 * step))
+    k, v = caches
+    q = torch.randn(1, QH, 128, generator=gen, device="cuda").to(BF16)
+    out = kda.gqa_decode_q4(q, k.raw, v.raw, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    want = torch.empty(QH, 128, dtype=torch.float64, device="cuda")
+    for g in range(KH):
+        kv, vv = (sum(c.head(0, g))[:n] for c in (k, v))
+        qs = q[0, 4 * g:4 * g + 4].double()
+        want[4 * g:4 * g + 4] = torch.softmax(qs @ kv.T / np.sqrt(128.0), -1) @ vv
+    err = float((out[0].double() - want).norm() / want.norm())
+    assert err <= 1.05 * 2.0 ** -8 / np.sqrt(3.0) + 2.0 ** -10, err
