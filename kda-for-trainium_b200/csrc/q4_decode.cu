@@ -213,6 +213,11 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? static_cast<unsigned>(a) / static_cast<unsigned>(b) : a / b;
 }
 
+// Whether the warps' shares lie without gaps between rows: with groups of 32 and 8 heads two CTAs find no
+// room on an SM otherwise.  (64 requests of 1 to 8,192 tokens: 4 query heads for each of 8 kv heads, two
+// together, 110 us with gaps, 87 without; 8 148 and 135.  Elsewhere gaps are up to 5 % faster.)
+constexpr bool compact_rows(int nt, int group, int warps) { return nt == 1 && group == 32 && warps == 8; }
+
 // NT: groups of 8 query heads a CTA works on.  PAIR: two kv heads of at most 4 query heads each;
 // a tile of 16 rows of the matrix instruction is then 8 tokens of either, and of S^T the two
 // quarters count in which rows and columns are of one kv head: a lane's two values instead of
@@ -365,9 +370,15 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load();
 
-  // [WARPS][held][kRow]; where the rings leave no room for it, in their place at the end
+  // [WARPS][held][kRow], in the rings' place at the end where they leave no room for it.  (COMPACT:
+  // [WARPS][held][kD], columns exchanged so that the heads which a warp writes at once meet different
+  // banks, then each row's maximum and sum.)
   float* parts = reinterpret_cast<float*>(smem + (WARPS == 16 ? 0 : WARPS * STAGES * kStage));
   const int held = PAIR ? 2 * p.rep : min(p.rep, H);
+  constexpr bool COMPACT = compact_rows(NT, GROUP, WARPS);
+  constexpr int kPart = COMPACT ? kD : kRow;
+  auto top_at = [&](int i) { return COMPACT ? WARPS * held * kD + 2 * i : i * kRow + kD; };  // of row i's maximum, sum
+  auto swap = [](int i) { return COMPACT ? (i & 6) << 2 : 0; };
   bool ok = true;
   int done = 0;       // this warp's chunks
   int piece_at = 0;   // the piece's first chunk in the run
@@ -712,17 +723,18 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
           for (int d = 4; d < 32; d <<= 1) add[j] += __shfl_xor_sync(kFull, add[j], d);
         }
         if (h < nh) {
-          float* dst = parts + (warp * held + h) * kRow;
+          float* dst = parts + (warp * held + h) * kPart;
           const float f0 = power(254 - vs[t][c]) * kUnit, f1 = f0 * 0.0625f;  // vs >= 32: 2^119 at most
           if (r == 0) {
-            dst[kD] = m[t][c];
-            dst[kD + 1] = sum;
+            float* top = parts + top_at(warp * held + h);
+            top[0] = m[t][c];
+            top[1] = sum;
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int st = 0; st < 2; ++st)
-              *reinterpret_cast<float2*>(dst + 32 * k + 4 * r + 2 * st) =
+              *reinterpret_cast<float2*>(dst + ((32 * k + 4 * r + 2 * st) ^ swap(warp * held + h))) =
                   make_float2(fmaf(o[t][k][st][c], f0, add[k / RUNS]),
                               fmaf(o[t][k][st][c + 2] - o[t][k][st][c], f1, add[k / RUNS]));
         }
@@ -737,15 +749,15 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
       float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        mw[w] = parts[(w * held + h) * kRow + kD];
+        mw[w] = parts[top_at(w * held + h)];
         mm = fmaxf(mm, mw[w]);
       }
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float* src = parts + (w * held + h) * kRow;
+        const float* src = parts + (w * held + h) * kPart;
         const float f = share_weight(mw[w], mm);
-        const float4 v = *reinterpret_cast<const float4*>(src + d);
-        ll += f * src[kD + 1];
+        const float4 v = *reinterpret_cast<const float4*>(src + (d ^ swap(w * held + h)));
+        ll += f * parts[top_at(w * held + h) + 1];
         oo.x += f * v.x, oo.y += f * v.y, oo.z += f * v.z, oo.w += f * v.w;
       }
       if (cut || size > 1) {
@@ -857,10 +869,14 @@ kda_status launch_decode(const DecodeParams& p, int ctas, int cluster, cudaStrea
   // cluster's short walks are 1 to 3 % faster with 3 stages there than with 4)
   constexpr int kStages = NT == 1 ? 2 : CLUSTER ? 3 : 4;
   constexpr int H = 8 * NT;
-  constexpr int kRing = WARPS * kStages * 4 * q4_block_bytes(GROUP), kRows = WARPS * kRow * 4;
+  constexpr int kRing = WARPS * kStages * 4 * q4_block_bytes(GROUP);
+  constexpr int kRows = WARPS * (compact_rows(NT, GROUP, WARPS) ? kD + 2 : kRow) * 4;
   static_assert((WARPS + 1) * H * kRow * 4 <= kRing, "shares in the rings' place");
   auto bytes = [](int held) { return static_cast<size_t>(kRing + (WARPS == 16 ? 0 : held * kRows)); };
-  static_assert(kRing + (WARPS == 16 ? 0 : H * kRows) <= (NT == 1 && WARPS == 8 ? 113 : 226) * 1024, "shared memory budget");
+  // an SM's 228 KB hold each CTA's static part (barriers and the run's place) and 1 KB of the system's too
+  constexpr int kStatic = (WARPS * kStages * 8 + WARPS * 8 + 16 + 127) / 128 * 128;
+  static_assert(kRing + (WARPS == 16 ? 0 : H * kRows) + kStatic + 1024 <= (NT == 1 && WARPS == 8 ? 114 : 228) * 1024,
+                "shared memory budget");
   auto* kernel = q4_decode_kernel<NT, GROUP, kStages, PAIR, CLUSTER, WARPS>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
