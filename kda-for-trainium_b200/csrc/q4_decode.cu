@@ -29,8 +29,8 @@
 // The products are transposed so that the few query heads are the narrow side of the
 // m16n8k16 matrix instruction:
 //   S^T (16 keys x 8 heads)  = K q^T          O^T (128 x 8 heads) += V^T P^T
-// The running maximum moves only when a score exceeds it by 2^8, which fp32 sums and bf16
-// weights hold exactly as well; so a block usually needs no exchange between lanes.
+// The running maximum moves only when a score exceeds it by 2^8, room for which fp32 sums and the
+// scale of the fp16 weights leave; so a block usually needs no exchange between lanes.
 //
 // A walk is a request's blocks of a kv head.  Short ones: a cluster of 1 to 16 CTAs for each; the
 // blocks go to their warps in turn, each through a ring of bulk copies of its own, and the
@@ -74,12 +74,12 @@ struct DecodeParams {
   int64_t q_b, q_h;          // element strides
   int64_t k_b, k_h, v_b, v_h;  // byte strides
   int cache_len, window, sinks;
-  int B, QH, KH, rep;
+  int B, QH, rep;
   int parts;                 // groups of 8 NT query heads per kv head; 0: two kv heads together
   int walks;                 // of a request
   float scale_log2;
   float* shares;             // [2 x CTAs][8 NT][kRow]
-  int4* pieces;              // [2 x CTAs]: walk, 0, chunks of the share, of the walk
+  int2* pieces;              // [2 x CTAs]: walk, chunks of the share (0: none)
   unsigned* length_err;
 };
 
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
       return;
     }
   } else {
-    if (threadIdx.x == 0) p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) p.pieces[2 * blockIdx.x] = p.pieces[2 * blockIdx.x + 1] = make_int2(0, 0);
     // The run: chunks [r0, r1) of all walks.  Each thread counts the requests [b0, b1).
     const int heads = p.walks;
     const int each = (p.B + THREADS - 1) / THREADS;
@@ -772,7 +772,7 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 && WARPS == 8 ? 2 : 1)
             make_uint2(pack_bf16x2(oo.x / ll, oo.y / ll), pack_bf16x2(oo.z / ll, oo.w / ll));
       }
     }
-    if (cut && threadIdx.x == 0) p.pieces[slot] = make_int4(at.b * p.walks + at.hp, 0, n, at.w.n);
+    if (cut && threadIdx.x == 0) p.pieces[slot] = make_int2(at.b * p.walks + at.hp, n);
     if (CLUSTER && size > 1) {
       cluster_sync_all();
       const uint32_t base = smem_u32(joined);
@@ -820,15 +820,15 @@ __global__ void __launch_bounds__(kThreads) q4_join_kernel(const DecodeParams p,
     const int slot = i == 0 ? 2 * x + 1 : 2 * min(x + i, ctas - 1);
     return p.shares + (static_cast<int64_t>(slot) * H + h) * kRow;
   };
-  const int4 w = p.pieces[2 * x + 1];
-  int4 next = p.pieces[2 * min(x + 1 + lane, ctas - 1)];
+  const int2 w = p.pieces[2 * x + 1];
+  int2 next = p.pieces[2 * min(x + 1 + lane, ctas - 1)];
   float mm = share(lane)[kD];
   const int b = w.x / p.walks;
   const Heads hs = heads_of(p, H, w.x - b * p.walks);
-  if (w.z == 0 || h >= hs.n) return;
+  if (w.y == 0 || h >= hs.n) return;
   int count = 1;
   for (;;) {
-    const unsigned others = ~__ballot_sync(kFull, x + count + lane < ctas && next.z > 0 && next.x == w.x);
+    const unsigned others = ~__ballot_sync(kFull, x + count + lane < ctas && next.y > 0 && next.x == w.x);
     count += others ? __ffs(static_cast<int>(others)) - 1 : 32;
     if (others) break;
     next = p.pieces[2 * min(x + count + lane, ctas - 1)];
@@ -973,7 +973,7 @@ using namespace kda;
 extern "C" size_t kda_gqa_decode_q4_workspace_size(int64_t QH, int64_t KH) {
   if (QH <= 0 || KH <= 0 || QH % KH || QH > 65535) return 0;
   const int64_t rep = QH / KH;
-  return static_cast<size_t>(2 * decode_ctas(rep)) * (16 + (rep > 8 ? 16 : 8) * kRow * 4);
+  return static_cast<size_t>(2 * decode_ctas(rep)) * (sizeof(int2) + (rep > 8 ? 16 : 8) * kRow * 4);
 }
 
 extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, const void* v_cache, const int* lengths,
@@ -1019,7 +1019,6 @@ extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, cons
   p.sinks = static_cast<int>(sinks < T ? sinks : T);
   p.B = static_cast<int>(B);
   p.QH = static_cast<int>(QH);
-  p.KH = static_cast<int>(KH);
   p.rep = static_cast<int>(QH / KH);
   p.parts = p.rep > 8 ? (p.rep + 15) / 16 : 1;
   const int64_t tokens = p.window + static_cast<int64_t>(p.sinks) < T ? p.window + static_cast<int64_t>(p.sinks) : T;
@@ -1032,7 +1031,7 @@ extern "C" kda_status kda_gqa_decode_q4(const void* q, const void* k_cache, cons
   p.walks = static_cast<int>(p.parts == 0 ? KH / 2 : KH * p.parts);
   p.scale_log2 = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(kD)));
   const int ctas = decode_ctas(p.rep);
-  p.pieces = static_cast<int4*>(workspace);
+  p.pieces = static_cast<int2*>(workspace);
   p.shares = reinterpret_cast<float*>(p.pieces + 2 * ctas);
   p.length_err = kda_err_ptr_q4_decode_length();
   // the longest run, and the number of walks
