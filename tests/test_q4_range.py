@@ -19,6 +19,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from test_q4_cache import DECODE_CASES, LONG_CASES  # noqa: E402
+
 BF16 = torch.bfloat16
 LOG2E = 1.4426950408889634
 GROUPS = [32, 64, 128]
@@ -263,3 +265,35 @@ def test_decode_of_131072_tokens(kda, group):
         want[4 * g:4 * g + 4] = torch.softmax(qs @ kv.T / np.sqrt(128.0), -1) @ vv
     err = float((out[0].double() - want).norm() / want.norm())
     assert err <= 1.05 * 2.0 ** -8 / np.sqrt(3.0) + 2.0 ** -10, err
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("case", range(len(DECODE_CASES) + len(LONG_CASES)))
+def test_decode_of_random_values(kda, group, case):
+    """Relative L2 of a request: rounding the result, 2^-8 at most, and 2^-10 for the fp16 operands: queries
+    and weights are off by 2^-11 of themselves each, independently of one another."""
+    B, blocks, QH, KH, window, sinks, *lens = (DECODE_CASES + LONG_CASES)[case]
+    gen = torch.Generator(device="cuda").manual_seed(case)
+    T, seen = 16 * blocks, 10 ** 9 if window is None else window
+    lens = lens[0] if lens else [T - (77 * b) % T for b in range(B)]
+    caches = []
+    for _ in range(2):
+        step = 0.3 + 0.1 * torch.rand(B, KH, T, 128 // group, generator=gen, device="cuda")
+        caches.append(Cache(gen, step, -step * (7 + torch.rand(step.shape, generator=gen, device="cuda"))))
+    k, v = caches
+    q = torch.randn(B, QH, 128, generator=gen, device="cuda").to(BF16)
+    out = kda.gqa_decode_q4(q, k.raw, v.raw, torch.tensor(lens, dtype=torch.int32, device="cuda"), window, sinks)
+    for b in range(0, B, 1 + B // 8):
+        n = lens[b]
+        if n <= 0:
+            assert not out[b].any()
+            continue
+        j = torch.arange(n, device="cuda")
+        want = []
+        for g in range(KH):
+            kv, vv = (sum(c.head(b, g))[:n] for c in caches)
+            s = q[b, g * QH // KH:(g + 1) * QH // KH].double() @ kv.T / np.sqrt(128.0)
+            want.append(torch.softmax(s.masked_fill((j < n - seen) & (j >= sinks), -torch.inf), -1) @ vv)
+        want = torch.cat(want)
+        assert float((out[b].double() - want).norm() / want.norm()) <= 2.0 ** -8 + 2.0 ** -10
