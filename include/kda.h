@@ -575,7 +575,9 @@ size_t kda_q4_block_bytes(int64_t group);
 
 /* kv_append_q4: new rows of k and v (bf16) into the caches, per group low =
  * min, step = bf16((max - low)/15), code = round((x - low)/step) (single fp32
- * operations; a group that holds an infinity or a NaN reads back as NaN).
+ * operations, the quotient by step as a product with its fp32 reciprocal; a step
+ * below 2^-126 becomes zero; a group that holds an infinity or a NaN, or whose
+ * max - low is past fp32's largest number, reads back as NaN).
  * offsets NULL: tokens/B rows of each request, k and v (B,S,KH,D) with strides
  * of request, token and head; else int32 [B+1]: rows [offsets[b], offsets[b+1])
  * of k, v (tokens,KH,D) are request b's (strides[0] is not used), rows of none

@@ -10,8 +10,9 @@
 // 16 lanes take a row, 8 channels each (one 16-byte load, one 4-byte store of codes), a
 // group's minimum and maximum by exchanges of bf16 pairs.  Bandwidth-bound: 656 bytes a
 // row of k and v; 20.4 us for 18,700 tokens of 8 heads, floor 15.0; 92 for 100,000, floor 80.
-// Reading back: 12.5 us for 32,768 tokens of 8 heads, floor 13.1 at the copy rate (13.7 with
-// codes converted one by one: the integer pipe was full).
+// Reading back, of buffers that do not stay in the L2: 54.5 us for 131,072 tokens of 8 heads, floor
+// 52.5; 15.9 for 32,768, floor 13.1.  (12.5 for those again and again into one buffer, 13.7 with codes
+// converted one by one: the integer pipe was full.)
 #include <cuda_fp16.h>
 
 #include "launch.cuh"
@@ -64,8 +65,8 @@ __device__ __forceinline__ void quantise(const uint4 x, unsigned mask, uint32_t*
   const float inv = step > 0.f ? __frcp_rn(step) : 0.f;  // NaN: zero codes beside a NaN pair
   // Adding 2^23 rounds to a whole number (ties to even), left in the low mantissa bits; the
   // shifted sum of the eight bit patterns is the word, and eight times 2^23's pattern shifted.
-  // No code is past 15: step is off by 2^-9 of itself at most, and (max - low) / step then
-  // below 15.03.
+  // No code is past 15: step is off by 2^-8 of itself at most, and (max - low) / step then
+  // below 15.06.
   float f[8];
   unpack_bf16x8(x, f);
   uint32_t w = 0u - 0x4b000000u * 0x11111111u;

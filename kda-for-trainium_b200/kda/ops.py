@@ -754,7 +754,8 @@ def kv_append_q4(k, v, k_cache, v_cache, lengths, offsets=None):
     ``offsets`` (int32 (B + 1,)) (T,KH,128): rows offsets[b] .. offsets[b + 1] - 1
     are request b's, rows of none are skipped.  Per group low is the minimum, step
     bf16((max - low) / 15), code round((x - low) / step): a value is at most about
-    half a step off.  A group with an infinity or a NaN reads back as NaN.  A
+    half a step off.  A group with an infinity or a NaN, or with a range past fp32's
+    largest number, reads back as NaN.  A
     negative length marks an idle slot: nothing is written.  A position past the
     cache is not written and sets ``device_error``.  ``lengths`` is left as it is."""
     _native.kv_append_q4(k, v, k_cache, v_cache, lengths, offsets)
@@ -771,7 +772,8 @@ def gqa_decode_q4(q, k_cache, v_cache, lengths, window=None, sinks=0, *, out=Non
     lengths[b] valid tokens of request b (int32, the newest among them), of which the
     last ``window`` are seen (None: all) and the first ``sinks``.  A request without
     tokens (length 0 or less) gives zeros; a length past the cache is cut to it and
-    sets ``device_error``.  Returns (B,QH,128)."""
+    sets ``device_error``.  ``include/kda.h`` states the range of q and of the caches'
+    values.  Returns (B,QH,128)."""
     return _native.gqa_decode_q4(q, k_cache, v_cache, lengths, window, sinks, out, workspace)
 
 
