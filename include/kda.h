@@ -547,7 +547,9 @@ kda_status kda_packed_plan(const int* offsets, int64_t sequences, int64_t tokens
  * log2-sum-exp of the scaled scores, for the backward.  Rows of no sequence are
  * never read into a result; in out and lse they become zeros (zero_rest != 0)
  * or stay as they are.  A plan for another number of tokens: nothing is done
- * and 8 is set in the device error word.  No workspace. */
+ * and 8 is set in the device error word.  A row's sums are divided at the end:
+ * they have to stay within fp32, 2^8 |v| times the row's keys at most.  No
+ * workspace. */
 kda_status kda_gqa_packed_bf16(const void* q, const void* k, const void* v, const void* plan, size_t plan_bytes,
                                void* out, float* lse, int zero_rest, int64_t tokens, int64_t QH, int64_t KH,
                                int64_t D, const int64_t* q_strides, const int64_t* k_strides,
